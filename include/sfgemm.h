@@ -388,6 +388,82 @@ int sf_cast(const void* x, sf_dtype in_dtype, void* y, sf_dtype out_dtype,
             int64_t n, void* stream);
 
 /* ------------------------------------------------------------------ */
+/* Experts: routing, row exchange, products over ragged groups         */
+/* ------------------------------------------------------------------ */
+/* No counterparts in the reference.  All operands are contiguous device
+ * memory; calls are asynchronous on `stream`, allocate nothing and may be
+ * captured. */
+
+/* Top-k routing of `tokens` rows of `experts` logits:
+ *   p = softmax(logits[t, :]) in fp32; the k largest logits are chosen, in
+ *   descending order, equal ones by ascending index, NaN above every number;
+ *   weights[t, j] = p[chosen_j], divided by their sum if `renormalize`.
+ * A token whose logits are all -inf gets weights 0 (and experts 0 .. k-1).
+ *   weights  fp32 [tokens, k]      expert  int32 [tokens, k]
+ *   offsets  int32 [experts + 1]: the assignments (t, j) ordered by expert,
+ *            within one by t k + j; expert e's are [offsets[e], offsets[e+1])
+ *   slots    int32 [tokens, k]: the place of (t, j) in that order
+ * 1 <= k <= min(experts, 16), experts <= 1024, tokens * k < 2^31.  `work`:
+ * sf_route_topk_work bytes of 4-byte aligned device memory, overwritten (may
+ * be NULL where that is 0).  tokens == 0 writes zeros to offsets. */
+int64_t sf_route_topk_work(int64_t tokens, int64_t experts);
+int sf_route_topk(const void* logits, int64_t tokens, int64_t experts, int64_t k, sf_dtype dtype, int renormalize,
+                  float* weights, int32_t* expert, int32_t* offsets, int32_t* slots, void* work, void* stream);
+
+/* Gradient of the logits from that of the weights (`weights`, `expert` as
+ * sf_route_topk wrote them, the same logits and `renormalize`); the choice
+ * itself has none.  grad_logits of `dtype`. */
+int sf_route_topk_backward(const float* grad_weights, const void* logits, const float* weights,
+                           const int32_t* expert, int64_t tokens, int64_t experts, int64_t k, sf_dtype dtype,
+                           int renormalize, void* grad_logits, void* stream);
+
+/* Rows between token order ([tokens, cols]) and expert order ([tokens * k,
+ * cols]); slots[t, j] as sf_route_topk writes them: every place once.  (A
+ * slot outside [0, tokens * k) is skipped; of a place that is named twice
+ * either row may win, and one that is not named is not written.)
+ *   sf_dispatch_rows   rows[slots[t, j]] = x[t]
+ *   sf_combine_rows    y[t] = sum_j weights[t, j] rows[slots[t, j]], in the
+ *                      order of j, fp32, one rounding; weights NULL: 1
+ *                      (the gradient of sf_dispatch_rows)
+ *   sf_combine_rows_backward   grad_rows[slots[t, j]] = weights[t, j] grad[t],
+ *                      grad_weights[t, j] = <grad[t], rows[slots[t, j]]>
+ * k >= 1, cols < 2^31. */
+int sf_dispatch_rows(const void* x, const int32_t* slots, void* rows, int64_t tokens, int64_t k, int64_t cols,
+                     sf_dtype dtype, void* stream);
+int sf_combine_rows(const void* rows, const int32_t* slots, const float* weights, void* y, int64_t tokens, int64_t k,
+                    int64_t cols, sf_dtype dtype, void* stream);
+int sf_combine_rows_backward(const void* grad, const void* rows, const int32_t* slots, const float* weights,
+                             void* grad_rows, float* grad_weights, int64_t tokens, int64_t k, int64_t cols,
+                             sf_dtype dtype, void* stream);
+
+/* A linear layer with one weight per group of rows:
+ *   y[r, :] = epi(W[e] x[r, :] (+ bias[e]))  for the rows r of group e
+ * x [rows, K], W [groups, N, K], bias [groups, N], y [rows, N], all `dtype`;
+ * sums as sf_gemm's.  Group e is the rows [offsets[e], offsets[e + 1]) of
+ * ascending `offsets` (int32, device, groups + 1 of them, the first 0) and
+ * may be empty; rows from offsets[groups] on are set to 0.  The sizes are
+ * read on the device, so a router's offsets need not reach the host.  (For
+ * other contents of offsets: group e ends at the largest of offsets[1..e+1],
+ * cut to [0, rows], and starts where the group before it ends.)
+ * groups <= 1024, rows < 2^31. */
+int sf_grouped_linear(const void* x, const void* W, const int32_t* offsets, const void* bias, void* y, int64_t rows,
+                      int64_t groups, int64_t N, int64_t K, sf_dtype dtype, sf_epilogue epi, void* stream);
+/* Its gradients (epi NONE or BIAS): grad_x[r] = W[e]^T grad[r], 0 for rows of
+ * no group; grad_W[e] = sum over the rows of e of grad[r] x[r]^T and
+ * grad_bias[e] = sum of grad[r], 0 for an empty group (grad_bias NULL: not
+ * formed).  fp32 sums in an order fixed by the sizes, one rounding. */
+int sf_grouped_linear_dx(const void* grad, const void* W, const int32_t* offsets, void* grad_x, int64_t rows,
+                         int64_t groups, int64_t N, int64_t K, sf_dtype dtype, void* stream);
+int sf_grouped_linear_dw(const void* grad, const void* x, const int32_t* offsets, void* grad_W, void* grad_bias,
+                         int64_t rows, int64_t groups, int64_t N, int64_t K, sf_dtype dtype, void* stream);
+
+/* out = grad * act'(pre) over n elements, act that of SF_EPI_SILU or
+ * SF_EPI_GELU_TANH: the gradient ahead of a fused activation, `pre` being the
+ * layer's output without it.  fp32 arithmetic; out may be grad or pre. */
+int sf_act_backward(const void* grad, const void* pre, void* out, int64_t n, sf_dtype dtype, sf_epilogue act,
+                    void* stream);
+
+/* ------------------------------------------------------------------ */
 /* Runtime: devices, memory, streams, events                           */
 /* (the CUDA runtime calls _cuda_ops.pyx:33-142 binds directly)        */
 /* ------------------------------------------------------------------ */

@@ -12,13 +12,13 @@ the package fails if the native extension has not been built
 (``python scaffolding_amd/build.py``).
 """
 from . import _cuda_ops as _cuops  # noqa: F401  (fails loudly if not built)
-from .dtype import bfloat16, dtype, float16, float32
+from .dtype import bfloat16, dtype, float16, float32, int32, uint8
 from .device import device
 from .tensor import Tensor, from_numpy, matmul, matmul_nt, tensor, zeros, empty
 from . import cuda, nn, backends  # noqa: E402
 
 __all__ = [
     "Tensor", "tensor", "from_numpy", "zeros", "empty", "matmul", "matmul_nt",
-    "dtype", "float32", "float16", "bfloat16", "device", "cuda", "nn", "backends",
+    "dtype", "float32", "float16", "bfloat16", "int32", "uint8", "device", "cuda", "nn", "backends",
 ]
 __version__ = "0.1.0"

@@ -26,7 +26,7 @@ Differences from the reference, on purpose:
 
 import numpy as np
 cimport numpy as cnp
-from libc.stdint cimport int64_t, uint64_t, uintptr_t
+from libc.stdint cimport int32_t, int64_t, uint64_t, uintptr_t
 from libc.string cimport memset
 from libc.math cimport sqrt
 
@@ -116,6 +116,28 @@ cdef extern from "sfgemm.h" nogil:
                    uint64_t offset, void* stream)
     int sf_sum_dim(const void* x, void* out, int64_t outer, int64_t dim_size, int64_t inner,
                    sf_dtype in_dtype, sf_dtype out_dtype, void* stream)
+    int64_t sf_route_topk_work(int64_t tokens, int64_t experts)
+    int sf_route_topk(const void* logits, int64_t tokens, int64_t experts, int64_t k, sf_dtype dtype, int renormalize,
+                      float* weights, int32_t* expert, int32_t* offsets, int32_t* slots, void* work, void* stream)
+    int sf_route_topk_backward(const float* grad_weights, const void* logits, const float* weights,
+                               const int32_t* expert, int64_t tokens, int64_t experts, int64_t k, sf_dtype dtype,
+                               int renormalize, void* grad_logits, void* stream)
+    int sf_dispatch_rows(const void* x, const int32_t* slots, void* rows, int64_t tokens, int64_t k, int64_t cols,
+                         sf_dtype dtype, void* stream)
+    int sf_combine_rows(const void* rows, const int32_t* slots, const float* weights, void* y, int64_t tokens,
+                        int64_t k, int64_t cols, sf_dtype dtype, void* stream)
+    int sf_combine_rows_backward(const void* grad, const void* rows, const int32_t* slots, const float* weights,
+                                 void* grad_rows, float* grad_weights, int64_t tokens, int64_t k, int64_t cols,
+                                 sf_dtype dtype, void* stream)
+    int sf_grouped_linear(const void* x, const void* W, const int32_t* offsets, const void* bias, void* y,
+                          int64_t rows, int64_t groups, int64_t N, int64_t K, sf_dtype dtype, sf_epilogue epi,
+                          void* stream)
+    int sf_grouped_linear_dx(const void* grad, const void* W, const int32_t* offsets, void* grad_x, int64_t rows,
+                             int64_t groups, int64_t N, int64_t K, sf_dtype dtype, void* stream)
+    int sf_grouped_linear_dw(const void* grad, const void* x, const int32_t* offsets, void* grad_W, void* grad_bias,
+                             int64_t rows, int64_t groups, int64_t N, int64_t K, sf_dtype dtype, void* stream)
+    int sf_act_backward(const void* grad, const void* pre, void* out, int64_t n, sf_dtype dtype, sf_epilogue act,
+                        void* stream)
     int sf_cast(const void* x, sf_dtype in_dtype, void* y, sf_dtype out_dtype, int64_t n, void* stream)
 
     int sf_get_device_count(int* count)
@@ -157,6 +179,9 @@ BFLOAT16 = np.dtype([('bf16', '<u2')])
 
 _F32 = np.dtype(np.float32)
 _F16 = np.dtype(np.float16)
+# Storage only (indices, packed weights): no operator computes in these.
+_I32 = np.dtype(np.int32)
+_U8 = np.dtype(np.uint8)
 
 
 cdef sf_dtype _sf_dtype(object dt) except *:
@@ -371,6 +396,12 @@ def gputensor_from_numpy(cnp.ndarray arr not None, int device_id=-1, dtype=None)
     if target < 0:
         target = _current_device()
     target_dt = resolve_dtype(dtype) if dtype is not None else arr.dtype
+    if (target_dt == _I32 or target_dt == _U8) and arr.dtype != target_dt:
+        # indices and packed bytes: never by way of fp32, and never wrapped
+        if arr.dtype.kind not in 'iu' or (arr.size and (arr.min() < np.iinfo(target_dt).min
+                                                        or arr.max() > np.iinfo(target_dt).max)):
+            raise TypeError("gputensor_from_numpy: %s values do not convert to %s" % (arr.dtype, target_dt))
+        arr = arr.astype(target_dt)
     if target_dt == BFLOAT16 and arr.dtype == BFLOAT16:
         src = np.ascontiguousarray(arr)
         host_dt = BFLOAT16
@@ -380,7 +411,7 @@ def gputensor_from_numpy(cnp.ndarray arr not None, int device_id=-1, dtype=None)
     else:
         src = np.ascontiguousarray(arr)
         host_dt = src.dtype
-    if host_dt != BFLOAT16 and host_dt not in (_F32, _F16):
+    if host_dt != BFLOAT16 and host_dt not in (_F32, _F16, _I32, _U8):
         raise TypeError("gputensor_from_numpy: unsupported dtype %r" % (arr.dtype,))
     cdef cnp.ndarray flat = src.reshape(-1)
     cdef size_t nbytes = flat.nbytes
@@ -1120,6 +1151,285 @@ def dev_multihead_attention(gt_q, gt_k, gt_v, int heads, scale=None):
     cdef int64_t D = C // heads
     s = (1.0 / sqrt(<double>D)) if scale is None else float(scale)
     return _mha_strided(gt_q, 0, C, gt_k, 0, C, gt_v, 0, C, qs[0], qs[1], ks[1], heads, D, s)
+
+
+# ================================================================
+#  Experts: routing, row exchange, products over ragged groups
+#  (no counterparts in the reference)
+# ================================================================
+
+cdef object _same_device(str name, first, tuple others):
+    for o in others:
+        if o is not None and o.device_id != first.device_id:
+            raise ValueError("%s: operands on devices %d and %d" % (name, first.device_id, o.device_id))
+
+
+cdef object _need_storage(gt, dt, str name, str what):
+    if gt.dtype is not dt and gt.dtype != dt:
+        raise TypeError("%s: %s must be %s, got %s" % (name, what, dt, gt.dtype))
+
+
+def dev_route_topk(gt_logits, int k, bint renormalize=True):
+    """Top-k routing of logits (..., E): (weights fp32 (..., k), experts
+    int32 (..., k), offsets int32 (E + 1,), slots int32 (..., k)).  p =
+    softmax(logits) in fp32; the k largest logits in descending order, equal
+    ones by ascending index, NaN above every number; weights p of the chosen,
+    divided by their sum with `renormalize`, 0 for a token whose logits are
+    all -inf.  With the assignments (t, j) ordered by expert, within one by
+    t k + j, slots holds each one's place and expert e's are places
+    [offsets[e], offsets[e + 1]).  E <= 1024, k <= min(E, 16)."""
+    shape = tuple(gt_logits.shape)
+    if len(shape) < 1:
+        raise ValueError("dev_route_topk: logits must be (..., E)")
+    cdef int64_t E = shape[-1]
+    cdef int64_t T = 1
+    for s in shape[:-1]:
+        T *= s
+    if E < 1 or k < 1 or k > E:
+        raise ValueError("dev_route_topk: k must be in [1, %d], got %d" % (E, k))
+    cdef int dev = gt_logits.device_id
+    cdef sf_dtype dt = _sf_dtype(gt_logits.dtype)
+    lead = shape[:-1] + (k,)
+    weights = _alloc_like(lead, _F32, dev)
+    experts = _alloc_like(lead, _I32, dev)
+    offsets = _alloc_like((int(E) + 1,), _I32, dev)
+    slots = _alloc_like(lead, _I32, dev)
+    cdef int64_t need = sf_route_topk_work(T, E)
+    cdef CudaBuffer work = None
+    cdef void* pk = NULL
+    if need > 0:
+        work = _make_buffer(need, dev)
+        pk = work.ptr
+    cdef void* pl = _ptr(gt_logits)
+    cdef float* pw = <float*>_ptr(weights)
+    cdef int32_t* pe = <int32_t*>_ptr(experts)
+    cdef int32_t* po = <int32_t*>_ptr(offsets)
+    cdef int32_t* ps = <int32_t*>_ptr(slots)
+    cdef int ret
+    with nogil:
+        ret = sf_route_topk(pl, T, E, k, dt, renormalize, pw, pe, po, ps, pk, NULL)
+    _check_kernel(ret)
+    return weights, experts, offsets, slots
+
+
+def dev_route_topk_backward(gt_grad, gt_logits, gt_weights, gt_experts, bint renormalize=True):
+    """Gradient of dev_route_topk's logits (..., E), in their dtype, from that
+    of its weights: grad, weights fp32 (..., k), experts int32 (..., k)."""
+    name = 'dev_route_topk_backward'
+    shape, lead = tuple(gt_logits.shape), tuple(gt_weights.shape)
+    _need_storage(gt_grad, _F32, name, 'grad')
+    _need_storage(gt_weights, _F32, name, 'weights')
+    _need_storage(gt_experts, _I32, name, 'experts')
+    if len(shape) < 1 or len(lead) != len(shape) or lead[:-1] != shape[:-1] or tuple(gt_grad.shape) != lead \
+            or tuple(gt_experts.shape) != lead or not 1 <= lead[-1] <= shape[-1]:
+        raise ValueError("%s: grad %s, weights %s and experts %s do not match logits %s"
+                         % (name, gt_grad.shape, lead, gt_experts.shape, shape))
+    _same_device(name, gt_logits, (gt_grad, gt_weights, gt_experts))
+    cdef int64_t E = shape[-1], k = lead[-1]
+    cdef int64_t T = gt_logits.numel // E
+    cdef sf_dtype dt = _sf_dtype(gt_logits.dtype)
+    out = _alloc_like(shape, gt_logits.dtype, gt_logits.device_id)
+    cdef float* pg = <float*>_ptr(gt_grad)
+    cdef void* pl = _ptr(gt_logits)
+    cdef float* pw = <float*>_ptr(gt_weights)
+    cdef int32_t* pe = <int32_t*>_ptr(gt_experts)
+    cdef void* po = _ptr(out)
+    cdef int ret
+    with nogil:
+        ret = sf_route_topk_backward(pg, pl, pw, pe, T, E, k, dt, renormalize, po, NULL)
+    _check_kernel(ret)
+    return out
+
+
+def dev_dispatch_rows(gt_x, gt_slots):
+    """Tokens x (..., D) in expert order: rows (T k, D) with rows[slots[t, j]]
+    = x[t], slots (..., k) as dev_route_topk gives them (every place once)."""
+    name = 'dev_dispatch_rows'
+    shape, lead = tuple(gt_x.shape), tuple(gt_slots.shape)
+    _need_storage(gt_slots, _I32, name, 'slots')
+    if len(shape) < 1 or len(lead) != len(shape) or lead[:-1] != shape[:-1] or lead[-1] < 1:
+        raise ValueError("%s: x %s and slots %s do not match" % (name, shape, lead))
+    _same_device(name, gt_x, (gt_slots,))
+    cdef int64_t D = shape[-1], k = lead[-1]
+    cdef int64_t T = gt_slots.numel // k
+    cdef sf_dtype dt = _sf_dtype(gt_x.dtype)
+    out = _alloc_like((int(T * k), int(D)), gt_x.dtype, gt_x.device_id)
+    cdef void* px = _ptr(gt_x)
+    cdef int32_t* ps = <int32_t*>_ptr(gt_slots)
+    cdef void* po = _ptr(out)
+    cdef int ret
+    with nogil:
+        ret = sf_dispatch_rows(px, ps, po, T, k, D, dt, NULL)
+    _check_kernel(ret)
+    return out
+
+
+cdef object _rows_shapes(str name, rows, slots, weights):
+    lead = tuple(slots.shape)
+    _need_storage(slots, _I32, name, 'slots')
+    if len(rows.shape) != 2 or len(lead) < 1 or lead[-1] < 1 or rows.shape[0] != slots.numel:
+        raise ValueError("%s: rows %s do not hold one row for each of slots %s" % (name, rows.shape, lead))
+    if weights is not None:
+        _need_storage(weights, _F32, name, 'weights')
+        if tuple(weights.shape) != lead:
+            raise ValueError("%s: weights %s and slots %s do not match" % (name, weights.shape, lead))
+    _same_device(name, rows, (slots, weights))
+    return lead
+
+
+def dev_combine_rows(gt_rows, gt_slots, gt_weights=None):
+    """Tokens from rows in expert order: y[t] = sum_j weights[t, j]
+    rows[slots[t, j]], fp32 sums in the order of j, one rounding.  rows (T k,
+    D), slots int32 (..., k), weights fp32 (..., k) or None for 1 (the
+    gradient of dev_dispatch_rows) -> (..., D)."""
+    lead = _rows_shapes('dev_combine_rows', gt_rows, gt_slots, gt_weights)
+    cdef int64_t D = gt_rows.shape[1], k = lead[-1]
+    cdef int64_t T = gt_slots.numel // k
+    cdef sf_dtype dt = _sf_dtype(gt_rows.dtype)
+    out = _alloc_like(lead[:-1] + (int(D),), gt_rows.dtype, gt_rows.device_id)
+    cdef void* pr = _ptr(gt_rows)
+    cdef int32_t* ps = <int32_t*>_ptr(gt_slots)
+    cdef float* pw = NULL
+    if gt_weights is not None:
+        pw = <float*>_ptr(gt_weights)
+    cdef void* po = _ptr(out)
+    cdef int ret
+    with nogil:
+        ret = sf_combine_rows(pr, ps, pw, po, T, k, D, dt, NULL)
+    _check_kernel(ret)
+    return out
+
+
+def dev_combine_rows_backward(gt_grad, gt_rows, gt_slots, gt_weights):
+    """(grad_rows, grad_weights) of dev_combine_rows with weights, from grad
+    (..., D): grad_rows[slots[t, j]] = weights[t, j] grad[t] in rows' dtype,
+    grad_weights[t, j] = <grad[t], rows[slots[t, j]]> in fp32."""
+    name = 'dev_combine_rows_backward'
+    lead = _rows_shapes(name, gt_rows, gt_slots, gt_weights)
+    _same_dtype(gt_grad, gt_rows, name)
+    _same_device(name, gt_rows, (gt_grad,))
+    cdef int64_t D = gt_rows.shape[1], k = lead[-1]
+    cdef int64_t T = gt_slots.numel // k
+    if tuple(gt_grad.shape) != lead[:-1] + (int(D),):
+        raise ValueError("%s: grad %s, rows %s and slots %s do not match" % (name, gt_grad.shape, gt_rows.shape, lead))
+    cdef sf_dtype dt = _sf_dtype(gt_rows.dtype)
+    grad_rows = _alloc_like(tuple(gt_rows.shape), gt_rows.dtype, gt_rows.device_id)
+    grad_weights = _alloc_like(lead, _F32, gt_rows.device_id)
+    cdef void* pg = _ptr(gt_grad)
+    cdef void* pr = _ptr(gt_rows)
+    cdef int32_t* ps = <int32_t*>_ptr(gt_slots)
+    cdef float* pw = <float*>_ptr(gt_weights)
+    cdef void* po = _ptr(grad_rows)
+    cdef float* pd = <float*>_ptr(grad_weights)
+    cdef int ret
+    with nogil:
+        ret = sf_combine_rows_backward(pg, pr, ps, pw, po, pd, T, k, D, dt, NULL)
+    _check_kernel(ret)
+    return grad_rows, grad_weights
+
+
+cdef object _grouped_shapes(str name, x, weight, offsets):
+    if len(x.shape) != 2 or len(weight.shape) != 3:
+        raise ValueError("%s: rows must be (R, C) and the weight (E, N, K), got %s and %s"
+                         % (name, x.shape, weight.shape))
+    _need_storage(offsets, _I32, name, 'offsets')
+    if tuple(offsets.shape) != (weight.shape[0] + 1,):
+        raise ValueError("%s: offsets must be (%d,), got %s" % (name, weight.shape[0] + 1, offsets.shape))
+    _same_device(name, x, (weight, offsets))
+
+
+def dev_grouped_linear(gt_x, gt_weight, gt_offsets, gt_bias=None, activation=None):
+    """y[r] = act(x[r] @ W[e]^T + b[e]) for the rows r of group e, one launch:
+    x (R, K), W (E, N, K), b (E, N) or None, offsets int32 (E + 1,) ascending
+    from 0 on the device: group e is the rows [offsets[e], offsets[e + 1])
+    and may be empty; rows from offsets[E] on give 0."""
+    name = 'dev_grouped_linear'
+    _same_dtype(gt_x, gt_weight, name)
+    _grouped_shapes(name, gt_x, gt_weight, gt_offsets)
+    cdef int64_t R = gt_x.shape[0], E = gt_weight.shape[0], N = gt_weight.shape[1], K = gt_weight.shape[2]
+    if gt_x.shape[1] != K:
+        raise ValueError("%s: x %s and W %s not aligned" % (name, gt_x.shape, gt_weight.shape))
+    if activation not in _ACTS:
+        raise ValueError("%s: unknown activation %r" % (name, activation))
+    cdef int act = _ACTS[activation]
+    cdef int epi
+    cdef void* pb = NULL
+    if gt_bias is not None:
+        _same_dtype(gt_x, gt_bias, name)
+        if tuple(gt_bias.shape) != (E, N):
+            raise ValueError("%s: bias must be (%d, %d), got %s" % (name, E, N, gt_bias.shape))
+        _same_device(name, gt_x, (gt_bias,))
+        pb = _ptr(gt_bias)
+        epi = (SF_EPI_BIAS, SF_EPI_BIAS_SILU, SF_EPI_BIAS_GELU_TANH)[act]
+    else:
+        epi = (SF_EPI_NONE, SF_EPI_SILU, SF_EPI_GELU_TANH)[act]
+    out = _alloc_like((int(R), int(N)), gt_x.dtype, gt_x.device_id)
+    cdef sf_dtype dt = _sf_dtype(gt_x.dtype)
+    cdef void* px = _ptr(gt_x)
+    cdef void* pw = _ptr(gt_weight)
+    cdef int32_t* po = <int32_t*>_ptr(gt_offsets)
+    cdef void* py = _ptr(out)
+    cdef int ret
+    with nogil:
+        ret = sf_grouped_linear(px, pw, po, pb, py, R, E, N, K, dt, <sf_epilogue>epi, NULL)
+    _check_kernel(ret)
+    return out
+
+
+def dev_grouped_linear_backward(gt_grad, gt_x, gt_weight, gt_offsets, bint has_bias=True, activation=None, pre=None):
+    """Gradients of dev_grouped_linear, (grad_x (R, K), grad_weight (E, N,
+    K), grad_bias (E, N) or None), from grad (R, N).  With the layer's
+    `activation`, `pre` (R, N) is its output without one (dev_grouped_linear
+    of the same operands), and grad is first multiplied by act'(pre) (rounded
+    to the operands' dtype, as the gradient of a separate activation is)."""
+    name = 'dev_grouped_linear_backward'
+    _same_dtype(gt_grad, gt_x, name)
+    _same_dtype(gt_grad, gt_weight, name)
+    _grouped_shapes(name, gt_grad, gt_weight, gt_offsets)
+    cdef int64_t R = gt_grad.shape[0], E = gt_weight.shape[0], N = gt_weight.shape[1], K = gt_weight.shape[2]
+    if gt_grad.shape[1] != N or tuple(gt_x.shape) != (R, K):
+        raise ValueError("%s: g %s, x %s and W %s not aligned" % (name, gt_grad.shape, gt_x.shape, gt_weight.shape))
+    if activation not in _ACTS:
+        raise ValueError("%s: unknown activation %r" % (name, activation))
+    _same_device(name, gt_grad, (gt_x, pre))
+    cdef int act = _ACTS[activation]
+    cdef int dev = gt_grad.device_id
+    cdef sf_dtype dt = _sf_dtype(gt_grad.dtype)
+    cdef int ret
+    cdef void* pg = _ptr(gt_grad)
+    cdef void* pp
+    cdef void* pq
+    cdef int64_t n = gt_grad.numel
+    if act != 0:
+        if pre is None:
+            raise ValueError("%s: the gradient of activation %r needs pre" % (name, activation))
+        _same_dtype(gt_grad, pre, name)
+        if tuple(pre.shape) != (R, N):
+            raise ValueError("%s: pre must be (%d, %d), got %s" % (name, R, N, pre.shape))
+        through = _alloc_like((int(R), int(N)), gt_grad.dtype, dev)
+        pp = _ptr(pre)
+        pq = _ptr(through)
+        with nogil:
+            ret = sf_act_backward(pg, pp, pq, n, dt, SF_EPI_SILU if act == 1 else SF_EPI_GELU_TANH, NULL)
+        _check_kernel(ret)
+        pg = pq
+    grad_x = _alloc_like((int(R), int(K)), gt_grad.dtype, dev)
+    grad_weight = _alloc_like(tuple(gt_weight.shape), gt_grad.dtype, dev)
+    grad_bias = _alloc_like((int(E), int(N)), gt_grad.dtype, dev) if has_bias else None
+    cdef void* px = _ptr(gt_x)
+    cdef void* pw = _ptr(gt_weight)
+    cdef int32_t* po = <int32_t*>_ptr(gt_offsets)
+    cdef void* pdx = _ptr(grad_x)
+    cdef void* pdw = _ptr(grad_weight)
+    cdef void* pdb = NULL
+    if has_bias:
+        pdb = _ptr(grad_bias)
+    with nogil:
+        ret = sf_grouped_linear_dx(pg, pw, po, pdx, R, E, N, K, dt, NULL)
+        if ret == SF_OK:
+            ret = sf_grouped_linear_dw(pg, px, po, pdw, pdb, R, E, N, K, dt, NULL)
+    _check_kernel(ret)
+    return grad_x, grad_weight, grad_bias
 
 
 # ================================================================

@@ -29,6 +29,8 @@ int fail(int code, const char* fmt, ...) {
   return code;
 }
 
+void clear_error() { g_err[0] = 0; }
+
 int check_hip(hipError_t e, const char* what) {
   if (e == hipSuccess) return SF_OK;
   // The runtime also keeps the error as the thread's last error; it is
@@ -133,7 +135,7 @@ static std::unordered_map<int, int> g_cu_count;
 // Without a device (sf_gemm_plan on a host with no GPU) the planner assumes
 // 256 CUs, or the count in SF_PLAN_CU_COUNT, so the plans of other parts
 // can be checked on the host; a visible device always reports its own.
-static int cu_count_current() {
+int cu_count_current() {
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess) {
     const char* s = getenv("SF_PLAN_CU_COUNT");

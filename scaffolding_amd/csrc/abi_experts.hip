@@ -1,0 +1,272 @@
+// abi_experts.hip — C entry points of the expert operators: argument checks
+// (before any HIP call) and the choice of tiles.
+#include "sf_internal.hpp"
+
+namespace sf {
+
+static bool known(sf_dtype d) { return d == SF_F32 || d == SF_F16 || d == SF_BF16; }
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+static int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Tile of a grouped product over `per` rows a group on average (the sizes
+// themselves are on the device).  `vec`: operands for the direct loads.
+static int rows_tile(int64_t per, bool vec, bool f32, bool b_kmajor) {
+  if (f32) return !vec ? TILE_GENERIC : (per > 96 ? TILE_128x128 : TILE_64x64);
+  if (!vec) return per > 96 ? TILE_RAG_128 : TILE_RAG_64;
+  if (per > 96) return TILE_MID_128;
+  return per <= 32 && b_kmajor ? TILE_MID_32 : TILE_MID_64;
+}
+
+static void tile_size(int cfg, int& bm, int& bn) {
+  switch (cfg) {
+    case TILE_MID_128:
+    case TILE_RAG_128:
+    case TILE_128x128: bm = bn = 128; return;
+    case TILE_MID_32: bm = 32; bn = 64; return;
+    default: bm = bn = 64; return;
+  }
+}
+
+template <typename P>
+static void fill(P& p, const void* A, const void* B, void* C, const void* bias, int64_t M, int64_t N, int64_t K,
+                 const int32_t* offsets, int64_t groups, int64_t rows, sf_epilogue epi) {
+  p = P{};
+  p.A = A;
+  p.B = B;
+  p.C = C;
+  p.bias = bias;
+  p.M = static_cast<int>(M);
+  p.N = static_cast<int>(N);
+  p.K = static_cast<int>(K);
+  p.alpha = 1.0f;
+  p.epi = epi;
+  p.offsets = offsets;
+  p.groups = static_cast<int>(groups);
+  p.rows = static_cast<int>(rows);
+}
+
+// The sizes that all entries of the grouped products share.
+static int grouped_check(const char* name, int64_t rows, int64_t groups, int64_t N, int64_t K, sf_dtype dtype) {
+  if (!known(dtype)) return fail(SF_ERR_INVALID_ARG, "%s: unknown dtype %d", name, (int)dtype);
+  if (rows < 0 || groups < 0 || N < 0 || K < 0) return fail(SF_ERR_INVALID_ARG, "%s: negative size", name);
+  if (groups > kMaxGroups) return fail(SF_ERR_UNSUPPORTED, "%s: %lld groups (at most %d)", name, (long long)groups, kMaxGroups);
+  if (rows >= INT32_MAX || N >= INT32_MAX || K >= INT32_MAX)
+    return fail(SF_ERR_UNSUPPORTED, "%s: sizes must be < 2^31 - 1", name);
+  return SF_OK;
+}
+
+// C rows = op(B[e]) A rows: M = rows, `N` columns out, `K` summed.
+static int grouped_rows(const char* name, const void* A, const void* B, const void* bias, void* C,
+                        const int32_t* offsets, int64_t rows, int64_t groups, int64_t N, int64_t K, bool b_kmajor,
+                        sf_dtype dtype, sf_epilogue epi, hipStream_t st) {
+  GroupedRows p;
+  fill(p, A, B, C, bias, rows, N, K, offsets, groups, rows, epi);
+  p.lda = K;
+  p.ldb = b_kmajor ? K : N;
+  p.ldc = N;
+  p.sB = N * K;
+  const bool f32 = dtype == SF_F32;
+  // 16-byte rows; one weight and one tile of A below the direct loads' 2 GiB
+  const bool vec = f32 ? K % 4 == 0 && (b_kmajor || N % 4 == 0) && aligned16(A) && aligned16(B)
+                       : K % 8 == 0 && (b_kmajor || N % 8 == 0) && aligned16(A) && aligned16(B) &&
+                             N * K < (int64_t(1) << 30) && K < (int64_t(1) << 22);
+  const int64_t per = rows / (groups < rows ? (groups > 0 ? groups : 1) : rows);
+  const int cfg = rows_tile(per, vec, f32, b_kmajor);
+  int bm, bn;
+  tile_size(cfg, bm, bn);
+  p.tiles_n = static_cast<int>(cdiv(N, bn));
+  const int64_t gx = grouped_max_tiles(rows, groups, bm) * p.tiles_n;
+  if (gx > (int64_t(1) << 22)) return fail(SF_ERR_UNSUPPORTED, "%s: more than 2^22 tiles", name);
+  const unsigned g = static_cast<unsigned>(gx);
+  switch (dtype) {
+    case SF_F16: return launch_grouped_rows_f16(b_kmajor, cfg, p, g, st);
+    case SF_BF16: return launch_grouped_rows_bf16(b_kmajor, cfg, p, g, st);
+    default: return launch_grouped_rows_f32(b_kmajor, cfg, p, g, st);
+  }
+}
+
+}  // namespace sf
+
+using namespace sf;
+
+extern "C" {
+
+int64_t sf_route_topk_work(int64_t tokens, int64_t experts) {
+  const int64_t nb = tokens > 0 ? route_blocks(tokens) : 0;
+  return nb > 1 && experts > 0 ? nb * experts * 4 : 0;
+}
+
+static int route_check(const char* name, int64_t tokens, int64_t experts, int64_t k, sf_dtype dtype) {
+  if (!known(dtype)) return fail(SF_ERR_INVALID_ARG, "%s: unknown dtype %d", name, (int)dtype);
+  if (tokens < 0 || experts < 1 || k < 1 || k > experts)
+    return fail(SF_ERR_INVALID_ARG, "%s: needs tokens >= 0 and 1 <= k <= experts (tokens=%lld experts=%lld k=%lld)",
+                name, (long long)tokens, (long long)experts, (long long)k);
+  if (experts > kMaxGroups || k > route_max_k())
+    return fail(SF_ERR_UNSUPPORTED, "%s: at most %d experts and k <= %d (experts=%lld k=%lld)", name, kMaxGroups,
+                route_max_k(), (long long)experts, (long long)k);
+  if (tokens * k >= INT32_MAX || tokens >= INT32_MAX)
+    return fail(SF_ERR_UNSUPPORTED, "%s: tokens * k must be < 2^31 - 1", name);
+  return SF_OK;
+}
+
+int sf_route_topk(const void* logits, int64_t tokens, int64_t experts, int64_t k, sf_dtype dtype, int renormalize,
+                  float* weights, int32_t* expert, int32_t* offsets, int32_t* slots, void* work, void* stream) {
+  clear_error();
+  const int rc = route_check("sf_route_topk", tokens, experts, k, dtype);
+  if (rc != SF_OK) return rc;
+  if (offsets == nullptr) return fail(SF_ERR_INVALID_ARG, "sf_route_topk: null pointer");
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (tokens == 0) return launch_zero(offsets, static_cast<size_t>(experts + 1) * 4, st);
+  if (logits == nullptr || weights == nullptr || expert == nullptr || slots == nullptr ||
+      (work == nullptr && sf_route_topk_work(tokens, experts) > 0))
+    return fail(SF_ERR_INVALID_ARG, "sf_route_topk: null pointer");
+  return launch_route(logits, tokens, experts, static_cast<int>(k), dtype, renormalize != 0, weights, expert, offsets,
+                      slots, static_cast<int*>(work), st);
+}
+
+int sf_route_topk_backward(const float* grad_weights, const void* logits, const float* weights,
+                           const int32_t* expert, int64_t tokens, int64_t experts, int64_t k, sf_dtype dtype,
+                           int renormalize, void* grad_logits, void* stream) {
+  clear_error();
+  const int rc = route_check("sf_route_topk_backward", tokens, experts, k, dtype);
+  if (rc != SF_OK) return rc;
+  if (tokens == 0) return SF_OK;
+  if (grad_weights == nullptr || logits == nullptr || weights == nullptr || expert == nullptr ||
+      grad_logits == nullptr)
+    return fail(SF_ERR_INVALID_ARG, "sf_route_topk_backward: null pointer");
+  return launch_route_backward(grad_weights, logits, weights, expert, tokens, experts, static_cast<int>(k), dtype,
+                               renormalize != 0, grad_logits, static_cast<hipStream_t>(stream));
+}
+
+static int rows_check(const char* name, int64_t tokens, int64_t k, int64_t cols, sf_dtype dtype) {
+  if (!known(dtype)) return fail(SF_ERR_INVALID_ARG, "%s: unknown dtype %d", name, (int)dtype);
+  if (tokens < 0 || k < 1 || cols < 0)
+    return fail(SF_ERR_INVALID_ARG, "%s: needs tokens >= 0, k >= 1 and cols >= 0 (tokens=%lld k=%lld cols=%lld)", name,
+                (long long)tokens, (long long)k, (long long)cols);
+  if (tokens >= INT32_MAX || k >= INT32_MAX || cols >= INT32_MAX || tokens * k >= INT32_MAX)
+    return fail(SF_ERR_UNSUPPORTED, "%s: tokens * k and cols must be < 2^31 - 1", name);
+  return SF_OK;
+}
+
+int sf_dispatch_rows(const void* x, const int32_t* slots, void* rows, int64_t tokens, int64_t k, int64_t cols,
+                     sf_dtype dtype, void* stream) {
+  clear_error();
+  const int rc = rows_check("sf_dispatch_rows", tokens, k, cols, dtype);
+  if (rc != SF_OK || tokens == 0 || cols == 0) return rc;
+  if (x == nullptr || slots == nullptr || rows == nullptr)
+    return fail(SF_ERR_INVALID_ARG, "sf_dispatch_rows: null pointer");
+  return launch_rows(0, x, nullptr, slots, nullptr, rows, nullptr, tokens, static_cast<int>(k), cols, dtype,
+                     static_cast<hipStream_t>(stream));
+}
+
+int sf_combine_rows(const void* rows, const int32_t* slots, const float* weights, void* y, int64_t tokens, int64_t k,
+                    int64_t cols, sf_dtype dtype, void* stream) {
+  clear_error();
+  const int rc = rows_check("sf_combine_rows", tokens, k, cols, dtype);
+  if (rc != SF_OK || tokens == 0 || cols == 0) return rc;
+  if (rows == nullptr || slots == nullptr || y == nullptr)
+    return fail(SF_ERR_INVALID_ARG, "sf_combine_rows: null pointer");
+  return launch_rows(1, rows, nullptr, slots, weights, y, nullptr, tokens, static_cast<int>(k), cols, dtype,
+                     static_cast<hipStream_t>(stream));
+}
+
+int sf_combine_rows_backward(const void* grad, const void* rows, const int32_t* slots, const float* weights,
+                             void* grad_rows, float* grad_weights, int64_t tokens, int64_t k, int64_t cols,
+                             sf_dtype dtype, void* stream) {
+  clear_error();
+  const int rc = rows_check("sf_combine_rows_backward", tokens, k, cols, dtype);
+  if (rc != SF_OK || tokens == 0) return rc;
+  if (slots == nullptr || weights == nullptr || grad_weights == nullptr ||
+      (cols > 0 && (grad == nullptr || rows == nullptr || grad_rows == nullptr)))
+    return fail(SF_ERR_INVALID_ARG, "sf_combine_rows_backward: null pointer");
+  return launch_rows(2, grad, rows, slots, weights, grad_rows, grad_weights, tokens, static_cast<int>(k), cols, dtype,
+                     static_cast<hipStream_t>(stream));
+}
+
+int sf_grouped_linear(const void* x, const void* W, const int32_t* offsets, const void* bias, void* y, int64_t rows,
+                      int64_t groups, int64_t N, int64_t K, sf_dtype dtype, sf_epilogue epi, void* stream) {
+  clear_error();
+  const int rc = grouped_check("sf_grouped_linear", rows, groups, N, K, dtype);
+  if (rc != SF_OK) return rc;
+  if (epi < SF_EPI_NONE || epi > SF_EPI_GELU_TANH)
+    return fail(SF_ERR_INVALID_ARG, "sf_grouped_linear: unknown epilogue %d", (int)epi);
+  if (epi_has_bias(epi) && bias == nullptr && groups > 0 && N > 0)
+    return fail(SF_ERR_INVALID_ARG, "sf_grouped_linear: the epilogue needs a bias");
+  if (rows == 0 || N == 0) return SF_OK;
+  if (y == nullptr || offsets == nullptr || (K > 0 && (x == nullptr || (groups > 0 && W == nullptr))))
+    return fail(SF_ERR_INVALID_ARG, "sf_grouped_linear: null pointer");
+  return grouped_rows("sf_grouped_linear", x, W, bias, y, offsets, rows, groups, N, K, true, dtype, epi,
+                      static_cast<hipStream_t>(stream));
+}
+
+int sf_grouped_linear_dx(const void* grad, const void* W, const int32_t* offsets, void* grad_x, int64_t rows,
+                         int64_t groups, int64_t N, int64_t K, sf_dtype dtype, void* stream) {
+  clear_error();
+  const int rc = grouped_check("sf_grouped_linear_dx", rows, groups, N, K, dtype);
+  if (rc != SF_OK || rows == 0 || K == 0) return rc;
+  if (grad_x == nullptr || offsets == nullptr || (N > 0 && (grad == nullptr || (groups > 0 && W == nullptr))))
+    return fail(SF_ERR_INVALID_ARG, "sf_grouped_linear_dx: null pointer");
+  return grouped_rows("sf_grouped_linear_dx", grad, W, nullptr, grad_x, offsets, rows, groups, K, N, false, dtype,
+                      SF_EPI_NONE, static_cast<hipStream_t>(stream));
+}
+
+int sf_grouped_linear_dw(const void* grad, const void* x, const int32_t* offsets, void* grad_W, void* grad_bias,
+                         int64_t rows, int64_t groups, int64_t N, int64_t K, sf_dtype dtype, void* stream) {
+  clear_error();
+  int rc = grouped_check("sf_grouped_linear_dw", rows, groups, N, K, dtype);
+  if (rc != SF_OK || groups == 0 || N == 0) return rc;
+  if (offsets == nullptr || (K > 0 && grad_W == nullptr) || (rows > 0 && grad == nullptr) ||
+      (rows > 0 && K > 0 && x == nullptr))
+    return fail(SF_ERR_INVALID_ARG, "sf_grouped_linear_dw: null pointer");
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (K > 0) {
+    GroupedSums p;
+    fill(p, grad, x, grad_W, nullptr, N, K, rows, offsets, groups, rows, SF_EPI_NONE);
+    p.lda = N;
+    p.ldb = K;
+    p.ldc = K;
+    p.sC = N * K;
+    const bool f32 = dtype == SF_F32;
+    // 16-byte rows; a group's rows, all rows at most, below the direct loads' 2 GiB
+    const bool vec = f32 ? N % 4 == 0 && K % 4 == 0 && aligned16(grad) && aligned16(x)
+                         : N % 8 == 0 && K % 8 == 0 && aligned16(grad) && aligned16(x) &&
+                               (rows + 64) * (N > K ? N : K) < (int64_t(1) << 30);
+    int cfg;
+    if (f32)
+      cfg = !vec ? TILE_GENERIC : (N > 64 && K > 64 ? TILE_128x128 : TILE_64x64);
+    else if (N > 64 && K > 64)
+      cfg = vec ? TILE_MID_128 : TILE_RAG_128;
+    else
+      cfg = vec ? TILE_MID_64 : TILE_RAG_64;
+    int bm, bn;
+    tile_size(cfg, bm, bn);
+    p.tiles_m = static_cast<int>(cdiv(N, bm));
+    p.tiles_n = static_cast<int>(cdiv(K, bn));
+    const int64_t gx = int64_t(p.tiles_m) * p.tiles_n;
+    if (gx * groups > (int64_t(1) << 22)) return fail(SF_ERR_UNSUPPORTED, "sf_grouped_linear_dw: more than 2^22 tiles");
+    const unsigned g = static_cast<unsigned>(gx), gy = static_cast<unsigned>(groups);
+    switch (dtype) {
+      case SF_F16: rc = launch_grouped_sums_f16(cfg, p, g, gy, st); break;
+      case SF_BF16: rc = launch_grouped_sums_bf16(cfg, p, g, gy, st); break;
+      default: rc = launch_grouped_sums_f32(cfg, p, g, gy, st); break;
+    }
+    if (rc != SF_OK) return rc;
+  }
+  if (grad_bias == nullptr) return SF_OK;
+  return launch_group_colsum(grad, offsets, rows, groups, N, grad_bias, dtype, st);
+}
+
+int sf_act_backward(const void* grad, const void* pre, void* out, int64_t n, sf_dtype dtype, sf_epilogue act,
+                    void* stream) {
+  clear_error();
+  if (!known(dtype)) return fail(SF_ERR_INVALID_ARG, "sf_act_backward: unknown dtype %d", (int)dtype);
+  if (n < 0) return fail(SF_ERR_INVALID_ARG, "sf_act_backward: negative size");
+  if (act != SF_EPI_SILU && act != SF_EPI_GELU_TANH)
+    return fail(SF_ERR_INVALID_ARG, "sf_act_backward: act must be SF_EPI_SILU or SF_EPI_GELU_TANH, got %d", (int)act);
+  if (n == 0) return SF_OK;
+  if (grad == nullptr || pre == nullptr || out == nullptr)
+    return fail(SF_ERR_INVALID_ARG, "sf_act_backward: null pointer");
+  return launch_act_backward(epi_act(act), grad, pre, out, n, dtype, static_cast<hipStream_t>(stream));
+}
+
+}  // extern "C"

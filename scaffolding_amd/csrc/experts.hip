@@ -1,0 +1,561 @@
+// experts.hip — the row kernels around the grouped products: top-k routing
+// and its gradient, the exchange between token order and expert order, the
+// gradient of a fused activation and the bias gradient per group.
+#include "grouped.hpp"
+#include "rowio.hpp"
+#include "sf_internal.hpp"
+
+namespace sf {
+
+// ---------------------------------------------------------------------
+// Routing.  One wave per token: lane l holds logits l, l + 64, ...  The k
+// largest are found one after the other as the largest 64-bit key (logit in
+// an order-preserving integer form, then the complement of its index, so ties
+// go to the lowest index); a NaN counts above every number.
+//
+// Places.  The assignments (t, j) are ordered by expert, within an expert by
+// t k + j.  A block covers kRouteTokens consecutive tokens: it counts its
+// assignments per expert, and an assignment's place is
+//   first place of its expert  +  that expert's assignments in earlier blocks
+//   +  those in earlier waves of its block  +  those in earlier lanes,
+// all integer counts, so the places do not depend on which block or wave ran
+// first.  With several blocks the counts of each go to `counts` and a second
+// launch forms the sums; one block needs neither.
+// ---------------------------------------------------------------------
+constexpr int kRouteTokens = 64;   // tokens per block
+constexpr int kRouteThreads = 1024;
+constexpr int kRouteMaxK = 16;
+
+__device__ __forceinline__ uint32_t order_key(float f) {
+  if (f != f) return 0xffffffffu;
+  const uint32_t u = __float_as_uint(f + 0.0f);  // -0 and +0 are equal
+  return (u >> 31) ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float order_value(uint32_t k) {
+  if (k == 0xffffffffu) return __uint_as_float(0x7fc00000u);
+  return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k);
+}
+
+// Places of the block's `n` <= 1024 assignments ex[] (experts, in order):
+// base[e] is the first place of this block's assignments of expert e.
+__device__ __forceinline__ void route_place(const int* ex, int n, int E, int (*hist)[kMaxGroups], const int* base,
+                                            int* __restrict__ slots) {
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  constexpr int NW = kRouteThreads / 64;
+  for (int i = tid; i < NW * E; i += kRouteThreads) hist[i / E][i % E] = 0;
+  __syncthreads();
+  const int e = tid < n ? ex[tid] : -1;
+  // earlier lanes of this wave with the same expert: one round per distinct expert
+  int rank = 0;
+  uint64_t left = __ballot(e >= 0);
+  while (left != 0) {
+    const int src = __builtin_ctzll(left);
+    const int v = __builtin_amdgcn_readlane(e, src);
+    const uint64_t same = __ballot(e == v);
+    if (e == v) rank = __popcll(same & ((1ull << lane) - 1));
+    if (lane == src) hist[wave][v] = __popcll(same);
+    left &= ~same;
+  }
+  __syncthreads();
+  if (e >= 0) {
+    int at = base[e] + rank;
+    for (int w = 0; w < wave; ++w) at += hist[w][e];
+    slots[tid] = at;
+  }
+}
+
+// Exclusive sums over experts of tot[0 .. E) into first[0 .. E], by one wave.
+__device__ __forceinline__ void route_scan(const int* tot, int E, int* first) {
+  const int lane = threadIdx.x & 63;
+  int run = 0;
+  for (int e0 = 0; e0 < E; e0 += 64) {
+    const int v = e0 + lane < E ? tot[e0 + lane] : 0;
+    const int s = wave_scan_sum(v);
+    if (e0 + lane < E) first[e0 + lane] = run + s - v;
+    run += __builtin_amdgcn_readlane(s, 63);
+  }
+  if (lane == 0) first[E] = run;
+}
+
+template <typename T, int CH>
+__global__ __launch_bounds__(kRouteThreads) void route_kernel(const void* __restrict__ logits, int rows, int E, int k,
+                                                              int renorm, float* __restrict__ weights,
+                                                              int* __restrict__ experts, int* __restrict__ offsets,
+                                                              int* __restrict__ slots, int* __restrict__ counts) {
+  __shared__ int ex[kRouteTokens * kRouteMaxK];
+  __shared__ int cnt[kMaxGroups];
+  __shared__ int first[kMaxGroups + 1];
+  __shared__ int hist[kRouteThreads / 64][kMaxGroups];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int t0 = blockIdx.x * kRouteTokens;
+  const int nt = rows - t0 < kRouteTokens ? rows - t0 : kRouteTokens;
+  for (int e = tid; e < E; e += kRouteThreads) cnt[e] = 0;
+  __syncthreads();
+  for (int t = wave; t < nt; t += kRouteThreads / 64) {
+    const int64_t row = t0 + t;
+    uint64_t key[CH];
+    float v[CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int e = c * 64 + lane;
+      v[c] = e < E ? Chunk8<T>::get(logits, row * E + e) : -INFINITY;
+      // 0 is below every key of an expert (its low half is not 0)
+      key[c] = e < E ? (uint64_t)order_key(v[c]) << 32 | (0xffffffffu - (uint32_t)e) : 0;
+    }
+    float most = 0.f, w = 0.f, sum = 0.f;
+    int mine = 0;
+    for (int j = 0; j < k; ++j) {
+      uint64_t best = key[0];
+#pragma unroll
+      for (int c = 1; c < CH; ++c) best = key[c] > best ? key[c] : best;
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) {
+        const uint64_t o = __shfl_xor(best, off, 64);
+        best = o > best ? o : best;
+      }
+      const int e = (int)(0xffffffffu - (uint32_t)best);
+      const float val = order_value((uint32_t)(best >> 32));
+      if (j == 0) most = val;
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+        if (key[c] == best) key[c] = 0;
+      // softmax numerator; a token with no expert allowed (all -inf) has none
+      const float p = most == -INFINITY ? 0.f : expf(val - most);
+      sum += p;
+      if (lane == j) {
+        w = p;
+        mine = e;
+      }
+    }
+    if (!renorm) {  // over every expert instead of the chosen ones
+      float s = 0.f;
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+        if (c * 64 + lane < E) s += most == -INFINITY ? 0.f : expf(v[c] - most);
+      sum = wave_sum(s);
+    }
+    if (lane < k) {
+      weights[row * k + lane] = most == -INFINITY ? 0.f : w / sum;
+      experts[row * k + lane] = mine;
+      ex[t * k + lane] = mine;
+      atomicAdd(&cnt[mine], 1);
+    }
+  }
+  __syncthreads();
+  if (counts != nullptr) {
+    for (int e = tid; e < E; e += kRouteThreads) counts[(int64_t)blockIdx.x * E + e] = cnt[e];
+    return;
+  }
+  if (wave == 0) route_scan(cnt, E, first);
+  __syncthreads();
+  for (int e = tid; e <= E; e += kRouteThreads) offsets[e] = first[e];
+  route_place(ex, nt * k, E, hist, first, slots);
+}
+
+// Second launch of several blocks: block b forms the sums over the blocks and
+// places its own assignments; block 0 writes the offsets.
+__global__ __launch_bounds__(kRouteThreads) void route_place_kernel(const int* __restrict__ experts, int rows, int E,
+                                                                    int k, const int* __restrict__ counts,
+                                                                    int* __restrict__ offsets,
+                                                                    int* __restrict__ slots) {
+  __shared__ int ex[kRouteTokens * kRouteMaxK];
+  __shared__ int before[kMaxGroups];
+  __shared__ int total[kMaxGroups];
+  __shared__ int first[kMaxGroups + 1];
+  __shared__ int hist[kRouteThreads / 64][kMaxGroups];
+  const int tid = threadIdx.x, wave = tid >> 6;
+  const int t0 = blockIdx.x * kRouteTokens;
+  const int nt = rows - t0 < kRouteTokens ? rows - t0 : kRouteTokens;
+  const int64_t a0 = (int64_t)t0 * k;
+  const int n = nt * k;
+  if (tid < n) ex[tid] = experts[a0 + tid];
+  for (int e = tid; e < E; e += kRouteThreads) before[e] = total[e] = 0;
+  __syncthreads();
+  // every thread sums a share of the blocks for one expert
+  const int nb = gridDim.x;
+  const int lanes = E < kRouteThreads ? E : kRouteThreads;
+  const int shares = kRouteThreads / lanes;
+  const int share = tid / lanes;
+  if (share < shares) {
+    for (int e = tid % lanes; e < E; e += lanes) {
+      int sum = 0, pre = 0;
+      for (int b = share; b < nb; b += shares) {
+        const int c = counts[(int64_t)b * E + e];
+        sum += c;
+        pre += b < (int)blockIdx.x ? c : 0;
+      }
+      atomicAdd(&total[e], sum);
+      atomicAdd(&before[e], pre);
+    }
+  }
+  __syncthreads();
+  if (wave == 0) route_scan(total, E, first);
+  __syncthreads();
+  if (blockIdx.x == 0)
+    for (int e = tid; e <= E; e += kRouteThreads) offsets[e] = first[e];
+  __syncthreads();
+  for (int e = tid; e < E; e += kRouteThreads) first[e] += before[e];
+  route_place(ex, n, E, hist, first, slots + a0);
+}
+
+// Gradient of the logits, one wave per token.  Renormalised weights are a
+// softmax over the chosen logits: dl = w (g - <g, w>) there, 0 elsewhere;
+// otherwise over all: dl = p ([chosen] g - <g, p>).  p is formed again from
+// the logits.  A token without an allowed expert has zero gradient.
+template <typename T, int CH>
+__global__ __launch_bounds__(256) void route_backward_kernel(const float* __restrict__ gw,
+                                                             const void* __restrict__ logits,
+                                                             const float* __restrict__ weights,
+                                                             const int* __restrict__ experts, int rows, int E, int k,
+                                                             int renorm, void* __restrict__ dl) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  float g = 0.f, w = 0.f;
+  int e = -1;
+  if (lane < k) {
+    g = gw[row * k + lane];
+    w = weights[row * k + lane];
+    e = experts[row * k + lane];
+  }
+  const float dot = wave_sum(g * w);
+  float p[CH], out[CH];
+  if (renorm) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) out[c] = 0.f;
+  } else {
+    float most = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      p[c] = c * 64 + lane < E ? Chunk8<T>::get(logits, row * E + c * 64 + lane) : -INFINITY;
+      most = fmaxf(most, p[c]);
+    }
+    most = wave_max(most);
+    float s = 0.f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      p[c] = most == -INFINITY ? 0.f : expf(p[c] - most);
+      s += p[c];
+    }
+    s = wave_sum(s);
+    const float inv = most == -INFINITY ? 0.f : 1.0f / s;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      p[c] *= inv;
+      out[c] = -p[c] * dot;
+    }
+  }
+  for (int j = 0; j < k; ++j) {  // the chosen experts, one lane each
+    const int ej = __builtin_amdgcn_readlane(e, j);
+    const float gj = __shfl(g, j, 64), wj = __shfl(w, j, 64);
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+      if (c * 64 + lane == ej) out[c] = wj * (gj - dot);
+  }
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+    if (c * 64 + lane < E) Chunk8<T>::put(dl, row * E + c * 64 + lane, out[c]);
+}
+
+int64_t route_blocks(int64_t rows) { return (rows + kRouteTokens - 1) / kRouteTokens; }
+int route_max_k() { return kRouteMaxK; }
+
+template <typename T>
+static int launch_route_t(const void* logits, int64_t rows, int64_t E, int k, bool renorm, float* weights,
+                          int* experts, int* offsets, int* slots, int* work, hipStream_t st) {
+  const unsigned nb = static_cast<unsigned>(route_blocks(rows));
+  int* counts = nb > 1 ? work : nullptr;
+  const int r = static_cast<int>(rows), e = static_cast<int>(E);
+#define SF_ROUTE(CH)                                                                                              \
+  hipLaunchKernelGGL((route_kernel<T, CH>), dim3(nb), dim3(kRouteThreads), 0, st, logits, r, e, k, renorm ? 1 : 0, \
+                     weights, experts, offsets, slots, counts)
+  if (E <= 64) SF_ROUTE(1);
+  else if (E <= 128) SF_ROUTE(2);
+  else if (E <= 256) SF_ROUTE(4);
+  else SF_ROUTE(16);
+#undef SF_ROUTE
+  int rc = check_launch("routing");
+  if (rc != SF_OK || nb == 1) return rc;
+  hipLaunchKernelGGL(route_place_kernel, dim3(nb), dim3(kRouteThreads), 0, st, experts, r, e, k, work, offsets, slots);
+  return check_launch("routing places");
+}
+
+int launch_route(const void* logits, int64_t rows, int64_t E, int k, sf_dtype dt, bool renorm, float* weights,
+                 int* experts, int* offsets, int* slots, int* work, hipStream_t st) {
+  switch (dt) {
+    case SF_F16: return launch_route_t<F16>(logits, rows, E, k, renorm, weights, experts, offsets, slots, work, st);
+    case SF_BF16: return launch_route_t<BF16>(logits, rows, E, k, renorm, weights, experts, offsets, slots, work, st);
+    default: return launch_route_t<float>(logits, rows, E, k, renorm, weights, experts, offsets, slots, work, st);
+  }
+}
+
+template <typename T>
+static int launch_route_backward_t(const float* gw, const void* logits, const float* weights, const int* experts,
+                                   int64_t rows, int64_t E, int k, bool renorm, void* dl, hipStream_t st) {
+  const dim3 g(static_cast<unsigned>((rows + 3) / 4));
+  const int r = static_cast<int>(rows), e = static_cast<int>(E);
+#define SF_ROUTE(CH)                                                                                              \
+  hipLaunchKernelGGL((route_backward_kernel<T, CH>), g, dim3(256), 0, st, gw, logits, weights, experts, r, e, k,   \
+                     renorm ? 1 : 0, dl)
+  if (E <= 64) SF_ROUTE(1);
+  else if (E <= 128) SF_ROUTE(2);
+  else if (E <= 256) SF_ROUTE(4);
+  else SF_ROUTE(16);
+#undef SF_ROUTE
+  return check_launch("routing gradient");
+}
+
+int launch_route_backward(const float* gw, const void* logits, const float* weights, const int* experts, int64_t rows,
+                          int64_t E, int k, sf_dtype dt, bool renorm, void* dl, hipStream_t st) {
+  switch (dt) {
+    case SF_F16: return launch_route_backward_t<F16>(gw, logits, weights, experts, rows, E, k, renorm, dl, st);
+    case SF_BF16: return launch_route_backward_t<BF16>(gw, logits, weights, experts, rows, E, k, renorm, dl, st);
+    default: return launch_route_backward_t<float>(gw, logits, weights, experts, rows, E, k, renorm, dl, st);
+  }
+}
+
+// ---------------------------------------------------------------------
+// Rows between token order and expert order: bound by memory, one pass.  A
+// token's row is shared by 2^lg consecutive threads of a block of 256, eight
+// columns each at a time; rows may start at any element (16-byte accesses at
+// element alignment).  Slots outside [0, n) are skipped.
+// ---------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ void load_cols(const void* p, int64_t i, int left, float v[8]) {
+  if (left >= 8) {
+    load8u<T>(p, i, v);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = q < left ? Chunk8<T>::get(p, i + q) : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store_cols(void* p, int64_t i, int left, const float v[8]) {
+  if (left >= 8) {
+    store8u<T>(p, i, v);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 7; ++q)
+      if (q < left) Chunk8<T>::put(p, i + q, v[q]);
+  }
+}
+
+struct RowsParams {
+  const void* x;  // dispatch: tokens; combine: rows; its gradient: token gradients
+  const void* y;  // combine's gradient: rows
+  const int* slots;
+  const float* w;  // NULL: 1
+  void* out;
+  float* dw;
+  int64_t tokens, n;  // n = tokens * k rows
+  int k, D, lg;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void dispatch_kernel(RowsParams p) {
+  const int64_t t = (int64_t)blockIdx.x * (256 >> p.lg) + (threadIdx.x >> p.lg);
+  if (t >= p.tokens) return;
+  const int step = 8 << p.lg;
+  for (int c = (threadIdx.x & ((1 << p.lg) - 1)) * 8; c < p.D; c += step) {
+    float v[8];
+    load_cols<T>(p.x, t * p.D + c, p.D - c, v);
+    for (int j = 0; j < p.k; ++j) {
+      const int s = p.slots[t * p.k + j];
+      if ((uint64_t)(int64_t)s < (uint64_t)p.n) store_cols<T>(p.out, (int64_t)s * p.D + c, p.D - c, v);
+    }
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void combine_kernel(RowsParams p) {
+  const int64_t t = (int64_t)blockIdx.x * (256 >> p.lg) + (threadIdx.x >> p.lg);
+  if (t >= p.tokens) return;
+  const int step = 8 << p.lg;
+  for (int c = (threadIdx.x & ((1 << p.lg) - 1)) * 8; c < p.D; c += step) {
+    float a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < p.k; ++j) {
+      const int s = p.slots[t * p.k + j];
+      if ((uint64_t)(int64_t)s < (uint64_t)p.n) {
+        float v[8];
+        load_cols<T>(p.x, (int64_t)s * p.D + c, p.D - c, v);
+        const float w = p.w != nullptr ? p.w[t * p.k + j] : 1.0f;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) a[q] = __builtin_fmaf(w, v[q], a[q]);
+      }
+    }
+    store_cols<T>(p.out, t * p.D + c, p.D - c, a);
+  }
+}
+
+// drows[s] = w g[t], dw = <g[t], rows[s]>; the sums over a row are formed per
+// thread, then over the lanes, then over the waves, in that order always.
+template <typename T>
+__global__ __launch_bounds__(256) void combine_backward_kernel(RowsParams p) {
+  __shared__ float part[4];
+  const int64_t t = (int64_t)blockIdx.x * (256 >> p.lg) + (threadIdx.x >> p.lg);
+  const bool live = t < p.tokens;
+  const int in = threadIdx.x & ((1 << p.lg) - 1);
+  const int step = 8 << p.lg;
+  for (int j = 0; j < p.k; ++j) {
+    const int s = live ? p.slots[t * p.k + j] : -1;
+    float dot = 0.f;
+    if ((uint64_t)(int64_t)s < (uint64_t)p.n) {
+      const float w = p.w[t * p.k + j];
+      for (int c = in * 8; c < p.D; c += step) {
+        float g[8], v[8], o[8];
+        load_cols<T>(p.x, t * p.D + c, p.D - c, g);
+        load_cols<T>(p.y, (int64_t)s * p.D + c, p.D - c, v);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          dot = __builtin_fmaf(g[q], v[q], dot);
+          o[q] = w * g[q];
+        }
+        store_cols<T>(p.out, (int64_t)s * p.D + c, p.D - c, o);
+      }
+    }
+    for (int off = p.lg < 6 ? 1 << p.lg >> 1 : 32; off > 0; off >>= 1) dot += __shfl_xor(dot, off, 64);
+    if (p.lg > 6) {  // a row over several waves of the block
+      if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = dot;
+      __syncthreads();
+      dot = 0.f;
+      const int w0 = (threadIdx.x >> p.lg) << (p.lg - 6);
+      for (int i = 0; i < 1 << (p.lg - 6); ++i) dot += part[w0 + i];
+      __syncthreads();
+    }
+    if (live && in == 0) p.dw[t * p.k + j] = dot;
+  }
+}
+
+template <typename T>
+static int launch_rows_t(int op, RowsParams p, hipStream_t st) {
+  // threads per token: enough for its columns, at most the block
+  int lg = 0;
+  while (lg < 8 && (8 << lg) < p.D) ++lg;
+  p.lg = lg;
+  const int64_t per = 256 >> lg;
+  const int64_t nb = (p.tokens + per - 1) / per;
+  if (nb > INT32_MAX) return fail(SF_ERR_UNSUPPORTED, "row exchange: too many tokens");
+  const dim3 g(static_cast<unsigned>(nb));
+  if (op == 0) hipLaunchKernelGGL((dispatch_kernel<T>), g, dim3(256), 0, st, p);
+  else if (op == 1) hipLaunchKernelGGL((combine_kernel<T>), g, dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((combine_backward_kernel<T>), g, dim3(256), 0, st, p);
+  return check_launch("row exchange");
+}
+
+int launch_rows(int op, const void* x, const void* y, const int* slots, const float* w, void* out, float* dw,
+                int64_t tokens, int k, int64_t D, sf_dtype dt, hipStream_t st) {
+  RowsParams p;
+  p.x = x; p.y = y; p.slots = slots; p.w = w; p.out = out; p.dw = dw;
+  p.tokens = tokens; p.n = tokens * k; p.k = k; p.D = static_cast<int>(D); p.lg = 0;
+  switch (dt) {
+    case SF_F16: return launch_rows_t<F16>(op, p, st);
+    case SF_BF16: return launch_rows_t<BF16>(op, p, st);
+    default: return launch_rows_t<float>(op, p, st);
+  }
+}
+
+// ---------------------------------------------------------------------
+// out = g act'(pre), elementwise.
+//   silu'(x) = s (1 + x (1 - s)),  s = 1 / (1 + e^-x)
+//   gelu(x) = x s(z), s the logistic function of z = x (c0 + c1 x^2), so
+//   gelu'(x) = s + x s (1 - s) (c0 + 3 c1 x^2)
+// Past |x| = 20 both are 1 or 0 to the last bit; x is cut there so that
+// x s (1 - s) does not become inf * 0.
+// ---------------------------------------------------------------------
+template <int ACT>
+__device__ __forceinline__ float act_slope(float t) {
+  const float x = t > 20.f ? 20.f : (t < -20.f ? -20.f : t);  // NaN passes
+  if constexpr (ACT == ACT_SILU) {
+    const float s = fast_rcp(1.0f + fast_exp(-x));
+    return s * __builtin_fmaf(x, 1.0f - s, 1.0f);
+  } else {
+    const float c0 = (float)(2.0 * 0.7978845608028654), c1 = (float)(2.0 * 0.7978845608028654 * 0.044715);
+    const float xx = x * x;
+    const float s = fast_rcp(1.0f + fast_exp(-x * __builtin_fmaf(c1, xx, c0)));
+    return __builtin_fmaf(x * s * (1.0f - s), __builtin_fmaf(3.0f * c1, xx, c0), s);
+  }
+}
+
+template <typename T, int ACT>
+__global__ __launch_bounds__(256) void act_backward_kernel(const void* __restrict__ g, const void* __restrict__ pre,
+                                                           void* __restrict__ out, int64_t n) {
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; i < n; i += (int64_t)gridDim.x * 2048) {
+    const int left = n - i < 8 ? (int)(n - i) : 8;
+    float a[8], b[8];
+    load_cols<T>(g, i, left, a);
+    load_cols<T>(pre, i, left, b);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) a[q] *= act_slope<ACT>(b[q]);
+    store_cols<T>(out, i, left, a);
+  }
+}
+
+template <typename T>
+static int launch_act_backward_t(int act, const void* g, const void* pre, void* out, int64_t n, hipStream_t st) {
+  int64_t nb = (n + 2047) / 2048;
+  if (nb > (1 << 20)) nb = 1 << 20;
+  const dim3 grid(static_cast<unsigned>(nb));
+  if (act == ACT_SILU)
+    hipLaunchKernelGGL((act_backward_kernel<T, ACT_SILU>), grid, dim3(256), 0, st, g, pre, out, n);
+  else
+    hipLaunchKernelGGL((act_backward_kernel<T, ACT_GELU>), grid, dim3(256), 0, st, g, pre, out, n);
+  return check_launch("activation gradient");
+}
+
+int launch_act_backward(int act, const void* g, const void* pre, void* out, int64_t n, sf_dtype dt, hipStream_t st) {
+  switch (dt) {
+    case SF_F16: return launch_act_backward_t<F16>(act, g, pre, out, n, st);
+    case SF_BF16: return launch_act_backward_t<BF16>(act, g, pre, out, n, st);
+    default: return launch_act_backward_t<float>(act, g, pre, out, n, st);
+  }
+}
+
+// ---------------------------------------------------------------------
+// Column sums of each group's rows (the bias gradients): out[e, n] = sum over
+// the rows r of group e of g[r, n].  A block takes 512 columns of one group,
+// its 16 waves every 16th row each, fp32 partial sums joined through LDS in
+// wave order.
+// ---------------------------------------------------------------------
+template <typename T>
+__global__ __launch_bounds__(1024) void group_colsum_kernel(const void* __restrict__ g, const int* __restrict__ offsets,
+                                                            int rows, int64_t N, void* __restrict__ out) {
+  __shared__ float part[16][512];
+  int first, cnt;
+  group_bounds(offsets, (int)blockIdx.y, rows, first, cnt);
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t c = (int64_t)blockIdx.x * 512 + lane * 8;
+  const int left = N - c >= 8 ? 8 : (int)(N - c);
+  float a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (left > 0) {
+#pragma unroll 4
+    for (int r = wave; r < cnt; r += 16) {
+      float v[8];
+      load_cols<T>(g, (int64_t)(first + r) * N + c, left, v);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) a[q] += v[q];
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < 8; ++q) part[wave][lane * 8 + q] = a[q];
+  __syncthreads();
+  if (threadIdx.x < 512) {
+    const int64_t n = (int64_t)blockIdx.x * 512 + threadIdx.x;
+    float s = 0.f;
+    for (int w = 0; w < 16; ++w) s += part[w][threadIdx.x];
+    if (n < N) Chunk8<T>::put(out, (int64_t)blockIdx.y * N + n, s);
+  }
+}
+
+int launch_group_colsum(const void* g, const int* offsets, int64_t rows, int64_t groups, int64_t N, void* out,
+                        sf_dtype dt, hipStream_t st) {
+  const dim3 grid(static_cast<unsigned>((N + 511) / 512), static_cast<unsigned>(groups));
+  const int r = static_cast<int>(rows);
+  switch (dt) {
+    case SF_F16: hipLaunchKernelGGL((group_colsum_kernel<F16>), grid, dim3(1024), 0, st, g, offsets, r, N, out); break;
+    case SF_BF16: hipLaunchKernelGGL((group_colsum_kernel<BF16>), grid, dim3(1024), 0, st, g, offsets, r, N, out); break;
+    default: hipLaunchKernelGGL((group_colsum_kernel<float>), grid, dim3(1024), 0, st, g, offsets, r, N, out); break;
+  }
+  return check_launch("group column sums");
+}
+
+}  // namespace sf

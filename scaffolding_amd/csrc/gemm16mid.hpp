@@ -44,6 +44,7 @@
 #pragma once
 
 #include "gemm16nt_pp.hpp"
+#include "grouped.hpp"
 
 namespace sf {
 
@@ -53,9 +54,11 @@ struct __attribute__((packed, aligned(2))) Chunk16 {
   u32x4 v;
 };
 
+// Prm: GemmParams, or one of grouped.hpp's (rows in ragged groups, one B and bias
+// each: GroupedRows; one sum over each group's rows: GroupedSums).
 template <typename TIn, typename TOut, int BM, int BN, int WVM, int WVN, int NST, bool A_KM, bool B_KM, bool DMA,
-          int OCC>
-__global__ __launch_bounds__(WVM* WVN * 64, OCC) void gemm16mid_kernel(GemmParams p) {
+          int OCC, typename Prm = GemmParams>
+__global__ __launch_bounds__(WVM* WVN * 64, OCC) void gemm16mid_kernel(Prm p) {
   constexpr int NW = WVM * WVN;
   constexpr int BK = 64;
   constexpr int WM = BM / WVM, WN = BN / WVN;
@@ -72,7 +75,30 @@ __global__ __launch_bounds__(WVM* WVN * 64, OCC) void gemm16mid_kernel(GemmParam
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WVN, wn = wave % WVN;
-  const int M = p.M, N = p.N, K = p.K;
+  const int N = p.N;
+  constexpr bool ROWS = std::is_same<Prm, GroupedRows>::value, SUMS = std::is_same<Prm, GroupedSums>::value;
+  typename GroupVar<ROWS>::type M = p.M, epi = p.epi;
+  typename GroupVar<ROWS || SUMS>::type K = p.K;
+  int64_t b = blockIdx.y;
+  int64_t row0 = 0;  // first row of this tile (ROWS) or of the sum (SUMS)
+  int gtn = 0;
+  if constexpr (ROWS) {
+    GroupTile g;
+    if (!group_find<BM>(p, g)) return;  // workgroup-uniform
+    b = g.e;
+    row0 = g.row;
+    M = g.rows;
+    gtn = g.tn;
+    if (g.e == p.groups) {  // rows of no group: zeros
+      K = 0;
+      epi = SF_EPI_NONE;
+    }
+  }
+  if constexpr (SUMS) {
+    int first;
+    group_bounds(p.offsets, (int)b, p.rows, first, K);
+    row0 = first;
+  }
   const int KT = (K + BK - 1) / BK;
 
   // Workgroup -> (tile, k part).  XCD x (workgroup id mod 8) owns a
@@ -91,11 +117,15 @@ __global__ __launch_bounds__(WVM* WVN * 64, OCC) void gemm16mid_kernel(GemmParam
     tile = xcd_remap(blockIdx.x, gridDim.x);
   }
   int tm, tn;
-  group_tile(tile, p.tiles_m, p.tiles_n, 8, tm, tn);
+  if constexpr (ROWS) {  // the row pointers start at the tile
+    tm = 0;
+    tn = gtn;
+  } else {
+    group_tile(tile, p.tiles_m, p.tiles_n, 8, tm, tn);
+  }
   const int m0 = tm * BM, n0 = tn * BN;
-  const int64_t b = blockIdx.y;
-  const uint16_t* __restrict__ A = static_cast<const uint16_t*>(p.A) + b * p.sA;
-  const uint16_t* __restrict__ B = static_cast<const uint16_t*>(p.B) + b * p.sB;
+  const uint16_t* __restrict__ A = static_cast<const uint16_t*>(p.A) + (ROWS || SUMS ? row0 * p.lda : b * p.sA);
+  const uint16_t* __restrict__ B = static_cast<const uint16_t*>(p.B) + (SUMS ? row0 * p.ldb : b * p.sB);
 
   // ---- loads ----------------------------------------------------------------
   // Instruction i of wave w fills the 8 lines 8 (i NW + w) .. + 7 of its
@@ -323,23 +353,25 @@ __global__ __launch_bounds__(WVM* WVN * 64, OCC) void gemm16mid_kernel(GemmParam
   }
 
   // ---- epilogue: alpha, bias, activation, residual; staged through LDS --------
-  const bool has_bias = epi_has_bias(p.epi);
+  const bool has_bias = epi_has_bias(epi);
   const float alpha = p.alpha;
+  const void* bias = p.bias;
+  if constexpr (ROWS) bias = static_cast<const uint16_t*>(p.bias) + b * N;
   float bv[FN][4];
 #pragma unroll
   for (int i = 0; i < FN; ++i) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) bv[i][q] = 0.f;
-    if (has_bias) load_bias4<TIn>(p.bias, n0 + wn * WN + i * 16 + 4 * (lane >> 4), N, bv[i]);
+    if (has_bias) load_bias4<TIn>(bias, n0 + wn * WN + i * 16 + 4 * (lane >> 4), N, bv[i]);
   }
   uint8_t* stage = smem + wave * (16 * PITCH);
-  uint16_t* C = static_cast<uint16_t*>(p.C) + b * p.sC;
+  uint16_t* C = static_cast<uint16_t*>(p.C) + (ROWS ? row0 * p.ldc : b * p.sC);
   const void* R = p.res != nullptr ? static_cast<const uint16_t*>(p.res) + b * p.sR : nullptr;
   const bool rvec = R != nullptr && res_vec_ok<TOut>(R, p.ldr);
   constexpr int LROW = WN / 8;       // lanes per staged row (16 bytes each)
   constexpr int RPI = 64 / LROW;     // rows per store instruction
   constexpr int NSTO = RPI >= 16 ? 1 : 16 / RPI;
-  with_act(epi_act(p.epi), [&](auto act_c) {
+  with_act(epi_act(epi), [&](auto act_c) {
     constexpr int ACT = decltype(act_c)::value;
 #pragma unroll
     for (int j = 0; j < FM; ++j) {

@@ -27,6 +27,7 @@
 #pragma once
 
 #include "gemm16.hpp"
+#include "grouped.hpp"
 
 namespace sf {
 
@@ -76,8 +77,10 @@ __device__ __forceinline__ bool split32_handoff(f32x4* acc, const GemmParams& p,
   return true;
 }
 
-template <int BM, int BN, int WAVES_M, int WAVES_N, bool B_KMAJOR, bool VEC, bool A_KMAJOR = true>
-__global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void gemm32_kernel(GemmParams p) {
+// Prm: GemmParams, or grouped.hpp's GroupedRows / GroupedSums.
+template <int BM, int BN, int WAVES_M, int WAVES_N, bool B_KMAJOR, bool VEC, bool A_KMAJOR = true,
+          typename Prm = GemmParams>
+__global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void gemm32_kernel(Prm p) {
   constexpr int NT = WAVES_M * WAVES_N * 64;
   constexpr int BK = 32;
   constexpr int CH = BK / 4;  // float4 chunks per K-contiguous row
@@ -108,17 +111,38 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void gemm32_kernel(GemmParam
   // x / split; part q covers k-slices [KT q / split, KT (q + 1) / split).
   const int part = p.split > 0 ? (int)(blockIdx.x % (unsigned)p.split) : -1;
   const int tile_id = p.split > 0 ? (int)(blockIdx.x / (unsigned)p.split) : 0;
+  constexpr bool ROWS = std::is_same<Prm, GroupedRows>::value, SUMS = std::is_same<Prm, GroupedSums>::value;
+  const int N = p.N;
+  typename GroupVar<ROWS>::type M = p.M, epi = p.epi;
+  typename GroupVar<ROWS || SUMS>::type K = p.K;
+  int64_t b = blockIdx.y;
+  int64_t row0 = 0;  // first row of this tile (ROWS) or of the sum (SUMS)
   int tm, tn;
-  {
+  if constexpr (ROWS) {  // the row pointers start at the tile
+    GroupTile gt;
+    if (!group_find<BM>(p, gt)) return;  // workgroup-uniform
+    b = gt.e;
+    row0 = gt.row;
+    M = gt.rows;
+    tm = 0;
+    tn = gt.tn;
+    if (gt.e == p.groups) {  // rows of no group: zeros
+      K = 0;
+      epi = SF_EPI_NONE;
+    }
+  } else {
     int pid = p.split > 0 ? tile_id : xcd_remap(blockIdx.x, gridDim.x);
     group_tile(pid, p.tiles_m, p.tiles_n, 8, tm, tn);
   }
+  if constexpr (SUMS) {
+    int first;
+    group_bounds(p.offsets, (int)b, p.rows, first, K);
+    row0 = first;
+  }
   const int m0 = tm * BM;
   const int n0 = tn * BN;
-  const int64_t b = blockIdx.y;
-  const float* __restrict__ A = static_cast<const float*>(p.A) + b * p.sA;
-  const float* __restrict__ B = static_cast<const float*>(p.B) + b * p.sB;
-  const int M = p.M, N = p.N, K = p.K;
+  const float* __restrict__ A = static_cast<const float*>(p.A) + (ROWS || SUMS ? row0 * p.lda : b * p.sA);
+  const float* __restrict__ B = static_cast<const float*>(p.B) + (SUMS ? row0 * p.ldb : b * p.sB);
   const int64_t lda = p.lda, ldb = p.ldb;
 
   f32x4 acc[FN][FM];
@@ -250,12 +274,12 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void gemm32_kernel(GemmParam
   // plain stores, the counter bumped by split_arrive, plain loads).
   if (part >= 0 && !split32_handoff<FN * FM, NT>(&acc[0][0], p, tile_id, part, tid)) return;
 
-  float* C = static_cast<float*>(p.C) + b * p.sC;
-  const bool has_bias = epi_has_bias(p.epi);
-  const int act = epi_act(p.epi);
+  float* C = static_cast<float*>(p.C) + (ROWS ? row0 * p.ldc : b * p.sC);
+  const bool has_bias = epi_has_bias(epi);
+  const int act = epi_act(epi);
   const float alpha = p.alpha;
   const bool vec_ok = ((p.ldc & 3) == 0) && ((reinterpret_cast<uintptr_t>(C) & 15) == 0);
-  const float* bias = static_cast<const float*>(p.bias);
+  const float* bias = static_cast<const float*>(p.bias) + (ROWS ? b * N : 0);
   const void* R = p.res != nullptr ? static_cast<const float*>(p.res) + b * p.sR : nullptr;
   const bool rvec = R != nullptr && res_vec_ok<float>(R, p.ldr);
   with_act(act, [&](auto act_c) {

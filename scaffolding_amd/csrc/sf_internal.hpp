@@ -7,12 +7,15 @@
 #include <atomic>
 
 #include "gemm16.hpp"
+#include "grouped.hpp"
 #include "sf_common.hpp"
 
 namespace sf {
 
 // Records a formatted message as this thread's last error; returns `code`.
 int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+// Forgets this thread's last error (at the start of an entry point).
+void clear_error();
 // Maps a pending launch error (hipGetLastError) to SF_ERR_HIP with context.
 int check_launch(const char* what);
 // Maps a HIP status to SF_OK / SF_ERR_HIP with context.
@@ -187,5 +190,29 @@ int launch_zero(void* p, size_t nbytes, hipStream_t st);
 int sum_dim_parts(int64_t outer, int64_t D, int64_t inner, int cus);
 int launch_sum_dim(const void* x, void* y, int64_t outer, int64_t D, int64_t inner, sf_dtype in, sf_dtype out,
                    float* ws, int S, hipStream_t st);
+
+// CUs of the current device (256 where there is none).
+int cu_count_current();
+// Grouped products (grouped.hpp): rows in groups, and sums over a group's rows.
+int launch_grouped_rows_bf16(bool b_kmajor, int cfg, const GroupedRows& p, unsigned gx, hipStream_t st);
+int launch_grouped_rows_f16(bool b_kmajor, int cfg, const GroupedRows& p, unsigned gx, hipStream_t st);
+int launch_grouped_rows_f32(bool b_kmajor, int cfg, const GroupedRows& p, unsigned gx, hipStream_t st);
+int launch_grouped_sums_bf16(int cfg, const GroupedSums& p, unsigned gx, unsigned gy, hipStream_t st);
+int launch_grouped_sums_f16(int cfg, const GroupedSums& p, unsigned gx, unsigned gy, hipStream_t st);
+int launch_grouped_sums_f32(int cfg, const GroupedSums& p, unsigned gx, unsigned gy, hipStream_t st);
+// The row kernels around them (experts.hip).
+int64_t route_blocks(int64_t rows);
+int route_max_k();
+int launch_route(const void* logits, int64_t rows, int64_t E, int k, sf_dtype dt, bool renorm, float* weights,
+                 int* experts, int* offsets, int* slots, int* work, hipStream_t st);
+int launch_route_backward(const float* gw, const void* logits, const float* weights, const int* experts, int64_t rows,
+                          int64_t E, int k, sf_dtype dt, bool renorm, void* dl, hipStream_t st);
+// op 0: x to rows; 1: weighted sums of rows (x); 2: its gradient (x: token
+// gradients, y: rows).
+int launch_rows(int op, const void* x, const void* y, const int* slots, const float* w, void* out, float* dw,
+                int64_t tokens, int k, int64_t D, sf_dtype dt, hipStream_t st);
+int launch_act_backward(int act, const void* g, const void* pre, void* out, int64_t n, sf_dtype dt, hipStream_t st);
+int launch_group_colsum(const void* g, const int* offsets, int64_t rows, int64_t groups, int64_t N, void* out,
+                        sf_dtype dt, hipStream_t st);
 
 }  // namespace sf

@@ -15,15 +15,22 @@ from . import _cuda_ops as _cuops
 
 _F32 = np.dtype(np.float32)
 _F16 = np.dtype(np.float16)
+_I32 = np.dtype(np.int32)
+_U8 = np.dtype(np.uint8)
 
 
 class dtype(enum.Enum):
     float16 = "float16"
     float32 = "float32"
     bfloat16 = "bfloat16"
+    # storage only (indices, packed 4-bit weights): no operator computes in them
+    int32 = "int32"
+    uint8 = "uint8"
 
     def to_numpy(self) -> np.dtype:
         """Host dtype of this dtype's values (reference dtype.py:25-39)."""
+        if self is dtype.int32 or self is dtype.uint8:
+            return np.dtype(self.value)
         return np.dtype(np.float16) if self is dtype.float16 else np.dtype(np.float32)
 
     def device_storage(self) -> np.dtype:
@@ -42,6 +49,10 @@ class dtype(enum.Enum):
             return dtype.bfloat16
         if d is _F16:
             return dtype.float16
+        if d is _I32:
+            return dtype.int32
+        if d is _U8:
+            return dtype.uint8
         if isinstance(d, dtype):
             return d
         if isinstance(d, str):
@@ -53,11 +64,17 @@ class dtype(enum.Enum):
             return dtype.float16
         if nd in (np.float32, np.float64):
             return dtype.float32
+        if nd == _I32:
+            return dtype.int32
+        if nd == _U8:
+            return dtype.uint8
         raise TypeError("unsupported dtype %r" % (d,))
 
     @property
     def itemsize(self) -> int:
-        return 4 if self is dtype.float32 else 2
+        if self is dtype.uint8:
+            return 1
+        return 4 if self is dtype.float32 or self is dtype.int32 else 2
 
     def __repr__(self) -> str:
         return "scaffolding_amd." + self.value
@@ -66,3 +83,5 @@ class dtype(enum.Enum):
 float16 = dtype.float16
 float32 = dtype.float32
 bfloat16 = dtype.bfloat16
+int32 = dtype.int32
+uint8 = dtype.uint8

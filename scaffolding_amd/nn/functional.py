@@ -5,16 +5,20 @@
   softmax                         reference nn/functional.py:113-145
   dropout                         reference nn/functional.py:231-238
   scaled_dot_product_attention    reference nn/functional.py:298-369
+  route_topk, dispatch_rows,
+  combine_rows, grouped_linear    experts, with their gradients (no reference
+                                  counterparts)
 
 GPU only; results carry no grad_fn (as the reference's GPU branches).
 """
 from __future__ import annotations
 
 import math
+from typing import NamedTuple
 
 from .. import _cuda_ops as _cuops
 from ..tensor import Tensor, _gpu_only
-from .layers import _linear
+from .layers import _linear, _on
 
 
 def linear(input: Tensor, weight: Tensor, bias: Tensor | None = None,
@@ -88,3 +92,91 @@ def scaled_dot_product_attention(q: Tensor, k: Tensor, v: Tensor, attn_mask=None
     s = (1.0 / math.sqrt(d)) if scale is None else float(scale)
     out = _cuops.dev_scaled_dot_product_attention(q._gpu, k._gpu, v._gpu, s, mask, dropout_p, seed, offset)
     return Tensor._wrap_gpu(out, q._device)
+
+
+class Routing(NamedTuple):
+    """What route_topk gives: weights (fp32) and experts (int32), both (..., k),
+    in descending order of the logits; offsets (int32, (E + 1,)) and slots
+    (int32, (..., k)): with the choices ordered by expert, within one by token,
+    slots holds each one's place, and expert e's places are offsets[e] to
+    offsets[e + 1] - 1."""
+    weights: Tensor
+    experts: Tensor
+    offsets: Tensor
+    slots: Tensor
+    renormalize: bool = True
+
+
+def _device_of(op: str, first: Tensor, *others) -> int:
+    """The device that `first` lives on, made current; every operand on a GPU."""
+    for t in (first,) + others:
+        if t is not None and t._gpu is None:
+            _gpu_only(op)
+    dev = first._gpu.device_id
+    _cuops.set_device(dev)
+    return dev
+
+
+def route_topk(logits: Tensor, k: int, renormalize: bool = True) -> Routing:
+    """Sends each token to the k experts of its largest logits (..., E):
+    weights softmax(logits) of the chosen in fp32, divided by their sum with
+    `renormalize`.  Equal logits go to the lower index, NaN counts above every
+    number, and a token whose logits are all -inf gets weights 0.  E <= 1024,
+    k <= min(E, 16)."""
+    _device_of("route_topk", logits)
+    out = _cuops.dev_route_topk(logits._gpu, k, renormalize)
+    return Routing(*(Tensor._wrap_gpu(t, logits._device) for t in out), renormalize)
+
+
+def route_topk_backward(grad_weights: Tensor, logits: Tensor, routing: Routing) -> Tensor:
+    """Gradient of route_topk's logits, in their dtype, from the fp32 gradient
+    of its weights (the choice itself has none)."""
+    dev = _device_of("route_topk_backward", logits, grad_weights, routing.weights, routing.experts)
+    out = _cuops.dev_route_topk_backward(_on(grad_weights, dev), logits._gpu, _on(routing.weights, dev),
+                                         _on(routing.experts, dev), routing.renormalize)
+    return Tensor._wrap_gpu(out, logits._device)
+
+
+def dispatch_rows(input: Tensor, slots: Tensor) -> Tensor:
+    """Tokens (..., D) in expert order: (T k, D) rows, rows[slots[t, j]] =
+    input[t].  Its gradient is combine_rows without weights."""
+    dev = _device_of("dispatch_rows", input, slots)
+    return Tensor._wrap_gpu(_cuops.dev_dispatch_rows(input._gpu, _on(slots, dev)), input._device)
+
+
+def combine_rows(rows: Tensor, slots: Tensor, weights: Tensor | None = None) -> Tensor:
+    """Tokens from rows in expert order: sum over j of weights[t, j]
+    rows[slots[t, j]] (fp32, one rounding); weights fp32 (..., k), None: 1."""
+    dev = _device_of("combine_rows", rows, slots, weights)
+    return Tensor._wrap_gpu(_cuops.dev_combine_rows(rows._gpu, _on(slots, dev), _on(weights, dev)), rows._device)
+
+
+def combine_rows_backward(grad: Tensor, rows: Tensor, slots: Tensor, weights: Tensor) -> tuple[Tensor, Tensor]:
+    """(grad_rows, grad_weights) of combine_rows; grad_weights is fp32."""
+    dev = _device_of("combine_rows_backward", rows, grad, slots, weights)
+    out = _cuops.dev_combine_rows_backward(_on(grad, dev), rows._gpu, _on(slots, dev), _on(weights, dev))
+    return tuple(Tensor._wrap_gpu(t, rows._device) for t in out)
+
+
+def grouped_linear(input: Tensor, weight: Tensor, offsets: Tensor, bias: Tensor | None = None,
+                   activation: str | None = None) -> Tensor:
+    """A linear layer with one weight per group of rows, in one launch:
+    act(input[r] W[e]^T + b[e]) for the rows r of group e.  input (R, K),
+    weight (E, N, K), bias (E, N); group e is the rows offsets[e] to
+    offsets[e + 1] - 1 of the int32 tensor offsets (E + 1,), ascending from 0,
+    and may be empty; rows from offsets[E] on give 0.  The sizes are read on
+    the device: offsets may come straight from route_topk."""
+    dev = _device_of("grouped_linear", input, weight, offsets, bias)
+    out = _cuops.dev_grouped_linear(input._gpu, _on(weight, dev), _on(offsets, dev), _on(bias, dev), activation)
+    return Tensor._wrap_gpu(out, input._device)
+
+
+def grouped_linear_backward(grad: Tensor, input: Tensor, weight: Tensor, offsets: Tensor, has_bias: bool = True,
+                            activation: str | None = None, pre: Tensor | None = None
+                            ) -> tuple[Tensor, Tensor, Tensor | None]:
+    """(grad_input, grad_weight, grad_bias or None) of grouped_linear; with an
+    activation, `pre` is the layer's output without it."""
+    dev = _device_of("grouped_linear_backward", input, grad, weight, offsets, pre)
+    out = _cuops.dev_grouped_linear_backward(_on(grad, dev), input._gpu, _on(weight, dev), _on(offsets, dev),
+                                             has_bias, activation, _on(pre, dev))
+    return tuple(None if t is None else Tensor._wrap_gpu(t, input._device) for t in out)
