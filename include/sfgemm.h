@@ -464,6 +464,33 @@ int sf_act_backward(const void* grad, const void* pre, void* out, int64_t n, sf_
                     void* stream);
 
 /* ------------------------------------------------------------------ */
+/* 4-bit weights                                                       */
+/* ------------------------------------------------------------------ */
+/* No counterparts in the reference.  A weight [N, K] in 4 bits, per weight of
+ * `groups` (1 for an ordinary linear layer):
+ *   q       uint8 [N, K / 2]: byte j of a row holds column 2 j in its low and
+ *           2 j + 1 in its high four bits
+ *   scales  `dtype` [K / group, N]
+ *   zeros   uint8 [K / group, N], or NULL for 8 everywhere
+ *   w[n, k] = (q[n, k] - zeros[k / group, n]) * scales[k / group, n]
+ * group is 32, 64 or a multiple of 128 and divides K; dtype F16 or BF16; q
+ * and x 16-byte aligned. */
+
+/* y[m, :] = epi(w x[m, :] (+ bias)) for `rows` rows of x [rows, K]; the
+ * unpacked integers are exact, scales and sums fp32, one rounding.  With
+ * offsets (int32 [groups + 1], device) row m uses the weight of its group, as
+ * sf_grouped_linear says, and bias is [groups, N]; without, groups is 1.
+ * Meant for few rows per weight: each block of 64 reads the weight again. */
+int sf_linear_q4(const void* x, const void* q, const void* scales, const void* zeros, const int32_t* offsets,
+                 const void* bias, void* y, int64_t rows, int64_t groups, int64_t N, int64_t K, int64_t group,
+                 sf_dtype dtype, sf_epilogue epi, void* stream);
+
+/* The weights themselves, w [groups, N, K] of `dtype`, each rounded once: for
+ * sf_gemm or sf_grouped_linear over many rows. */
+int sf_q4_expand(const void* q, const void* scales, const void* zeros, void* w, int64_t groups, int64_t N, int64_t K,
+                 int64_t group, sf_dtype dtype, void* stream);
+
+/* ------------------------------------------------------------------ */
 /* Runtime: devices, memory, streams, events                           */
 /* (the CUDA runtime calls _cuda_ops.pyx:33-142 binds directly)        */
 /* ------------------------------------------------------------------ */

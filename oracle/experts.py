@@ -109,3 +109,15 @@ def act_slope(v, name):
         t = np.tanh(c * (v + 0.044715 * v ** 3))
         return 0.5 * (1.0 + t) + 0.5 * v * (1.0 - t * t) * c * (1.0 + 3 * 0.044715 * v * v)
     return np.ones_like(v)
+
+
+def q4_weight(q, scales, zeros=None):
+    """The weight (..., N, K) that packed q (..., N, K / 2), scales (..., K /
+    G, N) and zero points stand for."""
+    q = np.asarray(q)
+    w = np.zeros(q.shape[:-1] + (2 * q.shape[-1],))
+    w[..., 0::2], w[..., 1::2] = q % 16, q // 16
+    s = np.swapaxes(np.asarray(scales, np.float64), -1, -2)
+    z = np.full(s.shape, 8.0) if zeros is None else np.swapaxes(np.asarray(zeros, np.float64), -1, -2)
+    of = np.arange(w.shape[-1]) // (w.shape[-1] // s.shape[-1])
+    return (w - z[..., of]) * s[..., of]

@@ -138,6 +138,11 @@ cdef extern from "sfgemm.h" nogil:
                              int64_t rows, int64_t groups, int64_t N, int64_t K, sf_dtype dtype, void* stream)
     int sf_act_backward(const void* grad, const void* pre, void* out, int64_t n, sf_dtype dtype, sf_epilogue act,
                         void* stream)
+    int sf_linear_q4(const void* x, const void* q, const void* scales, const void* zeros, const int32_t* offsets,
+                     const void* bias, void* y, int64_t rows, int64_t groups, int64_t N, int64_t K, int64_t group,
+                     sf_dtype dtype, sf_epilogue epi, void* stream)
+    int sf_q4_expand(const void* q, const void* scales, const void* zeros, void* w, int64_t groups, int64_t N,
+                     int64_t K, int64_t group, sf_dtype dtype, void* stream)
     int sf_cast(const void* x, sf_dtype in_dtype, void* y, sf_dtype out_dtype, int64_t n, void* stream)
 
     int sf_get_device_count(int* count)
@@ -1430,6 +1435,122 @@ def dev_grouped_linear_backward(gt_grad, gt_x, gt_weight, gt_offsets, bint has_b
             ret = sf_grouped_linear_dw(pg, px, po, pdw, pdb, R, E, N, K, dt, NULL)
     _check_kernel(ret)
     return grad_x, grad_weight, grad_bias
+
+
+# ================================================================
+#  4-bit weights (no counterpart in the reference)
+# ================================================================
+
+# Rows per weight from which dev_linear_q4 expands the weight and runs the
+# 16-bit product.
+_Q4_EXPAND_ROWS = 512
+
+
+def dev_linear_q4(gt_x, gt_q, gt_scales, gt_zeros=None, gt_bias=None, activation=None, gt_offsets=None):
+    """y = act(x @ W^T + b) with W in 4 bits: W[n, k] = (q[n, k] - z[k // G, n])
+    s[k // G, n].  x (..., K) fp16 or bf16; q uint8 (N, K / 2), the even column
+    in the low four bits; scales (K / G, N) of x's dtype; zeros uint8 (K / G,
+    N) or None for 8; b (N,).  G = K / scales' rows is 32, 64 or a multiple of
+    128.  With offsets (int32 (E + 1,), see dev_grouped_linear) q, scales,
+    zeros and b have a leading E and x is (R, K).  Sums are fp32 over exact
+    integers; from 512 rows per weight on, W is first rounded to x's dtype
+    (half a step of each weight, as a 16-bit copy of W has) and the 16-bit
+    products run."""
+    name = 'dev_linear_q4'
+    xs, qs = tuple(gt_x.shape), tuple(gt_q.shape)
+    lead = 0 if gt_offsets is None else 1
+    _need_storage(gt_q, _U8, name, 'q')
+    _same_dtype(gt_x, gt_scales, name)
+    cdef sf_dtype dt = _sf_dtype(gt_x.dtype)
+    if dt == SF_F32:
+        raise TypeError("%s: x must be float16 or bfloat16" % name)
+    if len(qs) != 2 + lead or len(gt_scales.shape) != 2 + lead or len(xs) < 1 or (lead and len(xs) != 2):
+        raise ValueError("%s: x %s, q %s and scales %s do not match" % (name, xs, qs, gt_scales.shape))
+    cdef int64_t E = qs[0] if lead else 1
+    cdef int64_t N = qs[lead], K = qs[lead + 1] * 2
+    cdef int64_t KG = gt_scales.shape[lead]
+    if xs[-1] != K or tuple(gt_scales.shape) != qs[:lead] + (int(KG), int(N)) or KG < 1 or K % KG != 0:
+        raise ValueError("%s: x %s, q %s and scales %s do not match" % (name, xs, qs, gt_scales.shape))
+    cdef int64_t G = K // KG
+    if G != 32 and G != 64 and (G < 128 or G % 128 != 0):
+        raise ValueError("%s: the group %d is not 32, 64 or a multiple of 128" % (name, G))
+    if gt_zeros is not None:
+        _need_storage(gt_zeros, _U8, name, 'zeros')
+        if tuple(gt_zeros.shape) != tuple(gt_scales.shape):
+            raise ValueError("%s: zeros %s and scales %s do not match" % (name, gt_zeros.shape, gt_scales.shape))
+    if gt_bias is not None:
+        _same_dtype(gt_x, gt_bias, name)
+        if tuple(gt_bias.shape) != qs[:lead] + (int(N),):
+            raise ValueError("%s: bias %s does not match q %s" % (name, gt_bias.shape, qs))
+    if lead:
+        _need_storage(gt_offsets, _I32, name, 'offsets')
+        if tuple(gt_offsets.shape) != (E + 1,):
+            raise ValueError("%s: offsets must be (%d,), got %s" % (name, E + 1, gt_offsets.shape))
+    _same_device(name, gt_x, (gt_q, gt_scales, gt_zeros, gt_bias, gt_offsets))
+    if activation not in _ACTS:
+        raise ValueError("%s: unknown activation %r" % (name, activation))
+    cdef int act = _ACTS[activation]
+    cdef int64_t R = 1
+    for s in xs[:-1]:
+        R *= s
+    cdef void* px = _ptr(gt_x)
+    cdef void* pq = _ptr(gt_q)
+    cdef void* ps = _ptr(gt_scales)
+    cdef void* pz = _ptr(gt_zeros) if gt_zeros is not None else NULL
+    cdef void* pw
+    cdef int ret
+    if R >= _Q4_EXPAND_ROWS * E:
+        w = dev_q4_expand(gt_q, gt_scales, gt_zeros)
+        if lead:
+            return dev_grouped_linear(gt_x, w, gt_offsets, gt_bias, activation)
+        return dev_linear_forward(gt_x, w, gt_bias, activation)
+    cdef int epi
+    cdef void* pb = NULL
+    if gt_bias is not None:
+        pb = _ptr(gt_bias)
+        epi = (SF_EPI_BIAS, SF_EPI_BIAS_SILU, SF_EPI_BIAS_GELU_TANH)[act]
+    else:
+        epi = (SF_EPI_NONE, SF_EPI_SILU, SF_EPI_GELU_TANH)[act]
+    out = _alloc_like(xs[:-1] + (int(N),), gt_x.dtype, gt_x.device_id)
+    cdef int32_t* po = <int32_t*>_ptr(gt_offsets) if lead else NULL
+    cdef void* py = _ptr(out)
+    with nogil:
+        ret = sf_linear_q4(px, pq, ps, pz, po, pb, py, R, E, N, K, G, dt, <sf_epilogue>epi, NULL)
+    _check_kernel(ret)
+    return out
+
+
+def dev_q4_expand(gt_q, gt_scales, gt_zeros=None):
+    """The weight that dev_linear_q4's q, scales and zeros stand for, in the
+    scales' dtype (one rounding): (N, K), or (E, N, K) with a leading E."""
+    name = 'dev_q4_expand'
+    qs = tuple(gt_q.shape)
+    _need_storage(gt_q, _U8, name, 'q')
+    if len(qs) not in (2, 3) or len(gt_scales.shape) != len(qs):
+        raise ValueError("%s: q %s and scales %s do not match" % (name, qs, gt_scales.shape))
+    cdef int lead = len(qs) - 2
+    cdef int64_t E = qs[0] if lead else 1
+    cdef int64_t N = qs[lead], K = qs[lead + 1] * 2, KG = gt_scales.shape[lead]
+    if tuple(gt_scales.shape) != qs[:lead] + (int(KG), int(N)) or KG < 1 or K % KG != 0:
+        raise ValueError("%s: q %s and scales %s do not match" % (name, qs, gt_scales.shape))
+    if gt_zeros is not None:
+        _need_storage(gt_zeros, _U8, name, 'zeros')
+        if tuple(gt_zeros.shape) != tuple(gt_scales.shape):
+            raise ValueError("%s: zeros %s and scales %s do not match" % (name, gt_zeros.shape, gt_scales.shape))
+    _same_device(name, gt_q, (gt_scales, gt_zeros))
+    cdef sf_dtype dt = _sf_dtype(gt_scales.dtype)
+    if dt == SF_F32:
+        raise TypeError("%s: scales must be float16 or bfloat16" % name)
+    out = _alloc_like(qs[:lead] + (int(N), int(K)), gt_scales.dtype, gt_scales.device_id)
+    cdef void* pq = _ptr(gt_q)
+    cdef void* ps = _ptr(gt_scales)
+    cdef void* pz = _ptr(gt_zeros) if gt_zeros is not None else NULL
+    cdef void* pw = _ptr(out)
+    cdef int ret
+    with nogil:
+        ret = sf_q4_expand(pq, ps, pz, pw, E, N, K, K // KG, dt, NULL)
+    _check_kernel(ret)
+    return out
 
 
 # ================================================================

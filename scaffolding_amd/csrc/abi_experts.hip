@@ -1,4 +1,5 @@
-// abi_experts.hip — C entry points of the expert operators: argument checks
+// abi_experts.hip — C entry points of the expert operators and the 4-bit
+// linear layer: argument checks
 // (before any HIP call) and the choice of tiles.
 #include "sf_internal.hpp"
 
@@ -267,6 +268,49 @@ int sf_act_backward(const void* grad, const void* pre, void* out, int64_t n, sf_
   if (grad == nullptr || pre == nullptr || out == nullptr)
     return fail(SF_ERR_INVALID_ARG, "sf_act_backward: null pointer");
   return launch_act_backward(epi_act(act), grad, pre, out, n, dtype, static_cast<hipStream_t>(stream));
+}
+
+static int q4_check(const char* name, int64_t rows, int64_t groups, int64_t N, int64_t K, int64_t group,
+                    sf_dtype dtype) {
+  int rc = grouped_check(name, rows, groups, N, K, dtype);
+  if (rc != SF_OK) return rc;
+  if (dtype == SF_F32) return fail(SF_ERR_UNSUPPORTED, "%s: scales and activations are F16 or BF16", name);
+  if (group != 32 && group != 64 && (group < 128 || group % 128 != 0))
+    return fail(SF_ERR_UNSUPPORTED, "%s: group %lld is not 32, 64 or a multiple of 128", name, (long long)group);
+  if (K % group != 0)
+    return fail(SF_ERR_INVALID_ARG, "%s: K = %lld is no multiple of the group %lld", name, (long long)K, (long long)group);
+  return SF_OK;
+}
+
+int sf_linear_q4(const void* x, const void* q, const void* scales, const void* zeros, const int32_t* offsets,
+                 const void* bias, void* y, int64_t rows, int64_t groups, int64_t N, int64_t K, int64_t group,
+                 sf_dtype dtype, sf_epilogue epi, void* stream) {
+  clear_error();
+  const int rc = q4_check("sf_linear_q4", rows, groups, N, K, group, dtype);
+  if (rc != SF_OK) return rc;
+  if (offsets == nullptr && groups != 1)
+    return fail(SF_ERR_INVALID_ARG, "sf_linear_q4: %lld weights need offsets", (long long)groups);
+  if (epi < SF_EPI_NONE || epi > SF_EPI_GELU_TANH)
+    return fail(SF_ERR_INVALID_ARG, "sf_linear_q4: unknown epilogue %d", (int)epi);
+  if (epi_has_bias(epi) && bias == nullptr && groups > 0 && N > 0)
+    return fail(SF_ERR_INVALID_ARG, "sf_linear_q4: the epilogue needs a bias");
+  if (rows == 0 || N == 0) return SF_OK;
+  if (y == nullptr || (K > 0 && (x == nullptr || (groups > 0 && (q == nullptr || scales == nullptr)))))
+    return fail(SF_ERR_INVALID_ARG, "sf_linear_q4: null pointer");
+  if (!aligned16(x) || !aligned16(q)) return fail(SF_ERR_UNSUPPORTED, "sf_linear_q4: x and q must be 16-byte aligned");
+  return launch_q4(x, q, scales, zeros, bias, y, offsets, groups, rows, N, K, group, dtype, epi,
+                   static_cast<hipStream_t>(stream));
+}
+
+int sf_q4_expand(const void* q, const void* scales, const void* zeros, void* w, int64_t groups, int64_t N, int64_t K,
+                 int64_t group, sf_dtype dtype, void* stream) {
+  clear_error();
+  const int rc = q4_check("sf_q4_expand", 0, groups, N, K, group, dtype);
+  if (rc != SF_OK || groups == 0 || N == 0 || K == 0) return rc;
+  if (q == nullptr || scales == nullptr || w == nullptr)
+    return fail(SF_ERR_INVALID_ARG, "sf_q4_expand: null pointer");
+  if (!aligned16(q) || !aligned16(w)) return fail(SF_ERR_UNSUPPORTED, "sf_q4_expand: q and w must be 16-byte aligned");
+  return launch_q4_expand(q, scales, zeros, w, groups, N, K, group, dtype, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

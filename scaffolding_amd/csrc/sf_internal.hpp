@@ -215,4 +215,11 @@ int launch_act_backward(int act, const void* g, const void* pre, void* out, int6
 int launch_group_colsum(const void* g, const int* offsets, int64_t rows, int64_t groups, int64_t N, void* out,
                         sf_dtype dt, hipStream_t st);
 
+// 4-bit weights (q4.hip).  z NULL: zero points 8; offsets NULL: one weight.
+int launch_q4(const void* x, const void* q, const void* s, const void* z, const void* bias, void* y,
+              const int* offsets, int64_t groups, int64_t rows, int64_t N, int64_t K, int64_t G, sf_dtype dt,
+              sf_epilogue epi, hipStream_t st);
+int launch_q4_expand(const void* q, const void* s, const void* z, void* w, int64_t groups, int64_t N, int64_t K,
+                     int64_t G, sf_dtype dt, hipStream_t st);
+
 }  // namespace sf

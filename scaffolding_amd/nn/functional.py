@@ -8,6 +8,7 @@
   route_topk, dispatch_rows,
   combine_rows, grouped_linear    experts, with their gradients (no reference
                                   counterparts)
+  quantize_q4, linear_q4          4-bit weights (no reference counterpart)
 
 GPU only; results carry no grad_fn (as the reference's GPU branches).
 """
@@ -15,6 +16,8 @@ from __future__ import annotations
 
 import math
 from typing import NamedTuple
+
+import numpy as np
 
 from .. import _cuda_ops as _cuops
 from ..tensor import Tensor, _gpu_only
@@ -180,3 +183,45 @@ def grouped_linear_backward(grad: Tensor, input: Tensor, weight: Tensor, offsets
     out = _cuops.dev_grouped_linear_backward(_on(grad, dev), input._gpu, _on(weight, dev), _on(offsets, dev),
                                              has_bias, activation, _on(pre, dev))
     return tuple(None if t is None else Tensor._wrap_gpu(t, input._device) for t in out)
+
+
+def quantize_q4(weight, group: int = 128, zeros: bool = False):
+    """A weight (..., N, K) (array or Tensor) in 4 bits, as NumPy arrays: (q
+    uint8 (..., N, K / 2), scales float32 (..., K / group, N), zero points
+    uint8 of the scales' shape or None), for linear_q4.  Symmetric by default
+    (values -7 .. 7 times max|w| / 7 of the group, so the largest is kept);
+    with `zeros` the group's range, widened to hold 0, is cut into 15 steps.
+    Runs on the host, once, when a model is loaded."""
+    w = weight.numpy() if isinstance(weight, Tensor) else np.asarray(weight)
+    w = w.astype(np.float32)
+    if w.ndim < 2 or group < 1 or w.shape[-1] % group != 0:
+        raise ValueError("quantize_q4: weight %s does not divide into groups of %d" % (w.shape, group))
+    if not np.isfinite(w).all():
+        raise ValueError("quantize_q4: the weight has values that are not finite")
+    g = w.reshape(w.shape[:-1] + (w.shape[-1] // group, group))
+    if zeros:
+        low, high = np.minimum(g.min(-1), 0.0), np.maximum(g.max(-1), 0.0)
+        scale = (high - low) / 15.0
+        zero = np.rint(-low / np.where(scale == 0.0, 1.0, scale))
+    else:
+        scale = np.abs(g).max(-1) / 7.0
+        zero = np.full(scale.shape, 8.0, np.float32)
+    q = np.rint(g / np.where(scale == 0.0, 1.0, scale)[..., None]) + zero[..., None]
+    q = np.clip(q, 0, 15).astype(np.uint8).reshape(w.shape)
+    packed = q[..., 0::2] | (q[..., 1::2] << 4)
+    return (packed, np.ascontiguousarray(np.swapaxes(scale, -1, -2).astype(np.float32)),
+            np.ascontiguousarray(np.swapaxes(zero, -1, -2).astype(np.uint8)) if zeros else None)
+
+
+def linear_q4(input: Tensor, qweight: Tensor, scales: Tensor, zeros: Tensor | None = None,
+              bias: Tensor | None = None, activation: str | None = None, offsets: Tensor | None = None) -> Tensor:
+    """A linear layer with a 4-bit weight W[n, k] = (q[n, k] - z[k // G, n])
+    s[k // G, n]: input (..., K) fp16 or bf16, qweight uint8 (N, K / 2) with
+    the even column in the low four bits, scales (K / G, N) of the input's
+    dtype, zeros uint8 (K / G, N) or None for 8, G = 32, 64 or a multiple of
+    128 (quantize_q4 makes them).  With offsets (see grouped_linear), one
+    weight, scales, zeros and bias per group of rows, a leading E each."""
+    dev = _device_of("linear_q4", input, qweight, scales, zeros, bias, offsets)
+    out = _cuops.dev_linear_q4(input._gpu, _on(qweight, dev), _on(scales, dev), _on(zeros, dev), _on(bias, dev),
+                               activation, _on(offsets, dev))
+    return Tensor._wrap_gpu(out, input._device)

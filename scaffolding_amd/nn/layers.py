@@ -129,7 +129,9 @@ class Module:
                     dst = _cuops.dev_cast(src, storage)
             else:
                 host = val.numpy() if isinstance(val, Tensor) else np.asarray(val)
-                dst = _cuops.gputensor_from_numpy(np.ascontiguousarray(host, dtype=np.float32), dev, storage)
+                if storage.kind not in "iu":  # indices and packed weights go as they are
+                    host = np.ascontiguousarray(host, dtype=np.float32)
+                dst = _cuops.gputensor_from_numpy(host, dev, storage)
             target._gpu = dst
             target._data = None
 
@@ -167,6 +169,60 @@ class Linear(Module):
     def __repr__(self) -> str:
         return "Linear(in_features=%d, out_features=%d, bias=%s)" % (
             self.in_features, self.out_features, self.bias is not None)
+
+
+class LinearQ4(Module):
+    """A Linear whose weight is held in 4 bits with a scale (and with `zeros` a
+    zero point) per `group` input features, for decoding: the weight's bytes
+    are what a step with few rows is bound by.  `weight` is packed (out, in /
+    2); scales are rounded to `dtype` (float16 or bfloat16).  Made from a
+    weight with from_linear; inference only."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, group: int = 128, zeros: bool = False,
+                 device=None, dtype="bfloat16", activation: str | None = None):
+        super().__init__()
+        if in_features % group != 0:
+            raise ValueError("LinearQ4: in_features %d is no multiple of the group %d" % (in_features, group))
+        self.in_features = in_features
+        self.out_features = out_features
+        self.group = group
+        self.activation = activation
+        dev = device or "cuda"
+        shape = (in_features // group, out_features)
+        self.weight = Parameter(np.full((out_features, in_features // 2), 0x88, np.uint8), False, "uint8", dev)
+        self.scales = Parameter(np.zeros(shape, np.float32), False, dtype, dev)
+        self.zeros = Parameter(np.full(shape, 8, np.uint8), False, "uint8", dev) if zeros else None
+        self.bias = Parameter(np.zeros(out_features, np.float32), False, dtype, dev) if bias else None
+
+    @classmethod
+    def from_linear(cls, linear: Linear, group: int = 128, zeros: bool = False, dtype=None) -> "LinearQ4":
+        from .functional import quantize_q4
+        dt = dtype if dtype is not None else linear.weight.dtype
+        out = cls(linear.in_features, linear.out_features, linear.bias is not None, group, zeros,
+                  linear.weight.device, dt, linear.activation)
+        q, scales, zero = quantize_q4(linear.weight, group, zeros)
+        state = {"weight": q, "scales": scales}
+        if zeros:
+            state["zeros"] = zero
+        if linear.bias is not None:
+            state["bias"] = linear.bias
+        out.load_state_dict(state)
+        return out
+
+    def to(self, device=None, dtype=None) -> "LinearQ4":
+        """Moves everything; `dtype` is that of the scales and the bias."""
+        for name, p in list(self._params.items()):
+            kept = p.dtype.value == "uint8"
+            setattr(self, name, Parameter(p.to(device, None if kept else dtype), requires_grad=False))
+        return self
+
+    def forward(self, x: Tensor) -> Tensor:
+        from .functional import linear_q4
+        return linear_q4(x, self.weight, self.scales, self.zeros, self.bias, self.activation)
+
+    def __repr__(self) -> str:
+        return "LinearQ4(in_features=%d, out_features=%d, bias=%s, group=%d)" % (
+            self.in_features, self.out_features, self.bias is not None, self.group)
 
 
 def _on(t: Tensor | None, dev: int):
@@ -303,5 +359,80 @@ class GELU(Module):
         return gelu(x)
 
 
-__all__ = ["Module", "Parameter", "Sequential", "Linear", "LayerNorm", "RMSNorm", "Dropout", "SiLU", "GELU",
+class MoE(Module):
+    """A feed-forward layer of experts: each token goes to the k of `experts`
+    two-layer networks (dim -> hidden -> dim, `activation` between) that the
+    router prefers, and their answers are summed with the router's weights.
+    router.weight (E, dim); up.weight (E, hidden, dim), up.bias (E, hidden);
+    down.weight (E, dim, hidden), down.bias (E, dim).  x (..., dim) ->
+    (..., dim); seven launches, none of which waits for the group sizes.
+    quantize() replaces the experts' weights by 4-bit ones for decoding.
+    Inference, as Linear (F.*_backward give the gradients)."""
+
+    def __init__(self, dim: int, hidden: int, experts: int, k: int = 2, bias: bool = True, activation: str = "silu",
+                 renormalize: bool = True, device=None, dtype=None):
+        super().__init__()
+        if not 1 <= k <= experts:
+            raise ValueError("MoE: k must be in [1, %d], got %d" % (experts, k))
+        self.dim, self.hidden, self.experts, self.k = dim, hidden, experts, k
+        self.activation = activation
+        self.renormalize = renormalize
+        self.router = Linear(dim, experts, bias=False, device=device, dtype=dtype)
+        self.up = _ExpertLinear(experts, dim, hidden, bias, device, dtype)
+        self.down = _ExpertLinear(experts, hidden, dim, bias, device, dtype)
+
+    def quantize(self, group: int = 128, zeros: bool = False) -> "MoE":
+        self.up.quantize(group, zeros)
+        self.down.quantize(group, zeros)
+        return self
+
+    def forward(self, x: Tensor) -> Tensor:
+        from . import functional as F
+        r = F.route_topk(self.router(x), self.k, self.renormalize)
+        h = self.up(F.dispatch_rows(x, r.slots), r.offsets, self.activation)
+        return F.combine_rows(self.down(h, r.offsets), r.slots, r.weights)
+
+
+class _ExpertLinear(Module):
+    """One linear layer per expert (F.grouped_linear), initialised as Linear
+    is; after quantize, F.linear_q4 over the same groups."""
+
+    def __init__(self, experts: int, in_features: int, out_features: int, bias: bool, device, dtype):
+        super().__init__()
+        s = 1.0 / math.sqrt(in_features)
+        dev = device or "cuda"
+        w = np.random.uniform(-s, s, (experts, out_features, in_features)).astype(np.float32)
+        self.weight = Parameter(w, dtype=dtype, device=dev)
+        self.scales = self.zeros = self.bias = None
+        if bias:
+            self.bias = Parameter(np.random.uniform(-s, s, (experts, out_features)).astype(np.float32), dtype=dtype,
+                                  device=dev)
+
+    def quantize(self, group: int, zeros: bool) -> None:
+        from .functional import quantize_q4
+        if self.scales is not None:
+            raise RuntimeError("the weight is quantized already")
+        if self.weight.dtype.value == "float32":
+            raise TypeError("4-bit weights need a float16 or bfloat16 layer")
+        dev, dt = self.weight.device, self.weight.dtype
+        q, scales, zero = quantize_q4(self.weight, group, zeros)
+        self.weight = Parameter(q, False, "uint8", dev)
+        self.scales = Parameter(scales, False, dt, dev)
+        if zeros:
+            self.zeros = Parameter(zero, False, "uint8", dev)
+
+    def to(self, device=None, dtype=None) -> "_ExpertLinear":
+        for name, p in list(self._params.items()):
+            kept = p.dtype.value == "uint8"
+            setattr(self, name, Parameter(p.to(device, None if kept else dtype), requires_grad=p.requires_grad))
+        return self
+
+    def forward(self, x: Tensor, offsets: Tensor, activation: str | None = None) -> Tensor:
+        from . import functional as F
+        if self.scales is None:
+            return F.grouped_linear(x, self.weight, offsets, self.bias, activation)
+        return F.linear_q4(x, self.weight, self.scales, self.zeros, self.bias, activation, offsets)
+
+
+__all__ = ["Module", "Parameter", "Sequential", "Linear", "LinearQ4", "MoE", "LayerNorm", "RMSNorm", "Dropout", "SiLU", "GELU",
            "_device_t", "_dtype_t"]
