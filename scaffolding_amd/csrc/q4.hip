@@ -30,6 +30,7 @@
 // A workgroup of NW waves takes 16 NB weight rows and up to 16 MB rows of x;
 // the waves take the blocks of 128 k in turn, and their sums are joined
 // through LDS in wave order.
+#include "gemm16nt_pp.hpp"
 #include "grouped.hpp"
 #include "rowio.hpp"
 #include "sf_internal.hpp"
@@ -47,7 +48,10 @@ struct Q4Params {
   int groups, rows, N, K, G;
   int tiles_n;
   int epi;
+  int sg;  // scale rows of a tile that are in LDS at a time (a multiple of 4, or all)
 };
+
+constexpr int kQ4ScaleBytes = 32768;  // most LDS for the scales of a tile
 
 template <typename T> struct Q4Bits;
 template <> struct Q4Bits<BF16> {
@@ -60,15 +64,17 @@ template <> struct Q4Bits<F16> {
 };
 
 // The eight weights of a dword as 16 + q, in the order 0 4 1 5 2 6 3 7.
+// `mask` and `exp` are Q4Bits' constants in registers, which one v_and_or_b32
+// takes (as literals they would need two instructions).
 template <typename T>
-__device__ __forceinline__ u32x4 q4_unpack(uint32_t w) {
+__device__ __forceinline__ u32x4 q4_unpack(uint32_t w, uint32_t mask, uint32_t exp) {
   typedef Q4Bits<T> B;
   u32x4 r;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int sh = B::kShift - 4 * i;
     const uint32_t t = sh >= 0 ? w << (sh & 31) : w >> (-sh & 31);
-    r[i] = (t & B::kMask) | B::kExp;
+    r[i] = (t & mask) | exp;
   }
   return r;
 }
@@ -92,11 +98,16 @@ __device__ __forceinline__ u32x4 lane_groups_transpose(u32x4 v) {
   return u32x4{c[0], c[1], d[0], d[1]};
 }
 
-// GB: scale groups per block of 128 k (1: G % 128 == 0; 2; 4).
-template <typename T, int NB, int MB, int NW, int GB, bool ZEROS, bool GROUPED>
+// GB: scale groups per block of 128 k (1: G % 128 == 0; 2; 4).  U: blocks whose
+// loads a wave issues together.
+template <typename T, int NB, int MB, int NW, int U, int GB, bool ZEROS, bool GROUPED>
 __global__ __launch_bounds__(NW * 64) void q4_kernel(Q4Params p) {
-  constexpr int BM = 16 * MB;
-  __shared__ f32x4 part[NW > 1 ? NW : 1][NB * MB][64];
+  constexpr int BM = 16 * MB, BN = 16 * NB;
+  constexpr int XP = 272;                        // bytes of a staged x row of 128 k: 16 rows on 16 bank groups
+  constexpr int XB = MB == 1 ? NW * 16 * XP : 0;  // staged x, one area per wave
+  constexpr int PB = NW * NB * 1024;             // the waves' partial sums of one row block
+  __shared__ __attribute__((aligned(16))) uint8_t area[XB > PB ? XB : PB];
+  extern __shared__ __attribute__((aligned(16))) uint8_t dyn[];  // scales, then zero points
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r16 = lane & 15, h = lane >> 4;
@@ -119,7 +130,7 @@ __global__ __launch_bounds__(NW * 64) void q4_kernel(Q4Params p) {
     rows = p.rows - row0 < BM ? p.rows - row0 : BM;
   }
   if (none) epi = SF_EPI_NONE;
-  const int n0 = tn * 16 * NB;
+  const int n0 = tn * BN;
   const int KG = K / p.G;  // scale rows
   const uint8_t* __restrict__ Q = p.q + e * (int64_t)N * (K / 2);
   const uint16_t* __restrict__ S = p.s + e * (int64_t)N * KG;
@@ -134,140 +145,278 @@ __global__ __launch_bounds__(NW * 64) void q4_kernel(Q4Params p) {
 
   const int nblk = none ? 0 : (K + 127) / 128;
   const int gstep = GB == 1 ? p.G / 128 : 1;  // blocks per scale group
+  uint32_t mask = Q4Bits<T>::kMask, exp = Q4Bits<T>::kExp;
+  asm("" : "+s"(mask));
+  asm("" : "+v"(exp));
   const u32x4 ones = {Q4Bits<T>::kOnes, Q4Bits<T>::kOnes, Q4Bits<T>::kOnes, Q4Bits<T>::kOnes};
-  // this lane's weight rows and x rows; rows past the edge read the last one
-  // (weights: their outputs are not stored) or zeros (x)
-  int64_t qrow[NB];
+
+  // The tile's scales and zero points go through LDS as [scale row][column], as
+  // many scale rows at a time as the launch gives room for (all of them but for
+  // very long K): read per block they would take as many load instructions as
+  // the weight, with 32 useful bytes each (28672 x 8192, 4 rows: 34 us against
+  // 29).
+  uint16_t* const sS = reinterpret_cast<uint16_t*>(dyn);
+  uint8_t* const sZ = dyn + p.sg * BN * 2;
+  const bool vec = (N & 3) == 0 && (reinterpret_cast<uintptr_t>(p.s) & 7) == 0 &&
+                   (!ZEROS || (reinterpret_cast<uintptr_t>(p.z) & 3) == 0);
+  auto stage_scales = [&](int kg0) {
+    const int cnt = KG - kg0 < p.sg ? KG - kg0 : p.sg;
+    for (int c = threadIdx.x; c < cnt * (BN / 4); c += NW * 64) {
+      const int kg = c / (BN / 4), n = c % (BN / 4) * 4;  // four columns, past N the last
+      const int64_t at = (int64_t)(kg0 + kg) * N;
+      u32x2 sc;
+      uint32_t zp = 0;
+      if (vec) {
+        const int g = n0 + n < N ? n0 + n : N - 4;
+        sc = *reinterpret_cast<const u32x2*>(S + at + g);
+        if constexpr (ZEROS) zp = *reinterpret_cast<const uint32_t*>(Z + at + g);
+      } else {
+        uint32_t v[4], z[4];
 #pragma unroll
-  for (int i = 0; i < NB; ++i) {
-    const int n = n0 + 16 * i + r16;
-    qrow[i] = (int64_t)(n < N ? n : N - 1) * (K / 2);
-  }
-  for (int blk = wave; blk < nblk; blk += NW) {
-    const int k0 = blk * 128;
-    u32x4 w[NB];
-#pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      const int k = k0 + 32 * h;
-      w[i] = k < K ? *reinterpret_cast<const u32x4*>(Q + qrow[i] + k / 2) : u32x4{0u, 0u, 0u, 0u};
-      if constexpr (GB > 1) w[i] = lane_groups_transpose(w[i]);
-    }
-    // the k of lane group h in dword d
-    auto k_of = [&](int d) { return GB == 1 ? k0 + 32 * h + 8 * d : k0 + 32 * d + 8 * h; };
-    u32x4 xs[MB][4];
-#pragma unroll
-    for (int j = 0; j < MB; ++j) {
-      const int m = 16 * j + r16;
-#pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        const int k = k_of(d);
-        u32x4 v = {0u, 0u, 0u, 0u};
-        if (m < rows && k < K) v = *reinterpret_cast<const u32x4*>(X + (int64_t)m * K + k);
-        xs[j][d] = q4_order(v);
-      }
-    }
-#pragma unroll
-    for (int gi = 0; gi < GB; ++gi) {
-      constexpr int DG = 4 / GB;  // dwords per scale group
-      const int kg = GB == 1 ? blk / gstep : blk * GB + gi;
-      if (GB > 1 && kg >= KG) break;
-      f32x4 xsum[MB];
-#pragma unroll
-      for (int j = 0; j < MB; ++j) {
-        xsum[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int d = gi * DG; d < gi * DG + DG; ++d) xsum[j] = Mfma16<T>::run(ones, xs[j][d], xsum[j]);
-      }
-#pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        f32x4 acc[MB];
-#pragma unroll
-        for (int j = 0; j < MB; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int d = gi * DG; d < gi * DG + DG; ++d) {
-          const u32x4 wf = q4_unpack<T>(w[i][d]);
-#pragma unroll
-          for (int j = 0; j < MB; ++j) acc[j] = Mfma16<T>::run(wf, xs[j][d], acc[j]);
+        for (int q = 0; q < 4; ++q) {
+          const int g = n0 + n + q < N ? n0 + n + q : N - 1;
+          v[q] = S[at + g];
+          z[q] = ZEROS ? Z[at + g] : 0;
         }
-        // this lane's outputs are n0 + 16 i + 4 h + 0..3 of x row r16
+        sc = u32x2{v[0] | v[1] << 16, v[2] | v[3] << 16};
+        if constexpr (ZEROS) zp = z[0] | z[1] << 8 | z[2] << 16 | z[3] << 24;
+      }
+      *reinterpret_cast<u32x2*>(sS + kg * BN + n) = sc;
+      if constexpr (ZEROS) *reinterpret_cast<uint32_t*>(sZ + kg * BN + n) = zp;
+    }
+  };
+
+  // Loads go through buffer resources whose ranges are this tile's weight rows
+  // and x rows: lanes past either read zeros without a branch (a weight row
+  // past N only reaches outputs that are not stored).  The range check leaves
+  // out the scalar offset, which moves along k within a row.
+  const int tile_rows = N - n0 < BN ? N - n0 : BN;
+  const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc(
+      (void*)(Q + (int64_t)n0 * (K / 2)), (short)0, none ? 0 : tile_rows * (K / 2), 0x00020000);
+  const __amdgpu_buffer_rsrc_t rx =
+      __builtin_amdgcn_make_buffer_rsrc((void*)X, (short)0, none ? 0 : rows * K * 2, 0x00020000);
+  constexpr uint32_t OOB = 0x80000000u;  // past every range
+  uint32_t vq[NB], vx[MB];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int n = n0 + 16 * i + 4 * h + c;
-          const int64_t at = (int64_t)kg * N + (n < N ? n : N - 1);
-          const float sc = Elem<T>::to_f32(S[at]);
-          const float off = ZEROS ? 16.0f + (float)Z[at] : 24.0f;
+  for (int i = 0; i < NB; ++i) vq[i] = (uint32_t)(16 * i + r16) * (uint32_t)(K / 2) + 16u * h;
+  // x of a single row block is loaded 16 bytes a lane, four rows of 128 k at a
+  // time, and put into MFMA order through the wave's LDS area: up to four rows
+  // take one load instruction a block (QX = 1) instead of four.  More row
+  // blocks are loaded in MFMA order straight away.
 #pragma unroll
-          for (int j = 0; j < MB; ++j) sum[i][j][c] += sc * __builtin_fmaf(-off, xsum[j][c], acc[j][c]);
+  for (int j = 0; j < MB; ++j)
+    vx[j] = MB == 1 ? (uint32_t)h * (uint32_t)K * 2u + 16u * r16
+                    : (uint32_t)(16 * j + r16) * (uint32_t)K * 2u + (GB == 1 ? 64u : 16u) * h;
+  uint8_t* const xw = area + (MB == 1 ? wave * 16 * XP : 0);
+
+  auto run = [&](auto qx_c) {
+    constexpr int QX = decltype(qx_c)::value;
+    u32x4 w[U][NB], xs[U][MB][4];
+    auto load = [&](int b0, int last) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int blk = b0 + u * NW, k0 = blk * 128;
+        const bool gone = blk >= last;                 // uniform
+        const bool tail = GB > 1 && k0 + 128 > K;      // uniform: a last block of 32, 64 or 96 k
+        const int ks = gone ? 0 : k0;
+#pragma unroll
+        for (int j = 0; j < MB; ++j)
+#pragma unroll
+          for (int d = 0; d < QX; ++d) {
+            uint32_t o;
+            if constexpr (MB == 1)
+              o = gone || (tail && k0 + 8 * r16 >= K) ? OOB : vx[j] + (uint32_t)(4 * d * K) * 2u;
+            else  // the k of lane group h in dword d: 32 h + 8 d, or 32 d + 8 h
+              o = gone || (tail && k0 + 32 * d >= K) ? OOB : vx[j] + (GB == 1 ? 16u : 64u) * d;
+            xs[u][j][d] = __builtin_amdgcn_raw_buffer_load_b128(rx, o, ks * 2, 0);
+          }
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+          const uint32_t o = gone || (tail && k0 + 32 * h >= K) ? OOB : vq[i];
+          w[u][i] = __builtin_amdgcn_raw_buffer_load_b128(rq, o, ks / 2, 0);
         }
       }
+    };
+    auto compute = [&](int b0, int last, int kg0) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int blk = b0 + u * NW;
+        if (u > 0 && blk >= last) break;  // uniform
+        if constexpr (MB == 1) {
+          // row 4 d + h, chunk r16 (8 k)
+#pragma unroll
+          for (int d = 0; d < QX; ++d)
+            *reinterpret_cast<u32x4*>(xw + (4 * d + h) * XP + r16 * 16) = q4_order(xs[u][0][d]);
+          wave_lds_sync();
+          // rows past the last: any staged bytes (their outputs are not stored)
+          const int m = QX == 4 ? r16 : r16 & 3;
+#pragma unroll
+          for (int d = 0; d < 4; ++d)
+            xs[u][0][d] = *reinterpret_cast<const u32x4*>(xw + m * XP + (GB == 1 ? 4 * h + d : 4 * d + h) * 16);
+          wave_lds_sync();
+        } else {
+#pragma unroll
+          for (int j = 0; j < MB; ++j)
+#pragma unroll
+            for (int d = 0; d < 4; ++d) xs[u][j][d] = q4_order(xs[u][j][d]);
+        }
+        if constexpr (GB > 1)
+#pragma unroll
+          for (int i = 0; i < NB; ++i) w[u][i] = lane_groups_transpose(w[u][i]);
+#pragma unroll
+        for (int gi = 0; gi < GB; ++gi) {
+          constexpr int DG = 4 / GB;  // dwords per scale group
+          const int kg = GB == 1 ? blk / gstep : blk * GB + gi;
+          if (GB > 1 && kg >= KG) break;  // past K
+          f32x4 xsum[MB];
+#pragma unroll
+          for (int j = 0; j < MB; ++j) {
+            xsum[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int d = gi * DG; d < gi * DG + DG; ++d) xsum[j] = Mfma16<T>::run(ones, xs[u][j][d], xsum[j]);
+          }
+#pragma unroll
+          for (int i = 0; i < NB; ++i) {
+            const u32x2 sc = *reinterpret_cast<const u32x2*>(sS + (kg - kg0) * BN + 16 * i + 4 * h);
+            uint32_t zp = 0;
+            if constexpr (ZEROS) zp = *reinterpret_cast<const uint32_t*>(sZ + (kg - kg0) * BN + 16 * i + 4 * h);
+            f32x4 acc[MB];
+#pragma unroll
+            for (int j = 0; j < MB; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int d = gi * DG; d < gi * DG + DG; ++d) {
+              const u32x4 wf = q4_unpack<T>(w[u][i][d], mask, exp);
+#pragma unroll
+              for (int j = 0; j < MB; ++j) acc[j] = Mfma16<T>::run(wf, xs[u][j][d], acc[j]);
+            }
+            // this lane's outputs are four columns of x row r16
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const float s = Elem<T>::to_f32(static_cast<uint16_t>(sc[c >> 1] >> ((c & 1) * 16)));
+              const float off = ZEROS ? 16.0f + (float)((zp >> (8 * c)) & 255u) : 24.0f;
+#pragma unroll
+              for (int j = 0; j < MB; ++j) sum[i][j][c] += s * __builtin_fmaf(-off, xsum[j][c], acc[j][c]);
+            }
+          }
+        }
+      }
+    };
+    // blocks whose scale rows are staged together
+    const int seg = GB == 1 ? p.sg * gstep : (p.sg + GB - 1) / GB;
+    for (int s0 = 0; s0 < nblk; s0 += seg) {
+      const int last = s0 + seg < nblk ? s0 + seg : nblk;
+      const int kg0 = GB == 1 ? s0 / gstep : s0 * GB;
+      int b0 = s0 + wave;
+      load(b0, last);  // in flight while the scales are staged
+      if (s0 > 0) __syncthreads();
+      stage_scales(kg0);
+      __syncthreads();
+      while (b0 < last) {
+        compute(b0, last, kg0);
+        b0 += NW * U;
+        if (b0 < last) load(b0, last);
+      }
     }
-  }
-  if constexpr (NW > 1) {
-#pragma unroll
-    for (int i = 0; i < NB; ++i)
-#pragma unroll
-      for (int j = 0; j < MB; ++j) part[wave][i * MB + j][lane] = sum[i][j];
-    __syncthreads();
-  }
-  // fragment f (of NB MB) is finished by wave f % NW
+  };
+  if (MB == 1 && rows <= 4)
+    run(std::integral_constant<int, 1>{});
+  else
+    run(std::integral_constant<int, 4>{});
+
+  // The waves' sums of one row block after the other through LDS, each column
+  // block i finished by wave i % NW.
   const bool has_bias = epi_has_bias(epi);
   const uint16_t* bias = has_bias ? static_cast<const uint16_t*>(p.bias) + e * N : nullptr;
+  const bool yvec = (N & 3) == 0 && (reinterpret_cast<uintptr_t>(p.y) & 7) == 0;
+  f32x4* const part = reinterpret_cast<f32x4*>(area);
   with_act(epi_act(epi), [&](auto act_c) {
     constexpr int ACT = decltype(act_c)::value;
 #pragma unroll
-    for (int f = 0; f < NB * MB; ++f) {
-      if (f % NW != wave) continue;
-      const int i = f / MB, j = f % MB;
-      f32x4 v = sum[i][j];
-      if constexpr (NW > 1) {
-        v = part[0][f][lane];
+    for (int j = 0; j < MB; ++j) {
+      __syncthreads();
 #pragma unroll
-        for (int w = 1; w < NW; ++w) v += part[w][f][lane];
-      }
-      const int m = 16 * j + r16, n = n0 + 16 * i + 4 * h;
-      if (m >= rows) continue;
+      for (int i = 0; i < NB; ++i) part[(wave * NB + i) * 64 + lane] = sum[i][j];
+      __syncthreads();
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        if (n + c >= N) continue;
-        float o = v[c];
-        if (has_bias) o += Elem<T>::to_f32(bias[n + c]);
-        p.y[(int64_t)(row0 + m) * N + n + c] = Elem<T>::from_f32(act_t<ACT>(o));
+      for (int i = 0; i < NB; ++i) {
+        if (i % NW != wave) continue;
+        f32x4 v = part[i * 64 + lane];
+#pragma unroll
+        for (int q = 1; q < NW; ++q) v += part[(q * NB + i) * 64 + lane];
+        const int m = 16 * j + r16, n = n0 + 16 * i + 4 * h;
+        if (m >= rows || n >= N) continue;
+        float o[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          o[c] = v[c];
+          if (has_bias && n + c < N) o[c] += Elem<T>::to_f32(bias[n + c]);
+          o[c] = act_t<ACT>(o[c]);
+        }
+        uint16_t* y = p.y + (int64_t)(row0 + m) * N + n;
+        if (yvec) {
+          *reinterpret_cast<u32x2*>(y) = u32x2{pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3])};
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (n + c < N) y[c] = Elem<T>::from_f32(o[c]);
+        }
       }
     }
   });
 }
 
-template <typename T, int NB, int MB, int NW, int GB>
-static void launch_q4_gz(const Q4Params& p, const dim3& g, hipStream_t st) {
+template <typename T, int NB, int MB, int NW, int U, int GB>
+static void launch_q4_gz(const Q4Params& p, const dim3& g, unsigned lds, hipStream_t st) {
   if (p.offsets != nullptr) {
-    if (p.z != nullptr) hipLaunchKernelGGL((q4_kernel<T, NB, MB, NW, GB, true, true>), g, dim3(NW * 64), 0, st, p);
-    else hipLaunchKernelGGL((q4_kernel<T, NB, MB, NW, GB, false, true>), g, dim3(NW * 64), 0, st, p);
+    if (p.z != nullptr) hipLaunchKernelGGL((q4_kernel<T, NB, MB, NW, U, GB, true, true>), g, dim3(NW * 64), lds, st, p);
+    else hipLaunchKernelGGL((q4_kernel<T, NB, MB, NW, U, GB, false, true>), g, dim3(NW * 64), lds, st, p);
   } else {
-    if (p.z != nullptr) hipLaunchKernelGGL((q4_kernel<T, NB, MB, NW, GB, true, false>), g, dim3(NW * 64), 0, st, p);
-    else hipLaunchKernelGGL((q4_kernel<T, NB, MB, NW, GB, false, false>), g, dim3(NW * 64), 0, st, p);
+    if (p.z != nullptr) hipLaunchKernelGGL((q4_kernel<T, NB, MB, NW, U, GB, true, false>), g, dim3(NW * 64), lds, st, p);
+    else hipLaunchKernelGGL((q4_kernel<T, NB, MB, NW, U, GB, false, false>), g, dim3(NW * 64), lds, st, p);
   }
 }
 
-template <typename T, int NB, int MB, int NW>
+template <typename T, int NB, int MB, int NW, int U>
 static int launch_q4_g(Q4Params p, hipStream_t st) {
   p.tiles_n = (p.N + 16 * NB - 1) / (16 * NB);
   int64_t gx = p.tiles_n, gy = 1;
   if (p.offsets != nullptr) gx *= grouped_max_tiles(p.rows, p.groups, 16 * MB);
   else gy = (p.rows + 16 * MB - 1) / (16 * MB);
   if (gx > (int64_t(1) << 22) || gy > 65535) return fail(SF_ERR_UNSUPPORTED, "sf_linear_q4: too many tiles");
+  const int row = 16 * NB * (p.z != nullptr ? 3 : 2);  // LDS bytes of a scale row
+  const int fit = kQ4ScaleBytes / row / 4 * 4;
+  p.sg = p.K / p.G < fit ? p.K / p.G : fit;
+  if (p.sg < 1) p.sg = 1;
+  const unsigned lds = static_cast<unsigned>((p.sg + 3) / 4 * 4 * row);
   const dim3 g(static_cast<unsigned>(gx), static_cast<unsigned>(gy));
-  if (p.G % 128 == 0) launch_q4_gz<T, NB, MB, NW, 1>(p, g, st);
-  else if (p.G == 64) launch_q4_gz<T, NB, MB, NW, 2>(p, g, st);
-  else launch_q4_gz<T, NB, MB, NW, 4>(p, g, st);
+  if (p.G % 128 == 0) launch_q4_gz<T, NB, MB, NW, U, 1>(p, g, lds, st);
+  else if (p.G == 64) launch_q4_gz<T, NB, MB, NW, U, 2>(p, g, lds, st);
+  else launch_q4_gz<T, NB, MB, NW, U, 4>(p, g, lds, st);
   return check_launch("4-bit linear");
 }
 
+// Variants by rows per weight (their mean where the sizes are on the device)
+// and by how many column tiles there are to share out.  Measured in us, bf16,
+// groups of 128 (28672 x 8192 x 4 rows, 11008 x 4096 x 1, 4096 x 11008 x 1,
+// 4096 x 4096 x 1, 8 experts 11008 x 4096 x 16 rows, 11008 x 4096 x 32, x 64,
+// x 128):
+//   32 columns, 4 waves     29.1   8.1  15.0  6.8  37.0  12.0  20.3
+//   32 columns, 8 waves     29.7   7.8  10.4  5.6  40.6  12.2  20.8
+//   16 columns, 8 waves     33.1   7.7   8.6  4.1  52.0  15.5  26.9
+//   16 columns, 16 waves    33.5   8.9   7.3  4.4  79.6  17.7  30.0
+//   64 columns, 4 waves     30.0   9.6  20.2  9.0  38.8  13.5  19.1
+//   64 columns x 32 rows, 4 waves                        15.4  25.6  37.5
 template <typename T>
 static int launch_q4_t(const Q4Params& p, hipStream_t st) {
-  const int per = p.offsets != nullptr ? (int)(p.rows / (p.groups < p.rows ? p.groups : p.rows)) : p.rows;
-  if (per <= 16) return launch_q4_g<T, 2, 1, 4>(p, st);
-  if (per <= 32) return launch_q4_g<T, 2, 2, 4>(p, st);
-  return launch_q4_g<T, 2, 4, 4>(p, st);
+  const int64_t reached = p.offsets == nullptr ? 1 : (p.groups < p.rows ? p.groups : p.rows);
+  const int64_t per = p.rows / reached;
+  if (per > 64) return launch_q4_g<T, 4, 2, 4, 1>(p, st);
+  if (per > 32) return launch_q4_g<T, 4, 1, 4, 1>(p, st);
+  const int64_t tiles = (p.N + 31) / 32 * reached * ((per + 15) / 16);
+  const int64_t cus = cu_count_current();
+  if (tiles >= 2 * cus) return launch_q4_g<T, 2, 1, 4, 1>(p, st);
+  if (tiles >= cus) return launch_q4_g<T, 2, 1, 8, 1>(p, st);
+  return p.K >= 8192 ? launch_q4_g<T, 1, 1, 16, 1>(p, st) : launch_q4_g<T, 1, 1, 8, 1>(p, st);
 }
 
 int launch_q4(const void* x, const void* q, const void* s, const void* z, const void* bias, void* y,
@@ -288,6 +437,7 @@ int launch_q4(const void* x, const void* q, const void* s, const void* z, const 
   p.G = static_cast<int>(G);
   p.tiles_n = 0;
   p.epi = epi;
+  p.sg = 0;
   return dt == SF_BF16 ? launch_q4_t<BF16>(p, st) : launch_q4_t<F16>(p, st);
 }
 
