@@ -9,23 +9,55 @@ static bool known(sf_dtype d) { return d == SF_F32 || d == SF_F16 || d == SF_BF1
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 static int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Tile of a grouped product over `per` rows a group on average (the sizes
-// themselves are on the device).  `vec`: operands for the direct loads.
-static int rows_tile(int64_t per, bool vec, bool f32, bool b_kmajor) {
-  if (f32) return !vec ? TILE_GENERIC : (per > 96 ? TILE_128x128 : TILE_64x64);
-  if (!vec) return per > 96 ? TILE_RAG_128 : TILE_RAG_64;
-  if (per > 96) return TILE_MID_128;
-  return per <= 32 && b_kmajor ? TILE_MID_32 : TILE_MID_64;
-}
-
 static void tile_size(int cfg, int& bm, int& bn) {
   switch (cfg) {
+    case TILE_NT_BIG: bm = bn = 256; return;
     case TILE_MID_128:
-    case TILE_RAG_128:
-    case TILE_128x128: bm = bn = 128; return;
+    case TILE_RAG_128: bm = bn = 128; return;
     case TILE_MID_32: bm = 32; bn = 64; return;
+    case TILE32_SMALL2: bm = 16; bn = 32; return;
     default: bm = bn = 64; return;
   }
+}
+
+// Estimated us of a grouped product on 256 x 256 tiles (one a CU and round)
+// and on 128 x 128 tiles (two a CU; the last of them by itself runs faster),
+// for groups that each leave half a tile.  Fitted to sweeps (bf16, us, 256 /
+// 128 measured): 8192 rows, 8 groups, K 1920 -> N 7680 282 / 298, 7680 -> 1920
+// 370 / 285; 4096 rows 164 / 176, 198 / 227; 2048 rows, 7680 -> 1920 201 / 125;
+// 16384 rows, 8 groups, 4096 -> 4096 520 / 625; 8192 rows, 64 groups, 2048 ->
+// 1408 129 / 111; 512 rows, 8 groups, 4096 -> 4096 101 / 73.
+static float big_us(int64_t rows, int64_t reached, int64_t N, int64_t K, int64_t cus) {
+  const int64_t tiles = (2 * rows + 256 * reached) / 512 * cdiv(N, 256);
+  return static_cast<float>(cdiv(tiles, cus)) * (12.4f + 0.0227f * static_cast<float>(K));
+}
+static float mid_us(int64_t rows, int64_t reached, int64_t N, int64_t K, int64_t cus) {
+  const int64_t tiles = (2 * rows + 128 * reached) / 256 * cdiv(N, 128);
+  const int64_t rem = tiles % (2 * cus);
+  const float rounds = static_cast<float>(tiles / (2 * cus)) + (rem == 0 ? 0.0f : (rem <= cus ? 0.65f : 1.0f));
+  return rounds * (2.6f + 0.018f * static_cast<float>(K));
+}
+
+// Tile of a grouped product whose `rows` rows fall into `reached` groups (the
+// sizes themselves are on the device; `per` rows each on average).  `vec`:
+// operands for the 16-byte direct loads; `dma`: for 4-byte ones (fp32).
+static int rows_tile(int64_t rows, int64_t reached, int64_t N, int64_t K, bool vec, bool dma, bool f32,
+                     bool b_kmajor) {
+  const int64_t per = rows / reached, cus = cu_count_current();
+  if (f32) {
+    if (!dma) return TILE_GENERIC;
+    if (!vec) return TILE32_RAG;
+    // as sf_gemm: few 64 x 64 tiles with a short k loop run as 16 x 32 blocks
+    // (64 rows, 4 groups, 512 -> 512: 17.6 us on 64 x 64 tiles, 6.0)
+    const int64_t t64 = (2 * rows + 64 * reached) / 128 * cdiv(N, 64);
+    return 4 * t64 <= cus && K <= 2048 ? TILE32_SMALL2 : TILE32_DMA;
+  }
+  if (!vec) return per > 96 ? TILE_RAG_128 : TILE_RAG_64;
+  // 256 rows, 8 groups, 4096 -> 4096: 59 us on 32 x 64, 61 on 64 x 64, 71 on
+  // 128 x 128 (dx, which has no 32 x 64: 61, 63)
+  if (per <= 32) return b_kmajor ? TILE_MID_32 : TILE_MID_64;
+  const bool big = N > 128 && K % 128 == 0 && K >= 128;
+  return big && big_us(rows, reached, N, K, cus) <= mid_us(rows, reached, N, K, cus) ? TILE_NT_BIG : TILE_MID_128;
 }
 
 template <typename P>
@@ -68,11 +100,12 @@ static int grouped_rows(const char* name, const void* A, const void* B, const vo
   p.sB = N * K;
   const bool f32 = dtype == SF_F32;
   // 16-byte rows; one weight and one tile of A below the direct loads' 2 GiB
-  const bool vec = f32 ? K % 4 == 0 && (b_kmajor || N % 4 == 0) && aligned16(A) && aligned16(B)
+  const bool dma = f32 && N * K < (int64_t(1) << 28) && K < (int64_t(1) << 20);
+  const bool vec = f32 ? dma && K % 4 == 0 && (b_kmajor || N % 4 == 0) && aligned16(A) && aligned16(B)
                        : K % 8 == 0 && (b_kmajor || N % 8 == 0) && aligned16(A) && aligned16(B) &&
                              N * K < (int64_t(1) << 30) && K < (int64_t(1) << 22);
-  const int64_t per = rows / (groups < rows ? (groups > 0 ? groups : 1) : rows);
-  const int cfg = rows_tile(per, vec, f32, b_kmajor);
+  const int64_t reached = groups < rows ? (groups > 0 ? groups : 1) : rows;
+  const int cfg = rows_tile(rows, reached, N, K, vec, dma, f32, b_kmajor);
   int bm, bn;
   tile_size(cfg, bm, bn);
   p.tiles_n = static_cast<int>(cdiv(N, bn));
@@ -229,14 +262,17 @@ int sf_grouped_linear_dw(const void* grad, const void* x, const int32_t* offsets
     p.sC = N * K;
     const bool f32 = dtype == SF_F32;
     // 16-byte rows; a group's rows, all rows at most, below the direct loads' 2 GiB
-    const bool vec = f32 ? N % 4 == 0 && K % 4 == 0 && aligned16(grad) && aligned16(x)
-                         : N % 8 == 0 && K % 8 == 0 && aligned16(grad) && aligned16(x) &&
-                               (rows + 64) * (N > K ? N : K) < (int64_t(1) << 30);
+    const int64_t wide = N > K ? N : K;
+    const bool small = (rows + 64) * wide < (int64_t(1) << (f32 ? 29 : 30));
+    const int64_t step = f32 ? 4 : 8;
+    const bool vec = small && N % step == 0 && K % step == 0 && aligned16(grad) && aligned16(x);
+    // 256 x 256 tiles lead from the first row (bf16, us, 256 / 128: 8192 rows,
+    // 8 groups, 1920 x 7680 253 / 302; 512 rows, 64 groups, 1024 x 1024 40 / 43)
     int cfg;
     if (f32)
-      cfg = !vec ? TILE_GENERIC : (N > 64 && K > 64 ? TILE_128x128 : TILE_64x64);
+      cfg = vec ? TILE32_DMA : (small ? TILE32_RAG : TILE_GENERIC);
     else if (N > 64 && K > 64)
-      cfg = vec ? TILE_MID_128 : TILE_RAG_128;
+      cfg = vec ? (N > 128 && K > 128 ? TILE_NT_BIG : TILE_MID_128) : TILE_RAG_128;
     else
       cfg = vec ? TILE_MID_64 : TILE_RAG_64;
     int bm, bn;

@@ -8,10 +8,12 @@
 namespace sf {
 
 // ---------------------------------------------------------------------
-// Routing.  One wave per token: lane l holds logits l, l + 64, ...  The k
-// largest are found one after the other as the largest 64-bit key (logit in
-// an order-preserving integer form, then the complement of its index, so ties
-// go to the lowest index); a NaN counts above every number.
+// Routing.  One wave per token: lane l holds logits l, l + 64, ... as integers
+// in the numbers' order (a NaN above every number).  The k largest are found
+// one after the other: the largest integer by a wave maximum in the lane
+// network, then the first lane that holds it, so ties go to the lowest index.
+// (With the index in the low half of a 64-bit key and the maximum by lane
+// permutes, 16384 x 64 bf16 with k = 8 took 24.5 us instead of 13.)
 //
 // Places.  The assignments (t, j) are ordered by expert, within an expert by
 // t k + j.  A block covers kRouteTokens consecutive tokens: it counts its
@@ -34,6 +36,19 @@ __device__ __forceinline__ uint32_t order_key(float f) {
 __device__ __forceinline__ float order_value(uint32_t k) {
   if (k == 0xffffffffu) return __uint_as_float(0x7fc00000u);
   return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k);
+}
+
+// Largest value of the 64 lanes, by the lane network (row shifts, then row
+// broadcasts; the last lane ends with it).
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+  auto step = [&](uint32_t o) { v = o > v ? o : v; };
+  step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false));
+  step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false));
+  step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false));
+  step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false));
+  step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false));
+  step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false));
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
 // Places of the block's `n` <= 1024 assignments ex[] (experts, in order):
@@ -93,40 +108,43 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(const void* __rest
   __syncthreads();
   for (int t = wave; t < nt; t += kRouteThreads / 64) {
     const int64_t row = t0 + t;
-    uint64_t key[CH];
+    uint32_t key[CH];
     float v[CH];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int e = c * 64 + lane;
       v[c] = e < E ? Chunk8<T>::get(logits, row * E + e) : -INFINITY;
-      // 0 is below every key of an expert (its low half is not 0)
-      key[c] = e < E ? (uint64_t)order_key(v[c]) << 32 | (0xffffffffu - (uint32_t)e) : 0;
+      key[c] = e < E ? order_key(v[c]) : 0;  // 0 is below the key of every number
     }
-    float most = 0.f, w = 0.f, sum = 0.f;
+    uint32_t top = 0, val = 0;  // the largest key, and lane j's: the j-th
     int mine = 0;
     for (int j = 0; j < k; ++j) {
-      uint64_t best = key[0];
+      uint32_t best = key[0];
 #pragma unroll
       for (int c = 1; c < CH; ++c) best = key[c] > best ? key[c] : best;
+      best = wave_max_u32(best);
+      int e = 0;
+      bool found = false;
 #pragma unroll
-      for (int off = 32; off > 0; off >>= 1) {
-        const uint64_t o = __shfl_xor(best, off, 64);
-        best = o > best ? o : best;
+      for (int c = 0; c < CH; ++c) {
+        const uint64_t has = __ballot(key[c] == best);
+        if (!found && has != 0) {  // uniform
+          const int src = __builtin_ctzll(has);
+          e = c * 64 + src;
+          if (lane == src) key[c] = 0;
+          found = true;
+        }
       }
-      const int e = (int)(0xffffffffu - (uint32_t)best);
-      const float val = order_value((uint32_t)(best >> 32));
-      if (j == 0) most = val;
-#pragma unroll
-      for (int c = 0; c < CH; ++c)
-        if (key[c] == best) key[c] = 0;
-      // softmax numerator; a token with no expert allowed (all -inf) has none
-      const float p = most == -INFINITY ? 0.f : expf(val - most);
-      sum += p;
+      if (j == 0) top = best;
       if (lane == j) {
-        w = p;
+        val = best;
         mine = e;
       }
     }
+    // softmax numerators; a token with no expert allowed (all -inf) has none
+    const float most = order_value(top);
+    const float w = lane < k && most != -INFINITY ? expf(order_value(val) - most) : 0.f;
+    float sum = wave_sum(w);
     if (!renorm) {  // over every expert instead of the chosen ones
       float s = 0.f;
 #pragma unroll
@@ -179,6 +197,7 @@ __global__ __launch_bounds__(kRouteThreads) void route_place_kernel(const int* _
   if (share < shares) {
     for (int e = tid % lanes; e < E; e += lanes) {
       int sum = 0, pre = 0;
+#pragma unroll 8
       for (int b = share; b < nb; b += shares) {
         const int c = counts[(int64_t)b * E + e];
         sum += c;
@@ -387,11 +406,12 @@ __global__ __launch_bounds__(256) void combine_kernel(RowsParams p) {
   }
 }
 
-// drows[s] = w g[t], dw = <g[t], rows[s]>; the sums over a row are formed per
-// thread, then over the lanes, then over the waves, in that order always.
+// drows[s] = w g[t], dw = <g[t], rows[s]>; a token's columns are shared by one
+// wave at most, so its sums are formed per thread and then over the lanes,
+// without a barrier (4096 x 2 rows of 1283 fp16: 16.8 us with a block of four
+// waves a token).
 template <typename T>
 __global__ __launch_bounds__(256) void combine_backward_kernel(RowsParams p) {
-  __shared__ float part[4];
   const int64_t t = (int64_t)blockIdx.x * (256 >> p.lg) + (threadIdx.x >> p.lg);
   const bool live = t < p.tokens;
   const int in = threadIdx.x & ((1 << p.lg) - 1);
@@ -401,6 +421,7 @@ __global__ __launch_bounds__(256) void combine_backward_kernel(RowsParams p) {
     float dot = 0.f;
     if ((uint64_t)(int64_t)s < (uint64_t)p.n) {
       const float w = p.w[t * p.k + j];
+#pragma unroll 2
       for (int c = in * 8; c < p.D; c += step) {
         float g[8], v[8], o[8];
         load_cols<T>(p.x, t * p.D + c, p.D - c, g);
@@ -413,24 +434,17 @@ __global__ __launch_bounds__(256) void combine_backward_kernel(RowsParams p) {
         store_cols<T>(p.out, (int64_t)s * p.D + c, p.D - c, o);
       }
     }
-    for (int off = p.lg < 6 ? 1 << p.lg >> 1 : 32; off > 0; off >>= 1) dot += __shfl_xor(dot, off, 64);
-    if (p.lg > 6) {  // a row over several waves of the block
-      if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = dot;
-      __syncthreads();
-      dot = 0.f;
-      const int w0 = (threadIdx.x >> p.lg) << (p.lg - 6);
-      for (int i = 0; i < 1 << (p.lg - 6); ++i) dot += part[w0 + i];
-      __syncthreads();
-    }
+    for (int off = 1 << p.lg >> 1; off > 0; off >>= 1) dot += __shfl_xor(dot, off, 64);
     if (live && in == 0) p.dw[t * p.k + j] = dot;
   }
 }
 
 template <typename T>
 static int launch_rows_t(int op, RowsParams p, hipStream_t st) {
-  // threads per token: enough for its columns, at most the block
+  // threads per token: enough for its columns, at most the block (the gradient:
+  // a wave)
   int lg = 0;
-  while (lg < 8 && (8 << lg) < p.D) ++lg;
+  while (lg < (op == 2 ? 6 : 8) && (8 << lg) < p.D) ++lg;
   p.lg = lg;
   const int64_t per = 256 >> lg;
   const int64_t nb = (p.tokens + per - 1) / per;
@@ -512,43 +526,48 @@ int launch_act_backward(int act, const void* g, const void* pre, void* out, int6
 
 // ---------------------------------------------------------------------
 // Column sums of each group's rows (the bias gradients): out[e, n] = sum over
-// the rows r of group e of g[r, n].  A block takes 512 columns of one group,
-// its 16 waves every 16th row each, fp32 partial sums joined through LDS in
-// wave order.
+// the rows r of group e of g[r, n].  A block takes 128 columns of one group:
+// 16 lanes eight columns each, the 64 quarter-waves of the block every 64th
+// row, fp32 partial sums joined through LDS in a fixed order.  Bound by
+// memory; narrow blocks give every CU some (4096 rows, 8 groups, 7680 columns
+// bf16: 24 us in 120 blocks of 512 columns, 480 of 128 take 12).
 // ---------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(1024) void group_colsum_kernel(const void* __restrict__ g, const int* __restrict__ offsets,
                                                             int rows, int64_t N, void* __restrict__ out) {
-  __shared__ float part[16][512];
+  __shared__ float part[64][132];
   int first, cnt;
   group_bounds(offsets, (int)blockIdx.y, rows, first, cnt);
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t c = (int64_t)blockIdx.x * 512 + lane * 8;
+  const int q = threadIdx.x >> 4, l = threadIdx.x & 15;
+  const int64_t c = (int64_t)blockIdx.x * 128 + l * 8;
   const int left = N - c >= 8 ? 8 : (int)(N - c);
   float a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   if (left > 0) {
 #pragma unroll 4
-    for (int r = wave; r < cnt; r += 16) {
+    for (int r = q; r < cnt; r += 64) {
       float v[8];
       load_cols<T>(g, (int64_t)(first + r) * N + c, left, v);
 #pragma unroll
-      for (int q = 0; q < 8; ++q) a[q] += v[q];
+      for (int i = 0; i < 8; ++i) a[i] += v[i];
     }
   }
 #pragma unroll
-  for (int q = 0; q < 8; ++q) part[wave][lane * 8 + q] = a[q];
+  for (int i = 0; i < 8; ++i) part[q][l * 8 + i] = a[i];
   __syncthreads();
-  if (threadIdx.x < 512) {
-    const int64_t n = (int64_t)blockIdx.x * 512 + threadIdx.x;
-    float s = 0.f;
-    for (int w = 0; w < 16; ++w) s += part[w][threadIdx.x];
-    if (n < N) Chunk8<T>::put(out, (int64_t)blockIdx.y * N + n, s);
-  }
+  // eight threads a column, eight partial sums each, then a fixed tree
+  const int col = threadIdx.x >> 3, o = threadIdx.x & 7;
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s += part[o * 8 + i][col];
+#pragma unroll
+  for (int off = 4; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
+  const int64_t n = (int64_t)blockIdx.x * 128 + col;
+  if (o == 0 && n < N) Chunk8<T>::put(out, (int64_t)blockIdx.y * N + n, s);
 }
 
 int launch_group_colsum(const void* g, const int* offsets, int64_t rows, int64_t groups, int64_t N, void* out,
                         sf_dtype dt, hipStream_t st) {
-  const dim3 grid(static_cast<unsigned>((N + 511) / 512), static_cast<unsigned>(groups));
+  const dim3 grid(static_cast<unsigned>((N + 127) / 128), static_cast<unsigned>(groups));
   const int r = static_cast<int>(rows);
   switch (dt) {
     case SF_F16: hipLaunchKernelGGL((group_colsum_kernel<F16>), grid, dim3(1024), 0, st, g, offsets, r, N, out); break;

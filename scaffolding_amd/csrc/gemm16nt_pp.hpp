@@ -78,6 +78,7 @@
 #pragma once
 
 #include "gemm16.hpp"
+#include "grouped.hpp"
 
 namespace sf {
 
@@ -144,11 +145,13 @@ constexpr int waitcnt_imm(int vm, int lgkm) {
   return (vm & 15) | (7 << 4) | ((lgkm & 15) << 8) | (((vm >> 4) & 3) << 14);
 }
 
+// Prm: GemmParams, or grouped.hpp's GroupedRows (K-contiguous A) or GroupedSums
+// (both M/N-contiguous), one tile per workgroup.
 // NSTAGE = 2, the pipelined kernel above: K % 128 == 0.  (K == 64 runs
 // gemm16nt_k64_kernel, which holds four workgroups per CU.)
 template <typename TIn, typename TOut, int NSTAGE = 2, bool A_KM = true, bool B_KM = true, bool PERSIST = false,
-          bool SHARED = false>
-__global__ __launch_bounds__(512) void gemm16nt_pp_kernel(GemmParams p) {
+          bool SHARED = false, typename Prm = GemmParams>
+__global__ __launch_bounds__(512) void gemm16nt_pp_kernel(Prm p) {
   static_assert(NSTAGE == 2, "two pair stages (K == 64 runs gemm16nt_k64_kernel)");
   static_assert(!PERSIST || A_KM, "persistent tiles: K-contiguous A");
   static_assert(!SHARED || PERSIST, "a shared split sum needs the persistent grid");
@@ -168,7 +171,31 @@ __global__ __launch_bounds__(512) void gemm16nt_pp_kernel(GemmParams p) {
   const int wm = wave >> 2;
   const int wn = wave & 3;
 
-  const int M = p.M, N = p.N, K = p.K;
+  constexpr bool ROWS = std::is_same<Prm, GroupedRows>::value, SUMS = std::is_same<Prm, GroupedSums>::value;
+  static_assert(!(ROWS || SUMS) || !PERSIST, "grouped products: one tile per workgroup");
+  const int N = p.N;
+  typename GroupVar<ROWS>::type M = p.M;
+  typename GroupVar<SUMS>::type K = p.K;
+  int64_t b = blockIdx.y;
+  int64_t row0 = 0;  // first row of this tile (ROWS) or of the sum (SUMS)
+  int gtn = 0;
+  if constexpr (ROWS) {
+    GroupTile g;
+    if (!group_find<BM>(p, g)) return;  // workgroup-uniform
+    b = g.e;
+    row0 = g.row;
+    M = g.rows;
+    gtn = g.tn;
+    if (g.e == p.groups) {  // rows of no group
+      group_zero_tile(static_cast<uint16_t*>(p.C) + row0 * p.ldc, p.ldc, M, gtn * BN, N, BN);
+      return;
+    }
+  }
+  if constexpr (SUMS) {
+    int first;
+    group_bounds(p.offsets, (int)b, p.rows, first, K);
+    row0 = first;
+  }
   // With two M/N-contiguous operands K need not be a multiple of 128: the
   // loop runs to the next multiple and the k-rows past K read as zeros
   // through both buffers' bounds.
@@ -181,7 +208,12 @@ __global__ __launch_bounds__(512) void gemm16nt_pp_kernel(GemmParams p) {
   const int xcd = blockIdx.x % kNumXcd, xo = blockIdx.x / kNumXcd;
   auto make_job = [&](int pid, int q, int st, Job& jb) {
     int tm, tn;
-    group_tile(pid, p.tiles_m, p.tiles_n, 8, tm, tn);
+    if constexpr (ROWS) {  // the row pointers start at the tile
+      tm = 0;
+      tn = gtn;
+    } else {
+      group_tile(pid, p.tiles_m, p.tiles_n, 8, tm, tn);
+    }
     jb.m0 = tm * BM;
     jb.n0 = tn * BN;
     jb.part = q;
@@ -248,9 +280,10 @@ __global__ __launch_bounds__(512) void gemm16nt_pp_kernel(GemmParams p) {
   bool has_next = job_at(1, nxt);
   int m0 = cur.m0, n0 = cur.n0;
   int t_begin = cur.t_begin, KT = cur.KT, part = cur.part, split_tile = cur.split_tile;
-  const int64_t b = blockIdx.y;
-  const uint16_t* __restrict__ A = static_cast<const uint16_t*>(p.A) + b * p.sA;
-  const uint16_t* __restrict__ B = static_cast<const uint16_t*>(p.B) + b * p.sB;
+  const uint16_t* __restrict__ A = static_cast<const uint16_t*>(p.A) + (ROWS || SUMS ? row0 * p.lda : b * p.sA);
+  const uint16_t* __restrict__ B = static_cast<const uint16_t*>(p.B) + (SUMS ? row0 * p.ldb : b * p.sB);
+  const void* bias = p.bias;
+  if constexpr (ROWS) bias = static_cast<const uint16_t*>(p.bias) + b * N;
   int KP = KT / 2;  // slice pairs (KT a multiple of 4)
 
   // A pair stage holds 64 k-columns: line r (128 B) is row r's 64 k values,
@@ -287,7 +320,7 @@ __global__ __launch_bounds__(512) void gemm16nt_pp_kernel(GemmParams p) {
   // spare for the next job's bias area).
   const bool bias_lds = B_KM && epi_has_bias(p.epi) && (N & 1) == 0;
   const __amdgpu_buffer_rsrc_t rBias = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<void*>(p.bias), (short)0, (int)((uint32_t)N * 2u), 0x00020000);
+      const_cast<void*>(bias), (short)0, (int)((uint32_t)N * 2u), 0x00020000);
   auto bias_dma = [&](int bn0, int area) {
     if (bias_lds && wave < 2)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rBias, (lds_ptr_t)(reinterpret_cast<uint8_t*>(&sBias[area][0]) + wave * 256),
@@ -627,7 +660,7 @@ __global__ __launch_bounds__(512) void gemm16nt_pp_kernel(GemmParams p) {
     for (int i = 0; i < FN; ++i) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) bv[i][q] = 0.f;
-      if (has_bias) load_bias4<TIn>(p.bias, n0 + wn * WN + i * 16 + 4 * (elane >> 4), N, bv[i]);
+      if (has_bias) load_bias4<TIn>(bias, n0 + wn * WN + i * 16 + 4 * (elane >> 4), N, bv[i]);
     }
   }
   constexpr int PITCH = WN * 2 + 16;             // 144 bytes
@@ -648,7 +681,7 @@ __global__ __launch_bounds__(512) void gemm16nt_pp_kernel(GemmParams p) {
   constexpr int LANES_ROW = WN * 2 / 16;
   constexpr int ROWS_I = 64 / LANES_ROW;
   static_assert(16 % ROWS_I == 0, "a store's rows lie in one 16-row block");
-  uint16_t* C = static_cast<uint16_t*>(p.C) + b * p.sC;
+  uint16_t* C = static_cast<uint16_t*>(p.C) + (ROWS ? row0 * p.ldc : b * p.sC);
   const bool vec_ok = ((p.ldc & 7) == 0) && ((reinterpret_cast<uintptr_t>(C) & 15) == 0);
   // Residual: read in the accumulator layout (4 consecutive columns of one
   // row per lane, as raw 16-bit pairs) and added before the single

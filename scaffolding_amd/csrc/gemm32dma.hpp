@@ -93,8 +93,10 @@ struct __attribute__((packed, aligned(4))) Float4u {
   f32x4 v;
 };
 
-template <int BM, int BN, bool A_KMAJOR, bool B_KMAJOR, int NSTG, int KG = 1, int CE = 4, bool TAIL = true>
-__global__ __launch_bounds__(256 * KG) void gemm32dma_kernel(GemmParams p) {
+// Prm: GemmParams, or grouped.hpp's GroupedRows / GroupedSums.
+template <int BM, int BN, bool A_KMAJOR, bool B_KMAJOR, int NSTG, int KG = 1, int CE = 4, bool TAIL = true,
+          typename Prm = GemmParams>
+__global__ __launch_bounds__(256 * KG) void gemm32dma_kernel(Prm p) {
   constexpr int NT = 256;  // threads of one k-group
   constexpr int BK = 32;
   constexpr int WM = BM / 2, WN = BN / 2;
@@ -127,13 +129,36 @@ __global__ __launch_bounds__(256 * KG) void gemm32dma_kernel(GemmParams p) {
   // Two k-groups never split across workgroups (the host passes split 0).
   const int part = (KG == 1 && p.split > 0) ? (int)(blockIdx.x % (unsigned)p.split) : -1;
   const int tile_id = p.split > 0 ? (int)(blockIdx.x / (unsigned)p.split) : 0;
+  constexpr bool ROWS = std::is_same<Prm, GroupedRows>::value, SUMS = std::is_same<Prm, GroupedSums>::value;
+  const int N = p.N;
+  typename GroupVar<ROWS>::type M = p.M, epi = p.epi;
+  typename GroupVar<ROWS || SUMS>::type K = p.K;
+  int64_t b = blockIdx.y;
+  int64_t row0 = 0;  // first row of this tile (ROWS) or of the sum (SUMS)
   int tm, tn;
-  group_tile(p.split > 0 ? tile_id : xcd_remap(blockIdx.x, gridDim.x), p.tiles_m, p.tiles_n, 8, tm, tn);
+  if constexpr (ROWS) {  // the row pointers start at the tile
+    GroupTile gt;
+    if (!group_find<BM>(p, gt)) return;  // workgroup-uniform
+    b = gt.e;
+    row0 = gt.row;
+    M = gt.rows;
+    tm = 0;
+    tn = gt.tn;
+    if (gt.e == p.groups) {  // rows of no group: zeros
+      K = 0;
+      epi = SF_EPI_NONE;
+    }
+  } else {
+    group_tile(p.split > 0 ? tile_id : xcd_remap(blockIdx.x, gridDim.x), p.tiles_m, p.tiles_n, 8, tm, tn);
+  }
+  if constexpr (SUMS) {
+    int first;
+    group_bounds(p.offsets, (int)b, p.rows, first, K);
+    row0 = first;
+  }
   const int m0 = tm * BM, n0 = tn * BN;
-  const int64_t b = blockIdx.y;
-  const float* A = static_cast<const float*>(p.A) + b * p.sA;
-  const float* B = static_cast<const float*>(p.B) + b * p.sB;
-  const int M = p.M, N = p.N, K = p.K;
+  const float* A = static_cast<const float*>(p.A) + (ROWS || SUMS ? row0 * p.lda : b * p.sA);
+  const float* B = static_cast<const float*>(p.B) + (SUMS ? row0 * p.ldb : b * p.sB);
 
   // This k-group's slices [kt0, kt1): with two groups the count is rounded
   // up to even (a slice past K is all zeros), so both run the same number of
@@ -369,12 +394,12 @@ __global__ __launch_bounds__(256 * KG) void gemm32dma_kernel(GemmParams p) {
   // wn*WN + 4 FN g + 4c + e, element e of run c from fragment (4c+e) % FN,
   // row (4c+e) / FN.  Fragment j's rows of C: 16 j + l % 16, or with an
   // M-contiguous A FM (l % 16) + j.
-  float* C = static_cast<float*>(p.C) + b * p.sC;
-  const bool has_bias = epi_has_bias(p.epi);
-  const int act = epi_act(p.epi);
+  float* C = static_cast<float*>(p.C) + (ROWS ? row0 * p.ldc : b * p.sC);
+  const bool has_bias = epi_has_bias(epi);
+  const int act = epi_act(epi);
   const float alpha = p.alpha;
   const bool vec_ok = ((p.ldc & 3) == 0) && ((reinterpret_cast<uintptr_t>(C) & 15) == 0);
-  const float* bias = static_cast<const float*>(p.bias);
+  const float* bias = static_cast<const float*>(p.bias) + (ROWS ? b * N : 0);
   const void* R = p.res != nullptr ? static_cast<const float*>(p.res) + b * p.sR : nullptr;
   const bool rvec = R != nullptr && res_vec_ok<float>(R, p.ldr);
   with_act(act, [&](auto act_c) {

@@ -27,20 +27,39 @@
 
 namespace sf {
 
-template <int FS, bool B_KMAJOR, int KW>
-__global__ __launch_bounds__(KW * 64) void gemm32small_kernel(GemmParams p) {
+// Prm: GemmParams, or grouped.hpp's GroupedRows.
+template <int FS, bool B_KMAJOR, int KW, typename Prm = GemmParams>
+__global__ __launch_bounds__(KW * 64) void gemm32small_kernel(Prm p) {
   constexpr int U = 4;  // 16-k steps per batch of loads
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, r = lane & 15;
 
-  const int tm = (int)(blockIdx.x / (unsigned)p.tiles_n), tn = (int)(blockIdx.x % (unsigned)p.tiles_n);
+  constexpr bool ROWS = std::is_same<Prm, GroupedRows>::value;
+  const int N = p.N;
+  typename GroupVar<ROWS>::type M = p.M, K = p.K, epi = p.epi;
+  int64_t b = blockIdx.y;
+  int64_t row0 = 0;
+  int tm = 0, tn;
+  if constexpr (ROWS) {  // the row pointers start at the tile
+    GroupTile gt;
+    if (!group_find<16>(p, gt)) return;  // workgroup-uniform
+    b = gt.e;
+    row0 = gt.row;
+    M = gt.rows;
+    tn = gt.tn;
+    if (gt.e == p.groups) {  // rows of no group: zeros
+      K = 0;
+      epi = SF_EPI_NONE;
+    }
+  } else {
+    tm = (int)(blockIdx.x / (unsigned)p.tiles_n);
+    tn = (int)(blockIdx.x % (unsigned)p.tiles_n);
+  }
   const int m0 = tm * 16, n0 = tn * 16 * FS;
-  const int64_t b = blockIdx.y;
-  const float* A = static_cast<const float*>(p.A) + b * p.sA;
+  const float* A = static_cast<const float*>(p.A) + (ROWS ? row0 * p.lda : b * p.sA);
   const float* B = static_cast<const float*>(p.B) + b * p.sB;
-  const int M = p.M, N = p.N, K = p.K;
 
   // Rows past M (N) are clamped to the last one: their products reach no
   // stored output.
@@ -109,12 +128,12 @@ __global__ __launch_bounds__(KW * 64) void gemm32small_kernel(GemmParams p) {
   for (int i = 0; i < FS; ++i) red[wave][i][lane] = acc[i];
   __syncthreads();
 
-  float* C = static_cast<float*>(p.C) + b * p.sC;
-  const bool has_bias = epi_has_bias(p.epi);
-  const int act = epi_act(p.epi);
+  float* C = static_cast<float*>(p.C) + (ROWS ? row0 * p.ldc : b * p.sC);
+  const bool has_bias = epi_has_bias(epi);
+  const int act = epi_act(epi);
   const float alpha = p.alpha;
   const bool vec_ok = ((p.ldc & 3) == 0) && ((reinterpret_cast<uintptr_t>(C) & 15) == 0);
-  const float* bias = static_cast<const float*>(p.bias);
+  const float* bias = static_cast<const float*>(p.bias) + (ROWS ? b * N : 0);
   const void* R = p.res != nullptr ? static_cast<const float*>(p.res) + b * p.sR : nullptr;
   const bool rvec = R != nullptr && res_vec_ok<float>(R, p.ldr);
   const int m = m0 + r;

@@ -151,6 +151,13 @@ __device__ __forceinline__ bool group_find(const P& p, GroupTile& out) {
   return group_find_at<BM>(p.offsets, p.groups, p.rows, p.tiles_n, (int)blockIdx.x, out);
 }
 
+// Zeros to `rows` rows of C (leading dimension ld) in columns n0 .. n0 + width
+// - 1 below N, by the whole workgroup.
+__device__ __forceinline__ void group_zero_tile(uint16_t* C, int64_t ld, int rows, int n0, int N, int width) {
+  const int w = N - n0 < width ? N - n0 : width;
+  for (int i = threadIdx.x; i < rows * w; i += blockDim.x) C[(int64_t)(i / w) * ld + n0 + i % w] = 0;
+}
+
 // First row and rows of group e, every wave for itself.
 __device__ __forceinline__ void group_bounds(const int* __restrict__ offsets, int e, int rows, int& first, int& cnt) {
   const int lane = threadIdx.x & 63;

@@ -1,21 +1,27 @@
-// grouped32.hip — fp32 grouped products on gemm32_kernel's register-staged
-// tiles.
+// grouped32.hip — fp32 grouped products: the direct-to-LDS tiles and, for few
+// rows in groups, the small blocks; register-staged tiles past the direct
+// loads' 2 GiB.
 #include "gemm32.hpp"
+#include "gemm32dma.hpp"
+#include "gemm32small.hpp"
 #include "sf_internal.hpp"
 
 namespace sf {
 
-template <bool KM, bool AKM, typename P>
-static int launch_grouped32_t(int cfg, const P& p, const dim3& g, hipStream_t st) {
+template <bool KM>
+static int launch_rows_t(int cfg, const GroupedRows& p, const dim3& g, hipStream_t st) {
   switch (cfg) {
-    case TILE_128x128:
-      hipLaunchKernelGGL((gemm32_kernel<128, 128, 2, 2, KM, true, AKM, P>), g, dim3(256), 0, st, p);
+    case TILE32_SMALL2:
+      hipLaunchKernelGGL((gemm32small_kernel<2, KM, 8, GroupedRows>), g, dim3(512), 0, st, p);
       break;
-    case TILE_64x64:
-      hipLaunchKernelGGL((gemm32_kernel<64, 64, 2, 2, KM, true, AKM, P>), g, dim3(256), 0, st, p);
+    case TILE32_DMA:
+      hipLaunchKernelGGL((gemm32dma_kernel<64, 64, true, KM, 2, 2, 4, true, GroupedRows>), g, dim3(512), 0, st, p);
+      break;
+    case TILE32_RAG:
+      hipLaunchKernelGGL((gemm32dma_kernel<64, 64, true, KM, 2, 2, 1, true, GroupedRows>), g, dim3(512), 0, st, p);
       break;
     case TILE_GENERIC:
-      hipLaunchKernelGGL((gemm32_kernel<64, 64, 2, 2, KM, false, AKM, P>), g, dim3(256), 0, st, p);
+      hipLaunchKernelGGL((gemm32_kernel<64, 64, 2, 2, KM, false, true, GroupedRows>), g, dim3(256), 0, st, p);
       break;
     default:
       return fail(SF_ERR_INVALID_ARG, "tile config %d has no grouped fp32 variant", cfg);
@@ -24,11 +30,25 @@ static int launch_grouped32_t(int cfg, const P& p, const dim3& g, hipStream_t st
 }
 
 int launch_grouped_rows_f32(bool b_kmajor, int cfg, const GroupedRows& p, unsigned gx, hipStream_t st) {
-  return b_kmajor ? launch_grouped32_t<true, true>(cfg, p, dim3(gx), st)
-                  : launch_grouped32_t<false, true>(cfg, p, dim3(gx), st);
+  return b_kmajor ? launch_rows_t<true>(cfg, p, dim3(gx), st) : launch_rows_t<false>(cfg, p, dim3(gx), st);
 }
+
 int launch_grouped_sums_f32(int cfg, const GroupedSums& p, unsigned gx, unsigned gy, hipStream_t st) {
-  return launch_grouped32_t<false, false>(cfg, p, dim3(gx, gy), st);
+  const dim3 g(gx, gy);
+  switch (cfg) {
+    case TILE32_DMA:
+      hipLaunchKernelGGL((gemm32dma_kernel<64, 64, false, false, 2, 2, 4, true, GroupedSums>), g, dim3(512), 0, st, p);
+      break;
+    case TILE32_RAG:
+      hipLaunchKernelGGL((gemm32dma_kernel<64, 64, false, false, 2, 2, 1, true, GroupedSums>), g, dim3(512), 0, st, p);
+      break;
+    case TILE_GENERIC:
+      hipLaunchKernelGGL((gemm32_kernel<64, 64, 2, 2, false, false, false, GroupedSums>), g, dim3(256), 0, st, p);
+      break;
+    default:
+      return fail(SF_ERR_INVALID_ARG, "tile config %d has no grouped fp32 variant", cfg);
+  }
+  return check_launch("grouped fp32 sums");
 }
 
 }  // namespace sf

@@ -4,6 +4,7 @@
 #pragma once
 
 #include "gemm16mid.hpp"
+#include "gemm16nt_pp.hpp"
 #include "sf_internal.hpp"
 
 namespace sf {
@@ -13,6 +14,10 @@ template <typename T, bool KM>
 static int launch_grouped_rows_t(int cfg, const GroupedRows& p, unsigned gx, hipStream_t st) {
   const dim3 g(gx);
   switch (cfg) {
+    case TILE_NT_BIG:
+      if (p.K % 128 != 0) return fail(SF_ERR_INVALID_ARG, "the grouped 256x256 kernel needs K %% 128 == 0");
+      hipLaunchKernelGGL((gemm16nt_pp_kernel<T, T, 2, true, KM, false, false, GroupedRows>), g, dim3(512), 0, st, p);
+      break;
     case TILE_MID_128:
       hipLaunchKernelGGL((gemm16mid_kernel<T, T, 128, 128, 2, 4, 2, true, KM, true, 4, GroupedRows>), g, dim3(512), 0,
                          st, p);
@@ -46,6 +51,9 @@ template <typename T>
 static int launch_grouped_sums_t(int cfg, const GroupedSums& p, unsigned gx, unsigned gy, hipStream_t st) {
   const dim3 g(gx, gy);
   switch (cfg) {
+    case TILE_NT_BIG:
+      hipLaunchKernelGGL((gemm16nt_pp_kernel<T, T, 2, false, false, false, false, GroupedSums>), g, dim3(512), 0, st, p);
+      break;
     case TILE_MID_128:
       hipLaunchKernelGGL((gemm16mid_kernel<T, T, 128, 128, 2, 4, 2, false, false, true, 4, GroupedSums>), g, dim3(512),
                          0, st, p);
