@@ -60,17 +60,14 @@ __device__ __forceinline__ void route_place(const int* ex, int n, int E, int (*h
   for (int i = tid; i < NW * E; i += kRouteThreads) hist[i / E][i % E] = 0;
   __syncthreads();
   const int e = tid < n ? ex[tid] : -1;
-  // earlier lanes of this wave with the same expert: one round per distinct expert
-  int rank = 0;
-  uint64_t left = __ballot(e >= 0);
-  while (left != 0) {
-    const int src = __builtin_ctzll(left);
-    const int v = __builtin_amdgcn_readlane(e, src);
-    const uint64_t same = __ballot(e == v);
-    if (e == v) rank = __popcll(same & ((1ull << lane) - 1));
-    if (lane == src) hist[wave][v] = __popcll(same);
-    left &= ~same;
+  // the lanes of this wave with the same expert: those that agree in every bit
+  uint64_t same = __ballot(e >= 0);
+  for (int bit = 1; bit < E; bit <<= 1) {
+    const uint64_t has = __ballot((e & bit) != 0);
+    same &= (e & bit) != 0 ? has : ~has;
   }
+  const int rank = __popcll(same & ((1ull << lane) - 1));  // earlier ones
+  if (e >= 0 && rank == 0) hist[wave][e] = __popcll(same);
   __syncthreads();
   if (e >= 0) {
     int at = base[e] + rank;
