@@ -84,7 +84,10 @@ __global__ __launch_bounds__(WVM* WVN * 64, OCC) void gemm16mid_kernel(Prm p) {
   int gtn = 0;
   if constexpr (ROWS) {
     GroupTile g;
-    if (!group_find<BM>(p, g)) return;  // workgroup-uniform
+    bool found;  // workgroup-uniform
+    if constexpr (BM == 128) found = group_find_rest(p, g);
+    else found = group_find<BM>(p, g);
+    if (!found) return;
     b = g.e;
     row0 = g.row;
     M = g.rows;
@@ -124,6 +127,7 @@ __global__ __launch_bounds__(WVM* WVN * 64, OCC) void gemm16mid_kernel(Prm p) {
     group_tile(tile, p.tiles_m, p.tiles_n, 8, tm, tn);
   }
   const int m0 = tm * BM, n0 = tn * BN;
+  if (ROWS && n0 >= N) return;  // a quarter past the last column
   const uint16_t* __restrict__ A = static_cast<const uint16_t*>(p.A) + (ROWS || SUMS ? row0 * p.lda : b * p.sA);
   const uint16_t* __restrict__ B = static_cast<const uint16_t*>(p.B) + (SUMS ? row0 * p.ldb : b * p.sB);
 

@@ -181,7 +181,7 @@ __global__ __launch_bounds__(512) void gemm16nt_pp_kernel(Prm p) {
   int gtn = 0;
   if constexpr (ROWS) {
     GroupTile g;
-    if (!group_find<BM>(p, g)) return;  // workgroup-uniform
+    if (!group_find_head(p, g)) return;  // workgroup-uniform
     b = g.e;
     row0 = g.row;
     M = g.rows;

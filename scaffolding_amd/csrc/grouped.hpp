@@ -32,6 +32,7 @@ namespace sf {
 struct GroupedRows : GemmParams {
   const int* offsets;
   int groups, rows;
+  int cus;  // > 0: one of a pair of launches (GroupPart), on this many CUs
 };
 struct GroupedSums : GemmParams {
   const int* offsets;
@@ -79,12 +80,24 @@ __device__ __forceinline__ int wave_scan_sum(int v) {
   return v;
 }
 
-// The tile of workgroup `pid` of `grid` (see above), every wave for itself;
-// false for a surplus workgroup.  Tiles run group by group, within a group in
-// the column bands of group_tile, and each XCD takes a contiguous range.
-template <int BM>
+// Which part of the tile list a launch works on.
+//   ALL   every tile
+//   HEAD  the whole rounds of one tile a CU (p.cus), and the rest where it is
+//         more than half a round
+//   REST  what HEAD leaves, in quarters: tile t's quarter q is the BM x BM / 2
+//         rows and columns at row (q & 1) BM and column tile 2 tn + (q >> 1) of
+//         a launch with tiles of half the edge
+// A last round of a few 256 x 256 tiles costs as much as a full one; in
+// quarters it runs on all CUs.
+enum GroupPart { GROUP_ALL, GROUP_HEAD, GROUP_REST };
+
+// The tile of workgroup `pid` (see above), every wave for itself; false for a
+// surplus workgroup.  Tiles run group by group, within a group in the column
+// bands of group_tile, and each XCD takes a contiguous range.  BM and tiles_n
+// are those of the tile list (REST: of HEAD's).
+template <int BM, GroupPart PART>
 __device__ __forceinline__ bool group_find_at(const int* __restrict__ offsets, int groups, int rows, int tiles_n,
-                                              int pid, GroupTile& out) {
+                                              int cus, int pid, GroupTile& out) {
   const int lane = threadIdx.x & 63;
   const int per = (groups + 1 + 63) / 64;  // groups per lane, the range behind the last among them
   const int i0 = lane * per;
@@ -110,8 +123,17 @@ __device__ __forceinline__ bool group_find_at(const int* __restrict__ offsets, i
   }
   const int upto = wave_scan_sum(tiles);
   const int active = __builtin_amdgcn_readlane(upto, 63) * tiles_n;
-  if (pid >= active) return false;
-  const int tile = xcd_remap(pid, active);
+  int lo = 0, hi = active;  // this launch's tiles
+  if constexpr (PART != GROUP_ALL) {
+    const int left = active % cus;
+    const int cut = 2 * left <= cus ? active - left : active;
+    if constexpr (PART == GROUP_HEAD) hi = cut;
+    else lo = cut;
+  }
+  constexpr int Q = PART == GROUP_REST ? 4 : 1;
+  if (pid >= (hi - lo) * Q) return false;
+  const int sub = xcd_remap(pid, (hi - lo) * Q);
+  const int tile = lo + sub / Q;
   const bool mine = tile >= (upto - tiles) * tiles_n && tile < upto * tiles_n;
   int e = 0, row = 0, cnt = 0, first = 0;  // group, its first row, its rows, its first tile
   if (mine) {
@@ -139,16 +161,31 @@ __device__ __forceinline__ bool group_find_at(const int* __restrict__ offsets, i
   first = __builtin_amdgcn_readlane(first, src);
   int tm, tn;
   group_tile(tile - first, (cnt + BM - 1) / BM, tiles_n, 8, tm, tn);
+  constexpr int H = PART == GROUP_REST ? BM / 2 : BM;  // rows of this launch's tiles
+  const int r0 = tm * BM + (PART == GROUP_REST ? (sub & 1) * H : 0);
+  if (PART == GROUP_REST && r0 >= cnt) return false;
   out.e = e;
-  out.row = row + tm * BM;
-  out.rows = cnt - tm * BM < BM ? cnt - tm * BM : BM;
-  out.tn = tn;
+  out.row = row + r0;
+  out.rows = cnt - r0 < H ? cnt - r0 : H;
+  out.tn = PART == GROUP_REST ? 2 * tn + ((sub >> 1) & 1) : tn;
   return true;
 }
 
 template <int BM, typename P>
 __device__ __forceinline__ bool group_find(const P& p, GroupTile& out) {
-  return group_find_at<BM>(p.offsets, p.groups, p.rows, p.tiles_n, (int)blockIdx.x, out);
+  return group_find_at<BM, GROUP_ALL>(p.offsets, p.groups, p.rows, p.tiles_n, 0, (int)blockIdx.x, out);
+}
+// 256-row tiles: all of them, or HEAD where the launch is one of a pair.
+template <typename P>
+__device__ __forceinline__ bool group_find_head(const P& p, GroupTile& out) {
+  if (p.cus == 0) return group_find<256>(p, out);
+  return group_find_at<256, GROUP_HEAD>(p.offsets, p.groups, p.rows, p.tiles_n, p.cus, (int)blockIdx.x, out);
+}
+// 128-row tiles: all of them, or the quarters of what the 256-row launch left.
+template <typename P>
+__device__ __forceinline__ bool group_find_rest(const P& p, GroupTile& out) {
+  if (p.cus == 0) return group_find<128>(p, out);
+  return group_find_at<256, GROUP_REST>(p.offsets, p.groups, p.rows, p.tiles_n, p.cus, (int)blockIdx.x, out);
 }
 
 // Zeros to `rows` rows of C (leading dimension ld) in columns n0 .. n0 + width

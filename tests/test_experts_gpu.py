@@ -251,6 +251,75 @@ def test_grouped_any_offsets(dtype, off):
         check_bound(down(a), want, gemm_bound(want, m, 72, dtype))
 
 
+@pytest.mark.parametrize("dtype,R,N,K,ends", [
+    # more 256 x 256 tiles than CUs: a short last round (in 128 x 128 tiles), a
+    # long one, columns and rows that end inside a quarter, rows of no group
+    ("bfloat16", 4096, 8192, 2048, [709, 1275, 1795, 2489, 2882, 3289, 3511, 4096]),
+    ("float16", 4096, 8200, 2048, [10, 10, 2300, 4000]),
+    ("bfloat16", 5000, 7000, 1920, [1, 1500, 1500, 2871, 4100]),
+    ("bfloat16", 4100, 8192, 2048, [40 * i for i in range(1, 101)]),
+])
+def test_grouped_linear_many_tiles(dtype, R, N, K, ends):
+    g = cu()
+    rng = np.random.default_rng(R)
+    E, off = len(ends), np.array([0] + ends)
+    x = rnd(rng, (R, K), 1.0, dtype)
+    # each group's weight: one matrix with its rows rotated
+    base = rnd(rng, (N, K), K ** -0.5, dtype)
+    w = np.stack([np.roll(base, e, 0) for e in range(E)]) if E < 10 else np.stack([base[:, ::(-1) ** e] for e in range(E)])
+    b = rnd(rng, (E, N), 0.1, dtype)
+    rows = np.unique(np.clip(np.concatenate([off[:-1], off[1:] - 1, off[:-1] + 127, off[:-1] + 128, off[:-1] + 256,
+                                             rng.integers(0, R, 12), [R - 1]]), 0, R - 1))
+    xt, wt, ot = up(x, dtype), up(w, dtype), ints(off)
+    got = down(g.dev_grouped_linear(xt, wt, ot, up(b, dtype), "silu"))
+    group = np.searchsorted(off[1:], rows, side="right")
+    for r, e in zip(rows, group):
+        if e == E:
+            assert (got[r] == 0).all()
+            continue
+        y = x[r].astype(np.float64) @ w[e].astype(np.float64).T + b[e]
+        mag = np.abs(x[r]).astype(np.float64) @ np.abs(w[e]).astype(np.float64).T
+        check_bound(got[r], ox.act(y, "silu"), gemm_bound(ox.act(y, "silu"), mag, K, dtype, "silu"), "row %d" % r)
+    assert (got[off[-1]:] == 0).all()
+    # every row of the same group with the same input gives the same result
+    same_rows = np.zeros((R, K), np.float32) + x[0]
+    got = down(g.dev_grouped_linear(up(same_rows, dtype), wt, ot))
+    for e in range(E):
+        lo, hi = off[e], off[e + 1]
+        assert (got[lo:hi] == got[lo:lo + 1]).all()
+
+
+@pytest.mark.parametrize("dtype,R,N,K,ends", [
+    ("bfloat16", 4096, 2048, 8192, [709, 1275, 1795, 2489, 2882, 3289, 3511, 4096]),
+    ("float16", 3000, 2048, 8200, [0, 1100, 2900]),
+])
+def test_grouped_backward_many_tiles(dtype, R, N, K, ends):
+    g = cu()
+    rng = np.random.default_rng(R)
+    E, off = len(ends), np.array([0] + ends)
+    gr, x = rnd(rng, (R, N), 1.0, dtype), rnd(rng, (R, K), 1.0, dtype)
+    base = rnd(rng, (N, K), N ** -0.5, dtype)
+    w = np.stack([np.roll(base, e, 0) for e in range(E)])
+    dx, dw, db = (down(t) for t in g.dev_grouped_linear_backward(up(gr, dtype), up(x, dtype), up(w, dtype), ints(off)))
+    for r in np.unique(np.concatenate([off[off < R], off[1:] - 1, rng.integers(0, R, 8)])):
+        if r < 0:
+            continue
+        e = int(np.searchsorted(off[1:], r, side="right"))
+        if e == E:
+            assert (dx[r] == 0).all()
+            continue
+        g64, w64 = gr[r].astype(np.float64), w[e].astype(np.float64)
+        y, mag = g64 @ w64, np.abs(g64) @ np.abs(w64)
+        check_bound(dx[r], y, gemm_bound(y, mag, N, dtype), "dx row %d" % r)
+    for e in range(E):
+        ge, xe = gr[off[e]:off[e + 1]].astype(np.float64), x[off[e]:off[e + 1]].astype(np.float64)
+        for n in (0, 255, 256, N - 1, int(rng.integers(N))):
+            y, mag = ge[:, n] @ xe, np.abs(ge[:, n]) @ np.abs(xe)
+            check_bound(dw[e, n], y, gemm_bound(y, mag, max(1, len(ge)), dtype), "dw row %d" % n)
+        s = ge.sum(0)
+        check_bound(db[e], s, gemm_bound(s, np.abs(ge).sum(0), max(1, len(ge)), dtype), "db")
+
+
 @pytest.mark.parametrize("R,E,N,K", [(0, 3, 8, 8), (8, 0, 8, 8), (8, 2, 0, 8), (8, 2, 8, 0)])
 def test_grouped_empty(R, E, N, K):
     g = cu()
