@@ -103,16 +103,27 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(const void* __rest
   const int nt = rows - t0 < kRouteTokens ? rows - t0 : kRouteTokens;
   for (int e = tid; e < E; e += kRouteThreads) cnt[e] = 0;
   __syncthreads();
-  for (int t = wave; t < nt; t += kRouteThreads / 64) {
-    const int64_t row = t0 + t;
-    uint32_t key[CH];
-    float v[CH];
+  // all of this wave's tokens' logits are loaded ahead of the first one's work
+  constexpr int PER = kRouteTokens * 64 / kRouteThreads;
+  float all[PER][CH];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int t = wave + i * (kRouteThreads / 64);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int e = c * 64 + lane;
-      v[c] = e < E ? Chunk8<T>::get(logits, row * E + e) : -INFINITY;
-      key[c] = e < E ? order_key(v[c]) : 0;  // 0 is below the key of every number
+      all[i][c] = t < nt && e < E ? Chunk8<T>::get(logits, (int64_t)(t0 + t) * E + e) : -INFINITY;
     }
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int t = wave + i * (kRouteThreads / 64);
+    if (t >= nt) break;
+    const int64_t row = t0 + t;
+    const float(&v)[CH] = all[i];
+    uint32_t key[CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) key[c] = c * 64 + lane < E ? order_key(v[c]) : 0;  // 0 is below the key of every number
     uint32_t top = 0, val = 0;  // the largest key, and lane j's: the j-th
     int mine = 0;
     for (int j = 0; j < k; ++j) {
@@ -263,7 +274,8 @@ __global__ __launch_bounds__(256) void route_backward_kernel(const float* __rest
   }
   for (int j = 0; j < k; ++j) {  // the chosen experts, one lane each
     const int ej = __builtin_amdgcn_readlane(e, j);
-    const float gj = __shfl(g, j, 64), wj = __shfl(w, j, 64);
+    const float gj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(g), j));
+    const float wj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), j));
 #pragma unroll
     for (int c = 0; c < CH; ++c)
       if (c * 64 + lane == ej) out[c] = wj * (gj - dot);
