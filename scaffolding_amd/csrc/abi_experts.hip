@@ -139,7 +139,7 @@ extern "C" {
 
 int64_t sf_route_topk_work(int64_t tokens, int64_t experts) {
   const int64_t nb = tokens > 0 ? route_blocks(tokens) : 0;
-  return nb > 1 && experts > 0 ? nb * experts * 4 : 0;
+  return nb > 1 && experts > 0 ? (nb + 1) * experts * 4 : 0;
 }
 
 static int route_check(const char* name, int64_t tokens, int64_t experts, int64_t k, sf_dtype dtype) {
@@ -323,6 +323,7 @@ static int q4_check(const char* name, int64_t rows, int64_t groups, int64_t N, i
   int rc = grouped_check(name, rows, groups, N, K, dtype);
   if (rc != SF_OK) return rc;
   if (dtype == SF_F32) return fail(SF_ERR_UNSUPPORTED, "%s: scales and activations are F16 or BF16", name);
+  if (K >= (int64_t(1) << 25)) return fail(SF_ERR_UNSUPPORTED, "%s: K must be < 2^25", name);
   if (group != 32 && group != 64 && (group < 128 || group % 128 != 0))
     return fail(SF_ERR_UNSUPPORTED, "%s: group %lld is not 32, 64 or a multiple of 128", name, (long long)group);
   if (K % group != 0)

@@ -22,11 +22,14 @@ namespace sf {
 //   +  those in earlier waves of its block  +  those in earlier lanes,
 // all integer counts, so the places do not depend on which block or wave ran
 // first.  With several blocks the counts of each go to `counts` and a second
-// launch forms the sums; one block needs neither.
+// launch forms the sums; one block needs neither.  Past kRouteDirect blocks,
+// where every block summing all counts would cost the square of the tokens, a
+// launch in between turns the counts into sums over the earlier blocks.
 // ---------------------------------------------------------------------
 constexpr int kRouteTokens = 64;   // tokens per block
 constexpr int kRouteThreads = 1024;
 constexpr int kRouteMaxK = 16;
+constexpr int kRouteDirect = 512;  // blocks
 
 __device__ __forceinline__ uint32_t order_key(float f) {
   if (f != f) return 0xffffffffu;
@@ -178,10 +181,41 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(const void* __rest
   route_place(ex, nt * k, E, hist, first, slots);
 }
 
-// Second launch of several blocks: block b forms the sums over the blocks and
-// places its own assignments; block 0 writes the offsets.
+// counts[b][e] -> assignments of e in blocks before b, for the nb blocks, and
+// counts[nb][e] -> all of them.  A block takes 16 experts: 64 threads each, a
+// contiguous share of the blocks per thread, the shares' sums scanned by lane.
+__global__ __launch_bounds__(1024) void route_scan_kernel(int* __restrict__ counts, int nb, int E) {
+  __shared__ int sums[16][65];
+  const int q = threadIdx.x & 15, share = threadIdx.x >> 4;
+  const int e = blockIdx.x * 16 + q;
+  const int b0 = (int)((int64_t)nb * share / 64), b1 = (int)((int64_t)nb * (share + 1) / 64);
+  int sum = 0;
+  if (e < E)
+#pragma unroll 8
+    for (int b = b0; b < b1; ++b) sum += counts[(int64_t)b * E + e];
+  sums[q][share] = sum;
+  __syncthreads();
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int v = sums[wave][lane];
+  const int upto = wave_scan_sum(v);
+  sums[wave][lane] = upto - v;
+  if (lane == 63) sums[wave][64] = upto;
+  __syncthreads();
+  if (e >= E) return;
+  int run = sums[q][share];
+  for (int b = b0; b < b1; ++b) {
+    const int c = counts[(int64_t)b * E + e];
+    counts[(int64_t)b * E + e] = run;
+    run += c;
+  }
+  if (share == 0) counts[(int64_t)nb * E + e] = sums[q][64];
+}
+
+// Last launch of several blocks: block b places its own assignments, after
+// summing the blocks' counts if they are not sums already; block 0 writes the
+// offsets.
 __global__ __launch_bounds__(kRouteThreads) void route_place_kernel(const int* __restrict__ experts, int rows, int E,
-                                                                    int k, const int* __restrict__ counts,
+                                                                    int k, const int* __restrict__ counts, int summed,
                                                                     int* __restrict__ offsets,
                                                                     int* __restrict__ slots) {
   __shared__ int ex[kRouteTokens * kRouteMaxK];
@@ -194,25 +228,32 @@ __global__ __launch_bounds__(kRouteThreads) void route_place_kernel(const int* _
   const int nt = rows - t0 < kRouteTokens ? rows - t0 : kRouteTokens;
   const int64_t a0 = (int64_t)t0 * k;
   const int n = nt * k;
-  if (tid < n) ex[tid] = experts[a0 + tid];
-  for (int e = tid; e < E; e += kRouteThreads) before[e] = total[e] = 0;
-  __syncthreads();
-  // every thread sums a share of the blocks for one expert
   const int nb = gridDim.x;
-  const int lanes = E < kRouteThreads ? E : kRouteThreads;
-  const int shares = kRouteThreads / lanes;
-  const int share = tid / lanes;
-  if (share < shares) {
-    for (int e = tid % lanes; e < E; e += lanes) {
-      int sum = 0, pre = 0;
+  if (tid < n) ex[tid] = experts[a0 + tid];
+  if (summed) {
+    for (int e = tid; e < E; e += kRouteThreads) {
+      before[e] = counts[(int64_t)blockIdx.x * E + e];
+      total[e] = counts[(int64_t)nb * E + e];
+    }
+  } else {
+    for (int e = tid; e < E; e += kRouteThreads) before[e] = total[e] = 0;
+    __syncthreads();
+    // every thread sums a share of the blocks for one expert
+    const int lanes = E < kRouteThreads ? E : kRouteThreads;
+    const int shares = kRouteThreads / lanes;
+    const int share = tid / lanes;
+    if (share < shares) {
+      for (int e = tid % lanes; e < E; e += lanes) {
+        int sum = 0, pre = 0;
 #pragma unroll 8
-      for (int b = share; b < nb; b += shares) {
-        const int c = counts[(int64_t)b * E + e];
-        sum += c;
-        pre += b < (int)blockIdx.x ? c : 0;
+        for (int b = share; b < nb; b += shares) {
+          const int c = counts[(int64_t)b * E + e];
+          sum += c;
+          pre += b < (int)blockIdx.x ? c : 0;
+        }
+        atomicAdd(&total[e], sum);
+        atomicAdd(&before[e], pre);
       }
-      atomicAdd(&total[e], sum);
-      atomicAdd(&before[e], pre);
     }
   }
   __syncthreads();
@@ -304,7 +345,14 @@ static int launch_route_t(const void* logits, int64_t rows, int64_t E, int k, bo
 #undef SF_ROUTE
   int rc = check_launch("routing");
   if (rc != SF_OK || nb == 1) return rc;
-  hipLaunchKernelGGL(route_place_kernel, dim3(nb), dim3(kRouteThreads), 0, st, experts, r, e, k, work, offsets, slots);
+  const int summed = nb > kRouteDirect ? 1 : 0;
+  if (summed) {
+    hipLaunchKernelGGL(route_scan_kernel, dim3((e + 15) / 16), dim3(1024), 0, st, work, static_cast<int>(nb), e);
+    rc = check_launch("routing sums");
+    if (rc != SF_OK) return rc;
+  }
+  hipLaunchKernelGGL(route_place_kernel, dim3(nb), dim3(kRouteThreads), 0, st, experts, r, e, k, work, summed, offsets,
+                     slots);
   return check_launch("routing places");
 }
 
@@ -482,12 +530,14 @@ int launch_rows(int op, const void* x, const void* y, const int* slots, const fl
 //   silu'(x) = s (1 + x (1 - s)),  s = 1 / (1 + e^-x)
 //   gelu(x) = x s(z), s the logistic function of z = x (c0 + c1 x^2), so
 //   gelu'(x) = s + x s (1 - s) (c0 + 3 c1 x^2)
-// Past |x| = 20 both are 1 or 0 to the last bit; x is cut there so that
-// x s (1 - s) does not become inf * 0.
+// Past |x| = 80 (silu) and 10 (gelu) both are 1 or 0 in fp32, and short of
+// them e^-x and e^-z are finite; x is cut there, so that an infinite x does not
+// become inf * 0.  NaN passes.
 // ---------------------------------------------------------------------
 template <int ACT>
 __device__ __forceinline__ float act_slope(float t) {
-  const float x = t > 20.f ? 20.f : (t < -20.f ? -20.f : t);  // NaN passes
+  constexpr float top = ACT == ACT_SILU ? 80.f : 10.f;
+  const float x = t > top ? top : (t < -top ? -top : t);
   if constexpr (ACT == ACT_SILU) {
     const float s = fast_rcp(1.0f + fast_exp(-x));
     return s * __builtin_fmaf(x, 1.0f - s, 1.0f);

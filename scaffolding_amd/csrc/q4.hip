@@ -146,8 +146,9 @@ __global__ __launch_bounds__(NW * 64) void q4_kernel(Q4Params p) {
   const int nblk = none ? 0 : (K + 127) / 128;
   const int gstep = GB == 1 ? p.G / 128 : 1;  // blocks per scale group
   uint32_t mask = Q4Bits<T>::kMask, exp = Q4Bits<T>::kExp;
-  asm("" : "+s"(mask));
+  asm("" : "+v"(mask));
   asm("" : "+v"(exp));
+  mask = __builtin_amdgcn_readfirstlane(mask);
   const u32x4 ones = {Q4Bits<T>::kOnes, Q4Bits<T>::kOnes, Q4Bits<T>::kOnes, Q4Bits<T>::kOnes};
 
   // The tile's scales and zero points go through LDS as [scale row][column], as

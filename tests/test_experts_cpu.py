@@ -111,7 +111,7 @@ def test_route_refusals(lib, kw, code, text):
 def test_route_work(lib):
     assert lib.sf_route_topk_work(I64(0), I64(8)) == 0
     assert lib.sf_route_topk_work(I64(64), I64(8)) == 0
-    assert lib.sf_route_topk_work(I64(65), I64(8)) == 2 * 8 * 4
+    assert lib.sf_route_topk_work(I64(65), I64(8)) == 3 * 8 * 4
 
 
 @pytest.mark.parametrize("kw,code", [

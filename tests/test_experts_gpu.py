@@ -99,6 +99,40 @@ def test_route_ties_nan_and_infinities():
     assert (d[6] == 0).all() and (d[4] == 0).all()
 
 
+@pytest.mark.parametrize("T,E,k", [(32768, 5, 1), (40001, 37, 3), (33000, 1000, 2)])
+def test_route_many_tokens(T, E, k):
+    """More blocks than are summed by every block: places and offsets exact."""
+    g = cu()
+    v = rnd(np.random.default_rng(T), (T, E), 1.0, "bfloat16")
+    w, e, off, slots = (raw(t) for t in g.dev_route_topk(up(v, "bfloat16"), k))
+    want = np.argsort(-v.astype(np.float64), axis=1, kind="stable")[:, :k]
+    assert np.array_equal(e, want)
+    flat = want.reshape(-1)
+    place = np.empty(T * k, np.int64)
+    place[np.argsort(flat, kind="stable")] = np.arange(T * k)
+    assert np.array_equal(slots.reshape(-1), place)
+    assert np.array_equal(off, np.concatenate([[0], np.bincount(flat, minlength=E).cumsum()]))
+    assert np.allclose(w.sum(1), 1, atol=1e-6)
+
+
+@pytest.mark.parametrize("act,code", [("silu", 4), ("gelu", 5)])
+def test_activation_slopes_far_out(act, code):
+    g = cu()
+    lib = ctypes.CDLL(os.path.join(ROOT, "scaffolding_amd", "libsfgemm.so"))
+    v = np.array([0.0, -0.0, 1e-30, 5, -5, 9.9, -9.9, 10.1, -10.1, 30, -30, 79, -79, 81, -81, 1e30, -1e30, np.inf, -np.inf,
+                  np.nan], np.float32)
+    a, b = f32(np.ones_like(v)), f32(v)
+    out = g.empty(v.shape)
+    assert lib.sf_act_backward(P(a.data_ptr), P(b.data_ptr), P(out.data_ptr), I64(v.size), 0, code, None) == 0
+    got = raw(out)
+    fin = v[:-3].astype(np.float64)
+    with np.errstate(over="ignore", under="ignore", invalid="ignore"):
+        want = np.where(np.abs(fin) > 100, fin > 0, ox.act_slope(np.clip(fin, -100, 100), act))
+    # the exponential's argument is off by a few steps of |x| (c0 + c1 x^2 at gelu)
+    assert (np.abs(got[:-3] - want) <= 200 * 2.0 ** -24 * np.abs(want) + 4e-7).all()
+    assert got[-3] == 1 and abs(got[-2]) < 1e-30 and np.isnan(got[-1])
+
+
 def test_route_no_tokens_and_leading_shapes():
     g = cu()
     w, e, off, slots = g.dev_route_topk(g.empty((0, 5)), 2)

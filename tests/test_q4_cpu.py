@@ -58,6 +58,7 @@ def test_quantize_zero_groups_and_refusals():
     (dict(epi=6), -2, b"epilogue"), (dict(epi=1), -2, b"bias"), (dict(x=None), -2, b"null"), (dict(q=None), -2, b"null"),
     (dict(s=None), -2, b"null"), (dict(y=None), -2, b"null"), (dict(x=P(4104)), -3, b"aligned"),
     (dict(q=P(4097)), -3, b"aligned"), (dict(R=2 ** 31), -3, b"2^31"), (dict(R=2 ** 30), -3, b"tiles"),
+    (dict(K=2 ** 25), -3, b"2^25"),
 ])
 def test_refusals(lib, kw, code, text):
     d = dict(x=A, q=A, s=A, o=None, y=A, R=4, E=1, N=16, K=128, G=64, dt=2, epi=0)
