@@ -480,7 +480,8 @@ int sf_act_backward(const void* grad, const void* pre, void* out, int64_t n, sf_
  * unpacked integers are exact, scales and sums fp32, one rounding.  With
  * offsets (int32 [groups + 1], device) row m uses the weight of its group, as
  * sf_grouped_linear says, and bias is [groups, N]; without, groups is 1.
- * Meant for few rows per weight: each block of 64 reads the weight again. */
+ * Meant for few rows per weight: each block of 16 unpacks it again (from a few
+ * hundred on, sf_q4_expand and a 16-bit product are faster). */
 int sf_linear_q4(const void* x, const void* q, const void* scales, const void* zeros, const int32_t* offsets,
                  const void* bias, void* y, int64_t rows, int64_t groups, int64_t N, int64_t K, int64_t group,
                  sf_dtype dtype, sf_epilogue epi, void* stream);

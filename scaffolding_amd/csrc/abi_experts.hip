@@ -20,44 +20,75 @@ static void tile_size(int cfg, int& bm, int& bn) {
   }
 }
 
-// Estimated us of a grouped product on 256 x 256 tiles (one a CU and round)
-// and on 128 x 128 tiles (two a CU; the last of them by itself runs faster),
-// for groups that each leave half a tile.  Fitted to sweeps (bf16, us, 256 /
-// 128 measured): 8192 rows, 8 groups, K 1920 -> N 7680 282 / 298, 7680 -> 1920
-// 370 / 285; 4096 rows 164 / 176, 198 / 227; 2048 rows, 7680 -> 1920 201 / 125;
-// 16384 rows, 8 groups, 4096 -> 4096 520 / 625; 8192 rows, 64 groups, 2048 ->
-// 1408 129 / 111; 512 rows, 8 groups, 4096 -> 4096 101 / 73.
-static float big_us(int64_t rows, int64_t reached, int64_t N, int64_t K, int64_t cus) {
-  const int64_t tiles = (2 * rows + 256 * reached) / 512 * cdiv(N, 256);
-  return static_cast<float>(cdiv(tiles, cus)) * (12.4f + 0.0227f * static_cast<float>(K));
-}
-static float mid_us(int64_t rows, int64_t reached, int64_t N, int64_t K, int64_t cus) {
-  const int64_t tiles = (2 * rows + 128 * reached) / 256 * cdiv(N, 128);
-  const int64_t rem = tiles % (2 * cus);
-  const float rounds = static_cast<float>(tiles / (2 * cus)) + (rem == 0 ? 0.0f : (rem <= cus ? 0.65f : 1.0f));
-  return rounds * (2.6f + 0.018f * static_cast<float>(K));
+// Estimated us of a grouped product.  The sizes of the groups are on the
+// device: `rows` rows in `reached` groups, each leaving half a tile.
+//   256 x 256 tiles, one a CU and round: 12.4 us and 0.0227 us per k
+//   smaller ones: tau[r - 1] us per 64 k when r workgroups share each CU
+// Fitted to sweeps (bf16, us, 256 / 128 / 64 / 32 x 64 measured): 8192 rows, 8
+// groups, K 1920 -> N 7680 282 / 298 / 467 / 632; 4096 rows 164 / 176 / 252 /
+// 339; 1024 rows 67 / 85 / 89 / 110; dx of 2048 rows, 7680 -> 1920 201 / 125 /
+// 153; 16384 rows, 8 groups, 4096 -> 4096 520 / 625 / 967; 256 rows 99 / 71 / 61
+// / 59; 8192 rows, 64 groups, 2048 -> 1408 129 / 111 / 129 / 163.
+struct TileCost {
+  int cfg, bm, bn, occ;
+  float tau[4];
+};
+static constexpr TileCost kDirect[] = {
+    {TILE_MID_128, 128, 128, 2, {0.72f, 1.15f}},
+    {TILE_MID_64, 64, 64, 3, {0.32f, 0.44f, 0.74f}},
+    {TILE_MID_32, 32, 64, 3, {0.22f, 0.30f, 0.48f}},
+};
+// Register-staged loads (unaligned rows).
+static constexpr TileCost kStaged[] = {
+    {TILE_RAG_128, 128, 128, 2, {0.90f, 1.50f}},
+    {TILE_RAG_64, 64, 64, 4, {0.45f, 0.85f, 1.10f, 1.75f}},
+};
+
+static int64_t row_tiles(int64_t rows, int64_t reached, int64_t bm) {
+  const int64_t t = (2 * rows + bm * reached) / (2 * bm);
+  return t > reached ? t : reached;
 }
 
-// Tile of a grouped product whose `rows` rows fall into `reached` groups (the
-// sizes themselves are on the device; `per` rows each on average).  `vec`:
-// operands for the 16-byte direct loads; `dma`: for 4-byte ones (fp32).
+static float tile_us(const TileCost& c, int64_t rows, int64_t reached, int64_t N, int64_t K, int64_t cus) {
+  const int64_t tiles = row_tiles(rows, reached, c.bm) * cdiv(N, c.bn), slots = c.occ * cus;
+  float t = static_cast<float>(tiles / slots) * c.tau[c.occ - 1];
+  const int64_t rem = tiles % slots;
+  if (rem > 0) t += c.tau[cdiv(rem, cus) - 1];
+  return t * static_cast<float>(cdiv(K, 64));
+}
+
+// Tile of a grouped product.  `vec`: operands for the 16-byte direct loads;
+// `dma`: for 4-byte ones (fp32).
 static int rows_tile(int64_t rows, int64_t reached, int64_t N, int64_t K, bool vec, bool dma, bool f32,
                      bool b_kmajor) {
-  const int64_t per = rows / reached, cus = cu_count_current();
+  const int64_t cus = cu_count_current();
   if (f32) {
     if (!dma) return TILE_GENERIC;
     if (!vec) return TILE32_RAG;
     // as sf_gemm: few 64 x 64 tiles with a short k loop run as 16 x 32 blocks
-    // (64 rows, 4 groups, 512 -> 512: 17.6 us on 64 x 64 tiles, 6.0)
-    const int64_t t64 = (2 * rows + 64 * reached) / 128 * cdiv(N, 64);
+    // (64 rows, 4 groups, 512 -> 512: 17.6 us on 64 x 64 tiles, 6.8)
+    const int64_t t64 = row_tiles(rows, reached, 64) * cdiv(N, 64);
     return 4 * t64 <= cus && K <= 2048 ? TILE32_SMALL2 : TILE32_DMA;
   }
-  if (!vec) return per > 96 ? TILE_RAG_128 : TILE_RAG_64;
-  // 256 rows, 8 groups, 4096 -> 4096: 59 us on 32 x 64, 61 on 64 x 64, 71 on
-  // 128 x 128 (dx, which has no 32 x 64: 61, 63)
-  if (per <= 32) return b_kmajor ? TILE_MID_32 : TILE_MID_64;
-  const bool big = N > 128 && K % 128 == 0 && K >= 128;
-  return big && big_us(rows, reached, N, K, cus) <= mid_us(rows, reached, N, K, cus) ? TILE_NT_BIG : TILE_MID_128;
+  float best = 3.0e38f;
+  int cfg = -1;
+  if (vec && N > 128 && K % 128 == 0 && K >= 128) {
+    const int64_t tiles = row_tiles(rows, reached, 256) * cdiv(N, 256), rem = tiles % cus;
+    // a short last round runs as quarters (grouped_rows)
+    const float last = rem == 0 ? 0.0f : (tiles > cus && 2 * rem <= cus ? 0.7f : 1.0f);
+    best = (static_cast<float>(tiles / cus) + last) * (12.4f + 0.0227f * static_cast<float>(K));
+    cfg = TILE_NT_BIG;
+  }
+  for (int i = 0; i < (vec ? 3 : 2); ++i) {
+    const TileCost& c = vec ? kDirect[i] : kStaged[i];
+    if (c.cfg == TILE_MID_32 && !b_kmajor) continue;
+    const float us = tile_us(c, rows, reached, N, K, cus) + 5.0f;  // launch, first loads, epilogue
+    if (us < best) {
+      best = us;
+      cfg = c.cfg;
+    }
+  }
+  return cfg;
 }
 
 template <typename P>

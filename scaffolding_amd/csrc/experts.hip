@@ -463,17 +463,22 @@ __global__ __launch_bounds__(256) void combine_kernel(RowsParams p) {
   }
 }
 
-// drows[s] = w g[t], dw = <g[t], rows[s]>; a token's columns are shared by one
-// wave at most, so its sums are formed per thread and then over the lanes,
-// without a barrier (4096 x 2 rows of 1283 fp16: 16.8 us with a block of four
-// waves a token).
-template <typename T>
+// drows[s] = w g[t], dw = <g[t], rows[s]>.  A wave at most takes a token and
+// its slots one after the other, so its sums are formed per thread and then
+// over the lanes, without a barrier (4096 x 2 rows of 1283 fp16: 16.8 us with a
+// block of four waves a token, 14.0).  Where the tokens are too few for that to
+// fill the GPU (PAIR), a block takes one slot of one token and the waves' sums
+// are joined in their order (387 x 3 rows of 7360 bf16: 36 -> 12 us).
+template <typename T, bool PAIR>
 __global__ __launch_bounds__(256) void combine_backward_kernel(RowsParams p) {
-  const int64_t t = (int64_t)blockIdx.x * (256 >> p.lg) + (threadIdx.x >> p.lg);
+  __shared__ float part[4];
+  const int64_t item = (int64_t)blockIdx.x * (256 >> p.lg) + (threadIdx.x >> p.lg);
+  const int64_t t = PAIR ? item / p.k : item;
   const bool live = t < p.tokens;
   const int in = threadIdx.x & ((1 << p.lg) - 1);
   const int step = 8 << p.lg;
-  for (int j = 0; j < p.k; ++j) {
+  const int j0 = PAIR ? (int)(item % p.k) : 0, j1 = PAIR ? j0 + 1 : p.k;
+  for (int j = j0; j < j1; ++j) {
     const int s = live ? p.slots[t * p.k + j] : -1;
     float dot = 0.f;
     if ((uint64_t)(int64_t)s < (uint64_t)p.n) {
@@ -491,7 +496,14 @@ __global__ __launch_bounds__(256) void combine_backward_kernel(RowsParams p) {
         store_cols<T>(p.out, (int64_t)s * p.D + c, p.D - c, o);
       }
     }
-    for (int off = 1 << p.lg >> 1; off > 0; off >>= 1) dot += __shfl_xor(dot, off, 64);
+    for (int off = p.lg < 6 ? 1 << p.lg >> 1 : 32; off > 0; off >>= 1) dot += __shfl_xor(dot, off, 64);
+    if (PAIR && p.lg > 6) {  // uniform: the slot's columns are over several waves
+      if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = dot;
+      __syncthreads();
+      const int w0 = (threadIdx.x >> p.lg) << (p.lg - 6);
+      dot = 0.f;
+      for (int i = 0; i < 1 << (p.lg - 6); ++i) dot += part[w0 + i];
+    }
     if (live && in == 0) p.dw[t * p.k + j] = dot;
   }
 }
@@ -499,17 +511,20 @@ __global__ __launch_bounds__(256) void combine_backward_kernel(RowsParams p) {
 template <typename T>
 static int launch_rows_t(int op, RowsParams p, hipStream_t st) {
   // threads per token: enough for its columns, at most the block (the gradient:
-  // a wave)
+  // a wave, or the block for each of its slots)
+  const bool pair = op == 2 && p.tokens < 4096;
   int lg = 0;
-  while (lg < (op == 2 ? 6 : 8) && (8 << lg) < p.D) ++lg;
+  while (lg < (op == 2 && !pair ? 6 : 8) && (8 << lg) < p.D) ++lg;
   p.lg = lg;
   const int64_t per = 256 >> lg;
-  const int64_t nb = (p.tokens + per - 1) / per;
+  const int64_t items = pair ? p.n : p.tokens;
+  const int64_t nb = (items + per - 1) / per;
   if (nb > INT32_MAX) return fail(SF_ERR_UNSUPPORTED, "row exchange: too many tokens");
   const dim3 g(static_cast<unsigned>(nb));
   if (op == 0) hipLaunchKernelGGL((dispatch_kernel<T>), g, dim3(256), 0, st, p);
   else if (op == 1) hipLaunchKernelGGL((combine_kernel<T>), g, dim3(256), 0, st, p);
-  else hipLaunchKernelGGL((combine_backward_kernel<T>), g, dim3(256), 0, st, p);
+  else if (pair) hipLaunchKernelGGL((combine_backward_kernel<T, true>), g, dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((combine_backward_kernel<T, false>), g, dim3(256), 0, st, p);
   return check_launch("row exchange");
 }
 

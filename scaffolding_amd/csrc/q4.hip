@@ -27,9 +27,15 @@
 // 4 x 4 transpose of dwords between the lane groups (four lane swaps) first
 // makes dword d cover k = 32 d .. 32 d + 31.
 //
-// A workgroup of NW waves takes 16 NB weight rows and up to 16 MB rows of x;
-// the waves take the blocks of 128 k in turn, and their sums are joined
-// through LDS in wave order.
+// A workgroup of NW waves takes 16 NB weight rows and up to 16 rows of x (more
+// rows read the weight again, from the caches); the waves take the blocks of
+// 128 k in turn, and their sums are joined through LDS in wave order.
+//
+// What bounds it.  With few rows the weight's bytes come in at 4.0 TB/s (28672
+// x 8192, past the 256 MB cache: a copy that only loads the weight reaches
+// 5.2); small weights run at the launch and one memory latency (11008 x 4096,
+// 1 row: 7.8 us, of them 3.4 the launch).  With more rows it is the unpacking's
+// VALU work.
 #include "gemm16nt_pp.hpp"
 #include "grouped.hpp"
 #include "rowio.hpp"
@@ -100,12 +106,12 @@ __device__ __forceinline__ u32x4 lane_groups_transpose(u32x4 v) {
 
 // GB: scale groups per block of 128 k (1: G % 128 == 0; 2; 4).  U: blocks whose
 // loads a wave issues together.
-template <typename T, int NB, int MB, int NW, int U, int GB, bool ZEROS, bool GROUPED>
+template <typename T, int NB, int NW, int U, int GB, bool ZEROS, bool GROUPED>
 __global__ __launch_bounds__(NW * 64) void q4_kernel(Q4Params p) {
-  constexpr int BM = 16 * MB, BN = 16 * NB;
+  constexpr int BM = 16, BN = 16 * NB;
   constexpr int XP = 272;                        // bytes of a staged x row of 128 k: 16 rows on 16 bank groups
-  constexpr int XB = MB == 1 ? NW * 16 * XP : 0;  // staged x, one area per wave
-  constexpr int PB = NW * NB * 1024;             // the waves' partial sums of one row block
+  constexpr int XB = NW * 16 * XP;               // staged x, one area per wave
+  constexpr int PB = NW * NB * 1024;             // the waves' partial sums
   __shared__ __attribute__((aligned(16))) uint8_t area[XB > PB ? XB : PB];
   extern __shared__ __attribute__((aligned(16))) uint8_t dyn[];  // scales, then zero points
   const int lane = threadIdx.x & 63;
@@ -137,11 +143,9 @@ __global__ __launch_bounds__(NW * 64) void q4_kernel(Q4Params p) {
   const uint8_t* __restrict__ Z = ZEROS ? p.z + e * (int64_t)N * KG : nullptr;
   const uint16_t* __restrict__ X = p.x + (int64_t)row0 * K;
 
-  f32x4 sum[NB][MB];
+  f32x4 sum[NB];
 #pragma unroll
-  for (int i = 0; i < NB; ++i)
-#pragma unroll
-    for (int j = 0; j < MB; ++j) sum[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < NB; ++i) sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   const int nblk = none ? 0 : (K + 127) / 128;
   const int gstep = GB == 1 ? p.G / 128 : 1;  // blocks per scale group
@@ -197,22 +201,19 @@ __global__ __launch_bounds__(NW * 64) void q4_kernel(Q4Params p) {
   const __amdgpu_buffer_rsrc_t rx =
       __builtin_amdgcn_make_buffer_rsrc((void*)X, (short)0, none ? 0 : rows * K * 2, 0x00020000);
   constexpr uint32_t OOB = 0x80000000u;  // past every range
-  uint32_t vq[NB], vx[MB];
+  uint32_t vq[NB];
 #pragma unroll
   for (int i = 0; i < NB; ++i) vq[i] = (uint32_t)(16 * i + r16) * (uint32_t)(K / 2) + 16u * h;
-  // x of a single row block is loaded 16 bytes a lane, four rows of 128 k at a
-  // time, and put into MFMA order through the wave's LDS area: up to four rows
-  // take one load instruction a block (QX = 1) instead of four.  More row
-  // blocks are loaded in MFMA order straight away.
-#pragma unroll
-  for (int j = 0; j < MB; ++j)
-    vx[j] = MB == 1 ? (uint32_t)h * (uint32_t)K * 2u + 16u * r16
-                    : (uint32_t)(16 * j + r16) * (uint32_t)K * 2u + (GB == 1 ? 64u : 16u) * h;
-  uint8_t* const xw = area + (MB == 1 ? wave * 16 * XP : 0);
+  // x is loaded 16 bytes a lane, four rows of 128 k at a time, and put into MFMA
+  // order through the wave's LDS area: up to four rows take one load
+  // instruction a block (QX = 1), which is what a launch with few rows is bound
+  // by next to the weight's own (11008 x 4096, 1 row: 9.0 us with four, 7.8).
+  const uint32_t vx = (uint32_t)h * (uint32_t)K * 2u + 16u * r16;
+  uint8_t* const xw = area + wave * 16 * XP;
 
   auto run = [&](auto qx_c) {
     constexpr int QX = decltype(qx_c)::value;
-    u32x4 w[U][NB], xs[U][MB][4];
+    u32x4 w[U][NB], xs[U][4];
     auto load = [&](int b0, int last) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -221,16 +222,10 @@ __global__ __launch_bounds__(NW * 64) void q4_kernel(Q4Params p) {
         const bool tail = GB > 1 && k0 + 128 > K;      // uniform: a last block of 32, 64 or 96 k
         const int ks = gone ? 0 : k0;
 #pragma unroll
-        for (int j = 0; j < MB; ++j)
-#pragma unroll
-          for (int d = 0; d < QX; ++d) {
-            uint32_t o;
-            if constexpr (MB == 1)
-              o = gone || (tail && k0 + 8 * r16 >= K) ? OOB : vx[j] + (uint32_t)(4 * d * K) * 2u;
-            else  // the k of lane group h in dword d: 32 h + 8 d, or 32 d + 8 h
-              o = gone || (tail && k0 + 32 * d >= K) ? OOB : vx[j] + (GB == 1 ? 16u : 64u) * d;
-            xs[u][j][d] = __builtin_amdgcn_raw_buffer_load_b128(rx, o, ks * 2, 0);
-          }
+        for (int d = 0; d < QX; ++d) {
+          const uint32_t o = gone || (tail && k0 + 8 * r16 >= K) ? OOB : vx + (uint32_t)(4 * d * K) * 2u;
+          xs[u][d] = __builtin_amdgcn_raw_buffer_load_b128(rx, o, ks * 2, 0);
+        }
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
           const uint32_t o = gone || (tail && k0 + 32 * h >= K) ? OOB : vq[i];
@@ -243,24 +238,18 @@ __global__ __launch_bounds__(NW * 64) void q4_kernel(Q4Params p) {
       for (int u = 0; u < U; ++u) {
         const int blk = b0 + u * NW;
         if (u > 0 && blk >= last) break;  // uniform
-        if constexpr (MB == 1) {
-          // row 4 d + h, chunk r16 (8 k)
+        // row 4 d + h, chunk r16 (8 k)
 #pragma unroll
-          for (int d = 0; d < QX; ++d)
-            *reinterpret_cast<u32x4*>(xw + (4 * d + h) * XP + r16 * 16) = q4_order(xs[u][0][d]);
-          wave_lds_sync();
-          // rows past the last: any staged bytes (their outputs are not stored)
-          const int m = QX == 4 ? r16 : r16 & 3;
+        for (int d = 0; d < QX; ++d)
+          *reinterpret_cast<u32x4*>(xw + (4 * d + h) * XP + r16 * 16) = q4_order(xs[u][d]);
+        wave_lds_sync();
+        // rows past the last: any staged bytes (their outputs are not stored)
+        const int m = QX == 4 ? r16 : r16 & 3;
+        // the k of lane group h in dword d: 32 h + 8 d, or 32 d + 8 h
 #pragma unroll
-          for (int d = 0; d < 4; ++d)
-            xs[u][0][d] = *reinterpret_cast<const u32x4*>(xw + m * XP + (GB == 1 ? 4 * h + d : 4 * d + h) * 16);
-          wave_lds_sync();
-        } else {
-#pragma unroll
-          for (int j = 0; j < MB; ++j)
-#pragma unroll
-            for (int d = 0; d < 4; ++d) xs[u][j][d] = q4_order(xs[u][j][d]);
-        }
+        for (int d = 0; d < 4; ++d)
+          xs[u][d] = *reinterpret_cast<const u32x4*>(xw + m * XP + (GB == 1 ? 4 * h + d : 4 * d + h) * 16);
+        wave_lds_sync();
         if constexpr (GB > 1)
 #pragma unroll
           for (int i = 0; i < NB; ++i) w[u][i] = lane_groups_transpose(w[u][i]);
@@ -269,34 +258,24 @@ __global__ __launch_bounds__(NW * 64) void q4_kernel(Q4Params p) {
           constexpr int DG = 4 / GB;  // dwords per scale group
           const int kg = GB == 1 ? blk / gstep : blk * GB + gi;
           if (GB > 1 && kg >= KG) break;  // past K
-          f32x4 xsum[MB];
+          f32x4 xsum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int j = 0; j < MB; ++j) {
-            xsum[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int d = gi * DG; d < gi * DG + DG; ++d) xsum[j] = Mfma16<T>::run(ones, xs[u][j][d], xsum[j]);
-          }
+          for (int d = gi * DG; d < gi * DG + DG; ++d) xsum = Mfma16<T>::run(ones, xs[u][d], xsum);
 #pragma unroll
           for (int i = 0; i < NB; ++i) {
             const u32x2 sc = *reinterpret_cast<const u32x2*>(sS + (kg - kg0) * BN + 16 * i + 4 * h);
             uint32_t zp = 0;
             if constexpr (ZEROS) zp = *reinterpret_cast<const uint32_t*>(sZ + (kg - kg0) * BN + 16 * i + 4 * h);
-            f32x4 acc[MB];
+            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int j = 0; j < MB; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int d = gi * DG; d < gi * DG + DG; ++d) {
-              const u32x4 wf = q4_unpack<T>(w[u][i][d], mask, exp);
-#pragma unroll
-              for (int j = 0; j < MB; ++j) acc[j] = Mfma16<T>::run(wf, xs[u][j][d], acc[j]);
-            }
+            for (int d = gi * DG; d < gi * DG + DG; ++d)
+              acc = Mfma16<T>::run(q4_unpack<T>(w[u][i][d], mask, exp), xs[u][d], acc);
             // this lane's outputs are four columns of x row r16
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               const float s = Elem<T>::to_f32(static_cast<uint16_t>(sc[c >> 1] >> ((c & 1) * 16)));
               const float off = ZEROS ? 16.0f + (float)((zp >> (8 * c)) & 255u) : 24.0f;
-#pragma unroll
-              for (int j = 0; j < MB; ++j) sum[i][j][c] += s * __builtin_fmaf(-off, xsum[j][c], acc[j][c]);
+              sum[i][c] += s * __builtin_fmaf(-off, xsum[c], acc[c]);
             }
           }
         }
@@ -319,70 +298,66 @@ __global__ __launch_bounds__(NW * 64) void q4_kernel(Q4Params p) {
       }
     }
   };
-  if (MB == 1 && rows <= 4)
+  if (rows <= 4)
     run(std::integral_constant<int, 1>{});
   else
     run(std::integral_constant<int, 4>{});
 
-  // The waves' sums of one row block after the other through LDS, each column
-  // block i finished by wave i % NW.
+  // The waves' sums through LDS, column block i finished by wave i % NW.
   const bool has_bias = epi_has_bias(epi);
   const uint16_t* bias = has_bias ? static_cast<const uint16_t*>(p.bias) + e * N : nullptr;
   const bool yvec = (N & 3) == 0 && (reinterpret_cast<uintptr_t>(p.y) & 7) == 0;
   f32x4* const part = reinterpret_cast<f32x4*>(area);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < NB; ++i) part[(wave * NB + i) * 64 + lane] = sum[i];
+  __syncthreads();
   with_act(epi_act(epi), [&](auto act_c) {
     constexpr int ACT = decltype(act_c)::value;
 #pragma unroll
-    for (int j = 0; j < MB; ++j) {
-      __syncthreads();
+    for (int i = 0; i < NB; ++i) {
+      if (i % NW != wave) continue;
+      f32x4 v = part[i * 64 + lane];
 #pragma unroll
-      for (int i = 0; i < NB; ++i) part[(wave * NB + i) * 64 + lane] = sum[i][j];
-      __syncthreads();
+      for (int q = 1; q < NW; ++q) v += part[(q * NB + i) * 64 + lane];
+      const int n = n0 + 16 * i + 4 * h;
+      if (r16 >= rows || n >= N) continue;
+      float o[4];
 #pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        if (i % NW != wave) continue;
-        f32x4 v = part[i * 64 + lane];
+      for (int c = 0; c < 4; ++c) {
+        o[c] = v[c];
+        if (has_bias && n + c < N) o[c] += Elem<T>::to_f32(bias[n + c]);
+        o[c] = act_t<ACT>(o[c]);
+      }
+      uint16_t* y = p.y + (int64_t)(row0 + r16) * N + n;
+      if (yvec) {
+        *reinterpret_cast<u32x2*>(y) = u32x2{pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3])};
+      } else {
 #pragma unroll
-        for (int q = 1; q < NW; ++q) v += part[(q * NB + i) * 64 + lane];
-        const int m = 16 * j + r16, n = n0 + 16 * i + 4 * h;
-        if (m >= rows || n >= N) continue;
-        float o[4];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          o[c] = v[c];
-          if (has_bias && n + c < N) o[c] += Elem<T>::to_f32(bias[n + c]);
-          o[c] = act_t<ACT>(o[c]);
-        }
-        uint16_t* y = p.y + (int64_t)(row0 + m) * N + n;
-        if (yvec) {
-          *reinterpret_cast<u32x2*>(y) = u32x2{pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3])};
-        } else {
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            if (n + c < N) y[c] = Elem<T>::from_f32(o[c]);
-        }
+        for (int c = 0; c < 4; ++c)
+          if (n + c < N) y[c] = Elem<T>::from_f32(o[c]);
       }
     }
   });
 }
 
-template <typename T, int NB, int MB, int NW, int U, int GB>
+template <typename T, int NB, int NW, int U, int GB>
 static void launch_q4_gz(const Q4Params& p, const dim3& g, unsigned lds, hipStream_t st) {
   if (p.offsets != nullptr) {
-    if (p.z != nullptr) hipLaunchKernelGGL((q4_kernel<T, NB, MB, NW, U, GB, true, true>), g, dim3(NW * 64), lds, st, p);
-    else hipLaunchKernelGGL((q4_kernel<T, NB, MB, NW, U, GB, false, true>), g, dim3(NW * 64), lds, st, p);
+    if (p.z != nullptr) hipLaunchKernelGGL((q4_kernel<T, NB, NW, U, GB, true, true>), g, dim3(NW * 64), lds, st, p);
+    else hipLaunchKernelGGL((q4_kernel<T, NB, NW, U, GB, false, true>), g, dim3(NW * 64), lds, st, p);
   } else {
-    if (p.z != nullptr) hipLaunchKernelGGL((q4_kernel<T, NB, MB, NW, U, GB, true, false>), g, dim3(NW * 64), lds, st, p);
-    else hipLaunchKernelGGL((q4_kernel<T, NB, MB, NW, U, GB, false, false>), g, dim3(NW * 64), lds, st, p);
+    if (p.z != nullptr) hipLaunchKernelGGL((q4_kernel<T, NB, NW, U, GB, true, false>), g, dim3(NW * 64), lds, st, p);
+    else hipLaunchKernelGGL((q4_kernel<T, NB, NW, U, GB, false, false>), g, dim3(NW * 64), lds, st, p);
   }
 }
 
-template <typename T, int NB, int MB, int NW, int U>
+template <typename T, int NB, int NW, int U>
 static int launch_q4_g(Q4Params p, hipStream_t st) {
   p.tiles_n = (p.N + 16 * NB - 1) / (16 * NB);
   int64_t gx = p.tiles_n, gy = 1;
-  if (p.offsets != nullptr) gx *= grouped_max_tiles(p.rows, p.groups, 16 * MB);
-  else gy = (p.rows + 16 * MB - 1) / (16 * MB);
+  if (p.offsets != nullptr) gx *= grouped_max_tiles(p.rows, p.groups, 16);
+  else gy = (p.rows + 15) / 16;
   if (gx > (int64_t(1) << 22) || gy > 65535) return fail(SF_ERR_UNSUPPORTED, "sf_linear_q4: too many tiles");
   const int row = 16 * NB * (p.z != nullptr ? 3 : 2);  // LDS bytes of a scale row
   const int fit = kQ4ScaleBytes / row / 4 * 4;
@@ -390,34 +365,37 @@ static int launch_q4_g(Q4Params p, hipStream_t st) {
   if (p.sg < 1) p.sg = 1;
   const unsigned lds = static_cast<unsigned>((p.sg + 3) / 4 * 4 * row);
   const dim3 g(static_cast<unsigned>(gx), static_cast<unsigned>(gy));
-  if (p.G % 128 == 0) launch_q4_gz<T, NB, MB, NW, U, 1>(p, g, lds, st);
-  else if (p.G == 64) launch_q4_gz<T, NB, MB, NW, U, 2>(p, g, lds, st);
-  else launch_q4_gz<T, NB, MB, NW, U, 4>(p, g, lds, st);
+  if (p.G % 128 == 0) launch_q4_gz<T, NB, NW, U, 1>(p, g, lds, st);
+  else if (p.G == 64) launch_q4_gz<T, NB, NW, U, 2>(p, g, lds, st);
+  else launch_q4_gz<T, NB, NW, U, 4>(p, g, lds, st);
   return check_launch("4-bit linear");
 }
 
-// Variants by rows per weight (their mean where the sizes are on the device)
-// and by how many column tiles there are to share out.  Measured in us, bf16,
-// groups of 128 (28672 x 8192 x 4 rows, 11008 x 4096 x 1, 4096 x 11008 x 1,
-// 4096 x 4096 x 1, 8 experts 11008 x 4096 x 16 rows, 11008 x 4096 x 32, x 64,
-// x 128):
-//   32 columns, 4 waves     29.1   8.1  15.0  6.8  37.0  12.0  20.3
-//   32 columns, 8 waves     29.7   7.8  10.4  5.6  40.6  12.2  20.8
+// Variants by how many tiles of 16 rows and 32 columns there are to share out
+// (rows per weight: their mean where the sizes are on the device), and 64
+// columns a tile once the rows of a weight fill more than two.  Measured in us,
+// bf16, groups of 128 (28672 x 8192 x 4 rows, 11008 x 4096 x 1, 4096 x 11008 x
+// 1, 4096 x 4096 x 1, 8 experts 11008 x 4096 x 16 rows, 11008 x 4096 x 32, x
+// 64, x 256, 4096 x 11008 x 48, x 128):
 //   16 columns, 8 waves     33.1   7.7   8.6  4.1  52.0  15.5  26.9
 //   16 columns, 16 waves    33.5   8.9   7.3  4.4  79.6  17.7  30.0
-//   64 columns, 4 waves     30.0   9.6  20.2  9.0  38.8  13.5  19.1
-//   64 columns x 32 rows, 4 waves                        15.4  25.6  37.5
+//   32 columns, 4 waves     29.1   8.1  15.0  6.8  37.0  12.0  20.3
+//   32 columns, 8 waves     29.7   7.8  10.4  5.6  40.6  12.2  20.8  74.5  24.9  45.7
+//   64 columns, 4 waves     30.0   9.6  20.2  9.0  38.8  13.5  19.1  60.7  38.9  49.3
+//   64 columns, 8 waves     29.5   8.1  14.8  7.6  39.6  13.5  19.3  65.8  26.1  39.2
+// (32 and 64 rows a tile, the weight unpacked once for them, were slower at
+// every size: 11008 x 4096 x 64 23.9 us at best, x 256 62.5.)
 template <typename T>
 static int launch_q4_t(const Q4Params& p, hipStream_t st) {
   const int64_t reached = p.offsets == nullptr ? 1 : (p.groups < p.rows ? p.groups : p.rows);
-  const int64_t per = p.rows / reached;
-  if (per > 64) return launch_q4_g<T, 4, 2, 4, 1>(p, st);
-  if (per > 32) return launch_q4_g<T, 4, 1, 4, 1>(p, st);
-  const int64_t tiles = (p.N + 31) / 32 * reached * ((per + 15) / 16);
+  const int64_t per = p.rows / reached, blocks = reached * ((per + 15) / 16);
   const int64_t cus = cu_count_current();
-  if (tiles >= 2 * cus) return launch_q4_g<T, 2, 1, 4, 1>(p, st);
-  if (tiles >= cus) return launch_q4_g<T, 2, 1, 8, 1>(p, st);
-  return p.K >= 8192 ? launch_q4_g<T, 1, 1, 16, 1>(p, st) : launch_q4_g<T, 1, 1, 8, 1>(p, st);
+  if (per > 32 && 2 * blocks * ((p.N + 63) / 64) >= 3 * cus)
+    return p.K >= 8192 ? launch_q4_g<T, 4, 8, 1>(p, st) : launch_q4_g<T, 4, 4, 1>(p, st);
+  const int64_t tiles = blocks * ((p.N + 31) / 32);
+  if (tiles >= 2 * cus) return launch_q4_g<T, 2, 4, 1>(p, st);
+  if (tiles >= cus) return launch_q4_g<T, 2, 8, 1>(p, st);
+  return p.K >= 8192 ? launch_q4_g<T, 1, 16, 1>(p, st) : launch_q4_g<T, 1, 8, 1>(p, st);
 }
 
 int launch_q4(const void* x, const void* q, const void* s, const void* z, const void* bias, void* y,
