@@ -15,7 +15,8 @@ static void tile_size(int cfg, int& bm, int& bn) {
     case TILE_MID_128:
     case TILE_RAG_128: bm = bn = 128; return;
     case TILE_MID_32: bm = 32; bn = 64; return;
-    case TILE32_SMALL2: bm = 16; bn = 32; return;
+    case TILE32_SMALL2:
+    case TILE32_SMALL2_ANY: bm = 16; bn = 32; return;
     default: bm = bn = 64; return;
   }
 }
@@ -63,12 +64,20 @@ static int rows_tile(int64_t rows, int64_t reached, int64_t N, int64_t K, bool v
                      bool b_kmajor) {
   const int64_t cus = cu_count_current();
   if (f32) {
-    if (!dma) return TILE_GENERIC;
-    if (!vec) return TILE32_RAG;
-    // as sf_gemm: few 64 x 64 tiles with a short k loop run as 16 x 32 blocks
-    // (64 rows, 4 groups, 512 -> 512: 17.6 us on 64 x 64 tiles, 6.8)
+    // 64 x 64 tiles, a round of one a CU: 0.0178 us per k (0.023 by 4-byte
+    // loads); 16 x 32 blocks, n a CU: 0.0065 n us per k, 0.008 n by shorter
+    // loads, 0.9 of one at least.  Fitted to sweeps (us, tiles / blocks):
+    // 3 rows, 5632 -> 195 100 / 29; 64 rows, 8 groups, 2048 -> 2048 42 / 31; 128
+    // rows 42 / 44; 512 rows 71 / 113; 64 groups, 1024 -> 1024, 256 rows 81 / 68;
+    // 1024 rows 83 / 97; 4-byte loads, 8 rows, 8 groups, 4095 -> 4095 171 / 102;
+    // 512 rows, 1 group, 1023 -> 1021 29 / 34.  (n < 4096 keeps the grid small.)
+    const float cu = static_cast<float>(cus);
     const int64_t t64 = row_tiles(rows, reached, 64) * cdiv(N, 64);
-    return 4 * t64 <= cus && K <= 2048 ? TILE32_SMALL2 : TILE32_DMA;
+    const float n = static_cast<float>(row_tiles(rows, reached, 16) * cdiv(N, 32)) / cu;
+    const float big = (vec ? 0.0178f : 0.023f) * static_cast<float>(cdiv(t64, cus));
+    if ((vec && b_kmajor ? 0.0065f : 0.008f) * (n > 0.9f ? n : 0.9f) < big && n < 4096.0f)
+      return vec ? TILE32_SMALL2 : TILE32_SMALL2_ANY;
+    return vec ? TILE32_DMA : dma ? TILE32_RAG : TILE_GENERIC;
   }
   float best = 3.0e38f;
   int cfg = -1;

@@ -24,11 +24,24 @@
 #pragma once
 
 #include "gemm32.hpp"
+#include "gemm32dma.hpp"
 
 namespace sf {
 
-// Prm: GemmParams, or grouped.hpp's GroupedRows.
-template <int FS, bool B_KMAJOR, int KW, typename Prm = GemmParams>
+// Four floats of a row from k on, zeros past K, at any 4-byte alignment.
+__device__ __forceinline__ f32x4 load4_any(const float* row, int k, int K) {
+  if (k + 4 <= K) return reinterpret_cast<const Float4u*>(row + k)->v;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int s = 0; s < 3; ++s)
+    if (k + s < K) v[s] = row[k + s];
+  return v;
+}
+
+// Prm: GemmParams, or grouped.hpp's GroupedRows.  ANY: any K and any row
+// alignment of a float (3 rows, 5633 -> 195: 130 us on 64 x 64 tiles by 4-byte
+// loads, 31 here).
+template <int FS, bool B_KMAJOR, int KW, typename Prm = GemmParams, bool ANY = false>
 __global__ __launch_bounds__(KW * 64) void gemm32small_kernel(Prm p) {
   constexpr int U = 4;  // 16-k steps per batch of loads
   const int tid = threadIdx.x;
@@ -81,14 +94,19 @@ __global__ __launch_bounds__(KW * 64) void gemm32small_kernel(Prm p) {
     for (int u = 0; u < U; ++u) {
       const int k = (st + u) * 16 + 4 * g;
       const bool ok = st + u < s1 && k < K;
-      a[u] = ok ? *reinterpret_cast<const f32x4*>(arow + k) : f32x4{0.f, 0.f, 0.f, 0.f};
+      if constexpr (ANY)
+        a[u] = st + u < s1 ? load4_any(arow, k, K) : f32x4{0.f, 0.f, 0.f, 0.f};
+      else
+        a[u] = ok ? *reinterpret_cast<const f32x4*>(arow + k) : f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < FS; ++i) {
-        if constexpr (B_KMAJOR) {
+        if constexpr (ANY && B_KMAJOR) {
+          x[u][i] = st + u < s1 ? load4_any(bptr[i], k, K) : f32x4{0.f, 0.f, 0.f, 0.f};
+        } else if constexpr (B_KMAJOR) {
           x[u][i] = ok ? *reinterpret_cast<const f32x4*>(bptr[i] + k) : f32x4{0.f, 0.f, 0.f, 0.f};
         } else {
 #pragma unroll
-          for (int s = 0; s < 4; ++s) x[u][i][s] = ok ? bptr[i][(int64_t)(k + s) * p.ldb] : 0.f;
+          for (int s = 0; s < 4; ++s) x[u][i][s] = ok && (!ANY || k + s < K) ? bptr[i][(int64_t)(k + s) * p.ldb] : 0.f;
         }
       }
     }

@@ -14,6 +14,9 @@ static int launch_rows_t(int cfg, const GroupedRows& p, const dim3& g, hipStream
     case TILE32_SMALL2:
       hipLaunchKernelGGL((gemm32small_kernel<2, KM, 8, GroupedRows>), g, dim3(512), 0, st, p);
       break;
+    case TILE32_SMALL2_ANY:
+      hipLaunchKernelGGL((gemm32small_kernel<2, KM, 8, GroupedRows, true>), g, dim3(512), 0, st, p);
+      break;
     case TILE32_DMA:
       hipLaunchKernelGGL((gemm32dma_kernel<64, 64, true, KM, 2, 2, 4, true, GroupedRows>), g, dim3(512), 0, st, p);
       break;

@@ -63,7 +63,8 @@ enum TileCfg {
   TILE_RAG_64 = 18,    // 64x64, likewise
   // fp32, operands at any 4-byte alignment (gemm32dma.hpp with 4-byte loads):
   TILE32_RAG = 19,       // as TILE32_DMA
-  TILE32_RAG_SPLIT = 20  // as TILE32_DMA_SPLIT
+  TILE32_RAG_SPLIT = 20,  // as TILE32_DMA_SPLIT
+  TILE32_SMALL2_ANY = 21  // as TILE32_SMALL2, rows of any alignment (grouped products)
 };
 const char* tile_name(int cfg);
 // Plans that sf_gemm_plan calls "split" rather than "split-tail".

@@ -212,6 +212,10 @@ CASES = [
     ("bfloat16", 900, 7, 256, 384, "one", None), ("bfloat16", 1500, 4, 520, 1, "any", None),
     ("bfloat16", 1500, 2, 512, 256, "any", "gelu"), ("float16", 2100, 3, 700, 128, "behind", None),
     ("bfloat16", 40, 1, 96, 4104, "any", None), ("float16", 3, 3, 1, 1, "any", None),
+    # few rows and a long sum, then 64 x 64 tiles, rows of four floats and others
+    ("float32", 3, 1, 195, 5632, "any", None), ("float32", 70, 3, 260, 4099, "any", "gelu"),
+    ("float32", 40, 9, 1027, 517, "behind", "silu"), ("float32", 1500, 3, 512, 640, "any", None),
+    ("float32", 1500, 3, 515, 700, "behind", "silu"), ("float32", 2000, 2, 600, 70, "any", None),
 ]
 
 
