@@ -477,7 +477,9 @@ int sf_act_backward(const void* grad, const void* pre, void* out, int64_t n, sf_
  * and x 16-byte aligned. */
 
 /* y[m, :] = epi(w x[m, :] (+ bias)) for `rows` rows of x [rows, K]; the
- * unpacked integers are exact, scales and sums fp32, one rounding.  With
+ * unpacked integers are exact, scales and sums fp32, one rounding.  The sums
+ * run over x (16 + w's integer) and take 16 x out again, so an infinite x (or
+ * one past 2^122) makes its row NaN.  With
  * offsets (int32 [groups + 1], device) row m uses the weight of its group, as
  * sf_grouped_linear says, and bias is [groups, N]; without, groups is 1.
  * Meant for few rows per weight: each block of 16 unpacks it again (from a few

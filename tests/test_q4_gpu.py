@@ -115,6 +115,20 @@ def test_known_values():
         assert np.array_equal(got, ox.q4_weight(q, s).T)
 
 
+def test_values_that_are_not_finite_stay_in_their_row():
+    g = cu()
+    rng = np.random.default_rng(4)
+    x = rnd(rng, (19, 256), 1.0, "bfloat16")
+    q, s, z = weight(rng, (), 40, 256, 64, "bfloat16", True)
+    w = ox.q4_weight(q, s, z)
+    x[3, 7], x[17, 200] = np.nan, np.inf
+    got = down(g.dev_linear_q4(up(x, "bfloat16"), *device(q, s, z, "bfloat16")))
+    assert np.isnan(got[[3, 17]]).all()
+    rest = np.delete(np.arange(19), [3, 17])
+    y = x[rest].astype(np.float64) @ w.T
+    check_bound(got[rest], y, bound(x[rest], w, y, s, "bfloat16"))
+
+
 def test_no_rows_and_shapes():
     g = cu()
     q, s = raw(np.zeros((8, 32)), np.uint8), up(np.ones((1, 8)), "bfloat16")
@@ -128,8 +142,7 @@ def test_large_activations_keep_their_sums():
     out of sums 5 times the result's."""
     g = cu()
     rng = np.random.default_rng(2)
-    x = np.full((4, 4096), 1.0, np.float32) + np.abs(rnd(rng, (4, 4096), 0.25, "float16"))
-    x = rnd(rng, (4, 4096), 0.0, "float16") + x.astype(np.float16).astype(np.float32)
+    x = (1.0 + 0.25 * rng.random((4, 4096))).astype(np.float16).astype(np.float32)
     q, s, z = weight(rng, (), 64, 4096, 128, "float16", True)
     w = ox.q4_weight(q, s, z)
     y = x.astype(np.float64) @ w.T
