@@ -403,7 +403,7 @@ int sf_cast(const void* x, sf_dtype in_dtype, void* y, sf_dtype out_dtype,
  *   offsets  int32 [experts + 1]: the assignments (t, j) ordered by expert,
  *            within one by t k + j; expert e's are [offsets[e], offsets[e+1])
  *   slots    int32 [tokens, k]: the place of (t, j) in that order
- * 1 <= k <= min(experts, 16), experts <= 1024, tokens * k < 2^31.  `work`:
+ * 1 <= k <= min(experts, 16), experts <= 1024, tokens < 2^26.  `work`:
  * sf_route_topk_work bytes of 4-byte aligned device memory, overwritten (may
  * be NULL where that is 0).  tokens == 0 writes zeros to offsets. */
 int64_t sf_route_topk_work(int64_t tokens, int64_t experts);
@@ -427,7 +427,8 @@ int sf_route_topk_backward(const float* grad_weights, const void* logits, const 
  *                      (the gradient of sf_dispatch_rows)
  *   sf_combine_rows_backward   grad_rows[slots[t, j]] = weights[t, j] grad[t],
  *                      grad_weights[t, j] = <grad[t], rows[slots[t, j]]>
- * k >= 1, cols < 2^31. */
+ * k >= 1, tokens * k < 2^31, cols <= 2^30, and fewer than 2^24 blocks of 256
+ * threads (8 columns each, at most a block a row). */
 int sf_dispatch_rows(const void* x, const int32_t* slots, void* rows, int64_t tokens, int64_t k, int64_t cols,
                      sf_dtype dtype, void* stream);
 int sf_combine_rows(const void* rows, const int32_t* slots, const float* weights, void* y, int64_t tokens, int64_t k,
@@ -445,7 +446,7 @@ int sf_combine_rows_backward(const void* grad, const void* rows, const int32_t* 
  * read on the device, so a router's offsets need not reach the host.  (For
  * other contents of offsets: group e ends at the largest of offsets[1..e+1],
  * cut to [0, rows], and starts where the group before it ends.)
- * groups <= 1024, rows < 2^31. */
+ * groups <= 1024; rows, N and K <= 2^30; at most 2^22 tiles. */
 int sf_grouped_linear(const void* x, const void* W, const int32_t* offsets, const void* bias, void* y, int64_t rows,
                       int64_t groups, int64_t N, int64_t K, sf_dtype dtype, sf_epilogue epi, void* stream);
 /* Its gradients (epi NONE or BIAS): grad_x[r] = W[e]^T grad[r], 0 for rows of

@@ -1454,9 +1454,9 @@ def dev_linear_q4(gt_x, gt_q, gt_scales, gt_zeros=None, gt_bias=None, activation
     N) or None for 8; b (N,).  G = K / scales' rows is 32, 64 or a multiple of
     128.  With offsets (int32 (E + 1,), see dev_grouped_linear) q, scales,
     zeros and b have a leading E and x is (R, K).  Sums are fp32 over exact
-    integers (an infinite x makes its row NaN); from 384 rows per weight on, W is first rounded to x's dtype
-    (half a step of each weight, as a 16-bit copy of W has) and the 16-bit
-    products run."""
+    integers (an infinite x makes its row NaN); from 384 rows per weight on, W
+    is first rounded to x's dtype (half a step of each weight, as a 16-bit copy
+    of W has) and the 16-bit products run."""
     name = 'dev_linear_q4'
     xs, qs = tuple(gt_x.shape), tuple(gt_q.shape)
     lead = 0 if gt_offsets is None else 1

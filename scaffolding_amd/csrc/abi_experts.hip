@@ -123,8 +123,9 @@ static int grouped_check(const char* name, int64_t rows, int64_t groups, int64_t
   if (!known(dtype)) return fail(SF_ERR_INVALID_ARG, "%s: unknown dtype %d", name, (int)dtype);
   if (rows < 0 || groups < 0 || N < 0 || K < 0) return fail(SF_ERR_INVALID_ARG, "%s: negative size", name);
   if (groups > kMaxGroups) return fail(SF_ERR_UNSUPPORTED, "%s: %lld groups (at most %d)", name, (long long)groups, kMaxGroups);
-  if (rows >= INT32_MAX || N >= INT32_MAX || K >= INT32_MAX)
-    return fail(SF_ERR_UNSUPPORTED, "%s: sizes must be < 2^31 - 1", name);
+  constexpr int64_t most = int64_t(1) << 30;
+  if (rows > most || N > most || K > most)
+    return fail(SF_ERR_UNSUPPORTED, "%s: sizes must be at most 2^30 (tiles past them stay below 2^31)", name);
   return SF_OK;
 }
 
@@ -192,6 +193,8 @@ static int route_check(const char* name, int64_t tokens, int64_t experts, int64_
                 route_max_k(), (long long)experts, (long long)k);
   if (tokens * k >= INT32_MAX || tokens >= INT32_MAX)
     return fail(SF_ERR_UNSUPPORTED, "%s: tokens * k must be < 2^31 - 1", name);
+  if (tokens >= int64_t(1) << 26)  // 64 threads a token, in a grid of fewer than 2^32
+    return fail(SF_ERR_UNSUPPORTED, "%s: tokens must be < 2^26", name);
   return SF_OK;
 }
 
@@ -231,6 +234,7 @@ static int rows_check(const char* name, int64_t tokens, int64_t k, int64_t cols,
                 (long long)tokens, (long long)k, (long long)cols);
   if (tokens >= INT32_MAX || k >= INT32_MAX || cols >= INT32_MAX || tokens * k >= INT32_MAX)
     return fail(SF_ERR_UNSUPPORTED, "%s: tokens * k and cols must be < 2^31 - 1", name);
+  if (cols > int64_t(1) << 30) return fail(SF_ERR_UNSUPPORTED, "%s: cols must be at most 2^30", name);
   return SF_OK;
 }
 

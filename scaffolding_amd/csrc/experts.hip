@@ -519,7 +519,7 @@ static int launch_rows_t(int op, RowsParams p, hipStream_t st) {
   const int64_t per = 256 >> lg;
   const int64_t items = pair ? p.n : p.tokens;
   const int64_t nb = (items + per - 1) / per;
-  if (nb > INT32_MAX) return fail(SF_ERR_UNSUPPORTED, "row exchange: too many tokens");
+  if (nb >= int64_t(1) << 24) return fail(SF_ERR_UNSUPPORTED, "row exchange: too many tokens of this width");
   const dim3 g(static_cast<unsigned>(nb));
   if (op == 0) hipLaunchKernelGGL((dispatch_kernel<T>), g, dim3(256), 0, st, p);
   else if (op == 1) hipLaunchKernelGGL((combine_kernel<T>), g, dim3(256), 0, st, p);
@@ -641,6 +641,7 @@ __global__ __launch_bounds__(1024) void group_colsum_kernel(const void* __restri
 
 int launch_group_colsum(const void* g, const int* offsets, int64_t rows, int64_t groups, int64_t N, void* out,
                         sf_dtype dt, hipStream_t st) {
+  if (N > int64_t(1) << 28) return fail(SF_ERR_UNSUPPORTED, "group column sums: more than 2^28 columns");
   const dim3 grid(static_cast<unsigned>((N + 127) / 128), static_cast<unsigned>(groups));
   const int r = static_cast<int>(rows);
   switch (dt) {

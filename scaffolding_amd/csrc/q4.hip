@@ -387,7 +387,8 @@ static int launch_q4_g(Q4Params p, hipStream_t st) {
 // every size: 11008 x 4096 x 64 23.9 us at best, x 256 62.5.)
 template <typename T>
 static int launch_q4_t(const Q4Params& p, hipStream_t st) {
-  const int64_t reached = p.offsets == nullptr ? 1 : (p.groups < p.rows ? p.groups : p.rows);
+  const int64_t some = p.groups < p.rows ? p.groups : p.rows;
+  const int64_t reached = p.offsets == nullptr || some < 1 ? 1 : some;  // no groups: all rows are set to 0
   const int64_t per = p.rows / reached, blocks = reached * ((per + 15) / 16);
   const int64_t cus = cu_count_current();
   if (per > 32 && 2 * blocks * ((p.N + 63) / 64) >= 3 * cus)

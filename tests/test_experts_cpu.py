@@ -99,7 +99,7 @@ def route(lib, T=4, E=8, k=2, dt=0, logits=A, w=A, e=A, o=A, s=A, work=A):
 @pytest.mark.parametrize("kw,code,text", [
     (dict(dt=7), -2, b"dtype"), (dict(T=-1), -2, b"tokens"), (dict(E=0), -2, b"experts"), (dict(k=0), -2, b"k"),
     (dict(k=9), -2, b"k"), (dict(E=1025), -3, b"experts"), (dict(E=40, k=17), -3, b"k"),
-    (dict(T=2 ** 31 - 1), -3, b"2^31"), (dict(T=2 ** 30, k=2), -3, b"2^31"),
+    (dict(T=2 ** 31 - 1), -3, b"2^31"), (dict(T=2 ** 30, k=2), -3, b"2^31"), (dict(T=2 ** 26, k=1), -3, b"2^26"),
     (dict(logits=None), -2, b"null"), (dict(w=None), -2, b"null"), (dict(e=None), -2, b"null"),
     (dict(o=None), -2, b"null"), (dict(s=None), -2, b"null"), (dict(T=65, work=None), -2, b"null"),
 ])
@@ -116,6 +116,7 @@ def test_route_work(lib):
 
 @pytest.mark.parametrize("kw,code", [
     (dict(dt=-1), -2), (dict(k=5, E=4), -2), (dict(E=1025), -3), (dict(g=None), -2), (dict(out=None), -2),
+    (dict(T=2 ** 26), -3),
 ])
 def test_route_backward_refusals(lib, kw, code):
     d = dict(T=4, E=8, k=2, dt=0, g=A, out=A)
@@ -127,7 +128,8 @@ def test_route_backward_refusals(lib, kw, code):
 
 @pytest.mark.parametrize("kw,code", [
     (dict(dt=9), -2), (dict(T=-1), -2), (dict(k=0), -2), (dict(D=-1), -2), (dict(T=2 ** 30, k=2), -3),
-    (dict(T=2 ** 40, k=2 ** 40), -3), (dict(D=2 ** 31), -3), (dict(a=None), -2), (dict(s=None), -2),
+    (dict(T=2 ** 40, k=2 ** 40), -3), (dict(D=2 ** 31), -3), (dict(D=2 ** 30 + 1), -3),
+    (dict(T=2 ** 26, k=1, D=2048), -3), (dict(a=None), -2), (dict(s=None), -2),
     (dict(out=None), -2),
 ])
 def test_row_exchange_refusals(lib, kw, code):
@@ -152,6 +154,7 @@ def test_row_exchange_empty(lib):
     (dict(dt=3), -2, b"dtype"), (dict(R=-1), -2, b"negative"), (dict(E=-1), -2, b"negative"),
     (dict(N=-1), -2, b"negative"), (dict(K=-1), -2, b"negative"), (dict(E=1025), -3, b"groups"),
     (dict(R=2 ** 31), -3, b"2^31"), (dict(N=2 ** 31), -3, b"2^31"), (dict(K=2 ** 31), -3, b"2^31"),
+    (dict(R=2 ** 30 + 1), -3, b"2^30"), (dict(N=2 ** 30 + 1), -3, b"2^30"), (dict(K=2 ** 30 + 1), -3, b"2^30"),
     (dict(a=None), -2, b"null"), (dict(b=None), -2, b"null"), (dict(o=None), -2, b"null"),
     (dict(out=None), -2, b"null"),
 ])
@@ -167,6 +170,8 @@ def test_grouped_refusals(lib, kw, code, text):
 
 
 def test_grouped_refusals_of_one_entry(lib):
+    assert lib.sf_grouped_linear_dw(A, None, A, None, A, I64(8), I64(2), I64(2 ** 28 + 1), I64(0), 2, None) == -3
+    assert b"2^28" in lib.sf_last_error()
     size = (I64(8), I64(2), I64(16), I64(16), 2)
     assert lib.sf_grouped_linear(A, A, A, None, A, *size, 6, None) == -2
     assert b"epilogue" in lib.sf_last_error()

@@ -137,6 +137,20 @@ def test_no_rows_and_shapes():
     assert g.dev_linear_q4(up(np.zeros(64), "bfloat16"), q, s).shape == (8,)
 
 
+def test_no_groups_give_zeros():
+    """Through the C ABI: offsets of no group at all, so every row is set to 0."""
+    g = cu()
+    lib = ctypes.CDLL(os.path.join(ROOT, "scaffolding_amd", "libsfgemm.so"))
+    x, y = up(np.ones((5, 64)), "bfloat16"), up(np.ones((5, 8)), "bfloat16")
+    off = raw(np.zeros(1), np.int32)
+    for bias, epi in ((None, 0), (y, 1)):
+        assert lib.sf_linear_q4(P(x.data_ptr), None, None, None, P(off.data_ptr), None if bias is None else P(bias.data_ptr),
+                                P(y.data_ptr), I64(5), I64(0), I64(8), I64(64), I64(32), 2, epi, None) == 0
+        assert (down(y) == 0).all()
+    assert g.dev_linear_q4(x, raw(np.zeros((0, 8, 32)), np.uint8), up(np.zeros((0, 2, 8)), "bfloat16"),
+                           gt_offsets=off).shape == (5, 8)
+
+
 def test_large_activations_keep_their_sums():
     """All x alike and positive: the offset of the packed integers is taken
     out of sums 5 times the result's."""
