@@ -181,8 +181,7 @@ class LinearQ4(Module):
     def __init__(self, in_features: int, out_features: int, bias: bool = True, group: int = 128, zeros: bool = False,
                  device=None, dtype="bfloat16", activation: str | None = None):
         super().__init__()
-        if in_features % group != 0:
-            raise ValueError("LinearQ4: in_features %d is no multiple of the group %d" % (in_features, group))
+        _check_q4_group("LinearQ4", in_features, group)
         self.in_features = in_features
         self.out_features = out_features
         self.group = group
@@ -223,6 +222,13 @@ class LinearQ4(Module):
     def __repr__(self) -> str:
         return "LinearQ4(in_features=%d, out_features=%d, bias=%s, group=%d)" % (
             self.in_features, self.out_features, self.bias is not None, self.group)
+
+
+def _check_q4_group(name: str, in_features: int, group: int) -> None:
+    if group not in (32, 64) and (group < 128 or group % 128 != 0):
+        raise ValueError("%s: the group %d is not 32, 64 or a multiple of 128" % (name, group))
+    if in_features % group != 0:
+        raise ValueError("%s: in_features %d is no multiple of the group %d" % (name, in_features, group))
 
 
 def _on(t: Tensor | None, dev: int):
@@ -382,8 +388,9 @@ class MoE(Module):
         self.down = _ExpertLinear(experts, hidden, dim, bias, device, dtype)
 
     def quantize(self, group: int = 128, zeros: bool = False) -> "MoE":
-        self.up.quantize(group, zeros)
-        self.down.quantize(group, zeros)
+        made = [layer.packed(group, zeros) for layer in (self.up, self.down)]  # both, or neither is changed
+        self.up.replace(*made[0])
+        self.down.replace(*made[1])
         return self
 
     def forward(self, x: Tensor) -> Tensor:
@@ -395,7 +402,7 @@ class MoE(Module):
 
 class _ExpertLinear(Module):
     """One linear layer per expert (F.grouped_linear), initialised as Linear
-    is; after quantize, F.linear_q4 over the same groups."""
+    is; after replace, F.linear_q4 over the same groups."""
 
     def __init__(self, experts: int, in_features: int, out_features: int, bias: bool, device, dtype):
         super().__init__()
@@ -408,17 +415,20 @@ class _ExpertLinear(Module):
             self.bias = Parameter(np.random.uniform(-s, s, (experts, out_features)).astype(np.float32), dtype=dtype,
                                   device=dev)
 
-    def quantize(self, group: int, zeros: bool) -> None:
+    def packed(self, group: int, zeros: bool) -> tuple:
         from .functional import quantize_q4
         if self.scales is not None:
             raise RuntimeError("the weight is quantized already")
         if self.weight.dtype.value == "float32":
             raise TypeError("4-bit weights need a float16 or bfloat16 layer")
+        _check_q4_group("MoE.quantize", self.weight.shape[-1], group)
+        return quantize_q4(self.weight, group, zeros)
+
+    def replace(self, q, scales, zero) -> None:
         dev, dt = self.weight.device, self.weight.dtype
-        q, scales, zero = quantize_q4(self.weight, group, zeros)
         self.weight = Parameter(q, False, "uint8", dev)
         self.scales = Parameter(scales, False, dt, dev)
-        if zeros:
+        if zero is not None:
             self.zeros = Parameter(zero, False, "uint8", dev)
 
     def to(self, device=None, dtype=None) -> "_ExpertLinear":

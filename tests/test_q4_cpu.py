@@ -127,6 +127,8 @@ def test_module_refusals():
     with pytest.raises(ValueError):
         nn.LinearQ4(100, 8, group=32)
     with pytest.raises(ValueError):
+        nn.LinearQ4(96, 8, group=48)
+    with pytest.raises(ValueError):
         nn.MoE(8, 8, 4, 5)
     t = sf.Tensor(np.zeros((4, 128), np.float16))
     with pytest.raises(RuntimeError):

@@ -268,3 +268,23 @@ def test_moe_module(dtype, T, E, k):
         # sums of 96 and 64 terms, with terms up to 31 / 7 of the weights'
         tol = 3 * out_half_ulp_rel(dtype) + 2 * 2 * 96 * 5 * 2.0 ** -24
         assert np.linalg.norm(got - want) <= tol * np.linalg.norm(want)
+
+
+def test_moe_module_shapes_and_refusals():
+    import scaffolding_amd as sf
+    from scaffolding_amd import nn
+
+    m = nn.MoE(64, 96, 4, 2, dtype="bfloat16")
+    with pytest.raises(ValueError):
+        m.quantize(64)  # 96 is no multiple of it: neither layer is changed
+    assert m.up.scales is None and m.down.scales is None
+    x = rnd(np.random.default_rng(0), (2, 3, 64), 1.0, "bfloat16")
+    for quantized in (False, True):
+        if quantized:
+            m.quantize(32)
+            with pytest.raises(RuntimeError):
+                m.quantize(32)
+        y = m(sf.Tensor(x, dtype="bfloat16", device="cuda")).numpy()
+        flat = m(sf.Tensor(x.reshape(6, 64), dtype="bfloat16", device="cuda")).numpy()
+        assert y.shape == x.shape and np.array_equal(y.reshape(6, 64), flat)
+        assert m(sf.empty(0, 64, dtype="bfloat16", device="cuda")).shape == (0, 64)
