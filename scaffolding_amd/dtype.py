@@ -39,6 +39,17 @@ class dtype(enum.Enum):
             return _cuops.BFLOAT16
         return np.dtype(self.value)
 
+    def of_host(self, arr: np.ndarray) -> np.ndarray:
+        """`arr` in this dtype's host type.  The integer types take whole
+        numbers of their range only: an index or a packed byte that was
+        truncated or wrapped would be another one."""
+        to = self.to_numpy()
+        if to.kind in "iu" and arr.dtype != to and arr.size:
+            info = np.iinfo(to)
+            if arr.dtype.kind not in "biu" or arr.min() < info.min or arr.max() > info.max:
+                raise TypeError("%s values do not convert to %s" % (arr.dtype, to))
+        return arr.astype(to, copy=False)
+
     @staticmethod
     def from_any(d) -> "dtype":
         # The storage dtypes' own objects first: this runs once per operator

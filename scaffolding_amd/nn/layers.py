@@ -116,7 +116,7 @@ class Module:
                 raise ValueError("load_state_dict: shape mismatch for %s: %s vs %s" % (name, shape, target.shape))
             if target._gpu is None:
                 host = val.numpy() if isinstance(val, Tensor) else np.asarray(val)
-                target._data = np.array(host, dtype=target._dtype.to_numpy(), copy=True)
+                target._data = np.array(target._dtype.of_host(host))
                 continue
             dev = target._gpu.device_id
             storage = target._dtype.device_storage()

@@ -36,7 +36,7 @@ class Tensor:
         arr = np.asarray(data)
         self._dtype = _dtype_t.from_any(dtype if dtype is not None else
                                         (arr.dtype if arr.dtype == np.float16 else "float32"))
-        host = arr.astype(self._dtype.to_numpy(), copy=False)
+        host = self._dtype.of_host(arr)
         if self._device.is_cuda:
             self._gpu = _cuops.gputensor_from_numpy(np.ascontiguousarray(host), self._device.ordinal(),
                                                     self._dtype.device_storage())
