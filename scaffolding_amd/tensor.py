@@ -139,7 +139,7 @@ class Tensor:
         if self._gpu is not None:
             return Tensor._wrap_gpu(_cuops.dev_reshape(self._gpu, tuple(shape)), self._device,
                                     self._requires_grad)
-        t = Tensor(self._data.reshape(shape), device="cpu", requires_grad=self._requires_grad)
+        t = Tensor(self._data.reshape(shape), dtype=self._dtype, device="cpu", requires_grad=self._requires_grad)
         return t
 
     view = reshape

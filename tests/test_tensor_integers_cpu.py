@@ -60,3 +60,11 @@ def test_state_dict_on_the_host():
     m.load_state_dict({"q": np.array([1, 2, 255]), "s": np.array([1, 2, 3])})
     assert m.q.numpy().tolist() == [1, 2, 255] and m.q.numpy().dtype == np.uint8
     assert m.s.numpy().tolist() == [1.0, 2.0, 3.0] and m.s.numpy().dtype == np.float32
+
+
+@pytest.mark.parametrize("dtype", ["int32", "uint8", "float16", "float32"])
+def test_reshape_keeps_the_type(dtype):
+    import scaffolding_amd as sf
+    t = sf.Tensor(np.arange(6), dtype=dtype, requires_grad=True).reshape(2, -1)
+    assert t.dtype is sf.dtype(dtype) and t.numpy().dtype == np.dtype(dtype) and t.requires_grad
+    assert t.numpy().tolist() == [[0, 1, 2], [3, 4, 5]] and t.view(6).dtype is sf.dtype(dtype)
