@@ -69,7 +69,14 @@ class Module:
         for mn, m in self._modules.items():
             yield from m.named_parameters(prefix + mn + ".")
 
+    def _check_dtype(self, dtype) -> None:
+        """Refuses a type that the module or one below it cannot take, before
+        anything is moved."""
+        for m in self._modules.values():
+            m._check_dtype(dtype)
+
     def to(self, device=None, dtype=None) -> "Module":
+        self._check_dtype(dtype)
         for name, p in list(self._params.items()):
             moved = Parameter(p.to(device, dtype), requires_grad=p.requires_grad)
             setattr(self, name, moved)
@@ -175,13 +182,15 @@ class LinearQ4(Module):
     """A Linear whose weight is held in 4 bits with a scale (and with `zeros` a
     zero point) per `group` input features, for decoding: the weight's bytes
     are what a step with few rows is bound by.  `weight` is packed (out, in /
-    2); scales are rounded to `dtype` (float16 or bfloat16).  Made from a
-    weight with from_linear; inference only."""
+    2); scales are rounded to `dtype` (float16 or bfloat16, the type of the
+    activations too).  Made from a weight with from_linear, whose dtype is the
+    Linear's by default (a float32 one needs it given); inference only."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, group: int = 128, zeros: bool = False,
                  device=None, dtype="bfloat16", activation: str | None = None):
         super().__init__()
         _check_q4_group("LinearQ4", in_features, group)
+        _check_q4_dtype("LinearQ4", dtype)
         self.in_features = in_features
         self.out_features = out_features
         self.group = group
@@ -210,10 +219,15 @@ class LinearQ4(Module):
 
     def to(self, device=None, dtype=None) -> "LinearQ4":
         """Moves everything; `dtype` is that of the scales and the bias."""
+        self._check_dtype(dtype)
         for name, p in list(self._params.items()):
             kept = p.dtype.value == "uint8"
             setattr(self, name, Parameter(p.to(device, None if kept else dtype), requires_grad=False))
         return self
+
+    def _check_dtype(self, dtype) -> None:
+        if dtype is not None:
+            _check_q4_dtype("LinearQ4", dtype)
 
     def forward(self, x: Tensor) -> Tensor:
         from .functional import linear_q4
@@ -229,6 +243,11 @@ def _check_q4_group(name: str, in_features: int, group: int) -> None:
         raise ValueError("%s: the group %d is not 32, 64 or a multiple of 128" % (name, group))
     if in_features % group != 0:
         raise ValueError("%s: in_features %d is no multiple of the group %d" % (name, in_features, group))
+
+
+def _check_q4_dtype(name: str, dtype) -> None:
+    if _dtype_t.from_any(dtype).value not in ("float16", "bfloat16"):
+        raise TypeError("%s: 4-bit weights need a float16 or bfloat16 layer, not %s" % (name, dtype))
 
 
 def _on(t: Tensor | None, dev: int):
@@ -419,8 +438,7 @@ class _ExpertLinear(Module):
         from .functional import quantize_q4
         if self.scales is not None:
             raise RuntimeError("the weight is quantized already")
-        if self.weight.dtype.value == "float32":
-            raise TypeError("4-bit weights need a float16 or bfloat16 layer")
+        _check_q4_dtype("MoE.quantize", self.weight.dtype)
         _check_q4_group("MoE.quantize", self.weight.shape[-1], group)
         return quantize_q4(self.weight, group, zeros)
 
@@ -431,7 +449,12 @@ class _ExpertLinear(Module):
         if zero is not None:
             self.zeros = Parameter(zero, False, "uint8", dev)
 
+    def _check_dtype(self, dtype) -> None:
+        if dtype is not None and self.scales is not None:
+            _check_q4_dtype("MoE", dtype)
+
     def to(self, device=None, dtype=None) -> "_ExpertLinear":
+        self._check_dtype(dtype)
         for name, p in list(self._params.items()):
             kept = p.dtype.value == "uint8"
             setattr(self, name, Parameter(p.to(device, None if kept else dtype), requires_grad=p.requires_grad))

@@ -133,3 +133,41 @@ def test_module_refusals():
     t = sf.Tensor(np.zeros((4, 128), np.float16))
     with pytest.raises(RuntimeError):
         F.linear_q4(t, t, t)
+
+
+def test_a_4_bit_layer_is_16_bit():
+    """Scales and activations are float16 or bfloat16: any other type is
+    refused where the layer is made or moved, and nothing is changed."""
+    import scaffolding_amd as sf
+    from scaffolding_amd import nn
+    with pytest.raises(TypeError):
+        nn.LinearQ4(64, 8, group=32, device="cpu", dtype="float32")
+    with pytest.raises(TypeError):
+        nn.LinearQ4(64, 8, group=32, device="cpu", dtype="int32")
+    lin = nn.Linear(64, 8, device="cpu")
+    with pytest.raises(TypeError):
+        nn.LinearQ4.from_linear(lin, 32)
+    lq = nn.LinearQ4.from_linear(lin, 32, dtype="float16")
+    assert lq.scales.dtype is sf.float16 and lq.bias.dtype is sf.float16 and lq.weight.dtype is sf.uint8
+    seq = nn.Sequential(nn.Linear(8, 64, device="cpu"), lq)
+    for m in (lq, seq):
+        with pytest.raises(TypeError):
+            m.to(dtype="float32")
+    assert seq._modules["0"].weight.dtype is sf.float32 and lq.scales.dtype is sf.float16
+    with pytest.raises(TypeError):
+        seq.to(dtype="uint8")
+    seq.to(device="cpu")
+    seq.to(dtype="float16")
+    assert seq._modules["0"].weight.dtype is sf.float16 and lq.weight.dtype is sf.uint8
+
+
+def test_a_quantized_expert_layer_is_16_bit():
+    import scaffolding_amd as sf
+    from scaffolding_amd import nn
+    m = nn.MoE(64, 32, 3, 2, device="cpu", dtype="float16")
+    m.to(dtype="float32").to(dtype="float16")
+    m.quantize(32)
+    with pytest.raises(TypeError):
+        m.to(dtype="float32")
+    assert {p.dtype for p in m.parameters()} == {sf.float16, sf.uint8}
+    m.to(device="cpu", dtype="float16")
