@@ -196,6 +196,8 @@ def quantize_q4(weight, group: int = 128, zeros: bool = False):
     w = w.astype(np.float32)
     if w.ndim < 2 or group < 1 or w.shape[-1] % group != 0:
         raise ValueError("quantize_q4: weight %s does not divide into groups of %d" % (w.shape, group))
+    if w.shape[-1] % 2:
+        raise ValueError("quantize_q4: two columns share a byte, %d is odd" % w.shape[-1])
     if not np.isfinite(w).all():
         raise ValueError("quantize_q4: the weight has values that are not finite")
     g = w.reshape(w.shape[:-1] + (w.shape[-1] // group, group))
