@@ -203,7 +203,9 @@ def quantize_q4(weight, group: int = 128, zeros: bool = False):
     g = w.reshape(w.shape[:-1] + (w.shape[-1] // group, group))
     if zeros:
         low, high = np.minimum(g.min(-1), 0.0), np.maximum(g.max(-1), 0.0)
-        scale = (high - low) / 15.0
+        with np.errstate(over="ignore"):
+            scale = (high - low) / 15.0
+        scale = np.where(np.isfinite(scale), scale, high / 15.0 - low / 15.0)  # a range past the largest number
         zero = np.rint(-low / np.where(scale == 0.0, 1.0, scale))
     else:
         scale = np.abs(g).max(-1) / 7.0

@@ -181,3 +181,17 @@ def test_quantize_needs_whole_bytes():
             F.quantize_q4(np.ones(shape, np.float32), group)
     q, s, z = F.quantize_q4(np.ones((2, 6), np.float32), 3)
     assert q.shape == (2, 3) and (ox.q4_weight(q, s) == 1).all()
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+def test_quantize_of_the_largest_weights(zeros):
+    """A group's range may pass the largest fp32 number; its step does not."""
+    from scaffolding_amd.nn import functional as F
+    top = np.finfo(np.float32).max
+    w = np.tile(np.array([top, -top, 0.0, top / 2], np.float32), (2, 8))
+    with np.errstate(all="raise", under="ignore"):
+        q, s, z = F.quantize_q4(w, 32, zeros)
+    assert np.isfinite(s).all()
+    back = ox.q4_weight(q, s, z)
+    step = np.repeat(np.swapaxes(s, -1, -2), 32, -1).astype(np.float64)
+    assert (np.abs(back - w) <= step * (1.001 if zeros else 0.501)).all()
