@@ -403,7 +403,7 @@ int sf_cast(const void* x, sf_dtype in_dtype, void* y, sf_dtype out_dtype,
  *   offsets  int32 [experts + 1]: the assignments (t, j) ordered by expert,
  *            within one by t k + j; expert e's are [offsets[e], offsets[e+1])
  *   slots    int32 [tokens, k]: the place of (t, j) in that order
- * 1 <= k <= min(experts, 16), experts <= 1024, tokens < 2^26.  `work`:
+ * 1 <= k <= min(experts, 16), experts <= 1024, tokens <= 2^26 - 4.  `work`:
  * sf_route_topk_work bytes of 4-byte aligned device memory, overwritten (may
  * be NULL where that is 0).  tokens == 0 writes zeros to offsets. */
 int64_t sf_route_topk_work(int64_t tokens, int64_t experts);

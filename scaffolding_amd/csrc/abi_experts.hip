@@ -193,8 +193,8 @@ static int route_check(const char* name, int64_t tokens, int64_t experts, int64_
                 route_max_k(), (long long)experts, (long long)k);
   if (tokens * k >= INT32_MAX || tokens >= INT32_MAX)
     return fail(SF_ERR_UNSUPPORTED, "%s: tokens * k must be < 2^31 - 1", name);
-  if (tokens >= int64_t(1) << 26)  // 64 threads a token, in a grid of fewer than 2^32
-    return fail(SF_ERR_UNSUPPORTED, "%s: tokens must be < 2^26", name);
+  // the gradient takes four tokens a block of 256 threads, in a grid of fewer than 2^32
+  if (tokens > (int64_t(1) << 26) - 4) return fail(SF_ERR_UNSUPPORTED, "%s: tokens must be at most 2^26 - 4", name);
   return SF_OK;
 }
 

@@ -268,3 +268,13 @@ def test_integer_tensors_on_the_host():
     assert sf.uint8.itemsize == 1
     # without a dtype, integers become float32 as before
     assert sf.Tensor(np.array([1, 2], np.int32)).dtype is sf.float32
+
+
+@pytest.mark.parametrize("T", [2 ** 26 - 3, 2 ** 26 - 1])
+def test_routing_refuses_grids_past_the_launch_limit(lib, T):
+    """The gradient takes 64 threads a token in blocks of four tokens: 2^26 - 4
+    tokens are the last whose grid stays below 2^32 threads."""
+    assert -(-T // 4) * 256 >= 2 ** 32 > -(-(2 ** 26 - 4) // 4) * 256
+    assert route(lib, T=T, k=1) == -3 and b"2^26" in lib.sf_last_error()
+    assert lib.sf_route_topk_backward(A, A, A, A, I64(T), I64(8), I64(1), 0, 1, A, None) == -3
+    assert b"2^26" in lib.sf_last_error()
