@@ -564,9 +564,9 @@ __device__ __forceinline__ float act_slope(float t) {
   }
 }
 
+// (out may be g or pre, so no pointer is marked as the only one to its memory.)
 template <typename T, int ACT>
-__global__ __launch_bounds__(256) void act_backward_kernel(const void* __restrict__ g, const void* __restrict__ pre,
-                                                           void* __restrict__ out, int64_t n) {
+__global__ __launch_bounds__(256) void act_backward_kernel(const void* g, const void* pre, void* out, int64_t n) {
   for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; i < n; i += (int64_t)gridDim.x * 2048) {
     const int left = n - i < 8 ? (int)(n - i) : 8;
     float a[8], b[8];

@@ -133,6 +133,29 @@ def test_activation_slopes_far_out(act, code):
     assert got[-3] == 1 and abs(got[-2]) < 1e-30 and np.isnan(got[-1])
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [1, 7, 2049, 2048 * 300 + 5])
+def test_activation_slopes_in_place(dtype, n):
+    """The result over the gradient or over the layer's output: the same bits
+    as into memory of its own."""
+    g = cu()
+    lib = ctypes.CDLL(os.path.join(ROOT, "scaffolding_amd", "libsfgemm.so"))
+    rng = np.random.default_rng(n)
+    gr, pre = rnd(rng, (n,), 1.0, dtype), rnd(rng, (n,), 3.0, dtype)
+
+    def run(into, code):
+        t = [up(gr, dtype), up(pre, dtype), g.empty((n,), up(gr, dtype).dtype)]
+        assert lib.sf_act_backward(P(t[0].data_ptr), P(t[1].data_ptr), P(t[into].data_ptr), I64(n), SFD[dtype], code,
+                                   None) == 0
+        return down(t[into])
+
+    for act, code in (("silu", 4), ("gelu", 5)):
+        own = run(2, code)
+        want = gr.astype(np.float64) * ox.act_slope(pre, act)
+        check_bound(own, want, out_half_ulp_rel(dtype) * np.abs(want) + 16 * 4 * 2.0 ** -24 * np.abs(gr) + 2.0 ** -25)
+        assert np.array_equal(run(0, code), own) and np.array_equal(run(1, code), own)
+
+
 def test_route_no_tokens_and_leading_shapes():
     g = cu()
     w, e, off, slots = g.dev_route_topk(g.empty((0, 5)), 2)
