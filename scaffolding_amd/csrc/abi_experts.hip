@@ -141,7 +141,10 @@ static int grouped_rows(const char* name, const void* A, const void* B, const vo
   p.sB = N * K;
   const bool f32 = dtype == SF_F32;
   // 16-byte rows; one weight and one tile of A below the direct loads' 2 GiB
-  const bool dma = f32 && N * K < (int64_t(1) << 28) && K < (int64_t(1) << 20);
+  // (fp32, an N-contiguous weight: and the 64 rows past its K that the last
+  // step's offsets reach, which would wrap at 4 GiB and read it again)
+  const bool dma = f32 && N * K < (int64_t(1) << 28) && K < (int64_t(1) << 20) &&
+                   (b_kmajor || N * (K + 64) < (int64_t(1) << 29));
   const bool vec = f32 ? dma && K % 4 == 0 && (b_kmajor || N % 4 == 0) && aligned16(A) && aligned16(B)
                        : K % 8 == 0 && (b_kmajor || N % 8 == 0) && aligned16(A) && aligned16(B) &&
                              N * K < (int64_t(1) << 30) && K < (int64_t(1) << 22);

@@ -624,3 +624,28 @@ def test_a_long_operand():
                              None) == 0
     pair = last.reshape(4, 2, C).astype(np.float64).sum(1)
     check_bound((got.astype(np.uint32) << 16).view(np.float32), pair, 2.0 ** -8 * np.abs(pair) + 1e-30)
+
+
+def test_fp32_gradient_of_a_very_wide_layer_with_few_outputs():
+    """The direct loads step through 64 rows of the weight at a time: with so
+    few outputs that those reach past 4 GiB from its start, an infinite weight
+    must still meet only its own product."""
+    g = cu()
+    N, K = 7, 2 ** 25
+    w = g.zeros((1, N, K), np.float32)
+    lib = ctypes.CDLL(os.path.join(ROOT, "scaffolding_amd", "libsfgemm.so"))
+    block = np.zeros((N, 8), np.float32)
+    block[0, 5], block[3, 1], block[6, 2] = np.inf, 2.0, -3.0
+    for n in range(N):
+        row = np.ascontiguousarray(block[n])
+        assert lib.sf_memcpy_h2d(P(w.data_ptr + n * K * 4), row.ctypes.data_as(P), ctypes.c_size_t(32), None) == 0
+    for R in (1, 70):
+        out = g.empty((R, K))
+        a, o = f32(np.ones((R, N))), ints([0, R])
+        assert lib.sf_grouped_linear_dx(P(a.data_ptr), P(w.data_ptr), P(o.data_ptr), P(out.data_ptr), I64(R), I64(1),
+                                        I64(N), I64(K), 0, None) == 0
+        for r in (0, R - 1):
+            got = np.empty(K if r == 0 else 4096, np.float32)
+            assert lib.sf_memcpy_d2h(got.ctypes.data_as(P), P(out.data_ptr + r * K * 4), ctypes.c_size_t(got.nbytes),
+                                     None) == 0
+            assert got[:8].tolist() == [0, 2, -3, 0, 0, np.inf, 0, 0] and (got[8:] == 0).all()
