@@ -285,18 +285,28 @@ cdef class CudaBuffer:
         return self.device_id
 
 
-cdef CudaBuffer _make_buffer(size_t nbytes, int device_id):
+cdef CudaBuffer _make_buffer_or_none(size_t nbytes, int device_id):
+    """_make_buffer's memory, or None where the device has no more."""
     cdef CudaBuffer buf = CudaBuffer.__new__(CudaBuffer)
     cdef size_t got = 0
     cdef void* p = NULL
     cdef int ret
     with nogil:
         ret = sf_cache_alloc(device_id, nbytes, &p, &got)
+    if ret == SF_ERR_OOM:
+        return None
     _check_cuda(ret)
     buf.ptr = p
     buf.nbytes = got
     buf.device_id = device_id
     buf.owns_memory = True
+    return buf
+
+
+cdef CudaBuffer _make_buffer(size_t nbytes, int device_id):
+    cdef CudaBuffer buf = _make_buffer_or_none(nbytes, device_id)
+    if buf is None:
+        _check_cuda(SF_ERR_OOM)  # with sf_cache_alloc's own text
     return buf
 
 
@@ -1456,7 +1466,7 @@ def dev_linear_q4(gt_x, gt_q, gt_scales, gt_zeros=None, gt_bias=None, activation
     zeros and b have a leading E and x is (R, K).  Sums are fp32 over exact
     integers (an infinite x makes its row NaN); from 384 rows per weight on, W
     is first rounded to x's dtype (half a step of each weight, as a 16-bit copy
-    of W has) and the 16-bit products run."""
+    of W has) and the 16-bit products run, unless there is no memory for it."""
     name = 'dev_linear_q4'
     xs, qs = tuple(gt_x.shape), tuple(gt_q.shape)
     lead = 0 if gt_offsets is None else 1
@@ -1501,10 +1511,11 @@ def dev_linear_q4(gt_x, gt_q, gt_scales, gt_zeros=None, gt_bias=None, activation
     cdef void* pw
     cdef int ret
     if R >= _Q4_EXPAND_ROWS * E:
-        w = dev_q4_expand(gt_q, gt_scales, gt_zeros)
-        if lead:
-            return dev_grouped_linear(gt_x, w, gt_offsets, gt_bias, activation)
-        return dev_linear_forward(gt_x, w, gt_bias, activation)
+        w = _q4_expand(gt_q, gt_scales, gt_zeros)
+        if w is not None:
+            if lead:
+                return dev_grouped_linear(gt_x, w, gt_offsets, gt_bias, activation)
+            return dev_linear_forward(gt_x, w, gt_bias, activation)
     cdef int epi
     cdef void* pb = NULL
     if gt_bias is not None:
@@ -1524,6 +1535,14 @@ def dev_linear_q4(gt_x, gt_q, gt_scales, gt_zeros=None, gt_bias=None, activation
 def dev_q4_expand(gt_q, gt_scales, gt_zeros=None):
     """The weight that dev_linear_q4's q, scales and zeros stand for, in the
     scales' dtype (one rounding): (N, K), or (E, N, K) with a leading E."""
+    out = _q4_expand(gt_q, gt_scales, gt_zeros)
+    if out is None:
+        _check_cuda(SF_ERR_OOM)
+    return out
+
+
+cdef object _q4_expand(gt_q, gt_scales, gt_zeros):
+    """dev_q4_expand's weight, or None where there is no memory for it."""
     name = 'dev_q4_expand'
     qs = tuple(gt_q.shape)
     _need_storage(gt_q, _U8, name, 'q')
@@ -1542,7 +1561,10 @@ def dev_q4_expand(gt_q, gt_scales, gt_zeros=None):
     cdef sf_dtype dt = _sf_dtype(gt_scales.dtype)
     if dt == SF_F32:
         raise TypeError("%s: scales must be float16 or bfloat16" % name)
-    out = _alloc_like(qs[:lead] + (int(N), int(K)), gt_scales.dtype, gt_scales.device_id)
+    cdef CudaBuffer buf = _make_buffer_or_none(<size_t>(E * N * K) * 2, gt_scales.device_id)
+    if buf is None:
+        return None
+    out = GpuTensor(buf, qs[:lead] + (int(N), int(K)), gt_scales.dtype, gt_scales.device_id)
     cdef void* pq = _ptr(gt_q)
     cdef void* ps = _ptr(gt_scales)
     cdef void* pz = _ptr(gt_zeros) if gt_zeros is not None else NULL

@@ -2,7 +2,10 @@
 from __future__ import annotations
 
 import ctypes
+import json
 import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -102,6 +105,16 @@ def test_many_rows_run_the_16_bit_product(E):
     got = down(g.dev_linear_q4(up(x, "bfloat16"), *args, None, None, raw(off, np.int32) if E else None))
     y, mag = ox.grouped_linear(x, wt if E else wt[None], off or [0, R])
     check_bound(got, y, gemm_bound(y, mag, K, "bfloat16"))
+
+
+def test_no_memory_left_for_a_16_bit_weight():
+    """Many rows run the direct kernel where the 16-bit weight cannot be
+    allocated."""
+    r = subprocess.run([sys.executable, os.path.join(ROOT, "tests", "low_memory_q4_process.py")], capture_output=True,
+                       text=True, timeout=100)
+    assert r.returncode == 0, r.stdout + r.stderr
+    out = json.loads(r.stdout.strip().splitlines()[-1])
+    assert out["error"] == "" and out["held"] > 0 and out["same"] and 0 <= out["worst"] <= 1.0, out
 
 
 def test_known_values():
