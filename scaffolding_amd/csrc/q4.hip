@@ -104,9 +104,8 @@ __device__ __forceinline__ u32x4 lane_groups_transpose(u32x4 v) {
   return u32x4{c[0], c[1], d[0], d[1]};
 }
 
-// GB: scale groups per block of 128 k (1: G % 128 == 0; 2; 4).  U: blocks whose
-// loads a wave issues together.
-template <typename T, int NB, int NW, int U, int GB, bool ZEROS, bool GROUPED>
+// GB: scale groups per block of 128 k (1: G % 128 == 0; 2; 4).
+template <typename T, int NB, int NW, int GB, bool ZEROS, bool GROUPED>
 __global__ __launch_bounds__(NW * 64) void q4_kernel(Q4Params p) {
   constexpr int BM = 16, BN = 16 * NB;
   constexpr int XP = 272;                        // bytes of a staged x row of 128 k: 16 rows on 16 bank groups
@@ -213,70 +212,61 @@ __global__ __launch_bounds__(NW * 64) void q4_kernel(Q4Params p) {
 
   auto run = [&](auto qx_c) {
     constexpr int QX = decltype(qx_c)::value;
-    u32x4 w[U][NB], xs[U][4];
-    auto load = [&](int b0, int last) {
+    u32x4 w[NB], xs[4];
+    auto load = [&](int blk, int last) {
+      const int k0 = blk * 128;
+      const bool gone = blk >= last;             // uniform
+      const bool tail = GB > 1 && k0 + 128 > K;  // uniform: a last block of 32, 64 or 96 k
+      const int ks = gone ? 0 : k0;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int blk = b0 + u * NW, k0 = blk * 128;
-        const bool gone = blk >= last;                 // uniform
-        const bool tail = GB > 1 && k0 + 128 > K;      // uniform: a last block of 32, 64 or 96 k
-        const int ks = gone ? 0 : k0;
+      for (int d = 0; d < QX; ++d) {
+        const uint32_t o = gone || (tail && k0 + 8 * r16 >= K) ? OOB : vx + (uint32_t)(4 * d * K) * 2u;
+        xs[d] = __builtin_amdgcn_raw_buffer_load_b128(rx, o, ks * 2, 0);
+      }
 #pragma unroll
-        for (int d = 0; d < QX; ++d) {
-          const uint32_t o = gone || (tail && k0 + 8 * r16 >= K) ? OOB : vx + (uint32_t)(4 * d * K) * 2u;
-          xs[u][d] = __builtin_amdgcn_raw_buffer_load_b128(rx, o, ks * 2, 0);
-        }
-#pragma unroll
-        for (int i = 0; i < NB; ++i) {
-          const uint32_t o = gone || (tail && k0 + 32 * h >= K) ? OOB : vq[i];
-          w[u][i] = __builtin_amdgcn_raw_buffer_load_b128(rq, o, ks / 2, 0);
-        }
+      for (int i = 0; i < NB; ++i) {
+        const uint32_t o = gone || (tail && k0 + 32 * h >= K) ? OOB : vq[i];
+        w[i] = __builtin_amdgcn_raw_buffer_load_b128(rq, o, ks / 2, 0);
       }
     };
-    auto compute = [&](int b0, int last, int kg0) {
+    auto compute = [&](int blk, int kg0) {
+      // row 4 d + h, chunk r16 (8 k)
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int blk = b0 + u * NW;
-        if (u > 0 && blk >= last) break;  // uniform
-        // row 4 d + h, chunk r16 (8 k)
+      for (int d = 0; d < QX; ++d) *reinterpret_cast<u32x4*>(xw + (4 * d + h) * XP + r16 * 16) = q4_order(xs[d]);
+      wave_lds_sync();
+      // rows past the last: any staged bytes (their outputs are not stored)
+      const int m = QX == 4 ? r16 : r16 & 3;
+      // the k of lane group h in dword d: 32 h + 8 d, or 32 d + 8 h
 #pragma unroll
-        for (int d = 0; d < QX; ++d)
-          *reinterpret_cast<u32x4*>(xw + (4 * d + h) * XP + r16 * 16) = q4_order(xs[u][d]);
-        wave_lds_sync();
-        // rows past the last: any staged bytes (their outputs are not stored)
-        const int m = QX == 4 ? r16 : r16 & 3;
-        // the k of lane group h in dword d: 32 h + 8 d, or 32 d + 8 h
+      for (int d = 0; d < 4; ++d)
+        xs[d] = *reinterpret_cast<const u32x4*>(xw + m * XP + (GB == 1 ? 4 * h + d : 4 * d + h) * 16);
+      wave_lds_sync();
+      if constexpr (GB > 1)
 #pragma unroll
-        for (int d = 0; d < 4; ++d)
-          xs[u][d] = *reinterpret_cast<const u32x4*>(xw + m * XP + (GB == 1 ? 4 * h + d : 4 * d + h) * 16);
-        wave_lds_sync();
-        if constexpr (GB > 1)
+        for (int i = 0; i < NB; ++i) w[i] = lane_groups_transpose(w[i]);
 #pragma unroll
-          for (int i = 0; i < NB; ++i) w[u][i] = lane_groups_transpose(w[u][i]);
+      for (int gi = 0; gi < GB; ++gi) {
+        constexpr int DG = 4 / GB;  // dwords per scale group
+        const int kg = GB == 1 ? blk / gstep : blk * GB + gi;
+        if (GB > 1 && kg >= KG) break;  // past K
+        f32x4 xsum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int gi = 0; gi < GB; ++gi) {
-          constexpr int DG = 4 / GB;  // dwords per scale group
-          const int kg = GB == 1 ? blk / gstep : blk * GB + gi;
-          if (GB > 1 && kg >= KG) break;  // past K
-          f32x4 xsum = {0.f, 0.f, 0.f, 0.f};
+        for (int d = gi * DG; d < gi * DG + DG; ++d) xsum = Mfma16<T>::run(ones, xs[d], xsum);
 #pragma unroll
-          for (int d = gi * DG; d < gi * DG + DG; ++d) xsum = Mfma16<T>::run(ones, xs[u][d], xsum);
+        for (int i = 0; i < NB; ++i) {
+          const u32x2 sc = *reinterpret_cast<const u32x2*>(sS + (kg - kg0) * BN + 16 * i + 4 * h);
+          uint32_t zp = 0;
+          if constexpr (ZEROS) zp = *reinterpret_cast<const uint32_t*>(sZ + (kg - kg0) * BN + 16 * i + 4 * h);
+          f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int i = 0; i < NB; ++i) {
-            const u32x2 sc = *reinterpret_cast<const u32x2*>(sS + (kg - kg0) * BN + 16 * i + 4 * h);
-            uint32_t zp = 0;
-            if constexpr (ZEROS) zp = *reinterpret_cast<const uint32_t*>(sZ + (kg - kg0) * BN + 16 * i + 4 * h);
-            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+          for (int d = gi * DG; d < gi * DG + DG; ++d)
+            acc = Mfma16<T>::run(q4_unpack<T>(w[i][d], mask, exp), xs[d], acc);
+          // this lane's outputs are four columns of x row r16
 #pragma unroll
-            for (int d = gi * DG; d < gi * DG + DG; ++d)
-              acc = Mfma16<T>::run(q4_unpack<T>(w[u][i][d], mask, exp), xs[u][d], acc);
-            // this lane's outputs are four columns of x row r16
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const float s = Elem<T>::to_f32(static_cast<uint16_t>(sc[c >> 1] >> ((c & 1) * 16)));
-              const float off = ZEROS ? 16.0f + (float)((zp >> (8 * c)) & 255u) : 24.0f;
-              sum[i][c] += s * __builtin_fmaf(-off, xsum[c], acc[c]);
-            }
+          for (int c = 0; c < 4; ++c) {
+            const float s = Elem<T>::to_f32(static_cast<uint16_t>(sc[c >> 1] >> ((c & 1) * 16)));
+            const float off = ZEROS ? 16.0f + (float)((zp >> (8 * c)) & 255u) : 24.0f;
+            sum[i][c] += s * __builtin_fmaf(-off, xsum[c], acc[c]);
           }
         }
       }
@@ -292,8 +282,8 @@ __global__ __launch_bounds__(NW * 64) void q4_kernel(Q4Params p) {
       stage_scales(kg0);
       __syncthreads();
       while (b0 < last) {
-        compute(b0, last, kg0);
-        b0 += NW * U;
+        compute(b0, kg0);
+        b0 += NW;
         if (b0 < last) load(b0, last);
       }
     }
@@ -341,18 +331,18 @@ __global__ __launch_bounds__(NW * 64) void q4_kernel(Q4Params p) {
   });
 }
 
-template <typename T, int NB, int NW, int U, int GB>
+template <typename T, int NB, int NW, int GB>
 static void launch_q4_gz(const Q4Params& p, const dim3& g, unsigned lds, hipStream_t st) {
   if (p.offsets != nullptr) {
-    if (p.z != nullptr) hipLaunchKernelGGL((q4_kernel<T, NB, NW, U, GB, true, true>), g, dim3(NW * 64), lds, st, p);
-    else hipLaunchKernelGGL((q4_kernel<T, NB, NW, U, GB, false, true>), g, dim3(NW * 64), lds, st, p);
+    if (p.z != nullptr) hipLaunchKernelGGL((q4_kernel<T, NB, NW, GB, true, true>), g, dim3(NW * 64), lds, st, p);
+    else hipLaunchKernelGGL((q4_kernel<T, NB, NW, GB, false, true>), g, dim3(NW * 64), lds, st, p);
   } else {
-    if (p.z != nullptr) hipLaunchKernelGGL((q4_kernel<T, NB, NW, U, GB, true, false>), g, dim3(NW * 64), lds, st, p);
-    else hipLaunchKernelGGL((q4_kernel<T, NB, NW, U, GB, false, false>), g, dim3(NW * 64), lds, st, p);
+    if (p.z != nullptr) hipLaunchKernelGGL((q4_kernel<T, NB, NW, GB, true, false>), g, dim3(NW * 64), lds, st, p);
+    else hipLaunchKernelGGL((q4_kernel<T, NB, NW, GB, false, false>), g, dim3(NW * 64), lds, st, p);
   }
 }
 
-template <typename T, int NB, int NW, int U>
+template <typename T, int NB, int NW>
 static int launch_q4_g(Q4Params p, hipStream_t st) {
   p.tiles_n = (p.N + 16 * NB - 1) / (16 * NB);
   int64_t gx = p.tiles_n, gy = 1;
@@ -365,9 +355,9 @@ static int launch_q4_g(Q4Params p, hipStream_t st) {
   if (p.sg < 1) p.sg = 1;
   const unsigned lds = static_cast<unsigned>((p.sg + 3) / 4 * 4 * row);
   const dim3 g(static_cast<unsigned>(gx), static_cast<unsigned>(gy));
-  if (p.G % 128 == 0) launch_q4_gz<T, NB, NW, U, 1>(p, g, lds, st);
-  else if (p.G == 64) launch_q4_gz<T, NB, NW, U, 2>(p, g, lds, st);
-  else launch_q4_gz<T, NB, NW, U, 4>(p, g, lds, st);
+  if (p.G % 128 == 0) launch_q4_gz<T, NB, NW, 1>(p, g, lds, st);
+  else if (p.G == 64) launch_q4_gz<T, NB, NW, 2>(p, g, lds, st);
+  else launch_q4_gz<T, NB, NW, 4>(p, g, lds, st);
   return check_launch("4-bit linear");
 }
 
@@ -392,11 +382,11 @@ static int launch_q4_t(const Q4Params& p, hipStream_t st) {
   const int64_t per = p.rows / reached, blocks = reached * ((per + 15) / 16);
   const int64_t cus = cu_count_current();
   if (per > 32 && 2 * blocks * ((p.N + 63) / 64) >= 3 * cus)
-    return p.K >= 8192 ? launch_q4_g<T, 4, 8, 1>(p, st) : launch_q4_g<T, 4, 4, 1>(p, st);
+    return p.K >= 8192 ? launch_q4_g<T, 4, 8>(p, st) : launch_q4_g<T, 4, 4>(p, st);
   const int64_t tiles = blocks * ((p.N + 31) / 32);
-  if (tiles >= 2 * cus) return launch_q4_g<T, 2, 4, 1>(p, st);
-  if (tiles >= cus) return launch_q4_g<T, 2, 8, 1>(p, st);
-  return p.K >= 8192 ? launch_q4_g<T, 1, 16, 1>(p, st) : launch_q4_g<T, 1, 8, 1>(p, st);
+  if (tiles >= 2 * cus) return launch_q4_g<T, 2, 4>(p, st);
+  if (tiles >= cus) return launch_q4_g<T, 2, 8>(p, st);
+  return p.K >= 8192 ? launch_q4_g<T, 1, 16>(p, st) : launch_q4_g<T, 1, 8>(p, st);
 }
 
 int launch_q4(const void* x, const void* q, const void* s, const void* z, const void* bias, void* y,
