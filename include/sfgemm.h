@@ -489,6 +489,13 @@ int sf_linear_q4(const void* x, const void* q, const void* scales, const void* z
                  const void* bias, void* y, int64_t rows, int64_t groups, int64_t N, int64_t K, int64_t group,
                  sf_dtype dtype, sf_epilogue epi, void* stream);
 
+/* Diagnostic twin of sf_linear_q4, as sf_gemm_plan is sf_gemm's: writes the
+ * kernel variant that these sizes take on the current device into buf[len]
+ * ("q4 16x32 4 waves, scales in 1": rows and columns of a tile, the waves
+ * that share its K, the parts in which its scales are staged).  Host-only. */
+int sf_linear_q4_plan(int64_t rows, int64_t groups, int64_t N, int64_t K, int64_t group, int zeros, int grouped,
+                      char* buf, int len);
+
 /* The weights themselves, w [groups, N, K] of `dtype`, each rounded once: for
  * sf_gemm or sf_grouped_linear over many rows. */
 int sf_q4_expand(const void* q, const void* scales, const void* zeros, void* w, int64_t groups, int64_t N, int64_t K,

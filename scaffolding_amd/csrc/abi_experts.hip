@@ -398,6 +398,24 @@ int sf_linear_q4(const void* x, const void* q, const void* scales, const void* z
                    static_cast<hipStream_t>(stream));
 }
 
+int sf_linear_q4_plan(int64_t rows, int64_t groups, int64_t N, int64_t K, int64_t group, int zeros, int grouped,
+                      char* buf, int len) {
+  clear_error();
+  if (buf == nullptr || len <= 0) return fail(SF_ERR_INVALID_ARG, "sf_linear_q4_plan: bad buffer");
+  buf[0] = 0;
+  const int rc = q4_check("sf_linear_q4_plan", rows, groups, N, K, group, SF_BF16);
+  if (rc != SF_OK) return rc;
+  if (grouped == 0 && groups != 1)
+    return fail(SF_ERR_INVALID_ARG, "sf_linear_q4_plan: %lld weights need offsets", (long long)groups);
+  if (rows == 0 || N == 0) {
+    snprintf(buf, static_cast<size_t>(len), "noop");
+    return SF_OK;
+  }
+  const Q4Variant v = q4_variant(rows, groups, grouped != 0, N, K, group, zeros != 0);
+  snprintf(buf, static_cast<size_t>(len), "q4 16x%d %d waves, scales in %d", v.columns, v.waves, v.segments);
+  return SF_OK;
+}
+
 int sf_q4_expand(const void* q, const void* scales, const void* zeros, void* w, int64_t groups, int64_t N, int64_t K,
                  int64_t group, sf_dtype dtype, void* stream) {
   clear_error();

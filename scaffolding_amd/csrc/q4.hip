@@ -342,6 +342,12 @@ static void launch_q4_gz(const Q4Params& p, const dim3& g, unsigned lds, hipStre
   }
 }
 
+// Scale rows that a tile of `columns` holds in LDS at a time.
+static int q4_staged(int columns, int64_t scale_rows, bool zeros) {
+  const int fit = kQ4ScaleBytes / (columns * (zeros ? 3 : 2)) / 4 * 4;
+  return scale_rows >= fit ? fit : (scale_rows > 1 ? static_cast<int>(scale_rows) : 1);
+}
+
 template <typename T, int NB, int NW>
 static int launch_q4_g(Q4Params p, hipStream_t st) {
   p.tiles_n = (p.N + 16 * NB - 1) / (16 * NB);
@@ -349,11 +355,8 @@ static int launch_q4_g(Q4Params p, hipStream_t st) {
   if (p.offsets != nullptr) gx *= grouped_max_tiles(p.rows, p.groups, 16);
   else gy = (p.rows + 15) / 16;
   if (gx > (int64_t(1) << 22) || gy > 65535) return fail(SF_ERR_UNSUPPORTED, "sf_linear_q4: too many tiles");
-  const int row = 16 * NB * (p.z != nullptr ? 3 : 2);  // LDS bytes of a scale row
-  const int fit = kQ4ScaleBytes / row / 4 * 4;
-  p.sg = p.K / p.G < fit ? p.K / p.G : fit;
-  if (p.sg < 1) p.sg = 1;
-  const unsigned lds = static_cast<unsigned>((p.sg + 3) / 4 * 4 * row);
+  p.sg = q4_staged(16 * NB, p.K / p.G, p.z != nullptr);
+  const unsigned lds = static_cast<unsigned>((p.sg + 3) / 4 * 4 * 16 * NB * (p.z != nullptr ? 3 : 2));
   const dim3 g(static_cast<unsigned>(gx), static_cast<unsigned>(gy));
   if (p.G % 128 == 0) launch_q4_gz<T, NB, NW, 1>(p, g, lds, st);
   else if (p.G == 64) launch_q4_gz<T, NB, NW, 2>(p, g, lds, st);
@@ -375,18 +378,28 @@ static int launch_q4_g(Q4Params p, hipStream_t st) {
 //   64 columns, 8 waves     29.5   8.1  14.8  7.6  39.6  13.5  19.3  65.8  26.1  39.2
 // (32 and 64 rows a tile, the weight unpacked once for them, were slower at
 // every size: 11008 x 4096 x 64 23.9 us at best, x 256 62.5.)
+Q4Variant q4_variant(int64_t rows, int64_t groups, bool grouped, int64_t N, int64_t K, int64_t G, bool zeros) {
+  const int64_t some = groups < rows ? groups : rows;
+  const int64_t reached = !grouped || some < 1 ? 1 : some;  // no groups: all rows are set to 0
+  const int64_t per = rows / reached, blocks = reached * ((per + 15) / 16);
+  const int64_t cus = cu_count_current(), tiles = blocks * ((N + 31) / 32);
+  Q4Variant v;
+  if (per > 32 && 2 * blocks * ((N + 63) / 64) >= 3 * cus) v = {64, K >= 8192 ? 8 : 4, 1};
+  else if (tiles >= cus) v = {32, tiles >= 2 * cus ? 4 : 8, 1};
+  else v = {16, K >= 8192 ? 16 : 8, 1};
+  // as q4_kernel counts them: segments of whole blocks of 128 k
+  const int64_t staged = q4_staged(v.columns, K / G, zeros), per_block = G < 128 ? 128 / G : 1;
+  const int64_t seg = G < 128 ? (staged + per_block - 1) / per_block : staged * (G / 128);
+  v.segments = static_cast<int>(((K + 127) / 128 + seg - 1) / seg);
+  return v;
+}
+
 template <typename T>
 static int launch_q4_t(const Q4Params& p, hipStream_t st) {
-  const int64_t some = p.groups < p.rows ? p.groups : p.rows;
-  const int64_t reached = p.offsets == nullptr || some < 1 ? 1 : some;  // no groups: all rows are set to 0
-  const int64_t per = p.rows / reached, blocks = reached * ((per + 15) / 16);
-  const int64_t cus = cu_count_current();
-  if (per > 32 && 2 * blocks * ((p.N + 63) / 64) >= 3 * cus)
-    return p.K >= 8192 ? launch_q4_g<T, 4, 8>(p, st) : launch_q4_g<T, 4, 4>(p, st);
-  const int64_t tiles = blocks * ((p.N + 31) / 32);
-  if (tiles >= 2 * cus) return launch_q4_g<T, 2, 4>(p, st);
-  if (tiles >= cus) return launch_q4_g<T, 2, 8>(p, st);
-  return p.K >= 8192 ? launch_q4_g<T, 1, 16>(p, st) : launch_q4_g<T, 1, 8>(p, st);
+  const Q4Variant v = q4_variant(p.rows, p.groups, p.offsets != nullptr, p.N, p.K, p.G, p.z != nullptr);
+  if (v.columns == 64) return v.waves == 8 ? launch_q4_g<T, 4, 8>(p, st) : launch_q4_g<T, 4, 4>(p, st);
+  if (v.columns == 32) return v.waves == 8 ? launch_q4_g<T, 2, 8>(p, st) : launch_q4_g<T, 2, 4>(p, st);
+  return v.waves == 16 ? launch_q4_g<T, 1, 16>(p, st) : launch_q4_g<T, 1, 8>(p, st);
 }
 
 int launch_q4(const void* x, const void* q, const void* s, const void* z, const void* bias, void* y,

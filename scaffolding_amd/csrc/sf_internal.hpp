@@ -216,7 +216,13 @@ int launch_act_backward(int act, const void* g, const void* pre, void* out, int6
 int launch_group_colsum(const void* g, const int* offsets, int64_t rows, int64_t groups, int64_t N, void* out,
                         sf_dtype dt, hipStream_t st);
 
-// 4-bit weights (q4.hip).  z NULL: zero points 8; offsets NULL: one weight.
+// 4-bit weights (q4.hip).  The columns of a tile, the waves that share its K,
+// and the parts in which its scales pass through LDS.
+struct Q4Variant {
+  int columns, waves, segments;
+};
+Q4Variant q4_variant(int64_t rows, int64_t groups, bool grouped, int64_t N, int64_t K, int64_t G, bool zeros);
+// z NULL: zero points 8; offsets NULL: one weight.
 int launch_q4(const void* x, const void* q, const void* s, const void* z, const void* bias, void* y,
               const int* offsets, int64_t groups, int64_t rows, int64_t N, int64_t K, int64_t G, sf_dtype dt,
               sf_epilogue epi, hipStream_t st);

@@ -196,3 +196,37 @@ def test_quantize_of_the_largest_weights(zeros):
     back = ox.q4_weight(q, s, z)
     step = np.repeat(np.swapaxes(s, -1, -2), 32, -1).astype(np.float64)
     assert (np.abs(back - w) <= step * (1.001 if zeros else 0.501)).all()
+
+
+# ---- which variant runs ------------------------------------------------------------
+
+def test_the_gpu_tests_reach_every_variant():
+    """On 256 CUs: each tile and wave count, dense and grouped, with scale
+    groups of 32, 64 and 128, with and without zero points, and scales that
+    pass through LDS in one part and in several."""
+    from q4_cases import DENSE, GROUPED, PARTS, plan, variant_cases
+    seen = set()
+    for R, E, N, K, G, zeros, cols, waves in variant_cases():
+        assert plan(R, E, N, K, G, zeros).startswith("q4 16x%d %d waves," % (cols, waves)), (R, E, N, K, G)
+        seen.add((cols, waves, E > 0, min(G, 128), zeros))
+    assert set(DENSE) == set(GROUPED) == {(c, w) for c, w, *_ in seen}
+    assert len(seen) == 6 * 2 * 3 * 2
+    parts = set()
+    for R, E, N, K, G, zeros, n in PARTS:
+        p = plan(R, E, N, K, G, zeros)
+        assert p.endswith("scales in %d" % n), (p, R, N, K)
+        parts.add((p.split("x")[1].split()[0], min(G, 128), n > 1))
+    assert {c for c, _, many in parts if many} == {"16", "32", "64"} and {g for _, g, many in parts if many} == {32, 64, 128}
+
+
+def test_plan_refusals(lib):
+    buf = ctypes.create_string_buffer(96)
+
+    def plan(R=4, E=1, N=16, K=128, G=64, zeros=0, grouped=0, to=buf, n=96):
+        return lib.sf_linear_q4_plan(I64(R), I64(E), I64(N), I64(K), I64(G), zeros, grouped, to, n)
+
+    assert plan() == 0 and buf.value == b"q4 16x16 8 waves, scales in 1"
+    assert plan(R=0) == 0 and buf.value == b"noop"
+    assert plan(n=4) == 0 and buf.value == b"q4 "
+    assert plan(to=None) == -2 and plan(n=0) == -2 and plan(E=2) == -2 and plan(G=48) == -3 and plan(K=100) == -2
+    assert plan(E=0, grouped=1) == 0
