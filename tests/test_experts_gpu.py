@@ -197,6 +197,26 @@ def test_row_exchange(dtype, T, k, D):
     check_bound(raw(dw), prod.sum(2), D * 2.0 ** -24 * np.abs(prod).sum(2) + 1e-30, "weights' gradient")
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,k,D", [(4095, 3, 72), (4096, 1, 1), (4096, 8, 500), (4096, 2, 512), (4099, 3, 513),
+                                   (4099, 8, 331), (5000, 2, 1283), (4200, 1, 2056)])
+def test_row_exchange_gradient_of_many_tokens(dtype, T, k, D):
+    """Tokens enough to fill the GPU: a wave a token, its slots in turn, rows
+    within a wave's columns and past them."""
+    g = cu()
+    rng = np.random.default_rng(T * D)
+    y, gr = rnd(rng, (T * k, D), 1.0, dtype), rnd(rng, (T, D), 1.0, dtype)
+    w = rng.random((T, k)).astype(np.float32)
+    slots = rng.permutation(T * k).reshape(T, k)
+    dy, dw = g.dev_combine_rows_backward(up(gr, dtype), up(y, dtype), ints(slots), f32(w))
+    dy, dw = down(dy), raw(dw)
+    for j in range(k):
+        want = w[:, j, None].astype(np.float64) * gr
+        check_bound(dy[slots[:, j]], want, (out_half_ulp_rel(dtype) + 2.0 ** -23) * np.abs(want) + 2.0 ** -25, "rows")
+        prod = gr.astype(np.float64) * y[slots[:, j]]
+        check_bound(dw[:, j], prod.sum(1), D * 2.0 ** -24 * np.abs(prod).sum(1) + 1e-30, "weights")
+
+
 def test_row_exchange_empty_and_skipped():
     g = cu()
     assert g.dev_dispatch_rows(g.empty((0, 8)), ints(np.zeros((0, 2)))).shape == (0, 8)
@@ -391,6 +411,56 @@ def test_grouped_empty(R, E, N, K):
     dx, dw, db = g.dev_grouped_linear_backward(z[3], z[0], z[1], off)
     assert dx.shape == (R, K) and dw.shape == (E, N, K) and db.shape == (E, N)
     assert all((down(t) == 0).all() for t in (dx, dw, db))
+
+
+def whole(rng, *shape):
+    """Whole numbers of at most 3: every sum of their products is exact in
+    fp32 up to 2^24 / 9 of them."""
+    return rng.integers(-3, 4, shape, dtype=np.int8).astype(np.float32)
+
+
+@pytest.mark.parametrize("N,K", [(2 ** 18 + 3, 1025), (1030, 2 ** 18 + 2)])
+def test_fp32_weights_past_the_direct_loads(N, K):
+    """One weight of more than 2^28 numbers: the register-staged tiles, and the
+    small blocks for a few rows, forward and dX."""
+    g = cu()
+    rng = np.random.default_rng(N)
+    w = whole(rng, 1, N, K)
+    wt = f32(w)
+    n, m = rng.integers(0, N, 40), rng.integers(0, K, 40)
+    n[:3], m[:3] = (0, N - 1, N - 2), (0, K - 1, K - 2)
+    for R, used in ((3, 3), (65, 61)):  # rows behind the only group too
+        x, gr, off = whole(rng, R, K), whole(rng, R, N), ints([0, used])
+        y = raw(g.dev_grouped_linear(f32(x), wt, off))
+        assert np.array_equal(y[:used][:, n], x[:used].astype(np.float64) @ w[0][n].T.astype(np.float64))
+        assert (y[used:] == 0).all()
+        out = g.empty((R, K))
+        a = f32(gr)
+        lib = ctypes.CDLL(os.path.join(ROOT, "scaffolding_amd", "libsfgemm.so"))
+        assert lib.sf_grouped_linear_dx(P(a.data_ptr), P(wt.data_ptr), P(off.data_ptr), P(out.data_ptr), I64(R), I64(1),
+                                        I64(N), I64(K), 0, None) == 0
+        dx = raw(out)
+        assert np.array_equal(dx[:used][:, m], gr[:used].astype(np.float64) @ w[0][:, m].astype(np.float64))
+        assert (dx[used:] == 0).all()
+
+
+@pytest.mark.parametrize("N,K", [(2 ** 22 + 5, 3), (5, 2 ** 22 + 4)])
+def test_fp32_weight_gradients_past_the_direct_loads(N, K):
+    """Rows of so many numbers that all of them pass 2 GiB: dW by the
+    register-staged tiles, an empty group and rows of none among them."""
+    g = cu()
+    rng = np.random.default_rng(N)
+    R, off = 66, [0, 20, 20, 63]
+    x, gr = whole(rng, R, K), whole(rng, R, N)
+    a, b, o = f32(gr), f32(x), ints(off)
+    dw, db = g.empty((3, N, K)), g.empty((3, N))
+    lib = ctypes.CDLL(os.path.join(ROOT, "scaffolding_amd", "libsfgemm.so"))
+    assert lib.sf_grouped_linear_dw(P(a.data_ptr), P(b.data_ptr), P(o.data_ptr), P(dw.data_ptr), P(db.data_ptr), I64(R),
+                                    I64(3), I64(N), I64(K), 0, None) == 0
+    dw, db = raw(dw), raw(db)
+    for e in range(3):
+        lo, hi = off[e], off[e + 1]
+        assert np.array_equal(dw[e], gr[lo:hi].T @ x[lo:hi]) and np.array_equal(db[e], gr[lo:hi].sum(0))
 
 
 def test_grouped_nan_stays_in_its_group():
