@@ -467,8 +467,11 @@ __global__ __launch_bounds__(256) void combine_kernel(RowsParams p) {
 // its slots one after the other, so its sums are formed per thread and then
 // over the lanes, without a barrier (4096 x 2 rows of 1283 fp16: 16.8 us with a
 // block of four waves a token, 14.0).  Where the tokens are too few for that to
-// fill the GPU (PAIR), a block takes one slot of one token and the waves' sums
-// are joined in their order (387 x 3 rows of 7360 bf16: 36 -> 12 us).
+// fill the GPU (PAIR: below 16 a CU), a block takes one slot of one token and
+// the waves' sums are joined in their order.  bf16, us, PAIR / a wave a token:
+// 512 x 8 rows of 4096 columns 19 / 52, 1024 x 2 of 1283 5.6 / 7.5, 2048 x 8 of
+// 512 7.9 / 13.2, of 1283 35.1 / 35.8; 4095 x 2 of 1283 19.3 / 13.3, of 4096
+// 31.3 / 30.5; 8192 x 8 of 1283 181 / 139, of 4096 253 / 296.
 template <typename T, bool PAIR>
 __global__ __launch_bounds__(256) void combine_backward_kernel(RowsParams p) {
   __shared__ float part[4];
@@ -512,7 +515,7 @@ template <typename T>
 static int launch_rows_t(int op, RowsParams p, hipStream_t st) {
   // threads per token: enough for its columns, at most the block (the gradient:
   // a wave, or the block for each of its slots)
-  const bool pair = op == 2 && p.tokens < 4096;
+  const bool pair = op == 2 && p.tokens < 16 * static_cast<int64_t>(cu_count_current());
   int lg = 0;
   while (lg < (op == 2 && !pair ? 6 : 8) && (8 << lg) < p.D) ++lg;
   p.lg = lg;
