@@ -84,6 +84,14 @@ def test_route(dtype, T, E, k, masked, renorm):
     check_bound(dl, d, bound + out_half_ulp_rel(dtype) * np.abs(d) + 2.0 ** -25, "logits' gradient")
 
 
+@pytest.mark.parametrize("renorm", [True, False])
+@pytest.mark.parametrize("T,E,k,masked", [(90, 100, 6, False), (70, 128, 4, True), (200, 129, 8, True), (66, 256, 16, False), (130, 700, 5, True)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_route_many_experts(dtype, T, E, k, masked, renorm):
+    """Two, four and sixteen logits a lane, in every type."""
+    test_route(dtype, T, E, k, masked, renorm)
+
+
 def test_route_ties_nan_and_infinities():
     g = cu()
     v = np.array([[3, 3, 3, 3], [-0.0, 0.0, -0.0, 0.0], [np.nan, 1, np.nan, 2], [np.inf, 1, 2, np.inf],
@@ -314,6 +322,14 @@ def test_grouped_linear_backward(dtype, R, E, N, K, kind, act):
         if off[e] == off[e + 1]:
             assert (down(got[1])[e] == 0).all() and (down(got[2])[e] == 0).all()
     assert g.dev_grouped_linear_backward(up(gr, dtype), up(x, dtype), up(w, dtype), ints(off), False)[2] is None
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("R,E,N,K,kind,act", [(2000, 2, 1283, 1285, "any", "silu"), (2100, 3, 1285, 1283, "behind", None)])
+def test_grouped_unaligned_128_tiles(dtype, R, E, N, K, kind, act):
+    """Rows that start at any element, enough of them for 128 x 128 tiles."""
+    test_grouped_linear(dtype, R, E, N, K, kind, act)
+    test_grouped_linear_backward(dtype, R, E, N, K, kind, act)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

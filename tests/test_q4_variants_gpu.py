@@ -62,13 +62,12 @@ def the_card_is_whole():
     return cu().get_device_properties(0)["multi_processor_count"] == 256
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
 @pytest.mark.parametrize("i,case", list(enumerate(variant_cases())))
-def test_variant(i, case):
+def test_variant(i, case, dtype):
     R, E, N, K, G, zeros, cols, waves = case
     if the_card_is_whole():
         assert plan(R, E, N, K, G, zeros).startswith("q4 16x%d %d waves," % (cols, waves))
-    # both types for each variant and width of the scale groups
-    dtype = ("bfloat16", "float16")[(i + i // 12) % 2]
     check(R, E, N, K, G, zeros, dtype, (None, "silu", "gelu")[i % 3], 255 if zeros else 8)
 
 
