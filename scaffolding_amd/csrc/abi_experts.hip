@@ -59,8 +59,8 @@ static float tile_us(const TileCost& c, int64_t rows, int64_t reached, int64_t N
 }
 
 // Tile of a grouped product.  `vec`: operands for the 16-byte direct loads;
-// `dma`: for 4-byte ones (fp32).
-static int rows_tile(int64_t rows, int64_t reached, int64_t N, int64_t K, bool vec, bool dma, bool f32,
+// `dma`: for 4-byte ones (fp32); `big`: a bias for the 256 x 256 tiles.
+static int rows_tile(int64_t rows, int64_t reached, int64_t N, int64_t K, bool vec, bool dma, bool big, bool f32,
                      bool b_kmajor) {
   const int64_t cus = cu_count_current();
   if (f32) {
@@ -81,7 +81,7 @@ static int rows_tile(int64_t rows, int64_t reached, int64_t N, int64_t K, bool v
   }
   float best = 3.0e38f;
   int cfg = -1;
-  if (vec && N > 128 && K % 128 == 0 && K >= 128) {
+  if (vec && big && N > 128 && K % 128 == 0 && K >= 128) {
     const int64_t tiles = row_tiles(rows, reached, 256) * cdiv(N, 256), rem = tiles % cus;
     // a short last round runs as quarters (grouped_rows)
     const float last = rem == 0 ? 0.0f : (tiles > cus && 2 * rem <= cus ? 0.7f : 1.0f);
@@ -149,7 +149,9 @@ static int grouped_rows(const char* name, const void* A, const void* B, const vo
                        : K % 8 == 0 && (b_kmajor || N % 8 == 0) && aligned16(A) && aligned16(B) &&
                              N * K < (int64_t(1) << 30) && K < (int64_t(1) << 22);
   const int64_t reached = groups < rows ? (groups > 0 ? groups : 1) : rows;
-  const int cfg = rows_tile(rows, reached, N, K, vec, dma, f32, b_kmajor);
+  // the 256 x 256 tiles load an even group's bias by dwords, straight into LDS
+  const bool big = !epi_has_bias(epi) || (reinterpret_cast<uintptr_t>(bias) & 3) == 0;
+  const int cfg = rows_tile(rows, reached, N, K, vec, dma, big, f32, b_kmajor);
   int bm, bn;
   tile_size(cfg, bm, bn);
   p.tiles_n = static_cast<int>(cdiv(N, bn));

@@ -429,6 +429,47 @@ def test_grouped_empty(R, E, N, K):
     assert all((down(t) == 0).all() for t in (dx, dw, db))
 
 
+def shifted(gt):
+    """A copy of gt one element past the start of its memory: (memory, address)."""
+    g = cu()
+    size = np.dtype(gt.dtype).itemsize
+    room = g.empty((gt.numel + 8,), gt.dtype)
+    lib = ctypes.CDLL(os.path.join(ROOT, "scaffolding_amd", "libsfgemm.so"))
+    assert lib.sf_memcpy_d2d(P(room.data_ptr + size), P(gt.data_ptr), ctypes.c_size_t(gt.nbytes), None) == 0
+    return room, room.data_ptr + size
+
+
+@pytest.mark.parametrize("dtype,R,E,N,K", [
+    ("bfloat16", 30, 3, 72, 136), ("float16", 700, 2, 264, 256), ("float32", 90, 2, 68, 36), ("float32", 1500, 3, 512, 640),
+    ("bfloat16", 9000, 2, 7168, 128),  # 256 x 256 tiles for aligned operands
+])
+@pytest.mark.parametrize("which", ["x", "w", "b", "y", "all"])
+def test_grouped_operands_at_any_element(dtype, R, E, N, K, which):
+    """Through the C ABI, each operand one element past an aligned address."""
+    g = cu()
+    rng = np.random.default_rng(R)
+    x, w, b = rnd(rng, (R, K), 1.0, dtype), rnd(rng, (E, N, K), K ** -0.5, dtype), rnd(rng, (E, N), 1.0, dtype)
+    off = np.array([R * i // (E + 1) for i in range(E + 1)])
+    t = {"x": up(x, dtype), "w": up(w, dtype), "b": up(b, dtype)}
+    t["y"] = g.zeros((R, N), t["x"].dtype)
+    keep = {n: shifted(v) for n, v in t.items() if which in (n, "all")}
+    at = {n: keep[n][1] if n in keep else v.data_ptr for n, v in t.items()}
+    o = ints(off)
+    lib = ctypes.CDLL(os.path.join(ROOT, "scaffolding_amd", "libsfgemm.so"))
+    assert lib.sf_grouped_linear(P(at["x"]), P(at["w"]), P(o.data_ptr), P(at["b"]), P(at["y"]), I64(R), I64(E), I64(N),
+                                 I64(K), SFD[dtype], 1, None) == 0
+    back = g.empty((R, N), t["x"].dtype)
+    assert lib.sf_memcpy_d2d(P(back.data_ptr), P(at["y"]), ctypes.c_size_t(back.nbytes), None) == 0
+    got = down(back)
+    rows = np.unique(np.concatenate([off[:-1], off[1:] - 1, rng.integers(0, off[-1], 60)]))
+    e = np.searchsorted(off[1:], rows, side="right")
+    for i in range(E):
+        xe = x[rows[e == i]].astype(np.float64)
+        y, mag = xe @ w[i].T.astype(np.float64) + b[i], np.abs(xe) @ np.abs(w[i]).T.astype(np.float64)
+        check_bound(got[rows[e == i]], y, gemm_bound(y, mag + np.abs(b[i]), K, dtype))
+    assert (got[off[-1]:] == 0).all()
+
+
 def whole(rng, *shape):
     """Whole numbers of at most 3: every sum of their products is exact in
     fp32 up to 2^24 / 9 of them."""

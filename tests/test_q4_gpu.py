@@ -107,6 +107,37 @@ def test_many_rows_run_the_16_bit_product(E):
     check_bound(got, y, gemm_bound(y, mag, K, "bfloat16"))
 
 
+@pytest.mark.parametrize("N,E", [(96, 0), (97, 0), (200, 3)])
+@pytest.mark.parametrize("which", ["s", "z", "b", "y", "all"])
+def test_operands_at_any_element(N, E, which):
+    """Through the C ABI: scales, zero points, bias and result one element past
+    an aligned address (x and q must be 16-byte aligned)."""
+    g = cu()
+    lib = ctypes.CDLL(os.path.join(ROOT, "scaffolding_amd", "libsfgemm.so"))
+    rng = np.random.default_rng(N)
+    M, K, G, dtype = 21, 320, 64, "bfloat16"
+    lead = (E,) if E else ()
+    x, b = rnd(rng, (M, K), 1.0, dtype), rnd(rng, lead + (N,), 1.0, dtype)
+    q, s, z = weight(rng, lead, N, K, G, dtype, True)
+    off = raw([0, 4, 4, 20], np.int32)
+    t = dict(zip("qsz", device(q, s, z, dtype)), x=up(x, dtype), b=up(b, dtype), y=g.zeros((M, N), g.BFLOAT16))
+    at, keep = {}, []
+    for n, v in t.items():
+        at[n] = v.data_ptr
+        if n in "szby" and which in (n, "all"):
+            size = np.dtype(v.dtype).itemsize
+            room = g.empty((v.numel + 16,), v.dtype)
+            at[n] = room.data_ptr + size
+            assert lib.sf_memcpy_d2d(P(at[n]), P(v.data_ptr), ctypes.c_size_t(v.nbytes), None) == 0
+            keep.append(room)
+    assert lib.sf_linear_q4(P(at["x"]), P(at["q"]), P(at["s"]), P(at["z"]), P(off.data_ptr) if E else None, P(at["b"]),
+                            P(at["y"]), I64(M), I64(max(1, E)), I64(N), I64(K), I64(G), 2, 1, None) == 0
+    back = g.empty((M, N), g.BFLOAT16)
+    assert lib.sf_memcpy_d2d(P(back.data_ptr), P(at["y"]), ctypes.c_size_t(back.nbytes), None) == 0
+    want = g.dev_linear_q4(t["x"], t["q"], t["s"], t["z"], t["b"], None, off if E else None)
+    assert np.array_equal(down(back), down(want))
+
+
 def test_no_memory_left_for_a_16_bit_weight():
     """Many rows run the direct kernel where the 16-bit weight cannot be
     allocated."""
