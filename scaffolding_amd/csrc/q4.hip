@@ -17,8 +17,9 @@
 // in fp32 brings in the scale and takes the offset out.  X comes from one
 // more MFMA with a matrix of ones (exact products, the same fp32 sums), shared
 // by all row blocks of the weight.  The sums run over terms of up to 31 |x|
-// where the result's are up to 15 |x|, in fp32: a few of its steps.  The order (0, 4, 1, 5, 2, 6, 3, 7) of the eight weights
-// of a dword is met by giving x the same order (v_perm).
+// where the result's are up to 15 |x|, in fp32: a few of its steps.  The order
+// (0, 4, 1, 5, 2, 6, 3, 7) of the eight weights of a dword is met by giving x
+// the same order (v_perm).
 //
 // k order.  v_mfma_f32_16x16x32 takes 8 consecutive k from each of four lane
 // groups.  Loaded as it lies, lane group h's 16 bytes are k = 32 h .. 32 h + 31

@@ -390,7 +390,8 @@ class MoE(Module):
     router prefers, and their answers are summed with the router's weights.
     router.weight (E, dim); up.weight (E, hidden, dim), up.bias (E, hidden);
     down.weight (E, dim, hidden), down.bias (E, dim).  x (..., dim) ->
-    (..., dim); seven launches, none of which waits for the group sizes.
+    (..., dim); six launches up to 64 tokens (more for many: routing in two or
+    three, large products in two), none of which waits for the group sizes.
     quantize() replaces the experts' weights by 4-bit ones for decoding.
     Inference, as Linear (F.*_backward give the gradients)."""
 
