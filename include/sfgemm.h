@@ -502,6 +502,70 @@ int sf_q4_expand(const void* q, const void* scales, const void* zeros, void* w, 
                  int64_t group, sf_dtype dtype, void* stream);
 
 /* ------------------------------------------------------------------ */
+/* Causal transformer blocks                                           */
+/* ------------------------------------------------------------------ */
+/* No counterparts in the reference.  A projection's rows are packed: `heads`
+ * query heads of D columns, then `kv_heads` key heads, then as many value
+ * heads. */
+
+typedef enum sf_norm { SF_NORM_RMS = 0, SF_NORM_LAYER = 1 } sf_norm;
+
+/* Norms of queries and keys per head, with the position rotation in the same
+ * pass, from packed rows x [batch * rows, ldx]:
+ *   hat = h r, r = 1 / sqrt(mean(h^2) + eps)            SF_NORM_RMS
+ *   hat = (h - mean) r, r = 1 / sqrt(var(h) + eps)      SF_NORM_LAYER
+ *   n   = hat weight[i] + bias[i]    (i: 0 queries, 1 keys; both [2, D], each
+ *                                     may be NULL)
+ * and the first `rot` columns of n (even, 0 .. D) turned in pairs (a, b) ->
+ * (a c_j - b s_j, b c_j + a s_j): columns (j, j + rot / 2), or (2 j, 2 j + 1)
+ * with `interleaved`.  c and s are the token's row of table [table_rows, rot]
+ * fp32: rot / 2 cosines, then as many sines.  Row i of sequence b stands at
+ * p = lengths[b] + i (lengths int32 [batch], or NULL for 0) and takes the
+ * table's row positions[b rows + i] (int32), or p without positions; a row
+ * that the table does not have turns its pairs to NaN.
+ * Queries go to q + b strideQ + i ldq; keys to k + b strideK + p ldk and
+ * values, unchanged, to v + b strideV + p ldv where 0 <= p < capacity (other
+ * rows are not written): a cache that holds lengths[b] rows takes the new ones
+ * behind them.  v NULL: values are not read (x then needs no columns for
+ * them).  q, k and v may be x's own columns (in place).  fp32 arithmetic, one
+ * rounding.  D <= 256, heads and kv_heads <= 4096, batch * rows <= 2^30. */
+int sf_qk_norm_rope(const void* x, int64_t ldx, void* q, int64_t ldq, int64_t strideQ, void* k, int64_t ldk,
+                    int64_t strideK, void* v, int64_t ldv, int64_t strideV, const float* table, int64_t table_rows,
+                    int64_t rot, const int32_t* positions, const int32_t* lengths, int64_t capacity,
+                    const void* weight, const void* bias, sf_norm norm, float eps, int interleaved, int64_t batch,
+                    int64_t rows, int64_t heads, int64_t kv_heads, int64_t D, sf_dtype dtype, void* stream);
+
+/* Its gradients (without lengths: row i stands at i): grad, x and grad_x are
+ * contiguous packed rows [batch * rows, (heads + 2 kv_heads) D]; grad is that
+ * of the packed result, values included, whose gradient goes through.
+ * grad_weight and grad_bias [2, D] of `dtype` (either may be NULL): fp32 sums
+ * in an order fixed by the sizes.  grad_x may be grad.  `work`:
+ * sf_qk_norm_rope_backward_work bytes of 4-byte aligned device memory,
+ * overwritten (may be NULL without grad_weight and grad_bias). */
+int64_t sf_qk_norm_rope_backward_work(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads, int64_t D,
+                                      int64_t rot);
+int sf_qk_norm_rope_backward(const void* grad, const void* x, const float* table, int64_t table_rows, int64_t rot,
+                             const int32_t* positions, const void* weight, sf_norm norm, float eps, int interleaved,
+                             void* grad_x, void* grad_weight, void* grad_bias, int64_t batch, int64_t rows,
+                             int64_t heads, int64_t kv_heads, int64_t D, sf_dtype dtype, void* work, void* stream);
+
+/* The up side of a gated feed-forward layer: with W [2 F, K] holding the
+ * gate's rows, then the up-projection's (bias [2 F] likewise, or NULL),
+ *   y[m, f] = act(x[m] . W[f] + bias[f]) (x[m] . W[F + f] + bias[F + f])
+ * x [M, K], y [M, F]; act SF_EPI_NONE, SF_EPI_SILU or SF_EPI_GELU_TANH; fp32
+ * sums, one rounding.  pre [M, 2 F] (or NULL) takes the two projections,
+ * rounded, for the backward pass; SF_F32 needs it (its products and the gate
+ * are two launches).  M, K <= 2^30, F <= 2^29, at most 2^22 tiles. */
+int sf_gated_linear(const void* x, const void* W, const void* bias, void* y, void* pre, int64_t M, int64_t F, int64_t K,
+                    sf_dtype dtype, sf_epilogue act, void* stream);
+/* The gradient of pre from that of y: grad_pre[m, f] = grad up act'(gate),
+ * grad_pre[m, F + f] = grad act(gate), each rounded once.  The rest is a
+ * linear layer's backward pass over grad_pre (sf_gemm, sf_sum_dim).  grad_pre
+ * may be pre. */
+int sf_gated_backward(const void* grad, const void* pre, void* grad_pre, int64_t M, int64_t F, sf_dtype dtype,
+                      sf_epilogue act, void* stream);
+
+/* ------------------------------------------------------------------ */
 /* Runtime: devices, memory, streams, events                           */
 /* (the CUDA runtime calls _cuda_ops.pyx:33-142 binds directly)        */
 /* ------------------------------------------------------------------ */

@@ -44,6 +44,9 @@ cdef extern from "sfgemm.h" nogil:
         SF_EPI_BIAS_GELU_TANH
         SF_EPI_SILU
         SF_EPI_GELU_TANH
+    ctypedef enum sf_norm:
+        SF_NORM_RMS
+        SF_NORM_LAYER
     int SF_OK
     int SF_ERR_HIP
     int SF_ERR_INVALID_ARG
@@ -143,6 +146,23 @@ cdef extern from "sfgemm.h" nogil:
                      sf_dtype dtype, sf_epilogue epi, void* stream)
     int sf_q4_expand(const void* q, const void* scales, const void* zeros, void* w, int64_t groups, int64_t N,
                      int64_t K, int64_t group, sf_dtype dtype, void* stream)
+    int sf_qk_norm_rope(const void* x, int64_t ldx, void* q, int64_t ldq, int64_t strideQ, void* k, int64_t ldk,
+                        int64_t strideK, void* v, int64_t ldv, int64_t strideV, const float* table,
+                        int64_t table_rows, int64_t rot, const int32_t* positions, const int32_t* lengths,
+                        int64_t capacity, const void* weight, const void* bias, sf_norm norm, float eps,
+                        int interleaved, int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads, int64_t D,
+                        sf_dtype dtype, void* stream)
+    int64_t sf_qk_norm_rope_backward_work(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads, int64_t D,
+                                          int64_t rot)
+    int sf_qk_norm_rope_backward(const void* grad, const void* x, const float* table, int64_t table_rows, int64_t rot,
+                                 const int32_t* positions, const void* weight, sf_norm norm, float eps,
+                                 int interleaved, void* grad_x, void* grad_weight, void* grad_bias, int64_t batch,
+                                 int64_t rows, int64_t heads, int64_t kv_heads, int64_t D, sf_dtype dtype, void* work,
+                                 void* stream)
+    int sf_gated_linear(const void* x, const void* W, const void* bias, void* y, void* pre, int64_t M, int64_t F,
+                        int64_t K, sf_dtype dtype, sf_epilogue act, void* stream)
+    int sf_gated_backward(const void* grad, const void* pre, void* grad_pre, int64_t M, int64_t F, sf_dtype dtype,
+                          sf_epilogue act, void* stream)
     int sf_cast(const void* x, sf_dtype in_dtype, void* y, sf_dtype out_dtype, int64_t n, void* stream)
 
     int sf_get_device_count(int* count)
@@ -1445,6 +1465,236 @@ def dev_grouped_linear_backward(gt_grad, gt_x, gt_weight, gt_offsets, bint has_b
             ret = sf_grouped_linear_dw(pg, px, po, pdw, pdb, R, E, N, K, dt, NULL)
     _check_kernel(ret)
     return grad_x, grad_weight, grad_bias
+
+
+# ================================================================
+#  Causal transformer blocks (no counterparts in the reference)
+# ================================================================
+
+_NORMS = {'rms': 0, 'layer': 1}
+_ACT_EPI = (SF_EPI_NONE, SF_EPI_SILU, SF_EPI_GELU_TANH)
+
+
+cdef tuple _packed_heads(str name, gt, int heads, int kv_heads):
+    """(B, N, D) of a packed projection (..., N, (heads + 2 kv_heads) D)."""
+    shape = tuple(gt.shape)
+    if heads < 1 or kv_heads < 1 or len(shape) not in (2, 3) or shape[-1] % (heads + 2 * kv_heads) != 0 \
+            or shape[-1] == 0:
+        raise ValueError("%s: the projection must be (B, N, (%d + 2 * %d) * D), got %s"
+                         % (name, heads, kv_heads, shape))
+    return (shape[0] if len(shape) == 3 else 1), shape[-2], shape[-1] // (heads + 2 * kv_heads)
+
+
+cdef object _norm_rope_operands(str name, x, table, positions, weight, bias, norm, tuple bnd):
+    B, N, D = bnd
+    if norm not in _NORMS:
+        raise ValueError("%s: norm must be 'rms' or 'layer', got %r" % (name, norm))
+    if table is not None:
+        _need_storage(table, _F32, name, 'table')
+        if len(table.shape) != 2 or table.shape[1] % 2 or table.shape[1] > D or 0 in table.shape:
+            raise ValueError("%s: table must be (rows, an even number of columns up to %d), got %s"
+                             % (name, D, table.shape))
+    if positions is not None:
+        _need_storage(positions, _I32, name, 'positions')
+        if tuple(positions.shape) != ((B, N) if len(x.shape) == 3 else (N,)):
+            raise ValueError("%s: positions must match the rows of %s, got %s" % (name, x.shape, positions.shape))
+    for what, p in (('weight', weight), ('bias', bias)):
+        if p is not None:
+            _same_dtype(x, p, name)
+            if tuple(p.shape) != (2, D):
+                raise ValueError("%s: %s must be (2, %d) (queries, keys), got %s" % (name, what, D, p.shape))
+    _same_device(name, x, (table, positions, weight, bias))
+
+
+def dev_qk_norm_rope(gt_x, int heads, int kv_heads, gt_table=None, gt_weight=None, gt_bias=None, norm='rms',
+                     float eps=1e-6, gt_positions=None, bint interleaved=False):
+    """Per-head norm and rotation of the queries and keys of a packed
+    projection x (B, N, (heads + 2 kv_heads) D) (values go through): weight and
+    bias (2, D), table (P, R) fp32 (R / 2 cosines, then sines, of each position;
+    None: no rotation), positions int32 (B, N) or None for 0 .. N - 1."""
+    name = 'dev_qk_norm_rope'
+    bnd = _packed_heads(name, gt_x, heads, kv_heads)
+    _norm_rope_operands(name, gt_x, gt_table, gt_positions, gt_weight, gt_bias, norm, bnd)
+    cdef int64_t B = bnd[0], N = bnd[1], D = bnd[2]
+    cdef int64_t ld = gt_x.shape[-1]
+    cdef int64_t rows = gt_table.shape[0] if gt_table is not None else 0
+    cdef int64_t rot = gt_table.shape[1] if gt_table is not None else 0
+    cdef sf_dtype dt = _sf_dtype(gt_x.dtype)
+    cdef int64_t es = _itemsize(gt_x.dtype)
+    cdef sf_norm nm = <sf_norm><int>_NORMS[norm]
+    out = _alloc_like(tuple(gt_x.shape), gt_x.dtype, gt_x.device_id)
+    cdef void* px = _ptr(gt_x)
+    cdef char* po = <char*>_ptr(out)
+    cdef float* pt = <float*>_ptr(gt_table) if gt_table is not None else NULL
+    cdef int32_t* pp = <int32_t*>_ptr(gt_positions) if gt_positions is not None else NULL
+    cdef void* pw = _ptr(gt_weight) if gt_weight is not None else NULL
+    cdef void* pb = _ptr(gt_bias) if gt_bias is not None else NULL
+    cdef int ret
+    with nogil:
+        ret = sf_qk_norm_rope(px, ld, po, ld, N * ld, po + heads * D * es, ld, N * ld,
+                              po + (heads + kv_heads) * D * es, ld, N * ld, pt, rows, rot, pp, NULL, N, pw, pb, nm,
+                              eps, interleaved, B, N, heads, kv_heads, D, dt, NULL)
+    _check_kernel(ret)
+    return out
+
+
+cdef object _cache_operands(str name, x, k, v, lengths, int64_t B, int64_t kv_cols):
+    _same_dtype(x, k, name)
+    _same_dtype(x, v, name)
+    if len(k.shape) != 3 or k.shape[0] != B or k.shape[2] != kv_cols or tuple(v.shape) != tuple(k.shape):
+        raise ValueError("%s: the caches must both be (%d, capacity, %d), got %s and %s"
+                         % (name, B, kv_cols, k.shape, v.shape))
+    _need_storage(lengths, _I32, name, 'lengths')
+    if tuple(lengths.shape) != (B,):
+        raise ValueError("%s: lengths must be (%d,), got %s" % (name, B, lengths.shape))
+    _same_device(name, x, (k, v, lengths))
+
+
+def dev_qk_norm_rope_cached(gt_x, int heads, int kv_heads, gt_table, gt_k, gt_v, gt_lengths, gt_weight=None,
+                            gt_bias=None, norm='rms', float eps=1e-6, gt_positions=None, bint interleaved=False):
+    """dev_qk_norm_rope of new tokens x (B, n, ...): row i of sequence b stands
+    at lengths[b] + i (int32 (B,)), and its keys and values go there in the
+    caches k, v (B, capacity, kv_heads D); rows past the capacity are dropped.
+    Returns the queries (B, n, heads D)."""
+    name = 'dev_qk_norm_rope_cached'
+    bnd = _packed_heads(name, gt_x, heads, kv_heads)
+    _norm_rope_operands(name, gt_x, gt_table, gt_positions, gt_weight, gt_bias, norm, bnd)
+    if len(gt_x.shape) != 3:
+        raise ValueError("%s: x must be (B, n, columns), got %s" % (name, gt_x.shape))
+    cdef int64_t B = bnd[0], N = bnd[1], D = bnd[2]
+    _cache_operands(name, gt_x, gt_k, gt_v, gt_lengths, B, kv_heads * D)
+    cdef int64_t cap = gt_k.shape[1], ld = gt_x.shape[-1], kc = kv_heads * D, qc = heads * D
+    cdef int64_t rows = gt_table.shape[0] if gt_table is not None else 0
+    cdef int64_t rot = gt_table.shape[1] if gt_table is not None else 0
+    cdef sf_dtype dt = _sf_dtype(gt_x.dtype)
+    cdef sf_norm nm = <sf_norm><int>_NORMS[norm]
+    out = _alloc_like((int(B), int(N), int(qc)), gt_x.dtype, gt_x.device_id)
+    cdef void* px = _ptr(gt_x)
+    cdef void* po = _ptr(out)
+    cdef void* pk = _ptr(gt_k)
+    cdef void* pv = _ptr(gt_v)
+    cdef int32_t* pl = <int32_t*>_ptr(gt_lengths)
+    cdef float* pt = <float*>_ptr(gt_table) if gt_table is not None else NULL
+    cdef int32_t* pp = <int32_t*>_ptr(gt_positions) if gt_positions is not None else NULL
+    cdef void* pw = _ptr(gt_weight) if gt_weight is not None else NULL
+    cdef void* pb = _ptr(gt_bias) if gt_bias is not None else NULL
+    cdef int ret
+    with nogil:
+        ret = sf_qk_norm_rope(px, ld, po, qc, N * qc, pk, kc, cap * kc, pv, kc, cap * kc, pt, rows, rot, pp, pl, cap,
+                              pw, pb, nm, eps, interleaved, B, N, heads, kv_heads, D, dt, NULL)
+    _check_kernel(ret)
+    return out
+
+
+def dev_qk_norm_rope_backward(gt_grad, gt_x, int heads, int kv_heads, gt_table=None, gt_weight=None, norm='rms',
+                              float eps=1e-6, gt_positions=None, bint interleaved=False):
+    """Gradients of dev_qk_norm_rope from grad, that of its result: (grad_x,
+    grad_weight (2, D), grad_bias (2, D)), the last for norm 'layer' only (else
+    None)."""
+    name = 'dev_qk_norm_rope_backward'
+    bnd = _packed_heads(name, gt_x, heads, kv_heads)
+    _norm_rope_operands(name, gt_x, gt_table, gt_positions, gt_weight, None, norm, bnd)
+    _same_dtype(gt_x, gt_grad, name)
+    _same_device(name, gt_x, (gt_grad,))
+    if tuple(gt_grad.shape) != tuple(gt_x.shape):
+        raise ValueError("%s: grad %s does not match x %s" % (name, gt_grad.shape, gt_x.shape))
+    cdef int64_t B = bnd[0], N = bnd[1], D = bnd[2]
+    cdef int64_t rows = gt_table.shape[0] if gt_table is not None else 0
+    cdef int64_t rot = gt_table.shape[1] if gt_table is not None else 0
+    cdef sf_dtype dt = _sf_dtype(gt_x.dtype)
+    cdef sf_norm nm = <sf_norm><int>_NORMS[norm]
+    cdef int dev = gt_x.device_id
+    out = _alloc_like(tuple(gt_x.shape), gt_x.dtype, dev)
+    dw = _alloc_like((2, int(D)), gt_x.dtype, dev)
+    db = _alloc_like((2, int(D)), gt_x.dtype, dev) if norm == 'layer' else None
+    cdef int64_t need = sf_qk_norm_rope_backward_work(B, N, heads, kv_heads, D, rot)
+    cdef CudaBuffer work = _make_buffer(need if need > 0 else 4, dev)
+    cdef void* px = _ptr(gt_x)
+    cdef void* pg = _ptr(gt_grad)
+    cdef void* po = _ptr(out)
+    cdef void* pdw = _ptr(dw)
+    cdef void* pdb = _ptr(db) if db is not None else NULL
+    cdef void* pk = work.ptr
+    cdef float* pt = <float*>_ptr(gt_table) if gt_table is not None else NULL
+    cdef int32_t* pp = <int32_t*>_ptr(gt_positions) if gt_positions is not None else NULL
+    cdef void* pw = _ptr(gt_weight) if gt_weight is not None else NULL
+    cdef int ret
+    with nogil:
+        ret = sf_qk_norm_rope_backward(pg, px, pt, rows, rot, pp, pw, nm, eps, interleaved, po, pdw, pdb, B, N, heads,
+                                       kv_heads, D, dt, pk, NULL)
+    _check_kernel(ret)
+    return out, dw, db
+
+
+def dev_gated_linear(gt_x, gt_weight, gt_bias=None, activation='silu', bint with_pre=False):
+    """y = act(x @ Wg^T + bg) * (x @ Wu^T + bu), W (2 F, K) holding Wg's rows,
+    then Wu's, b (2 F,) likewise: x (..., K) -> y (..., F), one launch (two in
+    fp32).  with_pre: (y, pre), pre (..., 2 F) the two projections."""
+    name = 'dev_gated_linear'
+    _same_dtype(gt_x, gt_weight, name)
+    if len(gt_x.shape) < 1 or len(gt_weight.shape) != 2 or gt_weight.shape[0] % 2 \
+            or gt_x.shape[-1] != gt_weight.shape[1]:
+        raise ValueError("%s: x must be (..., K) and W (2 F, K), got %s and %s" % (name, gt_x.shape, gt_weight.shape))
+    if activation not in _ACTS:
+        raise ValueError("%s: unknown activation %r" % (name, activation))
+    _same_device(name, gt_x, (gt_weight, gt_bias))
+    cdef int64_t F = gt_weight.shape[0] // 2, K = gt_weight.shape[1]
+    cdef int64_t M = 1
+    for s in gt_x.shape[:-1]:
+        M *= s
+    cdef void* pb = NULL
+    if gt_bias is not None:
+        _same_dtype(gt_x, gt_bias, name)
+        if tuple(gt_bias.shape) != (2 * F,):
+            raise ValueError("%s: bias must be (%d,), got %s" % (name, 2 * F, gt_bias.shape))
+        pb = _ptr(gt_bias)
+    cdef sf_dtype dt = _sf_dtype(gt_x.dtype)
+    cdef sf_epilogue act = <sf_epilogue><int>_ACT_EPI[_ACTS[activation]]
+    lead = tuple(gt_x.shape[:-1])
+    out = _alloc_like(lead + (int(F),), gt_x.dtype, gt_x.device_id)
+    pre = _alloc_like(lead + (int(2 * F),), gt_x.dtype, gt_x.device_id) if with_pre or dt == SF_F32 else None
+    cdef void* px = _ptr(gt_x)
+    cdef void* pw = _ptr(gt_weight)
+    cdef void* py = _ptr(out)
+    cdef void* pp = _ptr(pre) if pre is not None else NULL
+    cdef int ret
+    with nogil:
+        ret = sf_gated_linear(px, pw, pb, py, pp, M, F, K, dt, act, NULL)
+    _check_kernel(ret)
+    return (out, pre) if with_pre else out
+
+
+def dev_gated_linear_backward(gt_grad, gt_x, gt_weight, gt_pre, bint has_bias=False, activation='silu'):
+    """Gradients of dev_gated_linear from grad (..., F): (grad_x, grad_weight
+    (2 F, K), grad_bias (2 F,) or None).  The projections' gradient is rounded
+    to the operands' dtype ahead of the products, as a separate gate's is."""
+    name = 'dev_gated_linear_backward'
+    for o in (gt_x, gt_weight, gt_pre):
+        _same_dtype(gt_grad, o, name)
+    _same_device(name, gt_grad, (gt_x, gt_weight, gt_pre))
+    if activation not in _ACTS:
+        raise ValueError("%s: unknown activation %r" % (name, activation))
+    if len(gt_weight.shape) != 2 or gt_weight.shape[0] % 2 or len(gt_x.shape) < 1 or len(gt_grad.shape) < 1:
+        raise ValueError("%s: g must be (..., F), x (..., K) and W (2 F, K)" % name)
+    cdef int64_t F = gt_weight.shape[0] // 2, K = gt_weight.shape[1]
+    lead = tuple(gt_x.shape[:-1])
+    if gt_x.shape[-1] != K or tuple(gt_grad.shape) != lead + (F,) or tuple(gt_pre.shape) != lead + (2 * F,):
+        raise ValueError("%s: g %s, x %s, pre %s and W %s not aligned"
+                         % (name, gt_grad.shape, gt_x.shape, gt_pre.shape, gt_weight.shape))
+    cdef int64_t M = 1
+    for s in lead:
+        M *= s
+    cdef sf_dtype dt = _sf_dtype(gt_grad.dtype)
+    cdef sf_epilogue act = <sf_epilogue><int>_ACT_EPI[_ACTS[activation]]
+    through = _alloc_like(tuple(gt_pre.shape), gt_grad.dtype, gt_grad.device_id)
+    cdef void* pg = _ptr(gt_grad)
+    cdef void* pp = _ptr(gt_pre)
+    cdef void* pt = _ptr(through)
+    cdef int ret
+    with nogil:
+        ret = sf_gated_backward(pg, pp, pt, M, F, dt, act, NULL)
+    _check_kernel(ret)
+    return dev_linear_backward(through, gt_x, gt_weight, has_bias)
 
 
 # ================================================================

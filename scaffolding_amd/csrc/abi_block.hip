@@ -1,0 +1,251 @@
+// abi_block.hip — C entry points of the causal transformer block: norms of
+// queries and keys with the rotation, gated feed-forward layers, windowed
+// attention.  Argument checks (before any HIP call) and the choice of kernels.
+#include "sf_internal.hpp"
+
+namespace sf {
+
+static bool known(sf_dtype d) { return d == SF_F32 || d == SF_F16 || d == SF_BF16; }
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+static int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+constexpr int64_t kMostRows = int64_t(1) << 30;
+
+// ---- norms of queries and keys ----------------------------------------------
+
+static int norm_rope_check(const char* name, const float* table, int64_t table_rows, int64_t rot, sf_norm norm,
+                           float eps, int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads, int64_t D,
+                           sf_dtype dtype) {
+  if (!known(dtype)) return fail(SF_ERR_INVALID_ARG, "%s: unknown dtype %d", name, (int)dtype);
+  if (norm != SF_NORM_RMS && norm != SF_NORM_LAYER) return fail(SF_ERR_INVALID_ARG, "%s: unknown norm %d", name, (int)norm);
+  if (batch < 0 || rows < 0 || heads < 1 || kv_heads < 1 || D < 1)
+    return fail(SF_ERR_INVALID_ARG, "%s: needs batch, rows >= 0 and heads, kv_heads, D >= 1 (%lld, %lld, %lld, %lld, %lld)",
+                name, (long long)batch, (long long)rows, (long long)heads, (long long)kv_heads, (long long)D);
+  if (D > 256 || heads > 4096 || kv_heads > 4096)
+    return fail(SF_ERR_UNSUPPORTED, "%s: at most 256 columns a head and 4096 heads (D=%lld heads=%lld kv_heads=%lld)",
+                name, (long long)D, (long long)heads, (long long)kv_heads);
+  if (batch > 0 && rows > kMostRows / batch)
+    return fail(SF_ERR_UNSUPPORTED, "%s: batch * rows must be at most 2^30", name);
+  if (rot < 0 || rot > D || (rot & 1))
+    return fail(SF_ERR_INVALID_ARG, "%s: the rotated columns must be an even number up to D (rot=%lld D=%lld)", name,
+                (long long)rot, (long long)D);
+  if (rot > 0 && (table == nullptr || table_rows < 1))
+    return fail(SF_ERR_INVALID_ARG, "%s: the rotation needs a table", name);
+  if (!(eps >= 0.0f) || eps > 3.0e38f) return fail(SF_ERR_INVALID_ARG, "%s: eps must be finite and >= 0", name);
+  return SF_OK;
+}
+
+static void norm_rope_fill(NormRopeArgs& a, const void* x, int64_t ldx, const float* table, int64_t table_rows,
+                           int64_t rot, const int32_t* positions, const void* weight, sf_norm norm, float eps,
+                           int interleaved, int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads, int64_t D) {
+  a = NormRopeArgs{};
+  a.x = x;
+  a.ldx = ldx;
+  a.table = table;
+  a.table_rows = table_rows;
+  a.positions = positions;
+  a.weight = weight;
+  a.batch = batch;
+  a.rows = rows;
+  a.eps = eps;
+  a.heads = (int)heads;
+  a.kv_heads = (int)kv_heads;
+  a.D = (int)D;
+  a.rot = (int)rot;
+  a.layer = norm == SF_NORM_LAYER;
+  a.pairs = interleaved != 0;
+}
+
+// ---- gated feed-forward layers ----------------------------------------------
+
+static int gated_check(const char* name, int64_t M, int64_t F, int64_t K, sf_dtype dtype, sf_epilogue act) {
+  if (!known(dtype)) return fail(SF_ERR_INVALID_ARG, "%s: unknown dtype %d", name, (int)dtype);
+  if (M < 0 || F < 0 || K < 0) return fail(SF_ERR_INVALID_ARG, "%s: negative size", name);
+  if (act != SF_EPI_NONE && act != SF_EPI_SILU && act != SF_EPI_GELU_TANH)
+    return fail(SF_ERR_INVALID_ARG, "%s: the activation must be SF_EPI_NONE, SF_EPI_SILU or SF_EPI_GELU_TANH, got %d",
+                name, (int)act);
+  if (M > kMostRows || F > kMostRows / 2 || K > kMostRows)
+    return fail(SF_ERR_UNSUPPORTED, "%s: M and K must be at most 2^30, F 2^29", name);
+  return SF_OK;
+}
+
+// Tiles of a gated product: lines of W a tile takes are half gate, half up.
+struct GatedTile {
+  int cfg, bm, bn, occ;
+  float tau[4];  // us per 64 k when r workgroups share each CU
+};
+static constexpr GatedTile kGatedDirect[] = {
+    {TILE_MID_128, 128, 128, 2, {0.72f, 1.15f}},
+    {TILE_MID_64, 64, 64, 3, {0.32f, 0.44f, 0.74f}},
+    {TILE_MID_32, 32, 64, 3, {0.22f, 0.30f, 0.48f}},
+};
+static constexpr GatedTile kGatedStaged[] = {
+    {TILE_RAG_128, 128, 128, 2, {0.90f, 1.50f}},
+    {TILE_RAG_64, 64, 64, 4, {0.45f, 0.85f, 1.10f, 1.75f}},
+};
+
+static int gated_tile(int64_t M, int64_t F, int64_t K, bool rows16, bool direct, int& bm, int& bn) {
+  const int64_t cus = cu_count_current();
+  if (rows16 && M <= 16) {  // the weight is read once, as fast as it comes
+    bm = 16;
+    bn = 32;
+    return TILE_SKINNY;
+  }
+  float best = 3.0e38f;
+  int cfg = -1;
+  if (direct && K % 128 == 0 && K >= 128 && F > 64) {
+    const int64_t tiles = cdiv(M, 256) * cdiv(F, 128), rem = tiles % cus;
+    best = (static_cast<float>(tiles / cus) + (rem > 0 ? 1.0f : 0.0f)) * (12.4f + 0.0227f * static_cast<float>(K));
+    cfg = TILE_NT_BIG;
+    bm = bn = 256;
+  }
+  for (int i = 0; i < (direct ? 3 : 2); ++i) {
+    const GatedTile& c = direct ? kGatedDirect[i] : kGatedStaged[i];
+    const int64_t tiles = cdiv(M, c.bm) * cdiv(2 * F, c.bn), slots = c.occ * cus, rem = tiles % slots;
+    float us = static_cast<float>(tiles / slots) * c.tau[c.occ - 1];
+    if (rem > 0) us += c.tau[cdiv(rem, cus) - 1];
+    us = us * static_cast<float>(cdiv(K, 64)) + 5.0f;  // launch, first loads, epilogue
+    if (us < best) {
+      best = us;
+      cfg = c.cfg;
+      bm = c.bm;
+      bn = c.bn;
+    }
+  }
+  return cfg;
+}
+
+static int gated16(const void* x, const void* W, const void* bias, void* y, void* pre, int64_t M, int64_t F, int64_t K,
+                   sf_dtype dtype, sf_epilogue act, hipStream_t st) {
+  GatedParams p{};
+  p.A = x;
+  p.B = W;
+  p.C = y;
+  p.bias = bias;
+  p.pre = pre;
+  p.lda = p.ldb = K;
+  p.ldc = F;
+  p.M = (int)M;
+  p.N = (int)(2 * F);
+  p.F = (int)F;
+  p.K = (int)K;
+  p.alpha = 1.0f;
+  p.epi = bias == nullptr ? act
+          : act == SF_EPI_SILU ? SF_EPI_BIAS_SILU
+          : act == SF_EPI_GELU_TANH ? SF_EPI_BIAS_GELU_TANH : SF_EPI_BIAS;
+  const bool rows16 = K % 8 == 0 && aligned16(x) && aligned16(W);
+  // the direct loads' 32-bit offsets reach 2 GiB of either operand
+  const bool direct = rows16 && K > 0 && 2 * F * K < kMostRows && M * K < kMostRows;
+  int bm = 0, bn = 0;
+  const int cfg = gated_tile(M, F, K, rows16, direct, bm, bn);
+  p.tiles_m = (int)cdiv(M, bm);
+  p.tiles_n = (int)cdiv(2 * F, bn);
+  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, cus = cu_count_current();
+  if (tiles > (int64_t(1) << 22)) return fail(SF_ERR_UNSUPPORTED, "sf_gated_linear: more than 2^22 tiles");
+  // One workgroup a CU walks the tiles where the last round is at most half
+  // full, as sf_gemm's.
+  if (cfg == TILE_NT_BIG && tiles > cus && cus % kNumXcd == 0 && 2 * (tiles % cus) <= cus) p.persist = (int)cus;
+  const unsigned gx = p.persist > 0 ? (unsigned)p.persist : (unsigned)tiles;
+  return dtype == SF_BF16 ? launch_gated_bf16(cfg, p, gx, st) : launch_gated_f16(cfg, p, gx, st);
+}
+
+}  // namespace sf
+
+using namespace sf;
+
+extern "C" {
+
+int sf_qk_norm_rope(const void* x, int64_t ldx, void* q, int64_t ldq, int64_t strideQ, void* k, int64_t ldk,
+                    int64_t strideK, void* v, int64_t ldv, int64_t strideV, const float* table, int64_t table_rows,
+                    int64_t rot, const int32_t* positions, const int32_t* lengths, int64_t capacity,
+                    const void* weight, const void* bias, sf_norm norm, float eps, int interleaved, int64_t batch,
+                    int64_t rows, int64_t heads, int64_t kv_heads, int64_t D, sf_dtype dtype, void* stream) {
+  clear_error();
+  const char* name = "sf_qk_norm_rope";
+  const int rc = norm_rope_check(name, table, table_rows, rot, norm, eps, batch, rows, heads, kv_heads, D, dtype);
+  if (rc != SF_OK || batch == 0 || rows == 0) return rc;
+  if (x == nullptr || q == nullptr || k == nullptr) return fail(SF_ERR_INVALID_ARG, "%s: null pointer", name);
+  if (ldx < (heads + (v != nullptr ? 2 : 1) * kv_heads) * D || ldq < heads * D || ldk < kv_heads * D ||
+      (v != nullptr && ldv < kv_heads * D))
+    return fail(SF_ERR_INVALID_ARG, "%s: a row is shorter than its heads", name);
+  if (strideQ < 0 || strideK < 0 || strideV < 0) return fail(SF_ERR_INVALID_ARG, "%s: negative stride", name);
+  if (capacity < 0 || capacity > kMostRows) return fail(SF_ERR_INVALID_ARG, "%s: capacity out of range", name);
+  NormRopeArgs a;
+  norm_rope_fill(a, x, ldx, table, table_rows, rot, positions, weight, norm, eps, interleaved, batch, rows, heads,
+                 kv_heads, D);
+  a.q = q, a.ldq = ldq, a.sq = strideQ;
+  a.k = k, a.ldk = ldk, a.sk = strideK;
+  a.v = v, a.ldv = ldv, a.sv = strideV;
+  a.lengths = lengths;
+  a.capacity = capacity;
+  a.bias = bias;
+  return launch_norm_rope(a, dtype, false, static_cast<hipStream_t>(stream));
+}
+
+int64_t sf_qk_norm_rope_backward_work(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads, int64_t D,
+                                      int64_t rot) {
+  if (batch < 1 || rows < 1 || heads < 1 || kv_heads < 1 || D < 1 || D > 256 || rot < 0 || rot > D || (rot & 1) ||
+      heads > 4096 || kv_heads > 4096 || rows > kMostRows / batch)
+    return 0;
+  return norm_rope_work(batch, rows, (int)heads, (int)kv_heads, (int)D, (int)rot);
+}
+
+int sf_qk_norm_rope_backward(const void* grad, const void* x, const float* table, int64_t table_rows, int64_t rot,
+                             const int32_t* positions, const void* weight, sf_norm norm, float eps, int interleaved,
+                             void* grad_x, void* grad_weight, void* grad_bias, int64_t batch, int64_t rows,
+                             int64_t heads, int64_t kv_heads, int64_t D, sf_dtype dtype, void* work, void* stream) {
+  clear_error();
+  const char* name = "sf_qk_norm_rope_backward";
+  const int rc = norm_rope_check(name, table, table_rows, rot, norm, eps, batch, rows, heads, kv_heads, D, dtype);
+  if (rc != SF_OK) return rc;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (batch == 0 || rows == 0) {
+    const size_t bytes = static_cast<size_t>(2 * D) * (dtype == SF_F32 ? 4 : 2);
+    int z = grad_weight != nullptr ? launch_zero(grad_weight, bytes, st) : SF_OK;
+    if (z == SF_OK && grad_bias != nullptr) z = launch_zero(grad_bias, bytes, st);
+    return z;
+  }
+  const bool sums = grad_weight != nullptr || grad_bias != nullptr;
+  if (grad == nullptr || x == nullptr || grad_x == nullptr || (sums && work == nullptr))
+    return fail(SF_ERR_INVALID_ARG, "%s: null pointer", name);
+  NormRopeArgs a;
+  const int64_t ld = (heads + 2 * kv_heads) * D;
+  norm_rope_fill(a, x, ld, table, table_rows, rot, positions, weight, norm, eps, interleaved, batch, rows, heads,
+                 kv_heads, D);
+  a.g = grad, a.ldg = ld;
+  a.q = grad_x, a.ldq = ld;
+  a.v = grad_x;  // the values' gradient goes through
+  a.capacity = rows;
+  a.dw = grad_weight, a.db = grad_bias;
+  a.part = sums ? static_cast<float*>(work) : nullptr;
+  return launch_norm_rope(a, dtype, true, st);
+}
+
+int sf_gated_linear(const void* x, const void* W, const void* bias, void* y, void* pre, int64_t M, int64_t F, int64_t K,
+                    sf_dtype dtype, sf_epilogue act, void* stream) {
+  clear_error();
+  const char* name = "sf_gated_linear";
+  int rc = gated_check(name, M, F, K, dtype, act);
+  if (rc != SF_OK || M == 0 || F == 0) return rc;
+  if (y == nullptr || (K > 0 && (x == nullptr || W == nullptr)) || (dtype == SF_F32 && pre == nullptr))
+    return fail(SF_ERR_INVALID_ARG, "%s: null pointer", name);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype != SF_F32) return gated16(x, W, bias, y, pre, M, F, K, dtype, act, st);
+  rc = sf_gemm(0, 1, M, 2 * F, K, 1, x, K > 0 ? K : 1, 0, W, K > 0 ? K : 1, 0, pre, 2 * F, 0, SF_F32, SF_F32, 1.0f,
+               bias, bias != nullptr ? SF_EPI_BIAS : SF_EPI_NONE, stream);
+  if (rc != SF_OK) return rc;
+  return launch_gate(epi_act(act), false, nullptr, pre, y, M, F, dtype, st);
+}
+
+int sf_gated_backward(const void* grad, const void* pre, void* grad_pre, int64_t M, int64_t F, sf_dtype dtype,
+                      sf_epilogue act, void* stream) {
+  clear_error();
+  const char* name = "sf_gated_backward";
+  const int rc = gated_check(name, M, F, 0, dtype, act);
+  if (rc != SF_OK || M == 0 || F == 0) return rc;
+  if (grad == nullptr || pre == nullptr || grad_pre == nullptr)
+    return fail(SF_ERR_INVALID_ARG, "%s: null pointer", name);
+  return launch_gate(epi_act(act), true, grad, pre, grad_pre, M, F, dtype, static_cast<hipStream_t>(stream));
+}
+
+}  // extern "C"

@@ -396,26 +396,6 @@ int launch_route_backward(const float* gw, const void* logits, const float* weig
 // columns each at a time; rows may start at any element (16-byte accesses at
 // element alignment).  Slots outside [0, n) are skipped.
 // ---------------------------------------------------------------------
-template <typename T>
-__device__ __forceinline__ void load_cols(const void* p, int64_t i, int left, float v[8]) {
-  if (left >= 8) {
-    load8u<T>(p, i, v);
-  } else {
-#pragma unroll
-    for (int q = 0; q < 8; ++q) v[q] = q < left ? Chunk8<T>::get(p, i + q) : 0.f;
-  }
-}
-template <typename T>
-__device__ __forceinline__ void store_cols(void* p, int64_t i, int left, const float v[8]) {
-  if (left >= 8) {
-    store8u<T>(p, i, v);
-  } else {
-#pragma unroll
-    for (int q = 0; q < 7; ++q)
-      if (q < left) Chunk8<T>::put(p, i + q, v[q]);
-  }
-}
-
 struct RowsParams {
   const void* x;  // dispatch: tokens; combine: rows; its gradient: token gradients
   const void* y;  // combine's gradient: rows
@@ -544,29 +524,8 @@ int launch_rows(int op, const void* x, const void* y, const int* slots, const fl
 }
 
 // ---------------------------------------------------------------------
-// out = g act'(pre), elementwise.
-//   silu'(x) = s (1 + x (1 - s)),  s = 1 / (1 + e^-x)
-//   gelu(x) = x s(z), s the logistic function of z = x (c0 + c1 x^2), so
-//   gelu'(x) = s + x s (1 - s) (c0 + 3 c1 x^2)
-// Past |x| = 80 (silu) and 10 (gelu) both are 1 or 0 in fp32, and short of
-// them e^-x and e^-z are finite; x is cut there, so that an infinite x does not
-// become inf * 0.  NaN passes.
+// out = g act'(pre), elementwise (act_slope).
 // ---------------------------------------------------------------------
-template <int ACT>
-__device__ __forceinline__ float act_slope(float t) {
-  constexpr float top = ACT == ACT_SILU ? 80.f : 10.f;
-  const float x = t > top ? top : (t < -top ? -top : t);
-  if constexpr (ACT == ACT_SILU) {
-    const float s = fast_rcp(1.0f + fast_exp(-x));
-    return s * __builtin_fmaf(x, 1.0f - s, 1.0f);
-  } else {
-    const float c0 = (float)(2.0 * 0.7978845608028654), c1 = (float)(2.0 * 0.7978845608028654 * 0.044715);
-    const float xx = x * x;
-    const float s = fast_rcp(1.0f + fast_exp(-x * __builtin_fmaf(c1, xx, c0)));
-    return __builtin_fmaf(x * s * (1.0f - s), __builtin_fmaf(3.0f * c1, xx, c0), s);
-  }
-}
-
 // (out may be g or pre, so no pointer is marked as the only one to its memory.)
 template <typename T, int ACT>
 __global__ __launch_bounds__(256) void act_backward_kernel(const void* g, const void* pre, void* out, int64_t n) {

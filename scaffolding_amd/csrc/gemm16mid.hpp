@@ -43,6 +43,7 @@
 // within 3 %; the unaligned accesses themselves are the limit.)
 #pragma once
 
+#include "gated.hpp"
 #include "gemm16nt_pp.hpp"
 #include "grouped.hpp"
 
@@ -55,10 +56,13 @@ struct __attribute__((packed, aligned(2))) Chunk16 {
 };
 
 // Prm: GemmParams, or one of grouped.hpp's (rows in ragged groups, one B and bias
-// each: GroupedRows; one sum over each group's rows: GroupedSums).
+// each: GroupedRows; one sum over each group's rows: GroupedSums), or gated.hpp's
+// GatedParams (both K-contiguous, no split).
 template <typename TIn, typename TOut, int BM, int BN, int WVM, int WVN, int NST, bool A_KM, bool B_KM, bool DMA,
           int OCC, typename Prm = GemmParams>
 __global__ __launch_bounds__(WVM* WVN * 64, OCC) void gemm16mid_kernel(Prm p) {
+  constexpr bool GATED = std::is_same<Prm, GatedParams>::value;
+  static_assert(!GATED || (A_KM && B_KM), "gated products: K-contiguous operands");
   constexpr int NW = WVM * WVN;
   constexpr int BK = 64;
   constexpr int WM = BM / WVM, WN = BN / WVN;
@@ -69,7 +73,8 @@ __global__ __launch_bounds__(WVM* WVN * 64, OCC) void gemm16mid_kernel(Prm p) {
   static_assert((A_KM || BM % 64 == 0) && (B_KM || BN % 64 == 0), "k-row blocks of 64 columns");
   static_assert(DMA || NST == 2, "register-staged loads run one slice ahead");
   constexpr int PITCH = WN * 2 + 16;  // staged output row
-  constexpr int SMEM = NST * STAGE > NW * 16 * PITCH ? NST * STAGE : NW * 16 * PITCH;
+  constexpr int OUT = GATED ? NW * gated_stage_bytes<WN>() : NW * 16 * PITCH;
+  constexpr int SMEM = NST * STAGE > OUT ? NST * STAGE : OUT;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[SMEM];
 
   const int lane = threadIdx.x & 63;
@@ -126,7 +131,7 @@ __global__ __launch_bounds__(WVM* WVN * 64, OCC) void gemm16mid_kernel(Prm p) {
   } else {
     group_tile(tile, p.tiles_m, p.tiles_n, 8, tm, tn);
   }
-  const int m0 = tm * BM, n0 = tn * BN;
+  const int m0 = tm * BM, n0 = tn * (GATED ? BN / 2 : BN);  // GATED: the first column of the product
   if (ROWS && n0 >= N) return;  // a quarter past the last column
   const uint16_t* __restrict__ A = static_cast<const uint16_t*>(p.A) + (ROWS || SUMS ? row0 * p.lda : b * p.sA);
   const uint16_t* __restrict__ B = static_cast<const uint16_t*>(p.B) + (SUMS ? row0 * p.ldb : b * p.sB);
@@ -153,7 +158,11 @@ __global__ __launch_bounds__(WVM* WVN * 64, OCC) void gemm16mid_kernel(Prm p) {
       constexpr bool KM = ISA ? A_KM : B_KM;
       const int r = line_row(J), base = ISA ? m0 : n0, lim = ISA ? M : N;
       const uint32_t ld2 = (uint32_t)(ISA ? p.lda : p.ldb) * 2u;
-      if constexpr (KM) {
+      if constexpr (GATED && !ISA) {
+        bool in;
+        const int row = gated_row<WN>(r, n0, gated_columns(p), in);
+        vo[I] = in ? (uint32_t)row * ld2 + (uint32_t)(((lane & 7) ^ l3) * 16) : OOB;
+      } else if constexpr (KM) {
         vo[I] = base + r < lim ? (uint32_t)(base + r) * ld2 + (uint32_t)(((lane & 7) ^ l3) * 16) : OOB;
       } else {
         const int col = base + (r >> 6) * 64 + mn_chunk(r & 63) * 8;
@@ -199,7 +208,12 @@ __global__ __launch_bounds__(WVM* WVN * 64, OCC) void gemm16mid_kernel(Prm p) {
       const int64_t ld = ISA ? p.lda : p.ldb;
       // row (of ld elements), first element in it, elements valid from there
       int row, col, n_ok;
-      if constexpr (KM) {
+      if constexpr (GATED && !ISA) {
+        bool in;
+        row = gated_row<WN>(r, n0, gated_columns(p), in);
+        col = t * BK + ((lane & 7) ^ l3) * 8;
+        n_ok = in ? K - col : 0;
+      } else if constexpr (KM) {
         row = base + r;
         col = t * BK + ((lane & 7) ^ l3) * 8;
         n_ok = row < lim ? K - col : 0;
@@ -356,6 +370,11 @@ __global__ __launch_bounds__(WVM* WVN * 64, OCC) void gemm16mid_kernel(Prm p) {
     if (tid == 0) __hip_atomic_store(&p.counters[tile], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
 
+  if constexpr (GATED) {
+    gated_store<TIn, FM, FN, WN, false>(p, acc, m0 + wm * WM, n0 + wn * (WN / 2), M, lane,
+                                        smem + wave * gated_stage_bytes<WN>());
+    return;
+  } else {
   // ---- epilogue: alpha, bias, activation, residual; staged through LDS --------
   const bool has_bias = epi_has_bias(epi);
   const float alpha = p.alpha;
@@ -418,6 +437,7 @@ __global__ __launch_bounds__(WVM* WVN * 64, OCC) void gemm16mid_kernel(Prm p) {
       }
     }
   });
+  }
 }
 
 }  // namespace sf

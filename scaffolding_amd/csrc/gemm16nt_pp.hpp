@@ -77,6 +77,7 @@
 // instead of one part reading every partial through one CU.
 #pragma once
 
+#include "gated.hpp"
 #include "gemm16.hpp"
 #include "grouped.hpp"
 
@@ -124,17 +125,6 @@ __device__ __forceinline__ u32x2 ds_read_tr16(uint32_t addr) {
   return v;
 }
 
-// Orders a wave's LDS writes before its later LDS reads of other lanes'
-// data (and the reads before later writes).  A wave's LDS instructions
-// execute in issue order, so this only has to stop the compiler from
-// moving accesses across it; no workgroup barrier is needed for data that
-// never leaves the wave.
-__device__ __forceinline__ void wave_lds_sync() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 __device__ __forceinline__ uint32_t lds_addr(const void* p) {
   return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
 }
@@ -146,7 +136,8 @@ constexpr int waitcnt_imm(int vm, int lgkm) {
 }
 
 // Prm: GemmParams, or grouped.hpp's GroupedRows (K-contiguous A) or GroupedSums
-// (both M/N-contiguous), one tile per workgroup.
+// (both M/N-contiguous), one tile per workgroup, or gated.hpp's GatedParams (both
+// K-contiguous, no split).
 // NSTAGE = 2, the pipelined kernel above: K % 128 == 0.  (K == 64 runs
 // gemm16nt_k64_kernel, which holds four workgroups per CU.)
 template <typename TIn, typename TOut, int NSTAGE = 2, bool A_KM = true, bool B_KM = true, bool PERSIST = false,
@@ -173,6 +164,8 @@ __global__ __launch_bounds__(512) void gemm16nt_pp_kernel(Prm p) {
 
   constexpr bool ROWS = std::is_same<Prm, GroupedRows>::value, SUMS = std::is_same<Prm, GroupedSums>::value;
   static_assert(!(ROWS || SUMS) || !PERSIST, "grouped products: one tile per workgroup");
+  constexpr bool GATED = std::is_same<Prm, GatedParams>::value;
+  static_assert(!GATED || (A_KM && B_KM && !SHARED), "gated products: K-contiguous operands, no split");
   const int N = p.N;
   typename GroupVar<ROWS>::type M = p.M;
   typename GroupVar<SUMS>::type K = p.K;
@@ -215,7 +208,7 @@ __global__ __launch_bounds__(512) void gemm16nt_pp_kernel(Prm p) {
       group_tile(pid, p.tiles_m, p.tiles_n, 8, tm, tn);
     }
     jb.m0 = tm * BM;
-    jb.n0 = tn * BN;
+    jb.n0 = tn * (GATED ? BN / 2 : BN);  // GATED: the first column of the product
     jb.part = q;
     jb.split_tile = st;
     if (q >= 0) {
@@ -318,7 +311,7 @@ __global__ __launch_bounds__(512) void gemm16nt_pp_kernel(Prm p) {
   // loads the bias in the epilogue as before, and so does the NN layout
   // (dX = dY W has no bias; the persistent NN kernel has no registers to
   // spare for the next job's bias area).
-  const bool bias_lds = B_KM && epi_has_bias(p.epi) && (N & 1) == 0;
+  const bool bias_lds = !GATED && B_KM && epi_has_bias(p.epi) && (N & 1) == 0;
   const __amdgpu_buffer_rsrc_t rBias = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<void*>(bias), (short)0, (int)((uint32_t)N * 2u), 0x00020000);
   auto bias_dma = [&](int bn0, int area) {
@@ -344,8 +337,13 @@ __global__ __launch_bounds__(512) void gemm16nt_pp_kernel(Prm p) {
   if constexpr (B_KM) {
 #pragma unroll
     for (int i = 0; i < DMA_I; ++i) {
-      const int gb = n0 + drow + i * 8;
-      vob[i] = (uint32_t)(gb < N ? gb : N - 1) * (uint32_t)p.ldb * 2u + dchunk_b;
+      if constexpr (GATED) {
+        bool in;
+        vob[i] = (uint32_t)gated_row<WN>(drow + i * 8, n0, gated_columns(p), in) * (uint32_t)p.ldb * 2u + dchunk_b;
+      } else {
+        const int gb = n0 + drow + i * 8;
+        vob[i] = (uint32_t)(gb < N ? gb : N - 1) * (uint32_t)p.ldb * 2u + dchunk_b;
+      }
     }
   } else {
     vob[0] = ((uint32_t)mrow * (uint32_t)p.ldb + (uint32_t)(n0 + mch * 8)) * 2u;
@@ -370,8 +368,13 @@ __global__ __launch_bounds__(512) void gemm16nt_pp_kernel(Prm p) {
       if constexpr (B_KM) {
 #pragma unroll
         for (int i = 0; i < DMA_I; ++i) {
-          const int gb = bn0 + frow + i * 8;
-          vob[i] = (uint32_t)(gb < N ? gb : N - 1) * (uint32_t)p.ldb * 2u + fch;
+          if constexpr (GATED) {
+            bool in;
+            vob[i] = (uint32_t)gated_row<WN>(frow + i * 8, bn0, gated_columns(p), in) * (uint32_t)p.ldb * 2u + fch;
+          } else {
+            const int gb = bn0 + frow + i * 8;
+            vob[i] = (uint32_t)(gb < N ? gb : N - 1) * (uint32_t)p.ldb * 2u + fch;
+          }
         }
       } else {
         const int fmrow = wave * 8 + (fl >> 3);
@@ -632,6 +635,14 @@ __global__ __launch_bounds__(512) void gemm16nt_pp_kernel(Prm p) {
   }
 
   // ---- epilogue ------------------------------------------------------------
+  if constexpr (GATED) {
+    // staged through stage 1 (a persistent launch loads the next tile's first
+    // pair into stage 0), once every wave has read its last fragments
+    __syncthreads();
+    gated_store<TIn, FM, FN, WN, true>(p, acc, m0 + wm * WM, n0 + wn * (WN / 2), M, elane,
+                                       ((wave >> 2) ? sB1 : sA1) + (wave & 3) * (OP_BYTES / 4));
+    static_assert(gated_stage_bytes<WN>() <= OP_BYTES / 4, "a wave's share of stage 1");
+  } else {
   const bool has_bias = epi_has_bias(p.epi);
   const int act = epi_act(p.epi);
   const float alpha = p.alpha;
@@ -825,6 +836,7 @@ __global__ __launch_bounds__(512) void gemm16nt_pp_kernel(Prm p) {
       epilogue(std::false_type{});
   } else {
     epilogue(std::false_type{});
+  }
   }
   if (!has_next) break;
   // every wave is done with the staging area (stage 1) before the next

@@ -100,4 +100,24 @@ __device__ __forceinline__ void store8u(void* base, int64_t i, const float v[8])
   }
 }
 
+template <typename T>
+__device__ __forceinline__ void load_cols(const void* p, int64_t i, int left, float v[8]) {
+  if (left >= 8) {
+    load8u<T>(p, i, v);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = q < left ? Chunk8<T>::get(p, i + q) : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store_cols(void* p, int64_t i, int left, const float v[8]) {
+  if (left >= 8) {
+    store8u<T>(p, i, v);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 7; ++q)
+      if (q < left) Chunk8<T>::put(p, i + q, v[q]);
+  }
+}
+
 }  // namespace sf

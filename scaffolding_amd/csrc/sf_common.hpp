@@ -109,6 +109,28 @@ __device__ __forceinline__ float act_t(float v) {
     return v;
 }
 
+// Slope of the activation:
+//   silu'(x) = s (1 + x (1 - s)),  s = 1 / (1 + e^-x)
+//   gelu(x) = x s(z), s the logistic function of z = x (c0 + c1 x^2), so
+//   gelu'(x) = s + x s (1 - s) (c0 + 3 c1 x^2)
+// Past |x| = 80 (silu) and 10 (gelu) both are 1 or 0 in fp32, and short of
+// them e^-x and e^-z are finite; x is cut there, so that an infinite x does not
+// become inf * 0.  NaN passes.
+template <int ACT>
+__device__ __forceinline__ float act_slope(float t) {
+  constexpr float top = ACT == ACT_SILU ? 80.f : 10.f;
+  const float x = t > top ? top : (t < -top ? -top : t);
+  if constexpr (ACT == ACT_SILU) {
+    const float s = fast_rcp(1.0f + fast_exp(-x));
+    return s * __builtin_fmaf(x, 1.0f - s, 1.0f);
+  } else {
+    const float c0 = (float)(2.0 * 0.7978845608028654), c1 = (float)(2.0 * 0.7978845608028654 * 0.044715);
+    const float xx = x * x;
+    const float s = fast_rcp(1.0f + fast_exp(-x * __builtin_fmaf(c1, xx, c0)));
+    return __builtin_fmaf(x * s * (1.0f - s), __builtin_fmaf(3.0f * c1, xx, c0), s);
+  }
+}
+
 // Two fp32 values rounded (RNE) to the 16-bit type T and packed, a in the
 // low half: one v_cvt_pk_{f16,bf16}_f32.
 template <typename T>
@@ -208,6 +230,17 @@ __device__ __forceinline__ int lane_id_fresh() {
   int l;
   asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
   return l;
+}
+
+// Orders a wave's LDS writes before its later LDS reads of other lanes'
+// data (and the reads before later writes).  A wave's LDS instructions
+// execute in issue order, so this only has to stop the compiler from
+// moving accesses across it; no workgroup barrier is needed for data that
+// never leaves the wave.
+__device__ __forceinline__ void wave_lds_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
 // Wave-wide sum / max through cross-lane permutes (64 lanes).

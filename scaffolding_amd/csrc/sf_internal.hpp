@@ -6,6 +6,7 @@
 
 #include <atomic>
 
+#include "gated.hpp"
 #include "gemm16.hpp"
 #include "grouped.hpp"
 #include "sf_common.hpp"
@@ -228,5 +229,34 @@ int launch_q4(const void* x, const void* q, const void* s, const void* z, const 
               sf_epilogue epi, hipStream_t st);
 int launch_q4_expand(const void* q, const void* s, const void* z, void* w, int64_t groups, int64_t N, int64_t K,
                      int64_t G, sf_dtype dt, hipStream_t st);
+
+// Norms of queries and keys per head with the rotation (qknorm.hip).
+struct NormRopeArgs {
+  const void* x;        // packed rows: query, key and value heads
+  const void* g;        // backward: the gradient, packed likewise
+  void *q, *k, *v;      // outputs (backward: q is the packed gradient of x); v NULL: values left alone
+  int64_t ldx, ldg, ldq, ldk, ldv, sq, sk, sv;
+  const float* table;   // [table_rows, rot]: cosines, then sines
+  int64_t table_rows;
+  const int32_t* positions;  // of every token, or NULL
+  const int32_t* lengths;    // rows that precede each sequence's in k and v, or NULL
+  int64_t capacity;          // rows of k and v
+  const void *weight, *bias;  // [2, D] or NULL
+  void *dw, *db;
+  float* part;
+  int64_t batch, rows;
+  float eps;
+  int heads, kv_heads, D, rot;
+  bool layer, pairs;
+};
+int launch_norm_rope(const NormRopeArgs& a, sf_dtype dt, bool back, hipStream_t st);
+int64_t norm_rope_work(int64_t batch, int64_t rows, int heads, int kv_heads, int D, int rot);
+
+// Gated feed-forward layers (gated.hpp, gated.hip).
+int launch_gated_bf16(int cfg, const GatedParams& p, unsigned gx, hipStream_t st);
+int launch_gated_f16(int cfg, const GatedParams& p, unsigned gx, hipStream_t st);
+// back: out [M, 2 F] from g [M, F] and pre; otherwise out [M, F] from pre.
+int launch_gate(int act, bool back, const void* g, const void* pre, void* out, int64_t M, int64_t F, sf_dtype dt,
+                hipStream_t st);
 
 }  // namespace sf

@@ -23,12 +23,54 @@
 
 namespace sf {
 
-template <typename TIn, typename TOut, int KSPLIT, int NB, int UNROLL>
-__global__ __launch_bounds__(KSPLIT * 64) void skinny16_kernel(GemmParams p) {
+// The outputs of row m that a lane of a gated skinny block holds (4 consecutive
+// columns of each of NB / 2 blocks).
+template <typename T, int NB>
+__device__ __forceinline__ void gated_skinny_store(const GatedParams& p, const f32x4 (&acc)[NB], int m, int f0,
+                                                   int lane) {
+  const int F = p.F;
+  const bool has_bias = epi_has_bias(p.epi);
+  const bool vec = (F & 3) == 0 && ((reinterpret_cast<uintptr_t>(p.C) | reinterpret_cast<uintptr_t>(p.pre)) & 7) == 0;
+  uint16_t* y = static_cast<uint16_t*>(p.C) + (int64_t)m * F;
+  uint16_t* pre = p.pre != nullptr ? static_cast<uint16_t*>(p.pre) + (int64_t)m * 2 * F : nullptr;
+  with_act(epi_act(p.epi), [&](auto act_c) {
+    constexpr int ACT = decltype(act_c)::value;
+#pragma unroll
+    for (int j = 0; j < NB / 2; ++j) {
+      const int f = f0 + j * 16 + 4 * (lane >> 4);
+      if (f >= F) continue;
+      float g[4], u[4], v[4];
+      float bg[4] = {0.f, 0.f, 0.f, 0.f}, bu[4] = {0.f, 0.f, 0.f, 0.f};
+      if (has_bias) {
+        const uint16_t* b = static_cast<const uint16_t*>(p.bias);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (f + q < F) bg[q] = Elem<T>::to_f32(b[f + q]), bu[q] = Elem<T>::to_f32(b[F + f + q]);
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        g[q] = acc[j][q] + bg[q];
+        u[q] = acc[j + NB / 2][q] + bu[q];
+        v[q] = act_t<ACT>(g[q]) * u[q];
+      }
+      Store4<T>::run(y, f, F, vec, v);
+      if (pre != nullptr) {
+        Store4<T>::run(pre, f, F, vec, g);
+        Store4<T>::run(pre + F, f, F, vec, u);
+      }
+    }
+  });
+}
+
+// Prm: GemmParams, or gated.hpp's GatedParams: the first NB / 2 row blocks are
+// gate rows, the others the up rows of the same 8 NB outputs.
+template <typename TIn, typename TOut, int KSPLIT, int NB, int UNROLL, typename Prm = GemmParams>
+__global__ __launch_bounds__(KSPLIT * 64) void skinny16_kernel(Prm p) {
+  constexpr bool GATED = std::is_same<Prm, GatedParams>::value;
   const int lane = threadIdx.x & 63;
   const int wave = threadIdx.x >> 6;
   const int64_t b = blockIdx.y;
-  const int n0 = blockIdx.x * (16 * NB);
+  const int n0 = blockIdx.x * (GATED ? 8 * NB : 16 * NB);
   const uint16_t* __restrict__ X = static_cast<const uint16_t*>(p.A) + b * p.sA;
   const uint16_t* __restrict__ W = static_cast<const uint16_t*>(p.B) + b * p.sB;
   const int M = p.M, N = p.N, K = p.K;
@@ -47,8 +89,13 @@ __global__ __launch_bounds__(KSPLIT * 64) void skinny16_kernel(GemmParams p) {
   bool wrow_ok[NB];
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
-    int n = n0 + j * 16 + r;
-    wrow_ok[j] = n < N;
+    int n = n0 + (GATED ? j % (NB / 2) : j) * 16 + r;
+    if constexpr (GATED) {
+      wrow_ok[j] = n < p.F;
+      n += j < NB / 2 ? 0 : p.F;
+    } else {
+      wrow_ok[j] = n < N;
+    }
     wrow[j] = W + (int64_t)(wrow_ok[j] ? n : 0) * p.ldb + kc;
   }
 
@@ -93,6 +140,11 @@ __global__ __launch_bounds__(KSPLIT * 64) void skinny16_kernel(GemmParams p) {
       for (int j = 0; j < NB; ++j) acc[j] += red[w][j][lane];
   }
 
+  if constexpr (GATED) {
+    const int m = lane & 15;
+    if (m >= M) return;
+    gated_skinny_store<TIn, NB>(p, acc, m, n0, lane);
+  } else {
   typedef typename Elem<TOut>::storage OutS;
   OutS* C = static_cast<OutS*>(p.C) + b * p.sC;
   const bool has_bias = epi_has_bias(p.epi);
@@ -122,6 +174,7 @@ __global__ __launch_bounds__(KSPLIT * 64) void skinny16_kernel(GemmParams p) {
       Store4<TOut>::run(C + (int64_t)m * p.ldc, n, N, vec_ok, v);
     }
   });
+  }
 }
 
 

@@ -9,6 +9,11 @@
   combine_rows, grouped_linear    experts, with their gradients (no reference
                                   counterparts)
   quantize_q4, linear_q4          4-bit weights (no reference counterpart)
+  rope_table, qk_norm_rope        per-head norms and rotation, over a sequence
+                                  or into a cache, with their gradient (no
+                                  reference counterpart)
+  gated_linear                    gated feed-forward projections, with their
+                                  gradient (no reference counterpart)
 
 GPU only; results carry no grad_fn (as the reference's GPU branches).
 """
@@ -229,3 +234,87 @@ def linear_q4(input: Tensor, qweight: Tensor, scales: Tensor, zeros: Tensor | No
     out = _cuops.dev_linear_q4(input._gpu, _on(qweight, dev), _on(scales, dev), _on(zeros, dev), _on(bias, dev),
                                activation, _on(offsets, dev))
     return Tensor._wrap_gpu(out, input._device)
+
+
+def rope_table(length: int, columns: int, base: float = 10000.0, device=None) -> Tensor:
+    """The rotation's table for positions 0 .. length - 1, fp32 (length,
+    columns): cos(p base^(-2 j / columns)) for j < columns / 2, then the sines.
+    Angles are formed in 64 bits on the host, once; any table of this layout
+    will do (other spacings, several axes)."""
+    if length < 1 or columns < 2 or columns % 2:
+        raise ValueError("rope_table: needs a length and an even number of columns, got %d and %d" % (length, columns))
+    turn = np.arange(length)[:, None] * float(base) ** (-np.arange(0, columns, 2) / columns)
+    return Tensor(np.concatenate([np.cos(turn), np.sin(turn)], 1).astype(np.float32), device=device or "cuda")
+
+
+def qk_norm_rope(qkv: Tensor, heads: int, kv_heads: int, table: Tensor | None, weight: Tensor | None = None,
+                 bias: Tensor | None = None, norm: str = "rms", eps: float = 1e-6, positions: Tensor | None = None,
+                 interleaved: bool = False) -> Tensor:
+    """Norms each query and key head of a packed projection (B, N, (heads + 2
+    kv_heads) D) (norm 'rms' or 'layer'; weight and bias (2, D): queries, keys)
+    and rotates its first R columns by the token's row of `table` (P, R) (see
+    rope_table): columns (j, j + R / 2), or (2 j, 2 j + 1) with `interleaved`.
+    Token i takes row i, or positions[b, i] (int32 (B, N)); a position that the
+    table does not have gives NaN.  Values go through.  D <= 256."""
+    dev = _device_of("qk_norm_rope", qkv, table, weight, bias, positions)
+    out = _cuops.dev_qk_norm_rope(qkv._gpu, heads, kv_heads, _on(table, dev), _on(weight, dev), _on(bias, dev), norm,
+                                  eps, _on(positions, dev), interleaved)
+    return Tensor._wrap_gpu(out, qkv._device)
+
+
+def qk_norm_rope_cached(qkv: Tensor, heads: int, kv_heads: int, table: Tensor | None, k_cache: Tensor,
+                        v_cache: Tensor, lengths: Tensor, weight: Tensor | None = None, bias: Tensor | None = None,
+                        norm: str = "rms", eps: float = 1e-6, positions: Tensor | None = None,
+                        interleaved: bool = False) -> Tensor:
+    """qk_norm_rope of n new tokens a sequence, (B, n, ...), behind the
+    lengths[b] (int32 (B,)) that the caches (B, capacity, kv_heads D) hold: row
+    i stands at lengths[b] + i, its keys and values are written there (rows past
+    the capacity are dropped), and the queries (B, n, heads D) are returned.
+    `lengths` stays as it is."""
+    dev = _device_of("qk_norm_rope_cached", qkv, table, k_cache, v_cache, lengths, weight, bias, positions)
+    _written_on("qk_norm_rope_cached", dev, k_cache, v_cache)
+    out = _cuops.dev_qk_norm_rope_cached(qkv._gpu, heads, kv_heads, _on(table, dev), k_cache._gpu, v_cache._gpu,
+                                         _on(lengths, dev), _on(weight, dev), _on(bias, dev), norm, eps,
+                                         _on(positions, dev), interleaved)
+    return Tensor._wrap_gpu(out, qkv._device)
+
+
+def _written_on(op: str, dev: int, *written) -> None:
+    for t in written:  # a copy would take the writes
+        if t._gpu.device_id != dev:
+            raise ValueError("%s: the caches must be on the device of the new tokens" % op)
+
+
+def qk_norm_rope_backward(grad: Tensor, qkv: Tensor, heads: int, kv_heads: int, table: Tensor | None,
+                          weight: Tensor | None = None, norm: str = "rms", eps: float = 1e-6,
+                          positions: Tensor | None = None, interleaved: bool = False
+                          ) -> tuple[Tensor, Tensor, Tensor | None]:
+    """(grad_qkv, grad_weight (2, D), grad_bias (2, D)) of qk_norm_rope, qkv
+    being its input; the bias's for norm 'layer' only (else None)."""
+    dev = _device_of("qk_norm_rope_backward", qkv, grad, table, weight, positions)
+    out = _cuops.dev_qk_norm_rope_backward(_on(grad, dev), qkv._gpu, heads, kv_heads, _on(table, dev),
+                                           _on(weight, dev), norm, eps, _on(positions, dev), interleaved)
+    return tuple(None if t is None else Tensor._wrap_gpu(t, qkv._device) for t in out)
+
+
+def gated_linear(input: Tensor, weight: Tensor, bias: Tensor | None = None, activation: str | None = "silu",
+                 return_pre: bool = False):
+    """The up side of a gated feed-forward layer, one launch: act(input Wg^T +
+    bg) * (input Wu^T + bu), weight (2 F, K) holding Wg's rows, then Wu's, bias
+    (2 F,) likewise; (..., K) -> (..., F).  return_pre: (output, pre), pre
+    (..., 2 F) the two projections, for gated_linear_backward."""
+    dev = _device_of("gated_linear", input, weight, bias)
+    out = _cuops.dev_gated_linear(input._gpu, _on(weight, dev), _on(bias, dev), activation, return_pre)
+    if return_pre:
+        return tuple(Tensor._wrap_gpu(t, input._device) for t in out)
+    return Tensor._wrap_gpu(out, input._device)
+
+
+def gated_linear_backward(grad: Tensor, input: Tensor, weight: Tensor, pre: Tensor, has_bias: bool = False,
+                          activation: str | None = "silu") -> tuple[Tensor, Tensor, Tensor | None]:
+    """(grad_input, grad_weight, grad_bias or None) of gated_linear; `pre` from
+    return_pre (or linear of the same operands)."""
+    dev = _device_of("gated_linear_backward", input, grad, weight, pre)
+    out = _cuops.dev_gated_linear_backward(_on(grad, dev), input._gpu, _on(weight, dev), _on(pre, dev), has_bias,
+                                           activation)
+    return tuple(None if t is None else Tensor._wrap_gpu(t, input._device) for t in out)
