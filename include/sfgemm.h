@@ -549,6 +549,46 @@ int sf_qk_norm_rope_backward(const void* grad, const void* x, const float* table
                              void* grad_x, void* grad_weight, void* grad_bias, int64_t batch, int64_t rows,
                              int64_t heads, int64_t kv_heads, int64_t D, sf_dtype dtype, void* work, void* stream);
 
+/* Causal attention over a sliding window of keys and a few first ones that
+ * stay visible ("sinks"):
+ *   O[i] = sum_j softmax_j(scale Q[i] . K[j]) V[j] over the keys j <= p_i of
+ *   the sequence with j > p_i - window or j < sinks
+ * p_i being the position of query i; window 0: every key up to p_i.  Query
+ * head h reads key and value head h / (heads / kv_heads) (kv_heads divides
+ * heads).  Row i of entry (b, h) lies at Q + b strideQ + h headQ + i ldq
+ * elements, K and V likewise with kv_heads heads, O as Q.  dtype F16 or BF16,
+ * D a multiple of 8 up to 128, 16-byte aligned rows, a finite scale; row
+ * strides below 2^23, rows and capacity up to 2^29.  fp32 scores, softmax and
+ * sums, the weights rounded to dtype for their product with V, one rounding
+ * of O.  A row that sees no key gives 0; what is not seen does not matter, NaN
+ * and infinities included.  O may not overlap the operands.
+ *
+ * sf_window_attention: query i stands at i over `rows` keys of its own
+ * sequence.  lengths (int32 [batch], or NULL: rows each): keys from lengths[b]
+ * on are not read, and rows from there on give 0.  lse (fp32 [batch, heads,
+ * rows], or NULL) takes ln sum_j exp(scale Q[i] . K[j]), -inf for rows without
+ * a key, for the backward pass. */
+int sf_window_attention(const void* Q, int64_t ldq, int64_t strideQ, int64_t headQ, const void* K, int64_t ldk,
+                        int64_t strideK, int64_t headK, const void* V, int64_t ldv, int64_t strideV, int64_t headV,
+                        void* O, int64_t ldo, int64_t strideO, int64_t headO, float* lse, const int32_t* lengths,
+                        int64_t batch, int64_t heads, int64_t kv_heads, int64_t rows, int64_t D, int64_t window,
+                        int64_t sinks, float scale, sf_dtype dtype, void* stream);
+
+/* Over a cache of `capacity` rows: query i of sequence b stands at lengths[b]
+ * + i and sees keys up to its own, which are there already (sf_qk_norm_rope
+ * writes them).  lengths int32 [batch], cut to [0, capacity].  Few rows over
+ * many keys are split over ranges of the keys: `work` is
+ * sf_window_attention_cached_work bytes of 16-byte aligned device memory of
+ * the call's device (may be NULL where that is 0), overwritten. */
+int64_t sf_window_attention_cached_work(int64_t batch, int64_t heads, int64_t kv_heads, int64_t rows, int64_t capacity,
+                                        int64_t D, int64_t window, int64_t sinks);
+int sf_window_attention_cached(const void* Q, int64_t ldq, int64_t strideQ, int64_t headQ, const void* K, int64_t ldk,
+                               int64_t strideK, int64_t headK, const void* V, int64_t ldv, int64_t strideV,
+                               int64_t headV, void* O, int64_t ldo, int64_t strideO, int64_t headO,
+                               const int32_t* lengths, int64_t batch, int64_t heads, int64_t kv_heads, int64_t rows,
+                               int64_t capacity, int64_t D, int64_t window, int64_t sinks, float scale, sf_dtype dtype,
+                               void* work, void* stream);
+
 /* The up side of a gated feed-forward layer: with W [2 F, K] holding the
  * gate's rows, then the up-projection's (bias [2 F] likewise, or NULL),
  *   y[m, f] = act(x[m] . W[f] + bias[f]) (x[m] . W[F + f] + bias[F + f])

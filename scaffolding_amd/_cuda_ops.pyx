@@ -159,6 +159,21 @@ cdef extern from "sfgemm.h" nogil:
                                  int interleaved, void* grad_x, void* grad_weight, void* grad_bias, int64_t batch,
                                  int64_t rows, int64_t heads, int64_t kv_heads, int64_t D, sf_dtype dtype, void* work,
                                  void* stream)
+    int sf_window_attention(const void* Q, int64_t ldq, int64_t strideQ, int64_t headQ,
+                            const void* K, int64_t ldk, int64_t strideK, int64_t headK,
+                            const void* V, int64_t ldv, int64_t strideV, int64_t headV,
+                            void* O, int64_t ldo, int64_t strideO, int64_t headO, float* lse, const int32_t* lengths,
+                            int64_t batch, int64_t heads, int64_t kv_heads, int64_t rows, int64_t D, int64_t window,
+                            int64_t sinks, float scale, sf_dtype dtype, void* stream)
+    int64_t sf_window_attention_cached_work(int64_t batch, int64_t heads, int64_t kv_heads, int64_t rows,
+                                            int64_t capacity, int64_t D, int64_t window, int64_t sinks)
+    int sf_window_attention_cached(const void* Q, int64_t ldq, int64_t strideQ, int64_t headQ,
+                                   const void* K, int64_t ldk, int64_t strideK, int64_t headK,
+                                   const void* V, int64_t ldv, int64_t strideV, int64_t headV,
+                                   void* O, int64_t ldo, int64_t strideO, int64_t headO, const int32_t* lengths,
+                                   int64_t batch, int64_t heads, int64_t kv_heads, int64_t rows, int64_t capacity,
+                                   int64_t D, int64_t window, int64_t sinks, float scale, sf_dtype dtype, void* work,
+                                   void* stream)
     int sf_gated_linear(const void* x, const void* W, const void* bias, void* y, void* pre, int64_t M, int64_t F,
                         int64_t K, sf_dtype dtype, sf_epilogue act, void* stream)
     int sf_gated_backward(const void* grad, const void* pre, void* grad_pre, int64_t M, int64_t F, sf_dtype dtype,
@@ -1624,6 +1639,99 @@ def dev_qk_norm_rope_backward(gt_grad, gt_x, int heads, int kv_heads, gt_table=N
                                        kv_heads, D, dt, pk, NULL)
     _check_kernel(ret)
     return out, dw, db
+
+
+cdef tuple _window_args(str name, window, sinks, scale, int64_t D, x):
+    """(window, 0 for None; sinks; scale) of a windowed attention."""
+    if window is not None and int(window) < 1:
+        raise ValueError("%s: the window must be None or at least 1, got %r" % (name, window))
+    if int(sinks) < 0:
+        raise ValueError("%s: sinks must be at least 0, got %r" % (name, sinks))
+    if x.dtype is not _F16 and x.dtype is not BFLOAT16 and x.dtype != _F16 and x.dtype != BFLOAT16:
+        raise TypeError("%s: float16 or bfloat16 operands only, got %s" % (name, x.dtype))
+    if D < 8 or D > 128 or D % 8:
+        raise ValueError("%s: the head size must be a multiple of 8 up to 128, got %d" % (name, D))
+    return (0 if window is None else int(window)), int(sinks), \
+        (1.0 / sqrt(<double>D)) if scale is None else float(scale)
+
+
+cdef object _need_lengths(str name, x, lengths, int64_t B):
+    if lengths is not None:
+        _need_storage(lengths, _I32, name, 'lengths')
+        if tuple(lengths.shape) != (B,):
+            raise ValueError("%s: lengths must be (%d,), got %s" % (name, B, lengths.shape))
+        _same_device(name, x, (lengths,))
+
+
+def dev_window_attention(gt_x, int heads, int kv_heads, window=None, sinks=0, scale=None, gt_lengths=None,
+                         bint with_lse=False):
+    """Causal attention of a packed projection x (B, N, (heads + 2 kv_heads) D)
+    -> (B, N, heads D), heads read in place: query i sees the keys j <= i with
+    j > i - window (None: all) or j < sinks.  lengths (int32 (B,)): keys from
+    there on are unseen, rows from there on 0.  with_lse: (out, lse), lse fp32
+    (B, heads, N)."""
+    name = 'dev_window_attention'
+    bnd = _packed_heads(name, gt_x, heads, kv_heads)
+    if heads % kv_heads:
+        raise ValueError("%s: %d heads do not share %d key heads" % (name, heads, kv_heads))
+    cdef int64_t B = bnd[0], N = bnd[1], D = bnd[2]
+    cdef int64_t w, sk
+    cdef float s
+    w, sk, s = _window_args(name, window, sinks, scale, D, gt_x)
+    _need_lengths(name, gt_x, gt_lengths, B)
+    cdef sf_dtype dt = _sf_dtype(gt_x.dtype)
+    cdef int64_t es = 2, ld = gt_x.shape[-1], C = heads * D
+    out = _alloc_like(tuple(gt_x.shape[:-1]) + (int(C),), gt_x.dtype, gt_x.device_id)
+    lse = _alloc_like((int(B), int(heads), int(N)), _F32, gt_x.device_id) if with_lse else None
+    cdef char* px = <char*>_ptr(gt_x)
+    cdef void* po = _ptr(out)
+    cdef float* pl = <float*>_ptr(lse) if lse is not None else NULL
+    cdef int32_t* pn = <int32_t*>_ptr(gt_lengths) if gt_lengths is not None else NULL
+    cdef int ret
+    with nogil:
+        ret = sf_window_attention(px, ld, N * ld, D, px + heads * D * es, ld, N * ld, D,
+                                  px + (heads + kv_heads) * D * es, ld, N * ld, D, po, C, N * C, D, pl, pn, B, heads,
+                                  kv_heads, N, D, w, sk, s, dt, NULL)
+    _check_kernel(ret)
+    return (out, lse) if with_lse else out
+
+
+def dev_window_attention_cached(gt_q, gt_k, gt_v, gt_lengths, int heads, int kv_heads, window=None, sinks=0,
+                                scale=None):
+    """dev_window_attention of new tokens q (B, n, heads D) over caches k, v
+    (B, capacity, kv_heads D): query i of sequence b stands at lengths[b] + i
+    (int32 (B,)), and its own key and value are there already."""
+    name = 'dev_window_attention_cached'
+    if heads < 1 or kv_heads < 1 or heads % kv_heads or len(gt_q.shape) != 3 or gt_q.shape[2] % heads \
+            or gt_q.shape[2] == 0:
+        raise ValueError("%s: q must be (B, n, %d * D) and %d heads share %d key heads, got %s"
+                         % (name, heads, heads, kv_heads, gt_q.shape))
+    cdef int64_t B = gt_q.shape[0], N = gt_q.shape[1], C = gt_q.shape[2]
+    cdef int64_t D = C // heads, kc = kv_heads * D
+    cdef int64_t w, sk
+    cdef float s
+    w, sk, s = _window_args(name, window, sinks, scale, D, gt_q)
+    _cache_operands(name, gt_q, gt_k, gt_v, gt_lengths, B, kc)
+    cdef int64_t cap = gt_k.shape[1]
+    cdef sf_dtype dt = _sf_dtype(gt_q.dtype)
+    out = _alloc_like(tuple(gt_q.shape), gt_q.dtype, gt_q.device_id)
+    cdef int64_t need = sf_window_attention_cached_work(B, heads, kv_heads, N, cap, D, w, sk)
+    cdef CudaBuffer work = None
+    cdef void* pw = NULL
+    if need > 0:
+        work = _make_buffer(need, gt_q.device_id)
+        pw = work.ptr
+    cdef void* pq = _ptr(gt_q)
+    cdef void* pk = _ptr(gt_k)
+    cdef void* pv = _ptr(gt_v)
+    cdef void* po = _ptr(out)
+    cdef int32_t* pn = <int32_t*>_ptr(gt_lengths)
+    cdef int ret
+    with nogil:
+        ret = sf_window_attention_cached(pq, C, N * C, D, pk, kc, cap * kc, D, pv, kc, cap * kc, D, po, C, N * C, D,
+                                         pn, B, heads, kv_heads, N, cap, D, w, sk, s, dt, pw, NULL)
+    _check_kernel(ret)
+    return out
 
 
 def dev_gated_linear(gt_x, gt_weight, gt_bias=None, activation='silu', bint with_pre=False):

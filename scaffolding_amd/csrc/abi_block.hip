@@ -149,6 +149,67 @@ static int gated16(const void* x, const void* W, const void* bias, void* y, void
   return dtype == SF_BF16 ? launch_gated_bf16(cfg, p, gx, st) : launch_gated_f16(cfg, p, gx, st);
 }
 
+// ---- windowed attention -------------------------------------------------------
+
+// Sizes that every entry shares; *noop for an empty call.
+static int window_sizes(const char* name, int64_t batch, int64_t heads, int64_t kv_heads, int64_t rows,
+                        int64_t capacity, int64_t D, int64_t window, int64_t sinks, bool* noop) {
+  *noop = false;
+  if (batch < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || rows < 0 || capacity < 0)
+    return fail(SF_ERR_INVALID_ARG, "%s: needs batch, rows >= 0 and heads a multiple of kv_heads >= 1 (%lld, %lld, %lld, %lld)",
+                name, (long long)batch, (long long)rows, (long long)heads, (long long)kv_heads);
+  if (window < 0 || sinks < 0) return fail(SF_ERR_INVALID_ARG, "%s: negative window or sinks", name);
+  if (D < 8 || D > 128 || D % 8 != 0)
+    return fail(SF_ERR_UNSUPPORTED, "%s: head size %lld (multiples of 8 up to 128)", name, (long long)D);
+  if (rows > kMostRows / 2 || capacity > kMostRows / 2)
+    return fail(SF_ERR_UNSUPPORTED, "%s: at most 2^29 rows", name);
+  if (heads > (1 << 20) || batch > (1 << 24) || batch * heads > kMostRows / ((rows + 127) / 128 + 1))
+    return fail(SF_ERR_UNSUPPORTED, "%s: more than 2^30 blocks of rows", name);
+  *noop = batch == 0 || rows == 0;
+  return SF_OK;
+}
+
+static int window_operand(const char* name, const char* what, const void* p, int64_t ld, int64_t stride, int64_t head,
+                          int64_t D) {
+  if (p == nullptr) return fail(SF_ERR_INVALID_ARG, "%s: null pointer (%s)", name, what);
+  if (ld < D) return fail(SF_ERR_INVALID_ARG, "%s: row stride of %s below the head size", name, what);
+  if (stride < 0 || head < 0) return fail(SF_ERR_INVALID_ARG, "%s: negative stride of %s", name, what);
+  if (!aligned16(p) || ld % 8 || stride % 8 || head % 8)
+    return fail(SF_ERR_UNSUPPORTED, "%s: rows of %s must be 16-byte aligned", name, what);
+  if (ld >= (1 << 23)) return fail(SF_ERR_UNSUPPORTED, "%s: row stride of %s must be below 2^23", name, what);
+  return SF_OK;
+}
+
+static int window_fill(const char* name, WinShape& a, const void* Q, int64_t ldq, int64_t strideQ, int64_t headQ,
+                       const void* K, int64_t ldk, int64_t strideK, int64_t headK, const void* V, int64_t ldv,
+                       int64_t strideV, int64_t headV, void* O, int64_t ldo, int64_t strideO, int64_t headO,
+                       float scale, sf_dtype dtype) {
+  if (!known(dtype)) return fail(SF_ERR_INVALID_ARG, "%s: unknown dtype %d", name, (int)dtype);
+  if (dtype == SF_F32) return fail(SF_ERR_UNSUPPORTED, "%s: 16-bit dtypes only", name);
+  if (!(scale >= -1.0e30f && scale <= 1.0e30f))
+    return fail(SF_ERR_INVALID_ARG, "%s: the scale must be finite (at most 1e30 in size)", name);
+  int rc = window_operand(name, "Q", Q, ldq, strideQ, headQ, a.D);
+  if (rc == SF_OK) rc = window_operand(name, "K", K, ldk, strideK, headK, a.D);
+  if (rc == SF_OK) rc = window_operand(name, "V", V, ldv, strideV, headV, a.D);
+  if (rc == SF_OK) rc = window_operand(name, "O", O, ldo, strideO, headO, a.D);
+  if (rc != SF_OK) return rc;
+  a.Q = Q, a.ldq = ldq, a.sQ = strideQ, a.hQ = headQ;
+  a.K = K, a.ldk = ldk, a.sK = strideK, a.hK = headK;
+  a.V = V, a.ldv = ldv, a.sV = strideV, a.hV = headV;
+  a.O = O, a.ldo = ldo, a.sO = strideO, a.hO = headO;
+  a.scale = scale;
+  return SF_OK;
+}
+
+static void window_shape(WinShape& a, int64_t batch, int64_t heads, int64_t kv_heads, int64_t rows, int64_t capacity,
+                         int64_t D, int64_t window, int64_t sinks) {
+  a = WinShape{};
+  a.batch = batch, a.heads = heads, a.kv_heads = kv_heads;
+  a.Sq = rows, a.Sk = capacity, a.D = D;
+  a.window = window < kMostRows ? window : 0;  // past any position: none
+  a.sinks = sinks < kMostRows ? sinks : kMostRows;
+}
+
 }  // namespace sf
 
 using namespace sf;
@@ -219,6 +280,63 @@ int sf_qk_norm_rope_backward(const void* grad, const void* x, const float* table
   a.dw = grad_weight, a.db = grad_bias;
   a.part = sums ? static_cast<float*>(work) : nullptr;
   return launch_norm_rope(a, dtype, true, st);
+}
+
+int sf_window_attention(const void* Q, int64_t ldq, int64_t strideQ, int64_t headQ, const void* K, int64_t ldk,
+                        int64_t strideK, int64_t headK, const void* V, int64_t ldv, int64_t strideV, int64_t headV,
+                        void* O, int64_t ldo, int64_t strideO, int64_t headO, float* lse, const int32_t* lengths,
+                        int64_t batch, int64_t heads, int64_t kv_heads, int64_t rows, int64_t D, int64_t window,
+                        int64_t sinks, float scale, sf_dtype dtype, void* stream) {
+  clear_error();
+  const char* name = "sf_window_attention";
+  bool noop;
+  int rc = window_sizes(name, batch, heads, kv_heads, rows, rows, D, window, sinks, &noop);
+  if (rc != SF_OK || noop) return rc;
+  WinShape a;
+  window_shape(a, batch, heads, kv_heads, rows, rows, D, window, sinks);
+  rc = window_fill(name, a, Q, ldq, strideQ, headQ, K, ldk, strideK, headK, V, ldv, strideV, headV, O, ldo, strideO,
+                   headO, scale, dtype);
+  if (rc != SF_OK) return rc;
+  a.lse = lse;
+  a.lengths = lengths;
+  return launch_window(a, dtype, nullptr, static_cast<hipStream_t>(stream));
+}
+
+int64_t sf_window_attention_cached_work(int64_t batch, int64_t heads, int64_t kv_heads, int64_t rows, int64_t capacity,
+                                        int64_t D, int64_t window, int64_t sinks) {
+  bool noop;
+  if (window_sizes("", batch, heads, kv_heads, rows, capacity, D, window, sinks, &noop) != SF_OK || noop ||
+      capacity == 0) {
+    clear_error();
+    return 0;
+  }
+  WinShape a;
+  window_shape(a, batch, heads, kv_heads, rows, capacity, D, window, sinks);
+  return win_cached_work(a);
+}
+
+int sf_window_attention_cached(const void* Q, int64_t ldq, int64_t strideQ, int64_t headQ, const void* K, int64_t ldk,
+                               int64_t strideK, int64_t headK, const void* V, int64_t ldv, int64_t strideV,
+                               int64_t headV, void* O, int64_t ldo, int64_t strideO, int64_t headO,
+                               const int32_t* lengths, int64_t batch, int64_t heads, int64_t kv_heads, int64_t rows,
+                               int64_t capacity, int64_t D, int64_t window, int64_t sinks, float scale, sf_dtype dtype,
+                               void* work, void* stream) {
+  clear_error();
+  const char* name = "sf_window_attention_cached";
+  bool noop;
+  int rc = window_sizes(name, batch, heads, kv_heads, rows, capacity, D, window, sinks, &noop);
+  if (rc != SF_OK || noop) return rc;
+  if (capacity == 0) return fail(SF_ERR_INVALID_ARG, "%s: a cache without rows", name);
+  WinShape a;
+  window_shape(a, batch, heads, kv_heads, rows, capacity, D, window, sinks);
+  rc = window_fill(name, a, Q, ldq, strideQ, headQ, K, ldk, strideK, headK, V, ldv, strideV, headV, O, ldo, strideO,
+                   headO, scale, dtype);
+  if (rc != SF_OK) return rc;
+  if (lengths == nullptr || (work == nullptr && win_cached_work(a) > 0))
+    return fail(SF_ERR_INVALID_ARG, "%s: null pointer (lengths or work)", name);
+  a.lengths = lengths;
+  a.cached = 1;
+  return launch_window(a, dtype, static_cast<float*>(work), static_cast<hipStream_t>(stream));
 }
 
 int sf_gated_linear(const void* x, const void* W, const void* bias, void* y, void* pre, int64_t M, int64_t F, int64_t K,

@@ -259,4 +259,19 @@ int launch_gated_f16(int cfg, const GatedParams& p, unsigned gx, hipStream_t st)
 int launch_gate(int act, bool back, const void* g, const void* pre, void* out, int64_t M, int64_t F, sf_dtype dt,
                 hipStream_t st);
 
+// Windowed causal attention (attention_window.hpp): one call's operands.
+struct WinShape {
+  const void *Q, *K, *V;
+  void* O;
+  float* lse;
+  const int32_t* lengths;
+  int64_t ldq, ldk, ldv, ldo, sQ, sK, sV, sO, hQ, hK, hV, hO;
+  int64_t batch, heads, kv_heads, Sq, Sk, D;
+  int64_t window, sinks;  // window 0: none
+  float scale;
+  int cached;
+};
+int launch_window(const WinShape& a, sf_dtype dt, float* ws, hipStream_t st);
+int64_t win_cached_work(const WinShape& a);
+
 }  // namespace sf

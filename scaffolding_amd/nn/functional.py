@@ -12,6 +12,9 @@
   rope_table, qk_norm_rope        per-head norms and rotation, over a sequence
                                   or into a cache, with their gradient (no
                                   reference counterpart)
+  window_attention                causal attention over a window and sinks, over
+                                  a sequence or a cache, with its gradient (no
+                                  reference counterpart)
   gated_linear                    gated feed-forward projections, with their
                                   gradient (no reference counterpart)
 
@@ -295,6 +298,35 @@ def qk_norm_rope_backward(grad: Tensor, qkv: Tensor, heads: int, kv_heads: int, 
     out = _cuops.dev_qk_norm_rope_backward(_on(grad, dev), qkv._gpu, heads, kv_heads, _on(table, dev),
                                            _on(weight, dev), norm, eps, _on(positions, dev), interleaved)
     return tuple(None if t is None else Tensor._wrap_gpu(t, qkv._device) for t in out)
+
+
+def window_attention(qkv: Tensor, heads: int, kv_heads: int, window: int | None = None, sinks: int = 0,
+                     scale: float | None = None, lengths: Tensor | None = None, return_lse: bool = False):
+    """Causal attention of a packed projection (B, N, (heads + 2 kv_heads) D) ->
+    (B, N, heads D): token i sees the tokens j <= i with j > i - window (None:
+    all of them) or j < sinks; heads / kv_heads query heads share a key head;
+    scale defaults to 1 / sqrt(D).  lengths (int32 (B,)) ends each sequence:
+    nothing behind it is seen, and rows behind it give 0.  return_lse: (output,
+    lse), the rows' log-sums fp32 (B, heads, N), for
+    window_attention_backward.  float16 or bfloat16, D a multiple of 8 up to
+    128; one launch, heads read in place."""
+    dev = _device_of("window_attention", qkv, lengths)
+    out = _cuops.dev_window_attention(qkv._gpu, heads, kv_heads, window, sinks, scale, _on(lengths, dev), return_lse)
+    if return_lse:
+        return tuple(Tensor._wrap_gpu(t, qkv._device) for t in out)
+    return Tensor._wrap_gpu(out, qkv._device)
+
+
+def window_attention_cached(q: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: Tensor, heads: int, kv_heads: int,
+                            window: int | None = None, sinks: int = 0, scale: float | None = None) -> Tensor:
+    """window_attention of n new tokens a sequence, q (B, n, heads D), over
+    caches (B, capacity, kv_heads D) to which qk_norm_rope_cached has added
+    theirs: token i of sequence b stands at lengths[b] + i (int32 (B,), the
+    lengths before these tokens)."""
+    dev = _device_of("window_attention_cached", q, k_cache, v_cache, lengths)
+    out = _cuops.dev_window_attention_cached(q._gpu, _on(k_cache, dev), _on(v_cache, dev), _on(lengths, dev), heads,
+                                             kv_heads, window, sinks, scale)
+    return Tensor._wrap_gpu(out, q._device)
 
 
 def gated_linear(input: Tensor, weight: Tensor, bias: Tensor | None = None, activation: str | None = "silu",
