@@ -574,6 +574,27 @@ int sf_window_attention(const void* Q, int64_t ldq, int64_t strideQ, int64_t hea
                         int64_t batch, int64_t heads, int64_t kv_heads, int64_t rows, int64_t D, int64_t window,
                         int64_t sinks, float scale, sf_dtype dtype, void* stream);
 
+/* Gradients of sf_window_attention (the same operands, lengths, window, sinks
+ * and scale; O and lse as it wrote them) from dO, that of O: dQ laid out with
+ * strides of its own, dK and dV with kv_heads heads, summed over the query
+ * heads that share them; 0 for rows behind lengths.  P and dS are rounded to
+ * dtype for their products (dS unscaled: fp16 gradients past 65504 overflow);
+ * sums fp32, in an order fixed by the sizes.  A NaN or infinity reaches the
+ * gradients of the tokens around it.  The gradients may not overlap the
+ * operands or each other.  `work`: sf_window_attention_backward_work bytes of
+ * 256-byte aligned device memory, overwritten. */
+int64_t sf_window_attention_backward_work(int64_t batch, int64_t heads, int64_t kv_heads, int64_t rows, int64_t D,
+                                          int64_t window, int64_t sinks);
+int sf_window_attention_backward(const void* dO, int64_t lddo, int64_t strideDO, int64_t headDO, const void* Q,
+                                 int64_t ldq, int64_t strideQ, int64_t headQ, const void* K, int64_t ldk,
+                                 int64_t strideK, int64_t headK, const void* V, int64_t ldv, int64_t strideV,
+                                 int64_t headV, const void* O, int64_t ldo, int64_t strideO, int64_t headO,
+                                 const float* lse, const int32_t* lengths, void* dQ, int64_t lddq, int64_t strideDQ,
+                                 int64_t headDQ, void* dK, int64_t lddk, int64_t strideDK, int64_t headDK, void* dV,
+                                 int64_t lddv, int64_t strideDV, int64_t headDV, int64_t batch, int64_t heads,
+                                 int64_t kv_heads, int64_t rows, int64_t D, int64_t window, int64_t sinks, float scale,
+                                 sf_dtype dtype, void* work, void* stream);
+
 /* Over a cache of `capacity` rows: query i of sequence b stands at lengths[b]
  * + i and sees keys up to its own, which are there already (sf_qk_norm_rope
  * writes them).  lengths int32 [batch], cut to [0, capacity].  Few rows over

@@ -165,6 +165,18 @@ cdef extern from "sfgemm.h" nogil:
                             void* O, int64_t ldo, int64_t strideO, int64_t headO, float* lse, const int32_t* lengths,
                             int64_t batch, int64_t heads, int64_t kv_heads, int64_t rows, int64_t D, int64_t window,
                             int64_t sinks, float scale, sf_dtype dtype, void* stream)
+    int64_t sf_window_attention_backward_work(int64_t batch, int64_t heads, int64_t kv_heads, int64_t rows, int64_t D,
+                                              int64_t window, int64_t sinks)
+    int sf_window_attention_backward(const void* dO, int64_t lddo, int64_t strideDO, int64_t headDO,
+                                     const void* Q, int64_t ldq, int64_t strideQ, int64_t headQ,
+                                     const void* K, int64_t ldk, int64_t strideK, int64_t headK,
+                                     const void* V, int64_t ldv, int64_t strideV, int64_t headV,
+                                     const void* O, int64_t ldo, int64_t strideO, int64_t headO, const float* lse,
+                                     const int32_t* lengths, void* dQ, int64_t lddq, int64_t strideDQ, int64_t headDQ,
+                                     void* dK, int64_t lddk, int64_t strideDK, int64_t headDK,
+                                     void* dV, int64_t lddv, int64_t strideDV, int64_t headDV, int64_t batch,
+                                     int64_t heads, int64_t kv_heads, int64_t rows, int64_t D, int64_t window,
+                                     int64_t sinks, float scale, sf_dtype dtype, void* work, void* stream)
     int64_t sf_window_attention_cached_work(int64_t batch, int64_t heads, int64_t kv_heads, int64_t rows,
                                             int64_t capacity, int64_t D, int64_t window, int64_t sinks)
     int sf_window_attention_cached(const void* Q, int64_t ldq, int64_t strideQ, int64_t headQ,
@@ -1694,6 +1706,50 @@ def dev_window_attention(gt_x, int heads, int kv_heads, window=None, sinks=0, sc
                                   kv_heads, N, D, w, sk, s, dt, NULL)
     _check_kernel(ret)
     return (out, lse) if with_lse else out
+
+
+def dev_window_attention_backward(gt_grad, gt_x, gt_out, gt_lse, int heads, int kv_heads, window=None, sinks=0,
+                                  scale=None, gt_lengths=None):
+    """Gradient of dev_window_attention's packed projection x, in its layout,
+    from grad, that of its output; out and lse are what it gave for the same
+    arguments."""
+    name = 'dev_window_attention_backward'
+    bnd = _packed_heads(name, gt_x, heads, kv_heads)
+    if heads % kv_heads:
+        raise ValueError("%s: %d heads do not share %d key heads" % (name, heads, kv_heads))
+    cdef int64_t B = bnd[0], N = bnd[1], D = bnd[2]
+    cdef int64_t w, sk
+    cdef float s
+    w, sk, s = _window_args(name, window, sinks, scale, D, gt_x)
+    _need_lengths(name, gt_x, gt_lengths, B)
+    _same_dtype(gt_x, gt_grad, name)
+    _same_dtype(gt_x, gt_out, name)
+    _need_storage(gt_lse, _F32, name, 'lse')
+    want = tuple(gt_x.shape[:-1]) + (heads * D,)
+    if tuple(gt_grad.shape) != want or tuple(gt_out.shape) != want or tuple(gt_lse.shape) != (B, heads, N):
+        raise ValueError("%s: grad %s and out %s must be %s, lse %s (%d, %d, %d)"
+                         % (name, gt_grad.shape, gt_out.shape, want, gt_lse.shape, B, heads, N))
+    _same_device(name, gt_x, (gt_grad, gt_out, gt_lse))
+    cdef sf_dtype dt = _sf_dtype(gt_x.dtype)
+    cdef int64_t es = 2, ld = gt_x.shape[-1], C = heads * D
+    dx = _alloc_like(tuple(gt_x.shape), gt_x.dtype, gt_x.device_id)
+    cdef int64_t need = sf_window_attention_backward_work(B, heads, kv_heads, N, D, w, sk)
+    cdef CudaBuffer work = _make_buffer(need if need > 0 else 4, gt_x.device_id)
+    cdef void* pw = work.ptr
+    cdef char* px = <char*>_ptr(gt_x)
+    cdef char* pd = <char*>_ptr(dx)
+    cdef void* pg = _ptr(gt_grad)
+    cdef void* po = _ptr(gt_out)
+    cdef float* pl = <float*>_ptr(gt_lse)
+    cdef int32_t* pn = <int32_t*>_ptr(gt_lengths) if gt_lengths is not None else NULL
+    cdef int64_t k0 = heads * D * es, v0 = (heads + kv_heads) * D * es
+    cdef int ret
+    with nogil:
+        ret = sf_window_attention_backward(pg, C, N * C, D, px, ld, N * ld, D, px + k0, ld, N * ld, D, px + v0, ld,
+                                           N * ld, D, po, C, N * C, D, pl, pn, pd, ld, N * ld, D, pd + k0, ld, N * ld,
+                                           D, pd + v0, ld, N * ld, D, B, heads, kv_heads, N, D, w, sk, s, dt, pw, NULL)
+    _check_kernel(ret)
+    return dx
 
 
 def dev_window_attention_cached(gt_q, gt_k, gt_v, gt_lengths, int heads, int kv_heads, window=None, sinks=0,

@@ -302,6 +302,52 @@ int sf_window_attention(const void* Q, int64_t ldq, int64_t strideQ, int64_t hea
   return launch_window(a, dtype, nullptr, static_cast<hipStream_t>(stream));
 }
 
+int64_t sf_window_attention_backward_work(int64_t batch, int64_t heads, int64_t kv_heads, int64_t rows, int64_t D,
+                                          int64_t window, int64_t sinks) {
+  bool noop;
+  if (window_sizes("", batch, heads, kv_heads, rows, rows, D, window, sinks, &noop) != SF_OK || noop) {
+    clear_error();
+    return 0;
+  }
+  WinShape a;
+  window_shape(a, batch, heads, kv_heads, rows, rows, D, window, sinks);
+  return win_back_work(a);
+}
+
+int sf_window_attention_backward(const void* dO, int64_t lddo, int64_t strideDO, int64_t headDO, const void* Q,
+                                 int64_t ldq, int64_t strideQ, int64_t headQ, const void* K, int64_t ldk,
+                                 int64_t strideK, int64_t headK, const void* V, int64_t ldv, int64_t strideV,
+                                 int64_t headV, const void* O, int64_t ldo, int64_t strideO, int64_t headO,
+                                 const float* lse, const int32_t* lengths, void* dQ, int64_t lddq, int64_t strideDQ,
+                                 int64_t headDQ, void* dK, int64_t lddk, int64_t strideDK, int64_t headDK, void* dV,
+                                 int64_t lddv, int64_t strideDV, int64_t headDV, int64_t batch, int64_t heads,
+                                 int64_t kv_heads, int64_t rows, int64_t D, int64_t window, int64_t sinks, float scale,
+                                 sf_dtype dtype, void* work, void* stream) {
+  clear_error();
+  const char* name = "sf_window_attention_backward";
+  bool noop;
+  int rc = window_sizes(name, batch, heads, kv_heads, rows, rows, D, window, sinks, &noop);
+  if (rc != SF_OK || noop) return rc;
+  WinShape a;
+  window_shape(a, batch, heads, kv_heads, rows, rows, D, window, sinks);
+  rc = window_fill(name, a, Q, ldq, strideQ, headQ, K, ldk, strideK, headK, V, ldv, strideV, headV,
+                   const_cast<void*>(O), ldo, strideO, headO, scale, dtype);
+  if (rc == SF_OK) rc = window_operand(name, "dO", dO, lddo, strideDO, headDO, D);
+  if (rc == SF_OK) rc = window_operand(name, "dQ", dQ, lddq, strideDQ, headDQ, D);
+  if (rc == SF_OK) rc = window_operand(name, "dK", dK, lddk, strideDK, headDK, D);
+  if (rc == SF_OK) rc = window_operand(name, "dV", dV, lddv, strideDV, headDV, D);
+  if (rc != SF_OK) return rc;
+  if (lse == nullptr || work == nullptr) return fail(SF_ERR_INVALID_ARG, "%s: null pointer (lse or work)", name);
+  a.lse = const_cast<float*>(lse);
+  a.lengths = lengths;
+  WinBack g;
+  g.dO = dO, g.ldg = lddo, g.sG = strideDO, g.hG = headDO;
+  g.dQ = dQ, g.lddq = lddq, g.sDQ = strideDQ, g.hDQ = headDQ;
+  g.dK = dK, g.lddk = lddk, g.sDK = strideDK, g.hDK = headDK;
+  g.dV = dV, g.lddv = lddv, g.sDV = strideDV, g.hDV = headDV;
+  return launch_window_back(a, g, dtype, work, static_cast<hipStream_t>(stream));
+}
+
 int64_t sf_window_attention_cached_work(int64_t batch, int64_t heads, int64_t kv_heads, int64_t rows, int64_t capacity,
                                         int64_t D, int64_t window, int64_t sinks) {
   bool noop;

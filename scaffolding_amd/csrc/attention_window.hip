@@ -8,8 +8,8 @@ static int win_width(int64_t D) { return D <= 64 ? 64 : (D <= 96 ? 96 : 128); }
 
 static int64_t cdiv64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-static WinParams win_params(const WinShape& a) {
-  WinParams p{};
+void win_fill_params(const WinShape& a, WinParams& p) {
+  p = WinParams{};
   p.Q = a.Q, p.K = a.K, p.V = a.V, p.O = a.O;
   p.lse = a.lse;
   p.lengths = a.lengths;
@@ -23,7 +23,6 @@ static WinParams win_params(const WinShape& a) {
   p.cached = a.cached;
   p.QB = (int)cdiv64(a.Sq, WinCfg<64>::ROWS);
   p.scale_log2e = a.scale * 1.4426950408889634f;
-  return p;
 }
 
 // The key ranges of win_split_kernel, or 0 where whole rows of 128 queries are
@@ -83,7 +82,8 @@ static int launch_win(const WinParams& p, int parts, hipStream_t st) {
 }
 
 int launch_window(const WinShape& a, sf_dtype dt, float* ws, hipStream_t st) {
-  WinParams p = win_params(a);
+  WinParams p;
+  win_fill_params(a, p);
   int parts = 0;
   if (a.cached) {
     parts = win_split_parts(a, cu_count_current());

@@ -1,0 +1,491 @@
+// attention_window_bwd.hpp — gradients of win_attn_kernel (attention_window.hpp).
+//
+// With P = exp(scale Q K^T - lse) (0 where a query does not see a key), dO the
+// gradient of O, and delta[i] = dO[i] . O[i]:
+//
+//   dV = P^T dO,  dP = dO V^T,  dS = P (dP - delta),
+//   dQ = scale dS K,  dK = scale dS^T Q
+//
+// Two launches, each forming S and dP again (14 D flop a pair of query and key
+// instead of 10 D): the sums of dQ run over keys, those of dK and dV over
+// queries, so one launch for all would need atomic sums of one of them, whose
+// order changes the bits.
+//
+//   win_dq_kernel   128 query rows a workgroup (32 a wave), Q and dO in
+//                   registers, blocks of 64 keys of K and V through LDS; it
+//                   forms delta first and leaves it for the other launch
+//   win_dkv_kernel  128 keys a workgroup (32 a wave), K and V in registers,
+//                   blocks of 64 rows of Q and dO of every query head of the
+//                   group through LDS, so that the sum over heads needs no
+//                   further launch
+//
+// Both take the forward kernel's operand layouts: scores come out with the
+// summed index (keys here, rows there) across a lane's registers, where the
+// next product wants them, and the other operand of that product is read
+// transposed from the LDS tile that the scores were formed from.
+//
+// P and dS are rounded to the operands' type for the products (half a step
+// each); P of fp16 is held times 2^8, so that the weights of thousands of keys
+// stay normal numbers.  Everything else, sums included, is fp32.
+//
+// Key blocks that far more rows see than others (sinks; the first ones without
+// a window) are cut into parts of their rows, whose fp32 sums a third launch
+// adds in order (win_dkv_merge_kernel).
+#pragma once
+
+#include "attention_window.hpp"
+
+namespace sf {
+
+struct WinBackParams {
+  WinParams w;      // O: the forward output; lse its log-sums
+  const void* dO;   // strides as O's
+  void *dQ, *dK, *dV;  // strides as Q's, K's and V's
+  int64_t sG, hG, sDQ, hDQ, sDK, hDK, sDV, hDV;
+  int ldg, lddq, lddk, lddv;
+  float* delta;     // [B, H, Sq]
+  float* ws;        // parts of the heavy key blocks
+  int KBS;          // key blocks of 128
+  int heavy, parts;  // the first `heavy` of them run in `parts` parts
+  float scale;
+};
+
+template <typename T>
+struct WinBackScale {
+  static constexpr float up = 1.0f, down = 1.0f, log2 = 0.0f;
+};
+template <>
+struct WinBackScale<F16> {
+  static constexpr float up = 256.0f, down = 1.0f / 256.0f, log2 = 8.0f;
+};
+
+// Fragment offsets of a tile of 128-byte rows (64 d each half), as
+// win_attn_kernel's: rows of 16 (straight) and 16 columns of 32 rows
+// (transposed).
+struct WinFrag {
+  uint32_t row;   // straight, chunk l >> 4 of row l & 15
+  uint32_t trow;  // transposed
+  int tch, tsw;
+  __device__ __forceinline__ void set(int lane) {
+    row = (uint32_t)((lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) << 4));
+    const int vs = lane & 15, vrow = 4 * (lane >> 4) + (vs >> 2);
+    trow = (uint32_t)vrow * 128u + (uint32_t)((vs & 1) * 8);
+    tch = (vs & 3) >> 1;
+    tsw = vrow & 7;
+  }
+};
+
+// Rows NB 16 .. + 15 of the tile at `base`: KC chunks of 32 d.
+template <int NB, int KC, int HB>
+__device__ __forceinline__ void win_frag_rows(uint32_t base, const WinFrag& f, u32x4 (&out)[KC]) {
+  static_for<KC>([&](auto kc_c) {
+    constexpr int I = decltype(kc_c)::value;
+    out[I] = ds_read16<(I >> 1) * HB + NB * 2048>((I & 1) ? ((base + f.row) ^ 64u) : base + f.row);
+  });
+}
+// Columns 16 DBI .. + 15 of rows 32 C .. + 31, transposed.
+template <int C, int DBI, int HB>
+__device__ __forceinline__ u32x4 win_frag_cols(uint32_t base, const WinFrag& f) {
+  const uint32_t a = base + f.trow + (uint32_t)(((2 * (DBI & 3) + f.tch) ^ f.tsw) << 4);
+  const u32x2 x = ds_read_tr16<(DBI >> 2) * HB + C * 4096>(a), y = ds_read_tr16<(DBI >> 2) * HB + C * 4096 + 2048>(a);
+  return u32x4{x.x, x.y, y.x, y.y};
+}
+
+// One wave's share (16 rows) of the direct loads of a 64-row tile: rows from
+// row0 of `base`, those from `end` on and columns from D on read as zeros.
+template <int HV>
+__device__ __forceinline__ void win_load_tile(const uint16_t* base, int ld, int row0, int end, int D, uint8_t* dst,
+                                              int wave, int lane) {
+  constexpr int HB = 64 * 128;
+  const int left = end - row0 < 64 ? end - row0 : 64;  // >= 1
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+      (void*)(base + (int64_t)row0 * ld), (short)0, (int)(((uint32_t)(left - 1) * (uint32_t)ld + (uint32_t)D) * 2u),
+      0x00020000);
+  const int ch = (lane & 7) ^ (lane >> 3);
+  const uint32_t r0 = (uint32_t)(wave * 16 + (lane >> 3)) * (uint32_t)ld * 2u, r8 = 16u * (uint32_t)ld;
+#pragma unroll
+  for (int hf = 0; hf < HV; ++hf) {
+    const int d = hf * 64 + ch * 8;
+    const uint32_t o = d < D ? r0 + (uint32_t)d * 2u : 0x80000000u;
+    uint8_t* p = dst + hf * HB + wave * 2048;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)p, 16, o, 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(p + 1024), 16, o + r8, 0, 0, 0);
+  }
+}
+
+// Fragments of 16 rows from global memory (rows at or past `end` as zeros).
+template <int KC>
+__device__ __forceinline__ void win_load_rows(const uint16_t* base, int ld, int row0, int end, int D, int lane,
+                                              u32x4 (&out)[KC]) {
+  const int r = row0 + (lane & 15);
+#pragma unroll
+  for (int kc = 0; kc < KC; ++kc) {
+    const int d = kc * 32 + 8 * (lane >> 4);
+    out[kc] = r < end && d < D ? *reinterpret_cast<const u32x4*>(base + (int64_t)r * ld + d) : u32x4{0u, 0u, 0u, 0u};
+  }
+}
+
+template <typename T, int DW>
+__global__ __launch_bounds__(256, 2) void win_dq_kernel(WinBackParams bp) {
+  using C = WinCfg<DW>;
+  using S = WinBackScale<T>;
+  constexpr int MB = 2, HV = C::HALVES, KC = DW / 32, DB = DW / 16, KB = 64, HB = KB * 128, NS = 2;
+  const WinParams& p = bp.w;
+  __shared__ __attribute__((aligned(1024))) uint8_t sK[NS][HV * HB];
+  __shared__ __attribute__((aligned(1024))) uint8_t sV[NS][HV * HB];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int qb, b, h;
+  win_item(p, (int)blockIdx.x, qb, b, h);
+  const int hk = h / p.G;
+  const WinSeq sq = win_seq(p, b);
+  const int r0 = qb * 128, q0 = r0 + wave * 32;
+  const int r1 = r0 + 128 < sq.rows ? r0 + 128 : sq.rows;
+  const WinBlocks<KB> kbs = win_blocks<KB>(p, sq, r0, r1 > r0 ? r1 : r0);
+  const int nkb = r1 > r0 ? kbs.n : 0;
+  const uint16_t* Qb = static_cast<const uint16_t*>(p.Q) + b * p.sQ + h * p.hQ;
+  const uint16_t* Kb = static_cast<const uint16_t*>(p.K) + b * p.sK + hk * p.hK;
+  const uint16_t* Vb = static_cast<const uint16_t*>(p.V) + b * p.sV + hk * p.hV;
+  const uint16_t* Ob = static_cast<const uint16_t*>(p.O) + b * p.sO + h * p.hO;
+  const uint16_t* Gb = static_cast<const uint16_t*>(bp.dO) + b * bp.sG + h * bp.hG;
+  auto issue = [&](int i) {
+    const int j = kbs.at(i) * KB;
+    win_load_tile<HV>(Kb, p.ldk, j, sq.keys, p.D, &sK[i & 1][0], wave, lane);
+    win_load_tile<HV>(Vb, p.ldv, j, sq.keys, p.D, &sV[i & 1][0], wave, lane);
+  };
+  if (nkb > 0) issue(0);
+
+  u32x4 qf[MB][KC], gf[MB][KC];
+  float nl[MB], dl[MB];
+  const int64_t stat = ((int64_t)b * p.H + h) * p.Sq;
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) {
+    u32x4 of[KC];
+    const int row = q0 + mb * 16 + (lane & 15);
+    win_load_rows<KC>(Qb, p.ldq, q0 + mb * 16, sq.rows, p.D, lane, qf[mb]);
+    win_load_rows<KC>(Gb, bp.ldg, q0 + mb * 16, sq.rows, p.D, lane, gf[mb]);
+    win_load_rows<KC>(Ob, p.ldo, q0 + mb * 16, sq.rows, p.D, lane, of);
+    float d = 0.f;
+#pragma unroll
+    for (int kc = 0; kc < KC; ++kc)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t x = gf[mb][kc][e], y = of[kc][e];
+        d = __builtin_fmaf(Elem<T>::to_f32((uint16_t)(x & 0xffffu)), Elem<T>::to_f32((uint16_t)(y & 0xffffu)), d);
+        d = __builtin_fmaf(Elem<T>::to_f32((uint16_t)(x >> 16)), Elem<T>::to_f32((uint16_t)(y >> 16)), d);
+      }
+    d += __shfl_xor(d, 16, 64);
+    d += __shfl_xor(d, 32, 64);
+    dl[mb] = d;
+    nl[mb] = row < sq.rows ? S::log2 - p.lse[stat + row] * 1.4426950408889634f : 0.f;
+    if (row < sq.rows && lane < 16) bp.delta[stat + row] = d;
+  }
+  f32x4 dq[MB][DB];
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+    for (int db = 0; db < DB; ++db) dq[mb][db] = f32x4{0.f, 0.f, 0.f, 0.f};
+  WinFrag fr;
+  fr.set(lane);
+  const int pw0 = q0, pw1 = q0 + 31;
+
+  for (int i = 0; i < nkb; ++i) {
+    const int k0 = kbs.at(i) * KB, k1 = k0 + KB - 1;
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 0));
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    if (i + 1 < nkb) issue(i + 1);
+    __builtin_amdgcn_sched_barrier(0);
+    if (k0 > pw1 || (k1 <= pw0 - p.window && k0 >= p.sinks)) continue;
+    const bool edge = k1 > pw0 || k1 >= sq.keys || (k0 <= pw1 - p.window && k1 >= p.sinks);
+    const uint32_t ka = lds_addr(&sK[i & 1][0]), va = lds_addr(&sV[i & 1][0]);
+    static_for<2>([&](auto c_c) {
+      constexpr int CH = decltype(c_c)::value;  // keys 32 CH .. + 31 of the block
+      f32x4 s[MB][2], dp[MB][2];
+      static_for<2>([&](auto n_c) {
+        constexpr int N = decltype(n_c)::value, NB = 2 * CH + N;
+        u32x4 kf[KC], vf[KC];
+        win_frag_rows<NB, KC, HB>(ka, fr, kf);
+        win_frag_rows<NB, KC, HB>(va, fr, vf);
+        __builtin_amdgcn_s_waitcnt(waitcnt_imm(63, KC));
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) {
+          s[mb][N] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int kc = 0; kc < KC; ++kc) s[mb][N] = Mfma16<T>::run(kf[kc], qf[mb][kc], s[mb][N]);
+        }
+        __builtin_amdgcn_s_waitcnt(waitcnt_imm(63, 0));
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) {
+          dp[mb][N] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int kc = 0; kc < KC; ++kc) dp[mb][N] = Mfma16<T>::run(vf[kc], gf[mb][kc], dp[mb][N]);
+        }
+      });
+      u32x4 kt[DB];
+      __builtin_amdgcn_sched_barrier(0);
+      static_for<DB>([&](auto db_c) {
+        constexpr int I = decltype(db_c)::value;
+        kt[I] = win_frag_cols<CH, I, HB>(ka, fr);
+      });
+      __builtin_amdgcn_sched_barrier(0);
+      u32x4 ds[MB];
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) {
+        const int pos = pw0 + mb * 16 + (lane & 15);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          float v[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mb][n][q], p.scale_log2e, nl[mb]));
+            v[q] = e * ((dp[mb][n][q] - dl[mb]) * S::down);
+            if (edge && !win_sees(p, sq, pos, k0 + CH * 32 + n * 16 + 4 * (lane >> 4) + q)) v[q] = 0.f;
+          }
+          ds[mb][2 * n] = pack2<T>(v[0], v[1]);
+          ds[mb][2 * n + 1] = pack2<T>(v[2], v[3]);
+        }
+      }
+      __builtin_amdgcn_s_waitcnt(waitcnt_imm(63, 0));
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) dq[mb][db] = Mfma16<T>::run(kt[db], ds[mb], dq[mb][db]);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  }
+  uint16_t* Db = static_cast<uint16_t*>(bp.dQ) + b * bp.sDQ + h * bp.hDQ;
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) {
+    const int r = q0 + mb * 16 + (lane & 15);
+    if (r >= p.Sq) continue;
+    uint16_t* drow = Db + (int64_t)r * bp.lddq;
+    const bool in = r < sq.rows;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) {
+      const int d = db * 16 + 4 * (lane >> 4);
+      const f32x4 v = dq[mb][db];
+      if (d < p.D)
+        *reinterpret_cast<u32x2*>(drow + d) =
+            in ? u32x2{pack2<T>(v[0] * bp.scale, v[1] * bp.scale), pack2<T>(v[2] * bp.scale, v[3] * bp.scale)}
+               : u32x2{0u, 0u};
+    }
+  }
+}
+
+template <int DW>
+struct WinDkvCfg {
+  static constexpr int KEYS = 128;  // of a workgroup
+  static constexpr int PART = 2 * KEYS * DW;  // floats of one part
+};
+
+// Stores a wave's 32 keys; keys at or past `end` get 0.
+template <typename T, int DB>
+__device__ __forceinline__ void win_store_keys(uint16_t* base, int ld, int key0, int end, int rows, int D, float scale,
+                                               int lane, const f32x4 (&v)[2][DB]) {
+#pragma unroll
+  for (int mb = 0; mb < 2; ++mb) {
+    const int key = key0 + mb * 16 + (lane & 15);
+    if (key >= rows) continue;
+    uint16_t* out = base + (int64_t)key * ld;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) {
+      const int d = db * 16 + 4 * (lane >> 4);
+      const f32x4 x = v[mb][db];
+      if (d < D)
+        *reinterpret_cast<u32x2*>(out + d) =
+            key < end ? u32x2{pack2<T>(x[0] * scale, x[1] * scale), pack2<T>(x[2] * scale, x[3] * scale)}
+                      : u32x2{0u, 0u};
+    }
+  }
+}
+
+template <typename T, int DW>
+__global__ __launch_bounds__(256, 2) void win_dkv_kernel(WinBackParams bp) {
+  using S = WinBackScale<T>;
+  constexpr int HV = WinCfg<DW>::HALVES, KC = DW / 32, DB = DW / 16, RB = 64, HB = RB * 128, NS = 2;
+  const WinParams& p = bp.w;
+  __shared__ __attribute__((aligned(1024))) uint8_t sQ[NS][HV * HB];
+  __shared__ __attribute__((aligned(1024))) uint8_t sG[NS][HV * HB];
+  __shared__ __attribute__((aligned(256))) float sL[NS][2][RB];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // The key blocks in parts start first, then the others in order; a key head
+  // stays on one XCD where their number is a multiple of 8.
+  const int heads = p.B * p.Hk;
+  const int kv = (int)blockIdx.x % heads, x = (int)blockIdx.x / heads;
+  const bool cut = x < bp.heavy * bp.parts;
+  const int kb = cut ? x / bp.parts : bp.heavy + (x - bp.heavy * bp.parts);
+  const int part = cut ? x % bp.parts : 0, parts = cut ? bp.parts : 1;
+  const int b = kv / p.Hk, hk = kv % p.Hk;
+  const WinSeq sq = win_seq(p, b);
+  const int n = sq.rows;
+  const int k0 = kb * 128, kw0 = k0 + wave * 32;
+  // rows that see any of the 128 keys, in blocks of 64, of all G heads
+  int last = n - 1;
+  if (k0 >= p.sinks && k0 + 127 + p.window - 1 < last) last = k0 + 127 + p.window - 1;
+  const int rb0 = k0 / RB, nrb = last >= k0 ? last / RB - rb0 + 1 : 0;
+  const int64_t all = (int64_t)nrb * p.G;
+  const int t0 = (int)(all * part / parts), t1 = (int)(all * (part + 1) / parts);
+
+  const uint16_t* Kb = static_cast<const uint16_t*>(p.K) + b * p.sK + hk * p.hK;
+  const uint16_t* Vb = static_cast<const uint16_t*>(p.V) + b * p.sV + hk * p.hV;
+  const uint16_t* Qb = static_cast<const uint16_t*>(p.Q) + b * p.sQ + (int64_t)hk * p.G * p.hQ;
+  const uint16_t* Gb = static_cast<const uint16_t*>(bp.dO) + b * bp.sG + (int64_t)hk * p.G * bp.hG;
+  auto issue = [&](int t) {
+    const int g = t / nrb, row0 = (rb0 + t % nrb) * RB, st = t & 1;
+    win_load_tile<HV>(Qb + g * p.hQ, p.ldq, row0, n, p.D, &sQ[st][0], wave, lane);
+    win_load_tile<HV>(Gb + g * bp.hG, bp.ldg, row0, n, p.D, &sG[st][0], wave, lane);
+    if (wave < 2) {
+      const int left = n - row0 < RB ? n - row0 : RB;
+      const float* src = (wave == 0 ? p.lse : bp.delta) + ((int64_t)b * p.H + hk * p.G + g) * p.Sq + row0;
+      const __amdgpu_buffer_rsrc_t rs =
+          __builtin_amdgcn_make_buffer_rsrc((void*)src, (short)0, left * 4, 0x00020000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)&sL[st][wave][0], 4, (uint32_t)lane * 4u, 0, 0, 0);
+    }
+  };
+  if (t0 < t1) issue(t0);
+  u32x4 kf[2][KC], vf[2][KC];
+#pragma unroll
+  for (int mb = 0; mb < 2; ++mb) {
+    win_load_rows<KC>(Kb, p.ldk, kw0 + mb * 16, n, p.D, lane, kf[mb]);
+    win_load_rows<KC>(Vb, p.ldv, kw0 + mb * 16, n, p.D, lane, vf[mb]);
+  }
+  f32x4 dk[2][DB], dv[2][DB];
+#pragma unroll
+  for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+    for (int db = 0; db < DB; ++db) dk[mb][db] = dv[mb][db] = f32x4{0.f, 0.f, 0.f, 0.f};
+  WinFrag fr;
+  fr.set(lane);
+
+  for (int t = t0; t < t1; ++t) {
+    const int row0 = (rb0 + t % nrb) * RB, row1 = row0 + RB - 1, st = t & 1;
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 0));
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    if (t + 1 < t1) issue(t + 1);
+    __builtin_amdgcn_sched_barrier(0);
+    if (row1 < kw0 || (kw0 + 31 <= row0 - p.window && kw0 >= p.sinks)) continue;
+    const bool edge = kw0 + 31 > row0 || row1 >= n || (kw0 <= row1 - p.window && kw0 + 31 >= p.sinks);
+    const uint32_t qa = lds_addr(&sQ[st][0]), ga = lds_addr(&sG[st][0]);
+    const uint32_t la = lds_addr(&sL[st][0][0]) + (uint32_t)(lane >> 4) * 16u;
+    static_for<2>([&](auto c_c) {
+      constexpr int CH = decltype(c_c)::value;  // rows 32 CH .. + 31 of the block
+      u32x4 pf[2], ds[2];
+      static_for<2>([&](auto n_c) {
+        constexpr int N = decltype(n_c)::value, NB = 2 * CH + N;
+        u32x4 qf[KC], gf[KC];
+        const f32x4 ls = __builtin_bit_cast(f32x4, ds_read16<NB * 64>(la));
+        const f32x4 dl = __builtin_bit_cast(f32x4, ds_read16<RB * 4 + NB * 64>(la));
+        win_frag_rows<NB, KC, HB>(qa, fr, qf);
+        win_frag_rows<NB, KC, HB>(ga, fr, gf);
+        __builtin_amdgcn_s_waitcnt(waitcnt_imm(63, KC));
+        __builtin_amdgcn_sched_barrier(0);
+        f32x4 s[2], dp[2];
+#pragma unroll
+        for (int mb = 0; mb < 2; ++mb) {
+          s[mb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int kc = 0; kc < KC; ++kc) s[mb] = Mfma16<T>::run(qf[kc], kf[mb][kc], s[mb]);
+        }
+        __builtin_amdgcn_s_waitcnt(waitcnt_imm(63, 0));
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int mb = 0; mb < 2; ++mb) {
+          dp[mb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int kc = 0; kc < KC; ++kc) dp[mb] = Mfma16<T>::run(gf[kc], vf[mb][kc], dp[mb]);
+        }
+        const int row = row0 + NB * 16 + 4 * (lane >> 4);
+#pragma unroll
+        for (int mb = 0; mb < 2; ++mb) {
+          const int key = kw0 + mb * 16 + (lane & 15);
+          float e[4], v[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float nl = __builtin_fmaf(ls[q], -1.4426950408889634f, S::log2);
+            e[q] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mb][q], p.scale_log2e, nl));
+            v[q] = e[q] * ((dp[mb][q] - dl[q]) * S::down);
+            if (edge && !(row + q < n && win_sees(p, sq, row + q, key))) e[q] = v[q] = 0.f;
+          }
+          pf[mb][2 * N] = pack2<T>(e[0], e[1]);
+          pf[mb][2 * N + 1] = pack2<T>(e[2], e[3]);
+          ds[mb][2 * N] = pack2<T>(v[0], v[1]);
+          ds[mb][2 * N + 1] = pack2<T>(v[2], v[3]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      static_for<DB>([&](auto db_c) {
+        constexpr int I = decltype(db_c)::value;
+        const u32x4 gt = win_frag_cols<CH, I, HB>(ga, fr), qt = win_frag_cols<CH, I, HB>(qa, fr);
+        __builtin_amdgcn_s_waitcnt(waitcnt_imm(63, 0));
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int mb = 0; mb < 2; ++mb) {
+          dv[mb][I] = Mfma16<T>::run(gt, pf[mb], dv[mb][I]);
+          dk[mb][I] = Mfma16<T>::run(qt, ds[mb], dk[mb][I]);
+        }
+      });
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  }
+  if (cut) {
+    f32x4* out = reinterpret_cast<f32x4*>(bp.ws + ((int64_t)(kv * bp.heavy + kb) * parts + part) * WinDkvCfg<DW>::PART) +
+                 (wave * 2 * DB) * 64 + lane;
+#pragma unroll
+    for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        out[(mb * DB + db) * 64] = dk[mb][db];
+        out[(4 * 2 * DB + mb * DB + db) * 64] = dv[mb][db];
+      }
+    return;
+  }
+  win_store_keys<T, DB>(static_cast<uint16_t*>(bp.dK) + b * bp.sDK + hk * bp.hDK, bp.lddk, kw0, n, p.Sk, p.D, bp.scale,
+                        lane, dk);
+  win_store_keys<T, DB>(static_cast<uint16_t*>(bp.dV) + b * bp.sDV + hk * bp.hDV, bp.lddv, kw0, n, p.Sk, p.D, S::down,
+                        lane, dv);
+}
+
+// The parts of one key block, added in order.
+template <typename T, int DW>
+__global__ __launch_bounds__(256) void win_dkv_merge_kernel(WinBackParams bp) {
+  using S = WinBackScale<T>;
+  constexpr int DB = DW / 16;
+  const WinParams& p = bp.w;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kv = (int)blockIdx.x / bp.heavy, kb = (int)blockIdx.x % bp.heavy;
+  const int b = kv / p.Hk, hk = kv % p.Hk;
+  const WinSeq sq = win_seq(p, b);
+  const f32x4* in = reinterpret_cast<const f32x4*>(bp.ws + (int64_t)blockIdx.x * bp.parts * WinDkvCfg<DW>::PART) +
+                    (wave * 2 * DB) * 64 + lane;
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    f32x4 v[2][DB];
+#pragma unroll
+    for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+      for (int db = 0; db < DB; ++db) v[mb][db] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int q = 0; q < bp.parts; ++q)
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+          v[mb][db] += in[(int64_t)q * (WinDkvCfg<DW>::PART / 4) + (w * 4 * 2 * DB + mb * DB + db) * 64];
+    if (w == 0)
+      win_store_keys<T, DB>(static_cast<uint16_t*>(bp.dK) + b * bp.sDK + hk * bp.hDK, bp.lddk, kb * 128 + wave * 32,
+                            sq.rows, p.Sk, p.D, bp.scale, lane, v);
+    else
+      win_store_keys<T, DB>(static_cast<uint16_t*>(bp.dV) + b * bp.sDV + hk * bp.hDV, bp.lddv, kb * 128 + wave * 32,
+                            sq.rows, p.Sk, p.D, S::down, lane, v);
+  }
+}
+
+}  // namespace sf

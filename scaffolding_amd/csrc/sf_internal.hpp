@@ -274,4 +274,16 @@ struct WinShape {
 int launch_window(const WinShape& a, sf_dtype dt, float* ws, hipStream_t st);
 int64_t win_cached_work(const WinShape& a);
 
+struct WinParams;
+void win_fill_params(const WinShape& a, WinParams& p);
+// Its gradients: the operands beside the forward call's (WinShape, O and lse
+// being what it left).
+struct WinBack {
+  const void* dO;
+  void *dQ, *dK, *dV;
+  int64_t ldg, sG, hG, lddq, sDQ, hDQ, lddk, sDK, hDK, lddv, sDV, hDV;
+};
+int launch_window_back(const WinShape& a, const WinBack& g, sf_dtype dt, void* work, hipStream_t st);
+int64_t win_back_work(const WinShape& a);
+
 }  // namespace sf

@@ -317,6 +317,17 @@ def window_attention(qkv: Tensor, heads: int, kv_heads: int, window: int | None 
     return Tensor._wrap_gpu(out, qkv._device)
 
 
+def window_attention_backward(grad: Tensor, qkv: Tensor, out: Tensor, lse: Tensor, heads: int, kv_heads: int,
+                              window: int | None = None, sinks: int = 0, scale: float | None = None,
+                              lengths: Tensor | None = None) -> Tensor:
+    """grad_qkv of window_attention, in qkv's layout, from grad (B, N, heads
+    D); out and lse are what it gave with return_lse for the same arguments."""
+    dev = _device_of("window_attention_backward", qkv, grad, out, lse, lengths)
+    dx = _cuops.dev_window_attention_backward(_on(grad, dev), qkv._gpu, _on(out, dev), _on(lse, dev), heads, kv_heads,
+                                              window, sinks, scale, _on(lengths, dev))
+    return Tensor._wrap_gpu(dx, qkv._device)
+
+
 def window_attention_cached(q: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: Tensor, heads: int, kv_heads: int,
                             window: int | None = None, sinks: int = 0, scale: float | None = None) -> Tensor:
     """window_attention of n new tokens a sequence, q (B, n, heads D), over

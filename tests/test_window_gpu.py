@@ -224,3 +224,93 @@ def test_empty():
     assert tuple(y.shape) == (2, 0, 128) and tuple(lse.shape) == (2, 2, 0)
     q, k = g.empty((2, 0, 128), np.float16), g.empty((2, 5, 64), np.float16)
     assert tuple(g.dev_window_attention_cached(q, k, k, ints([0, 0]), 2, 1).shape) == (2, 0, 128)
+
+
+# ---- gradients -----------------------------------------------------------------------
+
+def backward_bound(g, x, H, Hk, window, sinks, scale, dtype, lengths=None):
+    """Per element of dx, in terms of the sums of magnitudes `mag` that
+    ob.window_attention_backward gives (dS by its parts |dP| + |delta|):
+      - P and dS are rounded once for their products: half a step each;
+      - delta comes of the rounded output (half a step of it) and lse carries
+        fp32 errors: both within another half step of the magnitudes;
+      - the scores' D fp32 roundings move P by D 2^-23 scale sum |q k|;
+      - the sums over up to N rows of every head (or keys) 2^-23 a term.
+    fp16's smallest step (2^-24, dS; P is held times 2^8) adds N H of them
+    times the operand."""
+    want, mag = ob.window_attention_backward(g, x, H, Hk, window, sinks, scale, lengths)
+    q, k, v = ob.split_heads(x, H, Hk)
+    D, N = q.shape[-1], q.shape[1]
+    size = np.abs(q).sum(-1).max() * np.abs(k).max()
+    hu = out_half_ulp_rel(dtype)
+    rel = 3 * hu + 4 * D * 2.0 ** -23 * abs(scale) * size + (N * H // Hk + D) * 2.0 ** -23 + 2.0 ** -16
+    tiny = 2.0 ** -24 * N * (H // Hk) * np.abs(x).max() * max(abs(scale), 1.0) if dtype == "float16" else 0.0
+    tol = rel * mag + tiny
+    return want, tol + hu * (np.abs(want) + tol) + 2.0 ** -24
+
+
+BACK = [
+    # dtype, B, N, H, Hk, D, window, sinks
+    ("bfloat16", 1, 1, 1, 1, 128, None, 0), ("float16", 1, 3, 2, 1, 8, 1, 0), ("bfloat16", 2, 63, 2, 2, 64, None, 0),
+    ("float16", 1, 64, 4, 1, 40, 64, 0), ("bfloat16", 1, 65, 3, 1, 72, 1, 1), ("float16", 2, 130, 4, 2, 96, 33, 4),
+    ("bfloat16", 1, 129, 2, 1, 128, 128, 200), ("float16", 1, 200, 2, 2, 128, 65, 63),
+    ("bfloat16", 1, 300, 6, 3, 104, 100, 70), ("float16", 3, 257, 2, 1, 64, 64, 65), ("bfloat16", 1, 500, 8, 8, 64, 37, 3),
+    ("bfloat16", 1, 520, 4, 2, 128, None, 0), ("float16", 1, 700, 2, 1, 128, 50, 150), ("bfloat16", 1, 390, 2, 1, 32, 129, 2 ** 40),
+]
+
+
+@pytest.mark.parametrize("dtype,B,N,H,Hk,D,window,sinks", BACK)
+def test_backward(dtype, B, N, H, Hk, D, window, sinks):
+    rng = np.random.default_rng(N + D)
+    x = rnd(rng, (B, N, (H + 2 * Hk) * D), 1.0, dtype)
+    g = rnd(rng, (B, N, H * D), 0.5, dtype)
+    gx, gg = up(x, dtype), up(g, dtype)
+    out, lse = cu().dev_window_attention(gx, H, Hk, window, sinks, None, None, True)
+    dx = down(cu().dev_window_attention_backward(gg, gx, out, lse, H, Hk, window, sinks))
+    want, tol = backward_bound(g, x, H, Hk, window, sinks, D ** -0.5, dtype)
+    check_bound(dx, want, tol)
+    again = down(cu().dev_window_attention_backward(gg, gx, out, lse, H, Hk, window, sinks))
+    assert (dx == again).all()
+
+
+@pytest.mark.parametrize("dtype,N,H,Hk,D,window,sinks,lengths", [
+    ("bfloat16", 200, 2, 1, 128, 50, 3, [200, 1, 0, 131, 64, 65]), ("float16", 270, 4, 2, 64, None, 0, [-5, 270, 900, 129]),
+    ("bfloat16", 300, 2, 2, 72, 20, 100, [90, 129, 128]),
+])
+def test_backward_lengths(dtype, N, H, Hk, D, window, sinks, lengths):
+    """What lies behind a sequence's end (NaN here) changes nothing, and gets
+    0."""
+    rng = np.random.default_rng(N)
+    B = len(lengths)
+    x = rnd(rng, (B, N, (H + 2 * Hk) * D), 1.0, dtype)
+    g = rnd(rng, (B, N, H * D), 0.5, dtype)
+    clean = x.copy()
+    for b, n in enumerate(lengths):
+        x[b, max(n, 0):] = np.nan
+        g[b, max(n, 0):] = np.nan
+    gx, gl = up(x, dtype), ints(lengths)
+    out, lse = cu().dev_window_attention(gx, H, Hk, window, sinks, 0.2, gl, True)
+    dx = down(cu().dev_window_attention_backward(up(g, dtype), gx, out, lse, H, Hk, window, sinks, 0.2, gl))
+    want, tol = backward_bound(np.nan_to_num(g), clean, H, Hk, window, sinks, 0.2, dtype, lengths)
+    check_bound(dx, want, tol)
+    for b, n in enumerate(lengths):
+        assert (dx[b, max(n, 0):] == 0).all()
+
+
+def test_backward_against_differences():
+    """The gradient along a few directions against central differences of the
+    oracle's loss: as far off as the elements' bounds allow, plus the
+    differences' own error (h^2 times a third derivative of order 10)."""
+    rng = np.random.default_rng(0)
+    N, H, Hk, D, window, sinks = 40, 2, 1, 64, 9, 2
+    x = rnd(rng, (1, N, (H + 2 * Hk) * D), 1.0, "float16")
+    g = rnd(rng, (1, N, H * D), 0.5, "float16")
+    out, lse = cu().dev_window_attention(up(x, "float16"), H, Hk, window, sinks, None, None, True)
+    dx = down(cu().dev_window_attention_backward(up(g, "float16"), up(x, "float16"), out, lse, H, Hk, window, sinks))
+    _, tol = backward_bound(g, x, H, Hk, window, sinks, D ** -0.5, "float16")
+    h = 1e-4
+    for _ in range(6):
+        way = rng.standard_normal(x.shape)
+        lo, hi = (ob.window_attention(x + s * way, H, Hk, window, sinks, D ** -0.5)[0] for s in (-h, h))
+        num = ((hi - lo) * g).sum() / (2 * h)
+        assert abs(num - (dx * way).sum()) < (tol * np.abs(way)).sum() + 1e-5
