@@ -93,8 +93,10 @@ __device__ __forceinline__ WinBlocks<KB> win_blocks(const WinParams& p, const Wi
   return w;
 }
 
+// (Without branches: it stands in the middle of code that must stay in one
+// piece to be scheduled.)
 __device__ __forceinline__ bool win_sees(const WinParams& p, const WinSeq& s, int pos, int key) {
-  return key <= pos && key < s.keys && (key > pos - p.window || key < p.sinks);
+  return (key <= pos) & (key < s.keys) & ((key > pos - p.window) | (key < p.sinks));
 }
 
 // Workgroup -> (row block, batch entry, query head).  The last row blocks, which

@@ -7,47 +7,37 @@ namespace sf {
 static int64_t cdiv64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 static int win_width(int64_t D) { return D <= 64 ? 64 : (D <= 96 ? 96 : 128); }
 
-// Which key blocks run in parts, and in how many.  A key block of 128 is seen
-// by the rows up to its window's end, one with sinks by every later row: with a
-// window the blocks of the sinks are cut to about the others' rows, without
-// one the first half of all blocks is cut in two.
-static void win_cut(const WinShape& a, int* heavy, int* parts) {
-  const int64_t blocks = cdiv64(a.Sk, 128), seen = a.window > 0 && a.window + 127 < a.Sq ? a.window + 127 : a.Sq;
-  *heavy = 0;
-  *parts = 1;
-  if (seen < a.Sq) {
-    const int64_t most = cdiv64(a.Sq, seen + 128);
-    if (a.sinks > 0 && most > 1) {
-      const int64_t with = cdiv64(a.sinks, 128);
-      *heavy = (int)(with < blocks ? with : blocks);
-      *parts = (int)(most < 16 ? most : 16);
-    }
-  } else if (blocks > 1) {
-    *heavy = (int)(blocks / 2);
-    *parts = 2;
-  }
+// Ranges of win_dkv_kernel's work: one a CU at head sizes past 64, two below
+// (128 registers a lane), but at least 8 products a range on average (each
+// leaves at most 2 sums to be added).
+static int64_t win_ranges(const WinShape& a) {
+  const int64_t blocks = cdiv64(a.Sk, 128), G = a.heads / a.kv_heads;
+  const int64_t seen = a.window > 0 && a.window + 127 < a.Sq ? a.window + 127 : a.Sq;
+  const int64_t products = a.batch * a.kv_heads * blocks * (cdiv64(seen, 64) + 1) * G;  // at most, but for the sinks'
+  int64_t n = (a.D > 64 ? 1 : 2) * static_cast<int64_t>(cu_count_current());
+  if (n > products / 8) n = products / 8;
+  return n < 1 ? 1 : n;
 }
 
+static int64_t round256(int64_t n) { return cdiv64(n, 256) * 256; }
 static size_t part_floats(int64_t D) { return static_cast<size_t>(2 * 128) * win_width(D); }
 
+// delta, the ranges' starts, their sums.
 int64_t win_back_work(const WinShape& a) {
-  int heavy, parts;
-  win_cut(a, &heavy, &parts);
-  const int64_t stats = cdiv64(a.batch * a.heads * a.Sq * 4, 256) * 256;
-  return stats + (heavy > 0 ? a.batch * a.kv_heads * heavy * parts * (int64_t)(part_floats(a.D) * sizeof(float)) : 0);
+  const int64_t n = win_ranges(a);
+  return round256(a.batch * a.heads * a.Sq * 4) + round256((n + 1) * static_cast<int64_t>(sizeof(WinStart))) +
+         2 * n * static_cast<int64_t>(part_floats(a.D) * sizeof(float));
 }
 
 template <typename T, int DW>
 static int launch_win_back_t(const WinBackParams& p, hipStream_t st) {
-  hipLaunchKernelGGL((win_dq_kernel<T, DW>), dim3((unsigned)((int64_t)p.w.B * p.w.H * p.w.QB)), dim3(256), 0, st, p);
+  hipLaunchKernelGGL((win_dq_kernel<T, DW>), dim3((unsigned)((int64_t)p.w.B * p.w.H * p.w.QB + 1)), dim3(256), 0, st, p);
   int rc = check_launch("window attention gradient (queries)");
   if (rc != SF_OK) return rc;
-  const int64_t kv = (int64_t)p.w.B * p.w.Hk;
-  hipLaunchKernelGGL((win_dkv_kernel<T, DW>), dim3((unsigned)(kv * (p.heavy * p.parts + p.KBS - p.heavy))), dim3(256), 0,
-                     st, p);
+  hipLaunchKernelGGL((win_dkv_kernel<T, DW>), dim3((unsigned)p.ranges), dim3(512), 0, st, p);
   rc = check_launch("window attention gradient (keys)");
-  if (rc != SF_OK || p.heavy == 0) return rc;
-  hipLaunchKernelGGL((win_dkv_merge_kernel<T, DW>), dim3((unsigned)(kv * p.heavy)), dim3(256), 0, st, p);
+  if (rc != SF_OK || p.ranges == 1) return rc;
+  hipLaunchKernelGGL((win_dkv_merge_kernel<T, DW>), dim3((unsigned)(2 * p.ranges)), dim3(512), 0, st, p);
   return check_launch("window attention gradient (merge)");
 }
 
@@ -60,11 +50,13 @@ int launch_window_back(const WinShape& a, const WinBack& g, sf_dtype dt, void* w
   p.dV = g.dV, p.lddv = (int)g.lddv, p.sDV = g.sDV, p.hDV = g.hDV;
   p.scale = a.scale;
   p.KBS = (int)cdiv64(a.Sk, 128);
-  win_cut(a, &p.heavy, &p.parts);
-  if (a.batch * a.kv_heads * ((int64_t)p.heavy * p.parts + p.KBS) > (int64_t(1) << 30))
-    return fail(SF_ERR_UNSUPPORTED, "window attention gradient: more than 2^30 workgroups");
+  if (a.batch * a.kv_heads * p.KBS > (int64_t(1) << 30) || p.KBS * (a.heads / a.kv_heads) > (int64_t(1) << 29))
+    return fail(SF_ERR_UNSUPPORTED, "window attention gradient: more than 2^30 blocks of keys");
+  p.ranges = (int)win_ranges(a);
   p.delta = static_cast<float*>(work);
-  p.ws = p.delta + cdiv64(a.batch * a.heads * a.Sq * 4, 256) * 64;
+  char* at = static_cast<char*>(work) + round256(a.batch * a.heads * a.Sq * 4);
+  p.start = reinterpret_cast<WinStart*>(at);
+  p.ws = reinterpret_cast<float*>(at + round256((p.ranges + 1) * static_cast<int64_t>(sizeof(WinStart))));
   const bool h = dt == SF_F16;
   switch (win_width(a.D)) {
     case 64: return h ? launch_win_back_t<F16, 64>(p, st) : launch_win_back_t<BF16, 64>(p, st);

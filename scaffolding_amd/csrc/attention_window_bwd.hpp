@@ -14,10 +14,9 @@
 //   win_dq_kernel   128 query rows a workgroup (32 a wave), Q and dO in
 //                   registers, blocks of 64 keys of K and V through LDS; it
 //                   forms delta first and leaves it for the other launch
-//   win_dkv_kernel  128 keys a workgroup (32 a wave), K and V in registers,
+//   win_dkv_kernel  128 keys a workgroup (16 a wave), K and V in registers,
 //                   blocks of 64 rows of Q and dO of every query head of the
-//                   group through LDS, so that the sum over heads needs no
-//                   further launch
+//                   group through LDS: the sum over heads is part of it
 //
 // Both take the forward kernel's operand layouts: scores come out with the
 // summed index (keys here, rows there) across a lane's registers, where the
@@ -28,14 +27,24 @@
 // each); P of fp16 is held times 2^8, so that the weights of thousands of keys
 // stay normal numbers.  Everything else, sums included, is fp32.
 //
-// Key blocks that far more rows see than others (sinks; the first ones without
-// a window) are cut into parts of their rows, whose fp32 sums a third launch
-// adds in order (win_dkv_merge_kernel).
+// How many rows see a block of keys differs widely (sinks, no window, short
+// sequences), so win_dkv_kernel's work is cut evenly whatever it is: the (key
+// block, row block, head) products of all key blocks in one list, as many equal
+// ranges of it as workgroups fit the chip (win_plan_ranges: one more workgroup
+// of the first launch, while the others work).  A key block whose products lie
+// in one range is stored by it; of one that is cut each range leaves its fp32
+// sums, and a third launch adds them in order (win_dkv_merge_kernel).
 #pragma once
 
 #include "attention_window.hpp"
 
 namespace sf {
+
+// A place in the list: product `at` of key block `block` (of (batch entry, key
+// head, key block) in this order).
+struct WinStart {
+  int block, at;
+};
 
 struct WinBackParams {
   WinParams w;      // O: the forward output; lse its log-sums
@@ -44,11 +53,29 @@ struct WinBackParams {
   int64_t sG, hG, sDQ, hDQ, sDK, hDK, sDV, hDV;
   int ldg, lddq, lddk, lddv;
   float* delta;     // [B, H, Sq]
-  float* ws;        // parts of the heavy key blocks
-  int KBS;          // key blocks of 128
-  int heavy, parts;  // the first `heavy` of them run in `parts` parts
+  float* ws;        // two sums (WinDkvCfg::PART floats) a range: its first and its last key block's
+  WinStart* start;  // where each range begins, and the end of the last
+  int ranges;
+  int KBS;          // key blocks of 128 of a sequence
   float scale;
 };
+
+// The rows that see a key of block kb (128 keys): blocks of 64 rows from
+// `first`; `products` of the list (every query head of the group times those,
+// or 1 for a block past the sequence's end, whose gradient is 0).
+struct WinKeyRows {
+  int first, n, products;
+};
+__device__ __forceinline__ WinKeyRows win_key_rows(const WinParams& p, const WinSeq& s, int kb) {
+  WinKeyRows r;
+  const int k0 = kb * 128;
+  int last = s.rows - 1;
+  if (k0 >= p.sinks && k0 + 127 + p.window - 1 < last) last = k0 + 127 + p.window - 1;
+  r.first = k0 / 64;
+  r.n = last >= k0 ? last / 64 - r.first + 1 : 0;
+  r.products = r.n > 0 ? r.n * p.G : 1;
+  return r;
+}
 
 template <typename T>
 struct WinBackScale {
@@ -125,6 +152,65 @@ __device__ __forceinline__ void win_load_rows(const uint16_t* base, int ld, int 
   }
 }
 
+// Cuts the list of products into bp.ranges equal ranges.  One workgroup.
+__device__ __forceinline__ void win_plan_ranges(const WinBackParams& bp, int64_t* scan) {
+  const WinParams& p = bp.w;
+  const int tid = (int)threadIdx.x, nt = (int)blockDim.x;
+  const int64_t all = (int64_t)p.B * p.Hk * bp.KBS;
+  auto products = [&](int64_t e) -> int64_t {
+    const int kb = (int)(e % bp.KBS);
+    return win_key_rows(p, win_seq(p, e / bp.KBS / p.Hk), kb).products;
+  };
+  // the sum over the threads' values up to this one; every thread calls it
+  auto running = [&](int64_t v) {
+    scan[tid] = v;
+    __syncthreads();
+    for (int off = 1; off < nt; off <<= 1) {
+      const int64_t o = tid >= off ? scan[tid - off] : 0;
+      __syncthreads();
+      scan[tid] += o;
+      __syncthreads();
+    }
+    return scan[tid];
+  };
+  int64_t v = 0;
+  for (int64_t e = tid; e < all; e += nt) v += products(e);
+  running(v);
+  const int64_t total = scan[nt - 1];
+  __syncthreads();
+  int64_t base = 0;
+  for (int64_t e0 = 0; e0 < all; e0 += nt) {
+    const int64_t e = e0 + tid, c = e < all ? products(e) : 0;
+    const int64_t end = base + running(c), begin = end - c;
+    base += scan[nt - 1];
+    __syncthreads();
+    // range w begins at product w total / ranges
+    for (int64_t w = (begin * bp.ranges + total - 1) / total; w < bp.ranges; ++w) {
+      const int64_t at = w * total / bp.ranges;
+      if (at >= end) break;
+      bp.start[w] = WinStart{(int)e, (int)(at - begin)};
+    }
+  }
+  if (tid == 0) bp.start[bp.ranges] = WinStart{(int)all, 0};
+}
+
+// Stores the lane's part of 16 rows (row: the lane's) of a gradient; rows at or
+// past `end` get 0, those past `rows` are not there.
+template <typename T, int DB>
+__device__ __forceinline__ void win_store_16(uint16_t* base, int ld, int row, int end, int rows, int D, float scale,
+                                             int lane, const f32x4 (&v)[DB]) {
+  if (row >= rows) return;
+  uint16_t* out = base + (int64_t)row * ld;
+#pragma unroll
+  for (int db = 0; db < DB; ++db) {
+    const int d = db * 16 + 4 * (lane >> 4);
+    const f32x4 x = v[db];
+    if (d < D)
+      *reinterpret_cast<u32x2*>(out + d) =
+          row < end ? u32x2{pack2<T>(x[0] * scale, x[1] * scale), pack2<T>(x[2] * scale, x[3] * scale)} : u32x2{0u, 0u};
+  }
+}
+
 template <typename T, int DW>
 __global__ __launch_bounds__(256, 2) void win_dq_kernel(WinBackParams bp) {
   using C = WinCfg<DW>;
@@ -133,10 +219,14 @@ __global__ __launch_bounds__(256, 2) void win_dq_kernel(WinBackParams bp) {
   const WinParams& p = bp.w;
   __shared__ __attribute__((aligned(1024))) uint8_t sK[NS][HV * HB];
   __shared__ __attribute__((aligned(1024))) uint8_t sV[NS][HV * HB];
+  if (blockIdx.x == 0) {  // the other launch's plan
+    win_plan_ranges(bp, reinterpret_cast<int64_t*>(&sK[0][0]));
+    return;
+  }
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int qb, b, h;
-  win_item(p, (int)blockIdx.x, qb, b, h);
+  win_item(p, (int)blockIdx.x - 1, qb, b, h);
   const int hk = h / p.G;
   const WinSeq sq = win_seq(p, b);
   const int r0 = qb * 128, q0 = r0 + wave * 32;
@@ -260,52 +350,17 @@ __global__ __launch_bounds__(256, 2) void win_dq_kernel(WinBackParams bp) {
   }
   uint16_t* Db = static_cast<uint16_t*>(bp.dQ) + b * bp.sDQ + h * bp.hDQ;
 #pragma unroll
-  for (int mb = 0; mb < MB; ++mb) {
-    const int r = q0 + mb * 16 + (lane & 15);
-    if (r >= p.Sq) continue;
-    uint16_t* drow = Db + (int64_t)r * bp.lddq;
-    const bool in = r < sq.rows;
-#pragma unroll
-    for (int db = 0; db < DB; ++db) {
-      const int d = db * 16 + 4 * (lane >> 4);
-      const f32x4 v = dq[mb][db];
-      if (d < p.D)
-        *reinterpret_cast<u32x2*>(drow + d) =
-            in ? u32x2{pack2<T>(v[0] * bp.scale, v[1] * bp.scale), pack2<T>(v[2] * bp.scale, v[3] * bp.scale)}
-               : u32x2{0u, 0u};
-    }
-  }
+  for (int mb = 0; mb < 2; ++mb)
+    win_store_16<T, DB>(Db, bp.lddq, q0 + mb * 16 + (lane & 15), sq.rows, p.Sq, p.D, bp.scale, lane, dq[mb]);
 }
 
 template <int DW>
 struct WinDkvCfg {
-  static constexpr int KEYS = 128;  // of a workgroup
-  static constexpr int PART = 2 * KEYS * DW;  // floats of one part
+  static constexpr int PART = 2 * 128 * DW;  // floats of the sums of a workgroup's 128 keys, dK and dV
 };
 
-// Stores a wave's 32 keys; keys at or past `end` get 0.
-template <typename T, int DB>
-__device__ __forceinline__ void win_store_keys(uint16_t* base, int ld, int key0, int end, int rows, int D, float scale,
-                                               int lane, const f32x4 (&v)[2][DB]) {
-#pragma unroll
-  for (int mb = 0; mb < 2; ++mb) {
-    const int key = key0 + mb * 16 + (lane & 15);
-    if (key >= rows) continue;
-    uint16_t* out = base + (int64_t)key * ld;
-#pragma unroll
-    for (int db = 0; db < DB; ++db) {
-      const int d = db * 16 + 4 * (lane >> 4);
-      const f32x4 x = v[mb][db];
-      if (d < D)
-        *reinterpret_cast<u32x2*>(out + d) =
-            key < end ? u32x2{pack2<T>(x[0] * scale, x[1] * scale), pack2<T>(x[2] * scale, x[3] * scale)}
-                      : u32x2{0u, 0u};
-    }
-  }
-}
-
 template <typename T, int DW>
-__global__ __launch_bounds__(256, 2) void win_dkv_kernel(WinBackParams bp) {
+__global__ __launch_bounds__(512, 2) void win_dkv_kernel(WinBackParams bp) {
   using S = WinBackScale<T>;
   constexpr int HV = WinCfg<DW>::HALVES, KC = DW / 32, DB = DW / 16, RB = 64, HB = RB * 128, NS = 2;
   const WinParams& p = bp.w;
@@ -314,178 +369,192 @@ __global__ __launch_bounds__(256, 2) void win_dkv_kernel(WinBackParams bp) {
   __shared__ __attribute__((aligned(256))) float sL[NS][2][RB];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // The key blocks in parts start first, then the others in order; a key head
-  // stays on one XCD where their number is a multiple of 8.
-  const int heads = p.B * p.Hk;
-  const int kv = (int)blockIdx.x % heads, x = (int)blockIdx.x / heads;
-  const bool cut = x < bp.heavy * bp.parts;
-  const int kb = cut ? x / bp.parts : bp.heavy + (x - bp.heavy * bp.parts);
-  const int part = cut ? x % bp.parts : 0, parts = cut ? bp.parts : 1;
-  const int b = kv / p.Hk, hk = kv % p.Hk;
-  const WinSeq sq = win_seq(p, b);
-  const int n = sq.rows;
-  const int k0 = kb * 128, kw0 = k0 + wave * 32;
-  // rows that see any of the 128 keys, in blocks of 64, of all G heads
-  int last = n - 1;
-  if (k0 >= p.sinks && k0 + 127 + p.window - 1 < last) last = k0 + 127 + p.window - 1;
-  const int rb0 = k0 / RB, nrb = last >= k0 ? last / RB - rb0 + 1 : 0;
-  const int64_t all = (int64_t)nrb * p.G;
-  const int t0 = (int)(all * part / parts), t1 = (int)(all * (part + 1) / parts);
-
-  const uint16_t* Kb = static_cast<const uint16_t*>(p.K) + b * p.sK + hk * p.hK;
-  const uint16_t* Vb = static_cast<const uint16_t*>(p.V) + b * p.sV + hk * p.hV;
-  const uint16_t* Qb = static_cast<const uint16_t*>(p.Q) + b * p.sQ + (int64_t)hk * p.G * p.hQ;
-  const uint16_t* Gb = static_cast<const uint16_t*>(bp.dO) + b * bp.sG + (int64_t)hk * p.G * bp.hG;
-  auto issue = [&](int t) {
-    const int g = t / nrb, row0 = (rb0 + t % nrb) * RB, st = t & 1;
-    win_load_tile<HV>(Qb + g * p.hQ, p.ldq, row0, n, p.D, &sQ[st][0], wave, lane);
-    win_load_tile<HV>(Gb + g * bp.hG, bp.ldg, row0, n, p.D, &sG[st][0], wave, lane);
-    if (wave < 2) {
-      const int left = n - row0 < RB ? n - row0 : RB;
-      const float* src = (wave == 0 ? p.lse : bp.delta) + ((int64_t)b * p.H + hk * p.G + g) * p.Sq + row0;
-      const __amdgpu_buffer_rsrc_t rs =
-          __builtin_amdgcn_make_buffer_rsrc((void*)src, (short)0, left * 4, 0x00020000);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)&sL[st][wave][0], 4, (uint32_t)lane * 4u, 0, 0, 0);
-    }
-  };
-  if (t0 < t1) issue(t0);
-  u32x4 kf[2][KC], vf[2][KC];
-#pragma unroll
-  for (int mb = 0; mb < 2; ++mb) {
-    win_load_rows<KC>(Kb, p.ldk, kw0 + mb * 16, n, p.D, lane, kf[mb]);
-    win_load_rows<KC>(Vb, p.ldv, kw0 + mb * 16, n, p.D, lane, vf[mb]);
-  }
-  f32x4 dk[2][DB], dv[2][DB];
-#pragma unroll
-  for (int mb = 0; mb < 2; ++mb)
-#pragma unroll
-    for (int db = 0; db < DB; ++db) dk[mb][db] = dv[mb][db] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // Each XCD takes a contiguous share of the ranges: neighbouring key blocks
+  // read the same rows.
+  const int w = xcd_remap((int)blockIdx.x, (int)gridDim.x);
+  const WinStart from = bp.start[w], to = bp.start[w + 1];
   WinFrag fr;
   fr.set(lane);
+  for (int e = from.block; e < to.block || (e == to.block && to.at > 0); ++e) {
+    const int kv = e / bp.KBS, kb = e % bp.KBS;
+    const int b = kv / p.Hk, hk = kv % p.Hk;
+    const WinSeq sq = win_seq(p, b);
+    const int n = sq.rows;
+    const WinKeyRows kr = win_key_rows(p, sq, kb);
+    const int begin = e == from.block ? from.at : 0, end = e == to.block ? to.at : kr.products;
+    const int t0 = begin, t1 = kr.n > 0 ? end : begin;  // past the sequence: nothing to add up
+    const int kw0 = kb * 128 + wave * 16, key = kw0 + (lane & 15);
+    const uint16_t* Kb = static_cast<const uint16_t*>(p.K) + b * p.sK + hk * p.hK;
+    const uint16_t* Vb = static_cast<const uint16_t*>(p.V) + b * p.sV + hk * p.hV;
+    const uint16_t* Qb = static_cast<const uint16_t*>(p.Q) + b * p.sQ + (int64_t)hk * p.G * p.hQ;
+    const uint16_t* Gb = static_cast<const uint16_t*>(bp.dO) + b * bp.sG + (int64_t)hk * p.G * bp.hG;
+    // waves 0-3 load Q's tile, 4-7 that of dO
+    auto issue = [&](int t) {
+      const int g = t / kr.n, row0 = (kr.first + t % kr.n) * RB, st = (t - t0) % NS;
+      if (wave < 4) win_load_tile<HV>(Qb + g * p.hQ, p.ldq, row0, n, p.D, &sQ[st][0], wave, lane);
+      else win_load_tile<HV>(Gb + g * bp.hG, bp.ldg, row0, n, p.D, &sG[st][0], wave - 4, lane);
+      if (wave < 2) {
+        const int left = n - row0 < RB ? n - row0 : RB;
+        const float* src = (wave == 0 ? p.lse : bp.delta) + ((int64_t)b * p.H + hk * p.G + g) * p.Sq + row0;
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)src, (short)0, left * 4, 0x00020000);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)&sL[st][wave][0], 4, (uint32_t)lane * 4u, 0, 0, 0);
+      }
+    };
+    __syncthreads();  // every wave has read the last block's tiles
+    if (t0 < t1) issue(t0);
+    u32x4 kf[KC], vf[KC];
+    f32x4 dk[DB], dv[DB];
+    win_load_rows<KC>(Kb, p.ldk, kw0, n, p.D, lane, kf);
+    win_load_rows<KC>(Vb, p.ldv, kw0, n, p.D, lane, vf);
+#pragma unroll
+    for (int db = 0; db < DB; ++db) dk[db] = dv[db] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  for (int t = t0; t < t1; ++t) {
-    const int row0 = (rb0 + t % nrb) * RB, row1 = row0 + RB - 1, st = t & 1;
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 0));
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_sched_barrier(0);
-    if (t + 1 < t1) issue(t + 1);
-    __builtin_amdgcn_sched_barrier(0);
-    if (row1 < kw0 || (kw0 + 31 <= row0 - p.window && kw0 >= p.sinks)) continue;
-    const bool edge = kw0 + 31 > row0 || row1 >= n || (kw0 <= row1 - p.window && kw0 + 31 >= p.sinks);
-    const uint32_t qa = lds_addr(&sQ[st][0]), ga = lds_addr(&sG[st][0]);
-    const uint32_t la = lds_addr(&sL[st][0][0]) + (uint32_t)(lane >> 4) * 16u;
-    static_for<2>([&](auto c_c) {
-      constexpr int CH = decltype(c_c)::value;  // rows 32 CH .. + 31 of the block
-      u32x4 pf[2], ds[2];
-      static_for<2>([&](auto n_c) {
-        constexpr int N = decltype(n_c)::value, NB = 2 * CH + N;
-        u32x4 qf[KC], gf[KC];
-        const f32x4 ls = __builtin_bit_cast(f32x4, ds_read16<NB * 64>(la));
-        const f32x4 dl = __builtin_bit_cast(f32x4, ds_read16<RB * 4 + NB * 64>(la));
-        win_frag_rows<NB, KC, HB>(qa, fr, qf);
-        win_frag_rows<NB, KC, HB>(ga, fr, gf);
-        __builtin_amdgcn_s_waitcnt(waitcnt_imm(63, KC));
-        __builtin_amdgcn_sched_barrier(0);
+    for (int t = t0; t < t1; ++t) {
+      const int row0 = (kr.first + t % kr.n) * RB, row1 = row0 + RB - 1, st = (t - t0) % NS;
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 0));
+      __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_sched_barrier(0);
+      if (t + 1 < t1) issue(t + 1);
+      __builtin_amdgcn_sched_barrier(0);
+      if (row1 < kw0 || (kw0 + 15 <= row0 - p.window && kw0 >= p.sinks)) continue;
+      const bool edge = kw0 + 15 > row0 || row1 >= n || (kw0 <= row1 - p.window && kw0 + 15 >= p.sinks);
+      const uint32_t qa = lds_addr(&sQ[st][0]), ga = lds_addr(&sG[st][0]);
+      const uint32_t la = lds_addr(&sL[st][0][0]) + (uint32_t)(lane >> 4) * 16u;
+      // Rows 32 CH .. + 31 of the block are one chunk; the second's are read while
+      // the first is worked on, in the registers that it has left.
+      u32x4 qf[2][2][KC], gf[2][2][KC];
+      f32x4 ls[2][2], dl[2][2];
+      auto q_rows = [&](auto c) {
+        constexpr int CH = decltype(c)::value;
+        static_for<2>([&](auto i) { win_frag_rows<2 * CH + decltype(i)::value, KC, HB>(qa, fr, qf[CH][decltype(i)::value]); });
+      };
+      auto g_rows = [&](auto c) {
+        constexpr int CH = decltype(c)::value;
+        static_for<2>([&](auto i) {
+          constexpr int N = decltype(i)::value, NB = 2 * CH + N;
+          win_frag_rows<NB, KC, HB>(ga, fr, gf[CH][N]);
+          ls[CH][N] = __builtin_bit_cast(f32x4, ds_read16<NB * 64>(la));
+          dl[CH][N] = __builtin_bit_cast(f32x4, ds_read16<RB * 4 + NB * 64>(la));
+        });
+      };
+      q_rows(std::integral_constant<int, 0>{});
+      g_rows(std::integral_constant<int, 0>{});
+      static_for<2>([&](auto c_c) {
+        constexpr int CH = decltype(c_c)::value;
+        u32x4 gt[DB], qt[DB], pf, ds;
         f32x4 s[2], dp[2];
-#pragma unroll
-        for (int mb = 0; mb < 2; ++mb) {
-          s[mb] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int kc = 0; kc < KC; ++kc) s[mb] = Mfma16<T>::run(qf[kc], kf[mb][kc], s[mb]);
-        }
+        __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_waitcnt(waitcnt_imm(63, 0));
         __builtin_amdgcn_sched_barrier(0);
+        static_for<DB>([&](auto d) { gt[decltype(d)::value] = win_frag_cols<CH, decltype(d)::value, HB>(ga, fr); });
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int mb = 0; mb < 2; ++mb) {
-          dp[mb] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < 2; ++i) s[i] = dp[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int kc = 0; kc < KC; ++kc) dp[mb] = Mfma16<T>::run(gf[kc], vf[mb][kc], dp[mb]);
+        for (int kc = 0; kc < KC; ++kc) {  // four sums side by side
+#pragma unroll
+          for (int i = 0; i < 2; ++i) s[i] = Mfma16<T>::run(qf[CH][i][kc], kf[kc], s[i]);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) dp[i] = Mfma16<T>::run(gf[CH][i][kc], vf[kc], dp[i]);
         }
-        const int row = row0 + NB * 16 + 4 * (lane >> 4);
+        __builtin_amdgcn_sched_barrier(0);
+        static_for<DB>([&](auto d) { qt[decltype(d)::value] = win_frag_cols<CH, decltype(d)::value, HB>(qa, fr); });
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int mb = 0; mb < 2; ++mb) {
-          const int key = kw0 + mb * 16 + (lane & 15);
-          float e[4], v[4];
+        for (int i = 0; i < 2; ++i) {
+          const int row = row0 + (2 * CH + i) * 16 + 4 * (lane >> 4);
+          float x[4], v[4];
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const float nl = __builtin_fmaf(ls[q], -1.4426950408889634f, S::log2);
-            e[q] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mb][q], p.scale_log2e, nl));
-            v[q] = e[q] * ((dp[mb][q] - dl[q]) * S::down);
-            if (edge && !(row + q < n && win_sees(p, sq, row + q, key))) e[q] = v[q] = 0.f;
+            const float nl = __builtin_fmaf(ls[CH][i][q], -1.4426950408889634f, S::log2);
+            x[q] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][q], p.scale_log2e, nl));
+            v[q] = x[q] * ((dp[i][q] - dl[CH][i][q]) * S::down);
           }
-          pf[mb][2 * N] = pack2<T>(e[0], e[1]);
-          pf[mb][2 * N + 1] = pack2<T>(e[2], e[3]);
-          ds[mb][2 * N] = pack2<T>(v[0], v[1]);
-          ds[mb][2 * N + 1] = pack2<T>(v[2], v[3]);
+          if (edge) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const bool see = (row + q < n) & win_sees(p, sq, row + q, key);
+              x[q] = see ? x[q] : 0.f;
+              v[q] = see ? v[q] : 0.f;
+            }
+          }
+          pf[2 * i] = pack2<T>(x[0], x[1]);
+          pf[2 * i + 1] = pack2<T>(x[2], x[3]);
+          ds[2 * i] = pack2<T>(v[0], v[1]);
+          ds[2 * i + 1] = pack2<T>(v[2], v[3]);
         }
         __builtin_amdgcn_sched_barrier(0);
-      });
-      static_for<DB>([&](auto db_c) {
-        constexpr int I = decltype(db_c)::value;
-        const u32x4 gt = win_frag_cols<CH, I, HB>(ga, fr), qt = win_frag_cols<CH, I, HB>(qa, fr);
-        __builtin_amdgcn_s_waitcnt(waitcnt_imm(63, 0));
+        __builtin_amdgcn_s_waitcnt(waitcnt_imm(63, 2 * DB < 16 ? 2 * DB : 15));  // dO columns
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int mb = 0; mb < 2; ++mb) {
-          dv[mb][I] = Mfma16<T>::run(gt, pf[mb], dv[mb][I]);
-          dk[mb][I] = Mfma16<T>::run(qt, ds[mb], dk[mb][I]);
-        }
-      });
-      __builtin_amdgcn_sched_barrier(0);
-    });
-  }
-  if (cut) {
-    f32x4* out = reinterpret_cast<f32x4*>(bp.ws + ((int64_t)(kv * bp.heavy + kb) * parts + part) * WinDkvCfg<DW>::PART) +
-                 (wave * 2 * DB) * 64 + lane;
+        for (int db = 0; db < DB; ++db) dv[db] = Mfma16<T>::run(gt[db], pf, dv[db]);
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(waitcnt_imm(63, 0));  // Q columns
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (CH == 0) q_rows(std::integral_constant<int, 1>{});
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int mb = 0; mb < 2; ++mb)
+        for (int db = 0; db < DB; ++db) dk[db] = Mfma16<T>::run(qt[db], ds, dk[db]);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (CH == 0) g_rows(std::integral_constant<int, 1>{});
+        __builtin_amdgcn_sched_barrier(0);
+      });
+    }
+    if (begin == 0 && end == kr.products) {
+      win_store_16<T, DB>(static_cast<uint16_t*>(bp.dK) + b * bp.sDK + hk * bp.hDK, bp.lddk, key, n, p.Sk, p.D, bp.scale,
+                          lane, dk);
+      win_store_16<T, DB>(static_cast<uint16_t*>(bp.dV) + b * bp.sDV + hk * bp.hDV, bp.lddv, key, n, p.Sk, p.D, S::down,
+                          lane, dv);
+    } else {
+      f32x4* out = reinterpret_cast<f32x4*>(bp.ws + (int64_t)(2 * w + (begin == 0 ? 1 : 0)) * WinDkvCfg<DW>::PART) +
+                   (wave * DB) * 64 + lane;
 #pragma unroll
       for (int db = 0; db < DB; ++db) {
-        out[(mb * DB + db) * 64] = dk[mb][db];
-        out[(4 * 2 * DB + mb * DB + db) * 64] = dv[mb][db];
+        out[db * 64] = dk[db];
+        out[(8 * DB + db) * 64] = dv[db];
       }
-    return;
+    }
   }
-  win_store_keys<T, DB>(static_cast<uint16_t*>(bp.dK) + b * bp.sDK + hk * bp.hDK, bp.lddk, kw0, n, p.Sk, p.D, bp.scale,
-                        lane, dk);
-  win_store_keys<T, DB>(static_cast<uint16_t*>(bp.dV) + b * bp.sDV + hk * bp.hDV, bp.lddv, kw0, n, p.Sk, p.D, S::down,
-                        lane, dv);
 }
 
-// The parts of one key block, added in order.
+// The key block that range w begins and does not end: its sums and those of the
+// ranges behind it that hold more of the block, added in order.
 template <typename T, int DW>
-__global__ __launch_bounds__(256) void win_dkv_merge_kernel(WinBackParams bp) {
+__global__ __launch_bounds__(512) void win_dkv_merge_kernel(WinBackParams bp) {
   using S = WinBackScale<T>;
-  constexpr int DB = DW / 16;
+  constexpr int DB = DW / 16, PART = WinDkvCfg<DW>::PART / 4;
   const WinParams& p = bp.w;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int kv = (int)blockIdx.x / bp.heavy, kb = (int)blockIdx.x % bp.heavy;
+  const int w = (int)blockIdx.x / 2, dv = (int)blockIdx.x % 2;
+  const WinStart from = bp.start[w], to = bp.start[w + 1];
+  const int e = to.block;
+  if (to.at == 0 || (from.block == e && from.at > 0) || (from.block == e && from.at == to.at)) return;
+  const int kv = e / bp.KBS, kb = e % bp.KBS;
   const int b = kv / p.Hk, hk = kv % p.Hk;
   const WinSeq sq = win_seq(p, b);
-  const f32x4* in = reinterpret_cast<const f32x4*>(bp.ws + (int64_t)blockIdx.x * bp.parts * WinDkvCfg<DW>::PART) +
-                    (wave * 2 * DB) * 64 + lane;
+  const f32x4* in = reinterpret_cast<const f32x4*>(bp.ws) + (dv * 8 * DB + wave * DB) * 64 + lane;
+  f32x4 v[DB];
 #pragma unroll
-  for (int w = 0; w < 2; ++w) {
-    f32x4 v[2][DB];
+  for (int db = 0; db < DB; ++db) v[db] = in[(int64_t)(2 * w + 1) * PART + db * 64];
+  WinStart at = to;
+  for (int f = w + 1; f < bp.ranges; ++f) {
+    const WinStart next = bp.start[f + 1];
+    if (next.block != at.block || next.at != at.at) {  // a range with products
 #pragma unroll
-    for (int mb = 0; mb < 2; ++mb)
-#pragma unroll
-      for (int db = 0; db < DB; ++db) v[mb][db] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int q = 0; q < bp.parts; ++q)
-#pragma unroll
-      for (int mb = 0; mb < 2; ++mb)
-#pragma unroll
-        for (int db = 0; db < DB; ++db)
-          v[mb][db] += in[(int64_t)q * (WinDkvCfg<DW>::PART / 4) + (w * 4 * 2 * DB + mb * DB + db) * 64];
-    if (w == 0)
-      win_store_keys<T, DB>(static_cast<uint16_t*>(bp.dK) + b * bp.sDK + hk * bp.hDK, bp.lddk, kb * 128 + wave * 32,
-                            sq.rows, p.Sk, p.D, bp.scale, lane, v);
-    else
-      win_store_keys<T, DB>(static_cast<uint16_t*>(bp.dV) + b * bp.sDV + hk * bp.hDV, bp.lddv, kb * 128 + wave * 32,
-                            sq.rows, p.Sk, p.D, S::down, lane, v);
+      for (int db = 0; db < DB; ++db) v[db] += in[(int64_t)2 * f * PART + db * 64];
+      if (next.block != e) break;
+      at = next;
+    }
   }
+  const int key = kb * 128 + wave * 16 + (lane & 15);
+  if (dv == 0)
+    win_store_16<T, DB>(static_cast<uint16_t*>(bp.dK) + b * bp.sDK + hk * bp.hDK, bp.lddk, key, sq.rows, p.Sk, p.D,
+                          bp.scale, lane, v);
+  else
+    win_store_16<T, DB>(static_cast<uint16_t*>(bp.dV) + b * bp.sDV + hk * bp.hDV, bp.lddv, key, sq.rows, p.Sk, p.D,
+                          S::down, lane, v);
 }
 
 }  // namespace sf
