@@ -72,7 +72,7 @@ static int launch_win(const WinParams& p, int parts, hipStream_t st) {
     hipLaunchKernelGGL((win_split_kernel<T, DW>), dim3((unsigned)(items * parts)), dim3(256), 0, st, p);
     int rc = check_launch("window attention (split)");
     if (rc != SF_OK || parts == 1) return rc;
-    hipLaunchKernelGGL((win_merge_kernel<T, DW>), dim3((unsigned)items), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((win_merge_kernel<T, DW>), dim3((unsigned)(items * (DW / 32))), dim3(256), 0, st, p);
     return check_launch("window attention (merge)");
   }
   const dim3 g((unsigned)((int64_t)p.B * p.H * p.QB));
@@ -91,7 +91,7 @@ int launch_window(const WinShape& a, sf_dtype dt, float* ws, hipStream_t st) {
     p.RB = (int)cdiv64(a.Sq * p.G, 16);
     p.ws = ws;
   }
-  if ((parts > 0 ? (int64_t)p.B * p.Hk * p.RB * parts : (int64_t)p.B * p.H * p.QB) > (int64_t(1) << 30))
+  if ((parts > 0 ? (int64_t)p.B * p.Hk * p.RB * (parts > 4 ? parts : 4) : (int64_t)p.B * p.H * p.QB) > (int64_t(1) << 30))
     return fail(SF_ERR_UNSUPPORTED, "window attention: more than 2^30 workgroups");
   const bool h = dt == SF_F16;
   switch (win_width(a.D)) {

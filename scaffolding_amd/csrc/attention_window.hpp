@@ -142,11 +142,12 @@ __device__ __forceinline__ float win_dot(const uint16_t* a, const uint16_t* b, i
 // global memory.  One wave; bit i of `rows` is the row at position pos0 + i,
 // whose query and output lie at Q + i ldq and O + i ldo.  Slow, for rows
 // beside values that are not finite.  Not inlined: it would cost the kernels
-// registers.
+// registers.  Columns d0 .. d1 - 1 are stored.
 template <typename T>
 __device__ __attribute__((noinline)) void win_exact_rows(const WinParams& p, const uint16_t* Q, int64_t ldq,
                                                          uint16_t* O, int64_t ldo, const uint16_t* K,
-                                                         const uint16_t* V, WinSeq s, int pos0, uint64_t rows) {
+                                                         const uint16_t* V, WinSeq s, int pos0, uint64_t rows, int d0,
+                                                         int d1) {
   const int lane = threadIdx.x & 63;
   const bool dok = 2 * lane < p.D;  // lane: columns 2 lane, 2 lane + 1
   while (rows != 0) {
@@ -191,7 +192,8 @@ __device__ __attribute__((noinline)) void win_exact_rows(const WinParams& p, con
       l = wave_sum(l);
     }
     const float inv = n > 0 ? 1.0f / l : 0.f;  // bad: 0 * inf = NaN
-    if (dok) *reinterpret_cast<uint32_t*>(O + (int64_t)i * ldo + 2 * lane) = pack2<T>(a0 * inv, a1 * inv);
+    if (dok && 2 * lane >= d0 && 2 * lane < d1)
+      *reinterpret_cast<uint32_t*>(O + (int64_t)i * ldo + 2 * lane) = pack2<T>(a0 * inv, a1 * inv);
   }
 }
 
@@ -536,7 +538,8 @@ __global__ __launch_bounds__(256, 2) void win_attn_kernel(WinParams p) {
   }
   if (__builtin_expect(odd != 0, 0)) {
     const WinParams& kp = *(const WinParams*)__builtin_amdgcn_kernarg_segment_ptr();
-    win_exact_rows<T>(kp, Qb + (int64_t)q0 * p.ldq, p.ldq, Ob + (int64_t)q0 * p.ldo, p.ldo, Kb, Vb, sq, pw0, odd);
+    win_exact_rows<T>(kp, Qb + (int64_t)q0 * p.ldq, p.ldq, Ob + (int64_t)q0 * p.ldo, p.ldo, Kb, Vb, sq, pw0, odd, 0,
+                      p.D);
   }
 }
 
@@ -578,26 +581,28 @@ __device__ __forceinline__ WinRow win_row(const WinParams& p, int hk, int r) {
   return w;
 }
 
-// Normalises and stores the columns of `mine` (DB / 4 blocks: db = wave + 4 i)
-// of 16 rows; rows that are not finite are formed again by wave 0.  The sums m,
-// l are those of the lane's row.
-template <typename T, int DB>
+// Normalises and stores 16 rows' blocks of 16 columns db0, db0 + step, ... (NB
+// of them, those below DB); rows that are not finite are formed again (columns
+// d0 .. d1 - 1, all that the workgroup stores) by wave 0.  l: the sum of the
+// lane's row.
+template <typename T, int DB, int NB>
 __device__ __forceinline__ void win_finish_rows(const WinParams& p, const WinSeq& sq, int b, int hk, int rb, int wave,
-                                                int lane, const f32x4 (&o)[(DB + 3) / 4], float l, uint32_t* flag) {
+                                                int lane, int db0, int step, int d0, int d1, const f32x4 (&o)[NB],
+                                                float l, uint32_t* flag) {
   const int rows = p.Sq * p.G, r = rb * 16 + (lane & 15);
   const WinRow w = win_row(p, hk, r < rows ? r : rows - 1);
   const int pos = sq.off + w.token;
   const bool row = r < rows, any = sq.keys > 0 && (sq.keys > pos - p.window + 1 || p.sinks > 0);
   const float inv = 1.0f / l;
   float fin = 0.f;
-  u32x2 v[(DB + 3) / 4];
+  u32x2 v[NB];
 #pragma unroll
-  for (int i = 0; i < (DB + 3) / 4; ++i) {
+  for (int i = 0; i < NB; ++i) {
     float x[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       x[q] = o[i][q] * inv;
-      if (wave + 4 * i < DB) fin = __builtin_fmaf(x[q], 0.f, fin);
+      if (db0 + step * i < DB) fin = __builtin_fmaf(x[q], 0.f, fin);
     }
     v[i] = any ? u32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])} : u32x2{0u, 0u};
   }
@@ -611,8 +616,8 @@ __device__ __forceinline__ void win_finish_rows(const WinParams& p, const WinSeq
   if (row && ((odd >> (lane & 15)) & 1) == 0) {
     uint16_t* orow = Ob + (int64_t)w.token * p.ldo + w.head * p.hO;
 #pragma unroll
-    for (int i = 0; i < (DB + 3) / 4; ++i) {
-      const int db = wave + 4 * i, d = db * 16 + 4 * (lane >> 4);
+    for (int i = 0; i < NB; ++i) {
+      const int db = db0 + step * i, d = db * 16 + 4 * (lane >> 4);
       if (db < DB && d < p.D) *reinterpret_cast<u32x2*>(orow + d) = v[i];
     }
   }
@@ -625,7 +630,7 @@ __device__ __forceinline__ void win_finish_rows(const WinParams& p, const WinSeq
       if ((odd >> i) & 1) {
         const WinRow x = win_row(p, hk, rb * 16 + i);
         win_exact_rows<T>(kp, Qb + (int64_t)x.token * p.ldq + x.head * p.hQ, 0,
-                          Ob + (int64_t)x.token * p.ldo + x.head * p.hO, 0, Kb, Vb, sq, sq.off + x.token, 1);
+                          Ob + (int64_t)x.token * p.ldo + x.head * p.hO, 0, Kb, Vb, sq, sq.off + x.token, 1, d0, d1);
       }
   }
 }
@@ -834,7 +839,7 @@ __global__ __launch_bounds__(256) void win_split_kernel(WinParams p) {
       for (int x = 0; x < 4; ++x) mine[i] += wt[x] * reinterpret_cast<const f32x4*>(&ring[x][0])[db * 64 + lane];
   }
   if (p.parts == 1) {
-    win_finish_rows<T, DB>(p, sq, b, hk, rb, wave, lane, mine, lt, &flag);
+    win_finish_rows<T, DB>(p, sq, b, hk, rb, wave, lane, wave, 4, 0, p.D, mine, lt, &flag);
     return;
   }
   float* ws = p.ws + (int64_t)blockIdx.x * C::PART;
@@ -847,40 +852,48 @@ __global__ __launch_bounds__(256) void win_split_kernel(WinParams p) {
   }
 }
 
-// The parts of one block of rows, merged in part order.
+// The parts of one block of rows.  A workgroup merges 32 columns, so that a few
+// sequences' many parts (1 of 131072 tokens, 8 key heads: 32 parts of each) are
+// read by enough of them; its waves take every fourth part, and their sums are
+// added in wave order.
 template <typename T, int DW>
 __global__ __launch_bounds__(256) void win_merge_kernel(WinParams p) {
   using C = WinSplitCfg<DW>;
   constexpr int DB = DW / 16;
+  __shared__ f32x4 so[4][2][64];
+  __shared__ float sl[4][16];
   __shared__ uint32_t flag;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int t = (int)blockIdx.x;
-  const int rb = t % p.RB;
-  t /= p.RB;
-  const int hk = t % p.Hk, b = t / p.Hk;
+  const int c2 = (int)blockIdx.x % (DB / 2), item = (int)blockIdx.x / (DB / 2);
+  const int rb = item % p.RB, hk = item / p.RB % p.Hk, b = item / p.RB / p.Hk;
   if (threadIdx.x == 0) flag = 0;
-  __syncthreads();
   const WinSeq sq = win_seq(p, b);
-  const float* ws = p.ws + (int64_t)blockIdx.x * p.parts * C::PART;
+  const float* ws = p.ws + (int64_t)item * p.parts * C::PART;
   const int lr = lane & 15;
   float big = -INFINITY;
 #pragma unroll 8
   for (int q = 0; q < p.parts; ++q) big = fmaxf(big, ws[(int64_t)q * C::PART + C::PART_O + lr]);
   float lt = 0.f;
-  f32x4 mine[(DB + 3) / 4];
-#pragma unroll
-  for (int i = 0; i < (DB + 3) / 4; ++i) mine[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  f32x4 mine[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll 4
-  for (int q = 0; q < p.parts; ++q) {
+  for (int q = wave; q < p.parts; q += 4) {
     const float* pq = ws + (int64_t)q * C::PART;
     const float m = pq[C::PART_O + lr], wt = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - big);
     lt += wt * pq[C::PART_O + 16 + lr];
 #pragma unroll
-    for (int i = 0; i < (DB + 3) / 4; ++i)
-      if (wave + 4 * i < DB) mine[i] += wt * reinterpret_cast<const f32x4*>(pq)[(wave + 4 * i) * 64 + lane];
+    for (int i = 0; i < 2; ++i) mine[i] += wt * reinterpret_cast<const f32x4*>(pq)[(2 * c2 + i) * 64 + lane];
   }
-  win_finish_rows<T, DB>(p, sq, b, hk, rb, wave, lane, mine, lt, &flag);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) so[wave][i][lane] = mine[i];
+  if (lane < 16) sl[wave][lane] = lt;
+  __syncthreads();
+  lt = (sl[0][lr] + sl[1][lr]) + (sl[2][lr] + sl[3][lr]);
+  // waves 0 and 1 store a block of 16 columns each
+  f32x4 out[1] = {f32x4{0.f, 0.f, 0.f, 0.f}};
+  if (wave < 2) out[0] = (so[0][wave][lane] + so[1][wave][lane]) + (so[2][wave][lane] + so[3][wave][lane]);
+  win_finish_rows<T, DB>(p, sq, b, hk, rb, wave, lane, wave < 2 ? 2 * c2 + wave : DB, 1, 32 * c2, 32 * c2 + 32, out, lt,
+                         &flag);
 }
 
 }  // namespace sf

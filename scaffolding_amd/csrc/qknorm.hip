@@ -159,8 +159,20 @@ __device__ __forceinline__ void turn(float* a, float* b, const float* c, const f
   }
 }
 
+// The sum over L = 2^n neighbouring lanes, in each of them: up to 16 by the
+// lane network (pairs, quads, halves and rows mirrored), without the trip
+// through LDS that a permute takes.
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
 __device__ __forceinline__ float sum_lanes(float v, int L) {
-  for (int off = L >> 1; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  if (L >= 2) v += dpp<0xb1>(v);    // quad_perm 1 0 3 2
+  if (L >= 4) v += dpp<0x4e>(v);    // quad_perm 2 3 0 1
+  if (L >= 8) v += dpp<0x141>(v);   // row_half_mirror
+  if (L >= 16) v += dpp<0x140>(v);  // row_mirror
+  if (L >= 32) v += __shfl_xor(v, 16, 64);
+  if (L >= 64) v += __shfl_xor(v, 32, 64);
   return v;
 }
 
@@ -459,36 +471,40 @@ __global__ __launch_bounds__(256) void qk_norm_rope_backward_kernel(NormRopePara
   }
 }
 
-// dw, db [2, D] from the blocks' sums: one block per 8 columns, 32 threads of
-// every column; the blocks of one kind are those whose number mod slices is in
-// its range.
+// dw, db [2, D] from the blocks' sums: one block of 1024 threads per 32 columns,
+// 32 threads of every column; the blocks of one kind are those whose number mod
+// slices is in its range.
 template <typename T>
-__global__ __launch_bounds__(256) void qk_norm_sums_kernel(NormRopeParams p, unsigned blocks) {
+__global__ __launch_bounds__(1024) void qk_norm_sums_kernel(NormRopeParams p, unsigned blocks) {
   const NormRopeArgs& a = p.a;
-  const int D = a.D, per = (D + 7) / 8;
-  const int kind = blockIdx.x / (2 * per), w = blockIdx.x / per % 2, d = blockIdx.x % per * 8 + (threadIdx.x & 7);
-  const int row = threadIdx.x >> 3;
+  const int D = a.D, per = (D + 31) / 32, x = threadIdx.x & 31;
+  const int kind = blockIdx.x / (2 * per), w = blockIdx.x / per % 2, d = blockIdx.x % per * 32 + x;
+  const int row = threadIdx.x >> 5;
   const unsigned slices = p.nq + p.nk + p.nv, first = kind ? p.nq : 0, count = kind ? p.nk : p.nq;
-  const unsigned groups = blocks / slices;
+  const unsigned n = blocks / slices * count;
   float v = 0.f;
-  if (d < D)
-    for (unsigned j = row; j < groups * count; j += 32)
+  if (d < D) {
+#pragma unroll 8
+    for (unsigned j = row; j < n; j += 32)
       v += a.part[((int64_t)(j / count) * slices + first + j % count) * 2 * D + w * D + d];
-  __shared__ float red[32][8];
-  red[row][threadIdx.x & 7] = v;
+  }
+  __shared__ float red[32][33];
+  red[row][x] = v;
   __syncthreads();
-  if (threadIdx.x < 8 && d < D) {
+  if (threadIdx.x < 32 && d < D) {
     float s = 0.f;
-    for (int j = 0; j < 32; ++j) s += red[j][threadIdx.x];
+    for (int j = 0; j < 32; ++j) s += red[j][x];
     void* out = w ? a.db : a.dw;
     if (out != nullptr) static_cast<typename Elem<T>::storage*>(out)[kind * D + d] = Elem<T>::from_f32(s);
   }
 }
 
 // The widest chunk that the sizes take: chunks divide the head and, in twos,
-// what is rotated of it.
-static int chunk_of(int D, int rot) {
-  if (D % 8 == 0 && rot % 16 == 0) return 8;
+// what is rotated of it.  Backward at most 4 columns: with 8, the sums and
+// operands take 230 registers, and half as many waves are there to hide the
+// memory's latency.
+static int chunk_of(int D, int rot, bool back) {
+  if (!back && D % 8 == 0 && rot % 16 == 0) return 8;
   if (D % 4 == 0 && rot % 8 == 0) return 4;
   return 1;
 }
@@ -496,7 +512,7 @@ static int chunk_of(int D, int rot) {
 // Fills the split of the work; returns its blocks.
 static unsigned norm_rope_split(NormRopeParams& p, bool back) {
   const NormRopeArgs& a = p.a;
-  const int V = chunk_of(a.D, a.rot);
+  const int V = chunk_of(a.D, a.rot, back);
   int pairs = a.rot / (2 * V) + (a.D - a.rot + 2 * V - 1) / (2 * V);
   p.lg = 0;
   while ((1 << p.lg) < pairs && p.lg < 6) ++p.lg;
@@ -510,10 +526,11 @@ static unsigned norm_rope_split(NormRopeParams& p, bool back) {
   p.nk = (int)cdiv(a.kv_heads, p.per);
   p.nv = a.v != nullptr ? p.nk : 0;
   const int64_t slices = p.nq + p.nk + p.nv;
-  // Blocks of four tokens: as many as there are forward (at most 16 a CU and
-  // slice keeps the grid small), backward fewer, each with sums to add.
+  // Blocks of four tokens at a time.  Forward up to 64 a CU and slice; backward
+  // 4 a CU over all slices, what the registers let run at once, since each
+  // leaves sums to be added (8 a CU: the same time here, twice the sums).
   int64_t groups = cdiv(tokens, 4);
-  const int64_t most = back ? cdiv(8 * cus, slices) : 64 * cus;
+  const int64_t most = back ? cdiv(4 * cus, slices) : 64 * cus;
   if (groups > most) groups = most;
   if (groups < 1) groups = 1;
   p.stride = groups * 4;
@@ -540,18 +557,24 @@ static void launch_norm_rope_v(const NormRopeParams& p, bool back, unsigned bloc
 }
 
 template <typename T>
+static void launch_norm_rope_8(const NormRopeParams& p, unsigned blocks, hipStream_t st) {
+  if (p.a.pairs) hipLaunchKernelGGL((qk_norm_rope_kernel<T, 8, 1, true>), dim3(blocks), dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((qk_norm_rope_kernel<T, 8, 1, false>), dim3(blocks), dim3(256), 0, st, p);
+}
+
+template <typename T>
 static int launch_norm_rope_t(const NormRopeArgs& a, bool back, hipStream_t st) {
   NormRopeParams p{};
   p.a = a;
   const unsigned blocks = norm_rope_split(p, back);
-  switch (chunk_of(a.D, a.rot)) {
-    case 8: launch_norm_rope_v<T, 8, 1>(p, back, blocks, st); break;
+  switch (chunk_of(a.D, a.rot, back)) {
+    case 8: launch_norm_rope_8<T>(p, blocks, st); break;
     case 4: launch_norm_rope_v<T, 4, 1>(p, back, blocks, st); break;
     default: launch_norm_rope_v<T, 1, 2>(p, back, blocks, st); break;
   }
   int rc = check_launch("query and key norm");
   if (rc != SF_OK || !back || a.part == nullptr) return rc;
-  hipLaunchKernelGGL((qk_norm_sums_kernel<T>), dim3(4 * ((a.D + 7) / 8)), dim3(256), 0, st, p, blocks);
+  hipLaunchKernelGGL((qk_norm_sums_kernel<T>), dim3(4 * ((a.D + 31) / 32)), dim3(1024), 0, st, p, blocks);
   return check_launch("query and key norm sums");
 }
 
