@@ -558,7 +558,8 @@ int sf_qk_norm_rope_backward(const void* grad, const void* x, const float* table
  * heads).  Row i of entry (b, h) lies at Q + b strideQ + h headQ + i ldq
  * elements, K and V likewise with kv_heads heads, O as Q.  dtype F16 or BF16,
  * D a multiple of 8 up to 128, 16-byte aligned rows, a finite scale; row
- * strides below 2^23, rows and capacity up to 2^29.  fp32 scores, softmax and
+ * strides below 2^23, rows and capacity up to 2^29, batch * heads * (blocks of
+ * 128 rows + 1) below 2^24.  fp32 scores, softmax and
  * sums, the weights rounded to dtype for their product with V, one rounding
  * of O.  A row that sees no key gives 0; what is not seen does not matter, NaN
  * and infinities included.  O may not overlap the operands.
@@ -615,16 +616,19 @@ int sf_window_attention_cached(const void* Q, int64_t ldq, int64_t strideQ, int6
  *   y[m, f] = act(x[m] . W[f] + bias[f]) (x[m] . W[F + f] + bias[F + f])
  * x [M, K], y [M, F]; act SF_EPI_NONE, SF_EPI_SILU or SF_EPI_GELU_TANH; fp32
  * sums, one rounding.  pre [M, 2 F] (or NULL) takes the two projections,
- * rounded, for the backward pass; SF_F32 needs it (its products and the gate
- * are two launches).  M, K <= 2^30, F <= 2^29, at most 2^22 tiles. */
+ * rounded, for the backward pass; SF_F32 needs it (past 16 rows its products
+ * and the gate are two launches).  M, K <= 2^30, F <= 2^29, at most 2^22 tiles. */
 int sf_gated_linear(const void* x, const void* W, const void* bias, void* y, void* pre, int64_t M, int64_t F, int64_t K,
                     sf_dtype dtype, sf_epilogue act, void* stream);
 /* The gradient of pre from that of y: grad_pre[m, f] = grad up act'(gate),
- * grad_pre[m, F + f] = grad act(gate), each rounded once.  The rest is a
- * linear layer's backward pass over grad_pre (sf_gemm, sf_sum_dim).  grad_pre
- * may be pre. */
-int sf_gated_backward(const void* grad, const void* pre, void* grad_pre, int64_t M, int64_t F, sf_dtype dtype,
-                      sf_epilogue act, void* stream);
+ * grad_pre[m, F + f] = grad act(gate), each rounded once; and with grad_bias
+ * [2 F] (or NULL) its sums over the rows, fp32 in an order fixed by the sizes.
+ * The rest is a linear layer's backward pass over grad_pre (sf_gemm).  grad_pre
+ * may be pre.  `work`: sf_gated_backward_work bytes of 4-byte aligned device
+ * memory of the call's device, overwritten (may be NULL without grad_bias). */
+int64_t sf_gated_backward_work(int64_t M, int64_t F);
+int sf_gated_backward(const void* grad, const void* pre, void* grad_pre, void* grad_bias, int64_t M, int64_t F,
+                      sf_dtype dtype, sf_epilogue act, void* work, void* stream);
 
 /* ------------------------------------------------------------------ */
 /* Runtime: devices, memory, streams, events                           */

@@ -188,8 +188,9 @@ cdef extern from "sfgemm.h" nogil:
                                    void* stream)
     int sf_gated_linear(const void* x, const void* W, const void* bias, void* y, void* pre, int64_t M, int64_t F,
                         int64_t K, sf_dtype dtype, sf_epilogue act, void* stream)
-    int sf_gated_backward(const void* grad, const void* pre, void* grad_pre, int64_t M, int64_t F, sf_dtype dtype,
-                          sf_epilogue act, void* stream)
+    int64_t sf_gated_backward_work(int64_t M, int64_t F)
+    int sf_gated_backward(const void* grad, const void* pre, void* grad_pre, void* grad_bias, int64_t M, int64_t F,
+                          sf_dtype dtype, sf_epilogue act, void* work, void* stream)
     int sf_cast(const void* x, sf_dtype in_dtype, void* y, sf_dtype out_dtype, int64_t n, void* stream)
 
     int sf_get_device_count(int* count)
@@ -1854,11 +1855,21 @@ def dev_gated_linear_backward(gt_grad, gt_x, gt_weight, gt_pre, bint has_bias=Fa
     cdef void* pg = _ptr(gt_grad)
     cdef void* pp = _ptr(gt_pre)
     cdef void* pt = _ptr(through)
+    cdef void* pb = NULL
+    cdef void* pk = NULL
+    cdef CudaBuffer work
+    db = None
+    if has_bias:
+        db = _alloc_like((int(2 * F),), gt_grad.dtype, gt_grad.device_id)
+        pb = _ptr(db)
+        work = _make_buffer(max(int(sf_gated_backward_work(M, F)), 4), gt_grad.device_id)
+        pk = work.ptr
     cdef int ret
     with nogil:
-        ret = sf_gated_backward(pg, pp, pt, M, F, dt, act, NULL)
+        ret = sf_gated_backward(pg, pp, pt, pb, M, F, dt, act, pk, NULL)
     _check_kernel(ret)
-    return dev_linear_backward(through, gt_x, gt_weight, has_bias)
+    dx, dw, _ = dev_linear_backward(through, gt_x, gt_weight, False)
+    return dx, dw, db
 
 
 # ================================================================

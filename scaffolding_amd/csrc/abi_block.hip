@@ -163,8 +163,10 @@ static int window_sizes(const char* name, int64_t batch, int64_t heads, int64_t 
     return fail(SF_ERR_UNSUPPORTED, "%s: head size %lld (multiples of 8 up to 128)", name, (long long)D);
   if (rows > kMostRows / 2 || capacity > kMostRows / 2)
     return fail(SF_ERR_UNSUPPORTED, "%s: at most 2^29 rows", name);
-  if (heads > (1 << 20) || batch > (1 << 24) || batch * heads > kMostRows / ((rows + 127) / 128 + 1))
-    return fail(SF_ERR_UNSUPPORTED, "%s: more than 2^30 blocks of rows", name);
+  // workgroups of 256 threads, one more for the backward pass: a launch holds
+  // fewer than 2^32 threads
+  if (heads > (1 << 20) || batch > (1 << 24) || batch * heads >= (int64_t(1) << 24) / ((rows + 127) / 128 + 1))
+    return fail(SF_ERR_UNSUPPORTED, "%s: batch * heads * (blocks of 128 rows + 1) must be below 2^24", name);
   *noop = batch == 0 || rows == 0;
   return SF_OK;
 }
@@ -395,21 +397,33 @@ int sf_gated_linear(const void* x, const void* W, const void* bias, void* y, voi
     return fail(SF_ERR_INVALID_ARG, "%s: null pointer", name);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype != SF_F32) return gated16(x, W, bias, y, pre, M, F, K, dtype, act, st);
+  // few rows: in one launch, bound by the weight's reading (FP32_RULE)
+  if (M <= 16 && K > 0 && K % 4 == 0 && aligned16(x) && aligned16(W) && F < (int64_t(1) << 26))
+    return launch_gated_skinny32(x, W, bias, y, pre, M, F, K, epi_act(act), st);
   rc = sf_gemm(0, 1, M, 2 * F, K, 1, x, K > 0 ? K : 1, 0, W, K > 0 ? K : 1, 0, pre, 2 * F, 0, SF_F32, SF_F32, 1.0f,
                bias, bias != nullptr ? SF_EPI_BIAS : SF_EPI_NONE, stream);
   if (rc != SF_OK) return rc;
   return launch_gate(epi_act(act), false, nullptr, pre, y, M, F, dtype, st);
 }
 
-int sf_gated_backward(const void* grad, const void* pre, void* grad_pre, int64_t M, int64_t F, sf_dtype dtype,
-                      sf_epilogue act, void* stream) {
+int64_t sf_gated_backward_work(int64_t M, int64_t F) {
+  if (M < 1 || F < 1 || M > kMostRows || F > kMostRows / 2) return 0;
+  return gate_sums_work(M, F);
+}
+
+int sf_gated_backward(const void* grad, const void* pre, void* grad_pre, void* grad_bias, int64_t M, int64_t F,
+                      sf_dtype dtype, sf_epilogue act, void* work, void* stream) {
   clear_error();
   const char* name = "sf_gated_backward";
   const int rc = gated_check(name, M, F, 0, dtype, act);
-  if (rc != SF_OK || M == 0 || F == 0) return rc;
-  if (grad == nullptr || pre == nullptr || grad_pre == nullptr)
+  if (rc != SF_OK || F == 0) return rc;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (M == 0) return grad_bias == nullptr ? SF_OK
+                     : launch_zero(grad_bias, static_cast<size_t>(2 * F) * (dtype == SF_F32 ? 4 : 2), st);
+  if (grad == nullptr || pre == nullptr || grad_pre == nullptr || (grad_bias != nullptr && work == nullptr))
     return fail(SF_ERR_INVALID_ARG, "%s: null pointer", name);
-  return launch_gate(epi_act(act), true, grad, pre, grad_pre, M, F, dtype, static_cast<hipStream_t>(stream));
+  if (grad_bias == nullptr) return launch_gate(epi_act(act), true, grad, pre, grad_pre, M, F, dtype, st);
+  return launch_gate_sums(epi_act(act), grad, pre, grad_pre, grad_bias, static_cast<float*>(work), M, F, dtype, st);
 }
 
 }  // extern "C"

@@ -39,7 +39,9 @@ static int win_split_parts(const WinShape& a, int cus) {
                        (5.0 + 1.0 * (double)cdiv64(keys, 64));
   double best = whole;
   int parts = 0;
-  for (int64_t q = 1; q <= 64 && (q == 1 || 8 * q <= blocks); ++q) {
+  // (workgroups of 256 threads: a launch holds fewer than 2^32; the merge takes
+  // up to four an item)
+  for (int64_t q = 1; q <= 64 && (q == 1 || 8 * q <= blocks) && items * (q > 4 ? q : 4) < (int64_t(1) << 24); ++q) {
     const double us = (double)cdiv64(items * q, slots) * (3.0 + 2.6 * (double)cdiv64(blocks, 4 * q)) +
                       (q > 1 ? 3.0 + 0.05 * (double)q : 0.0);
     if (us < best) {
@@ -91,8 +93,6 @@ int launch_window(const WinShape& a, sf_dtype dt, float* ws, hipStream_t st) {
     p.RB = (int)cdiv64(a.Sq * p.G, 16);
     p.ws = ws;
   }
-  if ((parts > 0 ? (int64_t)p.B * p.Hk * p.RB * (parts > 4 ? parts : 4) : (int64_t)p.B * p.H * p.QB) > (int64_t(1) << 30))
-    return fail(SF_ERR_UNSUPPORTED, "window attention: more than 2^30 workgroups");
   const bool h = dt == SF_F16;
   switch (win_width(a.D)) {
     case 64: return h ? launch_win<F16, 64>(p, parts, st) : launch_win<BF16, 64>(p, parts, st);

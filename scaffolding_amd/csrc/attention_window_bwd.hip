@@ -7,14 +7,13 @@ namespace sf {
 static int64_t cdiv64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 static int win_width(int64_t D) { return D <= 64 ? 64 : (D <= 96 ? 96 : 128); }
 
-// Ranges of win_dkv_kernel's work: one a CU at head sizes past 64, two below
-// (128 registers a lane), but at least 8 products a range on average (each
-// leaves at most 2 sums to be added).
+// Ranges of win_dkv_kernel's work: one a CU (its eight waves fill it), but at
+// least 8 products a range on average (each leaves at most 2 sums to be added).
 static int64_t win_ranges(const WinShape& a) {
   const int64_t blocks = cdiv64(a.Sk, 128), G = a.heads / a.kv_heads;
   const int64_t seen = a.window > 0 && a.window + 127 < a.Sq ? a.window + 127 : a.Sq;
   const int64_t products = a.batch * a.kv_heads * blocks * (cdiv64(seen, 64) + 1) * G;  // at most, but for the sinks'
-  int64_t n = (a.D > 64 ? 1 : 2) * static_cast<int64_t>(cu_count_current());
+  int64_t n = cu_count_current();
   if (n > products / 8) n = products / 8;
   return n < 1 ? 1 : n;
 }
@@ -50,8 +49,6 @@ int launch_window_back(const WinShape& a, const WinBack& g, sf_dtype dt, void* w
   p.dV = g.dV, p.lddv = (int)g.lddv, p.sDV = g.sDV, p.hDV = g.hDV;
   p.scale = a.scale;
   p.KBS = (int)cdiv64(a.Sk, 128);
-  if (a.batch * a.kv_heads * p.KBS > (int64_t(1) << 30) || p.KBS * (a.heads / a.kv_heads) > (int64_t(1) << 29))
-    return fail(SF_ERR_UNSUPPORTED, "window attention gradient: more than 2^30 blocks of keys");
   p.ranges = (int)win_ranges(a);
   p.delta = static_cast<float*>(work);
   char* at = static_cast<char*>(work) + round256(a.batch * a.heads * a.Sq * 4);

@@ -1,12 +1,17 @@
 // gated.hip — the elementwise parts of a gated feed-forward layer over its two
 // projections pre [M, 2 F] (gate, then up):
 //
-//   forward   y = act(gate) up                       (fp32, whose products have
-//                                                     no fused epilogue)
-//   backward  dgate = g up act'(gate), dup = g act(gate), as one [M, 2 F]
+//   forward   y = act(gate) up                       (fp32 of many rows, whose
+//                                                     products have no fused
+//                                                     epilogue)
+//   backward  dgate = g up act'(gate), dup = g act(gate), as one [M, 2 F], and
+//             their sums over the rows, a bias's gradient
 //
 // One read of each operand, one write: bound by HBM.  A thread takes eight
 // columns of a row, in 16-byte pieces at any alignment.
+//
+// And the fp32 layer for few rows, whole: gated_skinny32_kernel.
+#include "gemm16.hpp"
 #include "rowio.hpp"
 #include "sf_internal.hpp"
 
@@ -41,6 +46,200 @@ __global__ __launch_bounds__(256) void gate_kernel(const void* g, const void* pr
       store_cols<T>(out, m * F + f, left, gate);
     }
   }
+}
+
+// The backward pass with the sums over the rows: block (strip, chunk) takes TC *
+// 8 columns and p.rows rows, its 256 / TC thread rows every 256 / TC-th of them;
+// each thread row leaves its sums (fp32, of the gradients ahead of their
+// rounding) in a row of part [chunks * 256 / TC, 2 F].  The columns' threads
+// stay with their columns, so the sums need no reading of what was written
+// (4096 rows, F 7680, bf16: GATE_SUM_US).
+struct GateSums {
+  const void *g, *pre;
+  void *out, *db;
+  float* part;
+  int64_t M, rows;  // of a chunk
+  int F, strips, lg;  // TC = 2^lg threads for the columns
+  unsigned parts;
+};
+
+template <typename T, int ACT>
+__global__ __launch_bounds__(256) void gate_sums_kernel(GateSums p) {
+  const int tc = threadIdx.x & ((1 << p.lg) - 1), tr = threadIdx.x >> p.lg, step = 256 >> p.lg;
+  const int strip = blockIdx.x % (unsigned)p.strips, F = p.F;
+  const int64_t chunk = blockIdx.x / (unsigned)p.strips;
+  const int f = (strip << p.lg | tc) * 8, left = F - f < 8 ? F - f : 8;
+  if (left <= 0) return;
+  const int64_t end = (chunk + 1) * p.rows < p.M ? (chunk + 1) * p.rows : p.M;
+  float sg[8] = {}, su[8] = {};
+#pragma unroll 2
+  for (int64_t m = chunk * p.rows + tr; m < end; m += step) {
+    float gate[8], up[8], d[8];
+    load_cols<T>(p.pre, m * 2 * F + f, left, gate);
+    load_cols<T>(p.pre, m * 2 * F + F + f, left, up);
+    load_cols<T>(p.g, m * F + f, left, d);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float v = gate[e];
+      gate[e] = ACT == ACT_NONE ? d[e] * up[e] : d[e] * up[e] * act_slope<ACT>(v);
+      up[e] = d[e] * act_t<ACT>(v);
+      sg[e] += gate[e];
+      su[e] += up[e];
+    }
+    store_cols<T>(p.out, m * 2 * F + f, left, gate);
+    store_cols<T>(p.out, m * 2 * F + F + f, left, up);
+  }
+  float* row = p.part + (chunk * step + tr) * 2 * F + f;
+  for (int e = 0; e < left; ++e) {
+    row[e] = sg[e];
+    row[F + e] = su[e];
+  }
+}
+
+// db [2 F] from the parts: one block per 32 columns, 32 threads of each.
+template <typename T>
+__global__ __launch_bounds__(1024) void gate_bias_kernel(GateSums p) {
+  const int x = threadIdx.x & 31, row = threadIdx.x >> 5;
+  const int64_t N = 2 * (int64_t)p.F;
+  __shared__ float red[32][33];
+  for (int64_t c0 = (int64_t)blockIdx.x * 32; c0 < N; c0 += (int64_t)gridDim.x * 32) {
+    const int64_t c = c0 + x;
+    float v = 0.f;
+    if (c < N) {
+#pragma unroll 4
+      for (unsigned j = row; j < p.parts; j += 32) v += p.part[(int64_t)j * N + c];
+    }
+    red[row][x] = v;
+    __syncthreads();
+    if (threadIdx.x < 32 && c < N) {
+      float s = 0.f;
+      for (int j = 0; j < 32; ++j) s += red[j][x];
+      static_cast<typename Elem<T>::storage*>(p.db)[c] = Elem<T>::from_f32(s);
+    }
+    __syncthreads();
+  }
+}
+
+// Chunks of at least 16 rows a thread, in at most 8 workgroups a CU.
+static void gate_sums_split(int64_t M, int64_t F, GateSums& p) {
+  const int64_t pieces = (F + 7) / 8;
+  p.lg = 0;
+  while (p.lg < 8 && (int64_t(1) << p.lg) < pieces) ++p.lg;
+  const int64_t step = 256 >> p.lg, strips = (pieces + (1 << p.lg) - 1) >> p.lg;
+  int64_t chunks = (M + 16 * step - 1) / (16 * step);
+  const int64_t most = (8 * (int64_t)cu_count_current() + strips - 1) / strips;
+  if (chunks > most) chunks = most;
+  p.strips = (int)strips;
+  p.rows = (M + chunks - 1) / chunks;
+  chunks = (M + p.rows - 1) / p.rows;
+  p.parts = (unsigned)(chunks * step);
+}
+
+int64_t gate_sums_work(int64_t M, int64_t F) {
+  GateSums p;
+  gate_sums_split(M, F, p);
+  return (int64_t)p.parts * 2 * F * 4;
+}
+
+template <typename T>
+static int launch_gate_sums_t(int act, const GateSums& p, hipStream_t st) {
+  const dim3 grid(p.parts / (256u >> p.lg) * (unsigned)p.strips);
+  if (act == ACT_SILU) hipLaunchKernelGGL((gate_sums_kernel<T, ACT_SILU>), grid, dim3(256), 0, st, p);
+  else if (act == ACT_GELU) hipLaunchKernelGGL((gate_sums_kernel<T, ACT_GELU>), grid, dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((gate_sums_kernel<T, ACT_NONE>), grid, dim3(256), 0, st, p);
+  const int rc = check_launch("gate gradient");
+  if (rc != SF_OK) return rc;
+  int64_t blocks = (2 * (int64_t)p.F + 31) / 32;
+  if (blocks > (1 << 20)) blocks = 1 << 20;
+  hipLaunchKernelGGL((gate_bias_kernel<T>), dim3((unsigned)blocks), dim3(1024), 0, st, p);
+  return check_launch("gate gradient (sums)");
+}
+
+int launch_gate_sums(int act, const void* g, const void* pre, void* out, void* db, float* part, int64_t M, int64_t F,
+                     sf_dtype dt, hipStream_t st) {
+  GateSums p;
+  gate_sums_split(M, F, p);
+  p.g = g, p.pre = pre, p.out = out, p.db = db, p.part = part;
+  p.M = M;
+  p.F = (int)F;
+  switch (dt) {
+    case SF_F16: return launch_gate_sums_t<F16>(act, p, st);
+    case SF_BF16: return launch_gate_sums_t<BF16>(act, p, st);
+    default: return launch_gate_sums_t<float>(act, p, st);
+  }
+}
+
+// y = act(x Wg^T + bg) * (x Wu^T + bu), and the two projections, fp32, M <= 16:
+// bound by reading the weight once.  A workgroup takes 16 gate rows and their 16
+// up rows; its eight waves share K, each step of a wave 16 k: a lane loads four
+// of its row of W (and of x), and the k-th MFMA of 16 x 16 x 4 takes the k-th of
+// each, UNROLL steps asked for ahead of their products.  The waves' sums are
+// added in order through LDS.
+template <int UNROLL>
+__global__ __launch_bounds__(512) void gated_skinny32_kernel(const float* X, const float* W, const float* bias, float* Y,
+                                                             float* pre, int M, int F, int K, int act) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, kc = (lane >> 4) * 4;
+  const int n0 = blockIdx.x * 16;
+  const int steps = (K + 15) / 16, per = (steps + 7) / 8, begin = wave * per;
+  const int end = begin + per < steps ? begin + per : steps;
+  const bool wok = n0 + r < F, xok = r < M;
+  const float* wg = W + (int64_t)(wok ? n0 + r : 0) * K + kc;
+  const float* wu = wg + (int64_t)F * K;
+  const float* xr = X + (int64_t)(xok ? r : 0) * K + kc;
+  f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+  for (int s0 = begin; s0 < end; s0 += UNROLL) {
+    f32x4 w[UNROLL][2], x[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int s = s0 + u;
+      const bool in = s < end && s * 16 + kc < K;  // K % 4 == 0: all four or none
+      const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+      w[u][0] = in && wok ? __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(wg + s * 16)) : z;
+      w[u][1] = in && wok ? __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(wu + s * 16)) : z;
+      x[u] = in && xok ? *reinterpret_cast<const f32x4*>(xr + s * 16) : z;
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[u][j][e], x[u][e], acc[j], 0, 0, 0);
+  }
+  __shared__ f32x4 red[7][2][64];
+  if (wave > 0) {
+    red[wave - 1][0][lane] = acc[0];
+    red[wave - 1][1][lane] = acc[1];
+  }
+  __syncthreads();
+  if (wave != 0 || !xok) return;
+  for (int v = 0; v < 7; ++v)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) acc[j] += red[v][j][lane];
+  const int f = n0 + kc;  // this lane's outputs: row r, columns f .. f + 3
+  if (f >= F) return;
+  const bool vec = (F & 3) == 0 && ((reinterpret_cast<uintptr_t>(Y) | reinterpret_cast<uintptr_t>(pre)) & 15) == 0;
+  with_act(act, [&](auto act_c) {
+    constexpr int ACT = decltype(act_c)::value;
+    float g[4], u[4], y[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const bool has = bias != nullptr && f + q < F;
+      g[q] = acc[0][q] + (has ? bias[f + q] : 0.f);
+      u[q] = acc[1][q] + (has ? bias[F + f + q] : 0.f);
+      y[q] = act_t<ACT>(g[q]) * u[q];
+    }
+    Store4<float>::run(Y + (int64_t)r * F, f, F, vec, y);
+    Store4<float>::run(pre + (int64_t)r * 2 * F, f, F, vec, g);
+    Store4<float>::run(pre + (int64_t)r * 2 * F + F, f, F, vec, u);
+  });
+}
+
+int launch_gated_skinny32(const void* x, const void* W, const void* bias, void* y, void* pre, int64_t M, int64_t F,
+                          int64_t K, int act, hipStream_t st) {
+  hipLaunchKernelGGL((gated_skinny32_kernel<4>), dim3((unsigned)((F + 15) / 16)), dim3(512), 0, st,
+                     static_cast<const float*>(x), static_cast<const float*>(W), static_cast<const float*>(bias),
+                     static_cast<float*>(y), static_cast<float*>(pre), (int)M, (int)F, (int)K, act);
+  return check_launch("gated product (fp32, few rows)");
 }
 
 template <typename T>

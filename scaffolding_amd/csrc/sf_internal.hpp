@@ -256,6 +256,11 @@ int64_t norm_rope_work(int64_t batch, int64_t rows, int heads, int kv_heads, int
 int launch_gated_bf16(int cfg, const GatedParams& p, unsigned gx, hipStream_t st);
 int launch_gated_f16(int cfg, const GatedParams& p, unsigned gx, hipStream_t st);
 // back: out [M, 2 F] from g [M, F] and pre; otherwise out [M, F] from pre.
+int64_t gate_sums_work(int64_t M, int64_t F);
+int launch_gate_sums(int act, const void* g, const void* pre, void* out, void* db, float* part, int64_t M, int64_t F,
+                     sf_dtype dt, hipStream_t st);
+int launch_gated_skinny32(const void* x, const void* W, const void* bias, void* y, void* pre, int64_t M, int64_t F,
+                          int64_t K, int act, hipStream_t st);
 int launch_gate(int act, bool back, const void* g, const void* pre, void* out, int64_t M, int64_t F, sf_dtype dt,
                 hipStream_t st);
 

@@ -19,6 +19,7 @@ from .. import _cuda_ops as _cuops
 from ..device import device as _device_t
 from ..dtype import dtype as _dtype_t
 from ..tensor import Tensor, _gpu_only
+from ..tensor import zeros as _zeros
 
 
 class Parameter(Tensor):
@@ -468,5 +469,130 @@ class _ExpertLinear(Module):
         return F.linear_q4(x, self.weight, self.scales, self.zeros, self.bias, activation, offsets)
 
 
-__all__ = ["Module", "Parameter", "Sequential", "Linear", "LinearQ4", "MoE", "LayerNorm", "RMSNorm", "Dropout", "SiLU", "GELU",
-           "_device_t", "_dtype_t"]
+class GatedMLP(Module):
+    """A gated feed-forward layer: down(act(x Wg^T + bg) * (x Wu^T + bu)), the
+    part in brackets in one launch (F.gated_linear).  up.weight (2 hidden, dim)
+    holds Wg's rows, then Wu's, up.bias (2 hidden,) likewise; down.weight (dim,
+    hidden).  Inference, as Linear (F.gated_linear_backward gives the
+    gradients)."""
+
+    def __init__(self, dim: int, hidden: int, bias: bool = True, activation: str | None = "silu", device=None,
+                 dtype=None):
+        super().__init__()
+        self.dim, self.hidden, self.activation = dim, hidden, activation
+        self.up = Linear(dim, 2 * hidden, bias, device, dtype)
+        self.down = Linear(hidden, dim, bias, device, dtype)
+
+    def forward(self, x: Tensor, residual: Tensor | None = None) -> Tensor:
+        from . import functional as F
+        return self.down(F.gated_linear(x, self.up.weight, self.up.bias, self.activation), residual=residual)
+
+
+class WindowAttention(Module):
+    """Causal self-attention over a sliding window of tokens and `sinks` first
+    ones that stay visible (window None: every token up to its own): `heads`
+    query heads share `kv_heads` key heads, queries and keys are normed per head
+    (norm 'rms' or 'layer', norm_weight and, for 'layer', norm_bias (2,
+    head_dim): queries, keys) and their first `rotary` columns rotated by
+    position, up to max_positions.  qkv.weight ((heads + 2 kv_heads) head_dim,
+    dim), out.weight (dim, heads head_dim).  float16 or bfloat16.
+
+    forward(x) takes whole sequences (B, N, dim), lengths (int32 (B,)) ending
+    each.  With caches (cache()) it takes n new tokens a sequence behind the
+    lengths[b] that the caches hold, writes their keys and values there and
+    attends over all of them; the caller adds n to `lengths` after its last
+    layer.  Four launches either way, one more where few tokens attend over
+    many.  Inference, as Linear (F.*_backward give the gradients)."""
+
+    def __init__(self, dim: int, heads: int, kv_heads: int | None = None, head_dim: int | None = None,
+                 window: int | None = None, sinks: int = 0, max_positions: int = 4096, rotary: int | None = None,
+                 base: float = 10000.0, interleaved: bool = False, norm: str = "rms", eps: float = 1e-6,
+                 bias: bool = False, device=None, dtype="bfloat16"):
+        super().__init__()
+        kv_heads = heads if kv_heads is None else kv_heads
+        if heads < 1 or kv_heads < 1 or heads % kv_heads:
+            raise ValueError("WindowAttention: %d heads cannot share %d key heads" % (heads, kv_heads))
+        if head_dim is None:
+            if dim % heads:
+                raise ValueError("WindowAttention: %d columns do not split into %d heads" % (dim, heads))
+            head_dim = dim // heads
+        if head_dim < 8 or head_dim > 128 or head_dim % 8:
+            raise ValueError("WindowAttention: the head size must be a multiple of 8 up to 128, got %d" % head_dim)
+        if window is not None and window < 1 or sinks < 0:
+            raise ValueError("WindowAttention: needs a window of at least 1 (or None) and sinks >= 0")
+        rotary = head_dim if rotary is None else rotary
+        if rotary < 0 or rotary > head_dim or rotary % 2:
+            raise ValueError("WindowAttention: rotary must be an even number up to %d, got %d" % (head_dim, rotary))
+        if norm not in ("rms", "layer"):
+            raise ValueError("WindowAttention: unknown norm %r" % (norm,))
+        self._check_dtype(dtype)
+        from .functional import rope_table
+        self.heads, self.kv_heads, self.head_dim = heads, kv_heads, head_dim
+        self.window, self.sinks = window, sinks
+        self.interleaved, self.norm, self.eps = interleaved, norm, eps
+        dev = device or "cuda"
+        self.qkv = Linear(dim, (heads + 2 * kv_heads) * head_dim, bias, dev, dtype)
+        self.out = Linear(heads * head_dim, dim, bias, dev, dtype)
+        self.norm_weight = Parameter(np.ones((2, head_dim), np.float32), dtype=dtype, device=dev)
+        self.norm_bias = None
+        if norm == "layer":
+            self.norm_bias = Parameter(np.zeros((2, head_dim), np.float32), dtype=dtype, device=dev)
+        self.table = rope_table(max_positions, rotary, base, dev) if rotary else None
+
+    def _check_dtype(self, dtype) -> None:
+        if dtype is not None and _dtype_t.from_any(dtype).value not in ("float16", "bfloat16"):
+            raise TypeError("WindowAttention: float16 or bfloat16 layers only, not %s" % (dtype,))
+
+    def to(self, device=None, dtype=None) -> "WindowAttention":
+        super().to(device, dtype)
+        if self.table is not None:
+            self.table = self.table.to(device)  # stays fp32
+        return self
+
+    def cache(self, batch: int, capacity: int) -> tuple[Tensor, Tensor]:
+        """Zeroed caches of keys and values, (batch, capacity, kv_heads
+        head_dim), on the weights' device in their type."""
+        w = self.qkv.weight
+        shape = (batch, capacity, self.kv_heads * self.head_dim)
+        return _zeros(*shape, dtype=w.dtype, device=w.device), _zeros(*shape, dtype=w.dtype, device=w.device)
+
+    def forward(self, x: Tensor, lengths: Tensor | None = None, cache: tuple[Tensor, Tensor] | None = None,
+                residual: Tensor | None = None) -> Tensor:
+        from . import functional as F
+        qkv = self.qkv(x)
+        made = (self.norm_weight, self.norm_bias, self.norm, self.eps, None, self.interleaved)
+        heads = (self.heads, self.kv_heads)
+        if cache is None:
+            qkv = F.qk_norm_rope(qkv, *heads, self.table, *made)
+            y = F.window_attention(qkv, *heads, self.window, self.sinks, None, lengths)
+        else:
+            if lengths is None:
+                raise ValueError("WindowAttention: a cache needs the lengths that it holds")
+            q = F.qk_norm_rope_cached(qkv, *heads, self.table, *cache, lengths, *made)
+            y = F.window_attention_cached(q, *cache, lengths, *heads, self.window, self.sinks)
+        return self.out(y, residual=residual)
+
+
+class DecoderBlock(Module):
+    """A causal transformer block: x + attention(norm1(x)), then + mlp(norm2(
+    .)), with RMSNorm, WindowAttention (its arguments as there) and GatedMLP;
+    the two sums are in the layers' last launches."""
+
+    def __init__(self, dim: int, hidden: int, heads: int, kv_heads: int | None = None, eps: float = 1e-6,
+                 activation: str | None = "silu", device=None, dtype="bfloat16", **attention):
+        super().__init__()
+        self.norm1 = RMSNorm(dim, eps, device, dtype)
+        self.attention = WindowAttention(dim, heads, kv_heads, eps=eps, device=device, dtype=dtype, **attention)
+        self.norm2 = RMSNorm(dim, eps, device, dtype)
+        self.mlp = GatedMLP(dim, hidden, False, activation, device, dtype)
+
+    def cache(self, batch: int, capacity: int) -> tuple[Tensor, Tensor]:
+        return self.attention.cache(batch, capacity)
+
+    def forward(self, x: Tensor, lengths: Tensor | None = None, cache: tuple[Tensor, Tensor] | None = None) -> Tensor:
+        h = self.attention(self.norm1(x), lengths, cache, residual=x)
+        return self.mlp(self.norm2(h), residual=h)
+
+
+__all__ = ["Module", "Parameter", "Sequential", "Linear", "LinearQ4", "MoE", "GatedMLP", "WindowAttention",
+           "DecoderBlock", "LayerNorm", "RMSNorm", "Dropout", "SiLU", "GELU", "_device_t", "_dtype_t"]
