@@ -397,7 +397,9 @@ int sf_gated_linear(const void* x, const void* W, const void* bias, void* y, voi
     return fail(SF_ERR_INVALID_ARG, "%s: null pointer", name);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype != SF_F32) return gated16(x, W, bias, y, pre, M, F, K, dtype, act, st);
-  // few rows: in one launch, bound by the weight's reading (FP32_RULE)
+  // few rows: in one launch, bound by the weight's reading (F 5312, K 2416: 25 us
+  // for one row and 36 for 16, the product and the gate 86; F 11008, K 4096: 81
+  // and 122, 145)
   if (M <= 16 && K > 0 && K % 4 == 0 && aligned16(x) && aligned16(W) && F < (int64_t(1) << 26))
     return launch_gated_skinny32(x, W, bias, y, pre, M, F, K, epi_act(act), st);
   rc = sf_gemm(0, 1, M, 2 * F, K, 1, x, K > 0 ? K : 1, 0, W, K > 0 ? K : 1, 0, pre, 2 * F, 0, SF_F32, SF_F32, 1.0f,

@@ -11,7 +11,6 @@
 // columns of a row, in 16-byte pieces at any alignment.
 //
 // And the fp32 layer for few rows, whole: gated_skinny32_kernel.
-#include "gemm16.hpp"
 #include "rowio.hpp"
 #include "sf_internal.hpp"
 
@@ -52,8 +51,9 @@ __global__ __launch_bounds__(256) void gate_kernel(const void* g, const void* pr
 // 8 columns and p.rows rows, its 256 / TC thread rows every 256 / TC-th of them;
 // each thread row leaves its sums (fp32, of the gradients ahead of their
 // rounding) in a row of part [chunks * 256 / TC, 2 F].  The columns' threads
-// stay with their columns, so the sums need no reading of what was written
-// (4096 rows, F 7680, bf16: GATE_SUM_US).
+// stay with their columns, so the sums need no reading of what was written:
+// 4096 rows, F 7680, bf16 in 73 us (315 MB, 4.3 TB/s) and 5 for the parts' sums,
+// where the gate alone takes 63 and summing its result 25.
 struct GateSums {
   const void *g, *pre;
   void *out, *db;
@@ -72,7 +72,6 @@ __global__ __launch_bounds__(256) void gate_sums_kernel(GateSums p) {
   if (left <= 0) return;
   const int64_t end = (chunk + 1) * p.rows < p.M ? (chunk + 1) * p.rows : p.M;
   float sg[8] = {}, su[8] = {};
-#pragma unroll 2
   for (int64_t m = chunk * p.rows + tr; m < end; m += step) {
     float gate[8], up[8], d[8];
     load_cols<T>(p.pre, m * 2 * F + f, left, gate);
@@ -120,7 +119,8 @@ __global__ __launch_bounds__(1024) void gate_bias_kernel(GateSums p) {
   }
 }
 
-// Chunks of at least 16 rows a thread, in at most 8 workgroups a CU.
+// Chunks of at least 16 rows a thread, in at most 8 workgroups a CU (32 rows,
+// half as many workgroups at 4096 rows: 103 us instead of 73).
 static void gate_sums_split(int64_t M, int64_t F, GateSums& p) {
   const int64_t pieces = (F + 7) / 8;
   p.lg = 0;
@@ -170,73 +170,65 @@ int launch_gate_sums(int act, const void* g, const void* pre, void* out, void* d
 }
 
 // y = act(x Wg^T + bg) * (x Wu^T + bu), and the two projections, fp32, M <= 16:
-// bound by reading the weight once.  A workgroup takes 16 gate rows and their 16
-// up rows; its eight waves share K, each step of a wave 16 k: a lane loads four
-// of its row of W (and of x), and the k-th MFMA of 16 x 16 x 4 takes the k-th of
-// each, UNROLL steps asked for ahead of their products.  The waves' sums are
-// added in order through LDS.
+// bound by reading the weight once.  A workgroup takes 8 gate rows and their 8
+// up rows, the 16 rows of one MFMA operand; its eight waves share K, each step
+// of a wave 16 k: a lane loads four of its row of W (and of x), and the k-th
+// MFMA of 16 x 16 x 4 takes the k-th of each, UNROLL steps asked for ahead of
+// their products (8 steps: 10 % slower; 16 gate rows a workgroup: 33 us for 25 at
+// F 5312, whose 332 workgroups fill 256 CUs badly).  The waves' sums are added in
+// order through LDS.  One row, F 11008, K 4096: 81 us, 361 MB, 4.5 TB/s; 16 rows
+// 122 us, with x read from L2 by every workgroup.
 template <int UNROLL>
 __global__ __launch_bounds__(512) void gated_skinny32_kernel(const float* X, const float* W, const float* bias, float* Y,
                                                              float* pre, int M, int F, int K, int act) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, kc = (lane >> 4) * 4;
-  const int n0 = blockIdx.x * 16;
+  const int n0 = blockIdx.x * 8, n = n0 + (r & 7);
   const int steps = (K + 15) / 16, per = (steps + 7) / 8, begin = wave * per;
   const int end = begin + per < steps ? begin + per : steps;
-  const bool wok = n0 + r < F, xok = r < M;
-  const float* wg = W + (int64_t)(wok ? n0 + r : 0) * K + kc;
-  const float* wu = wg + (int64_t)F * K;
+  const bool wok = n < F, xok = r < M;
+  const float* wr = W + ((wok ? n : 0) + (r < 8 ? 0 : (int64_t)F)) * K + kc;
   const float* xr = X + (int64_t)(xok ? r : 0) * K + kc;
-  f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   for (int s0 = begin; s0 < end; s0 += UNROLL) {
-    f32x4 w[UNROLL][2], x[UNROLL];
+    f32x4 w[UNROLL], x[UNROLL];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
       const int s = s0 + u;
       const bool in = s < end && s * 16 + kc < K;  // K % 4 == 0: all four or none
       const f32x4 z = {0.f, 0.f, 0.f, 0.f};
-      w[u][0] = in && wok ? __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(wg + s * 16)) : z;
-      w[u][1] = in && wok ? __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(wu + s * 16)) : z;
+      w[u] = in && wok ? __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(wr + s * 16)) : z;
       x[u] = in && xok ? *reinterpret_cast<const f32x4*>(xr + s * 16) : z;
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(w[u][e], x[u][e], acc, 0, 0, 0);
+  }
+  // Lane (g, m) holds rows 4 g .. 4 g + 3 of token m: rows 0 .. 7 gates, 8 .. 15
+  // the up rows.
+  __shared__ float red[8][4][64];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[u][j][e], x[u][e], acc[j], 0, 0, 0);
-  }
-  __shared__ f32x4 red[7][2][64];
-  if (wave > 0) {
-    red[wave - 1][0][lane] = acc[0];
-    red[wave - 1][1][lane] = acc[1];
-  }
+  for (int q = 0; q < 4; ++q) red[wave][q][lane] = acc[q];
   __syncthreads();
-  if (wave != 0 || !xok) return;
-  for (int v = 0; v < 7; ++v)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) acc[j] += red[v][j][lane];
-  const int f = n0 + kc;  // this lane's outputs: row r, columns f .. f + 3
-  if (f >= F) return;
-  const bool vec = (F & 3) == 0 && ((reinterpret_cast<uintptr_t>(Y) | reinterpret_cast<uintptr_t>(pre)) & 15) == 0;
-  with_act(act, [&](auto act_c) {
-    constexpr int ACT = decltype(act_c)::value;
-    float g[4], u[4], y[4];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const bool has = bias != nullptr && f + q < F;
-      g[q] = acc[0][q] + (has ? bias[f + q] : 0.f);
-      u[q] = acc[1][q] + (has ? bias[F + f + q] : 0.f);
-      y[q] = act_t<ACT>(g[q]) * u[q];
-    }
-    Store4<float>::run(Y + (int64_t)r * F, f, F, vec, y);
-    Store4<float>::run(pre + (int64_t)r * 2 * F, f, F, vec, g);
-    Store4<float>::run(pre + (int64_t)r * 2 * F + F, f, F, vec, u);
-  });
+  const int m = threadIdx.x >> 3, c = threadIdx.x & 7, f = n0 + c;
+  if (m >= M || f >= F) return;
+  float g = 0.f, u = 0.f;
+  for (int v = 0; v < 8; ++v) {
+    g += red[v][c & 3][(c >> 2) * 16 + m];
+    u += red[v][c & 3][(c >> 2) * 16 + 32 + m];
+  }
+  if (bias != nullptr) {
+    g += bias[f];
+    u += bias[F + f];
+  }
+  Y[(int64_t)m * F + f] = (act == ACT_SILU ? act_t<ACT_SILU>(g) : act == ACT_GELU ? act_t<ACT_GELU>(g) : g) * u;
+  pre[(int64_t)m * 2 * F + f] = g;
+  pre[(int64_t)m * 2 * F + F + f] = u;
 }
 
 int launch_gated_skinny32(const void* x, const void* W, const void* bias, void* y, void* pre, int64_t M, int64_t F,
                           int64_t K, int act, hipStream_t st) {
-  hipLaunchKernelGGL((gated_skinny32_kernel<4>), dim3((unsigned)((F + 15) / 16)), dim3(512), 0, st,
+  hipLaunchKernelGGL((gated_skinny32_kernel<4>), dim3((unsigned)((F + 7) / 8)), dim3(512), 0, st,
                      static_cast<const float*>(x), static_cast<const float*>(W), static_cast<const float*>(bias),
                      static_cast<float*>(y), static_cast<float*>(pre), (int)M, (int)F, (int)K, act);
   return check_launch("gated product (fp32, few rows)");
