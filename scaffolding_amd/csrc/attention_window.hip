@@ -67,8 +67,16 @@ int64_t win_cached_work(const WinShape& a) {
          (int64_t)(win_part_floats(a.D) * sizeof(float));
 }
 
+template <typename T, int DW, bool FEW>
+static int launch_win_rows(const WinParams& p, hipStream_t st) {
+  const dim3 g((unsigned)((int64_t)p.B * p.H * p.QB));
+  if (p.lse != nullptr) hipLaunchKernelGGL((win_attn_kernel<T, DW, true, FEW>), g, dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((win_attn_kernel<T, DW, false, FEW>), g, dim3(256), 0, st, p);
+  return check_launch("window attention");
+}
+
 template <typename T, int DW>
-static int launch_win(const WinParams& p, int parts, hipStream_t st) {
+static int launch_win(const WinParams& p, int parts, bool few, hipStream_t st) {
   if (parts > 0) {
     const int64_t items = (int64_t)p.B * p.Hk * p.RB;
     hipLaunchKernelGGL((win_split_kernel<T, DW>), dim3((unsigned)(items * parts)), dim3(256), 0, st, p);
@@ -77,10 +85,7 @@ static int launch_win(const WinParams& p, int parts, hipStream_t st) {
     hipLaunchKernelGGL((win_merge_kernel<T, DW>), dim3((unsigned)(items * (DW / 32))), dim3(256), 0, st, p);
     return check_launch("window attention (merge)");
   }
-  const dim3 g((unsigned)((int64_t)p.B * p.H * p.QB));
-  if (p.lse != nullptr) hipLaunchKernelGGL((win_attn_kernel<T, DW, true>), g, dim3(256), 0, st, p);
-  else hipLaunchKernelGGL((win_attn_kernel<T, DW, false>), g, dim3(256), 0, st, p);
-  return check_launch("window attention");
+  return few ? launch_win_rows<T, DW, true>(p, st) : launch_win_rows<T, DW, false>(p, st);
 }
 
 int launch_window(const WinShape& a, sf_dtype dt, float* ws, hipStream_t st) {
@@ -93,12 +98,15 @@ int launch_window(const WinShape& a, sf_dtype dt, float* ws, hipStream_t st) {
     p.RB = (int)cdiv64(a.Sq * p.G, 16);
     p.ws = ws;
   }
+  const int64_t halves = a.batch * a.heads * cdiv64(a.Sq, WinCfg<64, true>::ROWS);
+  const bool few = halves <= (a.D > 64 ? 1 : 2) * cu_count_current();
+  if (few) p.QB = (int)cdiv64(a.Sq, WinCfg<64, true>::ROWS);
   const bool h = dt == SF_F16;
   switch (win_width(a.D)) {
-    case 64: return h ? launch_win<F16, 64>(p, parts, st) : launch_win<BF16, 64>(p, parts, st);
-    case 96: return h ? launch_win<F16, 96>(p, parts, st) : launch_win<BF16, 96>(p, parts, st);
+    case 64: return h ? launch_win<F16, 64>(p, parts, few, st) : launch_win<BF16, 64>(p, parts, few, st);
+    case 96: return h ? launch_win<F16, 96>(p, parts, few, st) : launch_win<BF16, 96>(p, parts, few, st);
   }
-  return h ? launch_win<F16, 128>(p, parts, st) : launch_win<BF16, 128>(p, parts, st);
+  return h ? launch_win<F16, 128>(p, parts, few, st) : launch_win<BF16, 128>(p, parts, few, st);
 }
 
 }  // namespace sf

@@ -197,17 +197,23 @@ __device__ __attribute__((noinline)) void win_exact_rows(const WinParams& p, con
   }
 }
 
-template <int DW>
+// FEW: where all workgroups of half the rows run at once, one a CU (two at head
+// sizes up to 64): a workgroup's few blocks do not hide their loads' latency, so
+// three of them are under way.  3 x 777 rows, 6 + 2 heads of 72, window 100: 10.2
+// us (else 14.2); 1024 rows, 16 + 4 heads of 128: 22.6 (27.0); 4096 rows of 4 + 1:
+// 73.7 (86.2).  Where twice as many would run, 25.2 instead of 20.6 (2 x 1024 rows,
+// 16 + 4 heads of 128, window 200).
+template <int DW, bool FEW = false>
 struct WinCfg {
-  static constexpr int MB = 2;                 // 16-row query blocks per wave
+  static constexpr int MB = FEW ? 1 : 2;       // 16-row query blocks per wave
   static constexpr int ROWS = 4 * MB * 16;     // query rows per workgroup
   static constexpr int HALVES = (DW + 63) / 64;
-  static constexpr int NS = DW > 64 ? 2 : 3;   // key blocks of 64 in LDS
+  static constexpr int NS = FEW ? 4 : (DW > 64 ? 2 : 3);  // key blocks of 64 in LDS
 };
 
-template <typename T, int DW, bool LSE>
-__global__ __launch_bounds__(256, 2) void win_attn_kernel(WinParams p) {
-  using C = WinCfg<DW>;
+template <typename T, int DW, bool LSE, bool FEW>
+__global__ __launch_bounds__(256, FEW && DW > 64 ? 1 : 2) void win_attn_kernel(WinParams p) {
+  using C = WinCfg<DW, FEW>;
   constexpr int MB = C::MB, HV = C::HALVES, NS = C::NS;
   constexpr int KC = DW / 32, DB = DW / 16;
   constexpr int KB = 64;
@@ -265,8 +271,9 @@ __global__ __launch_bounds__(256, 2) void win_attn_kernel(WinParams p) {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rV, (lds_ptr_t)(v + 1024), 16, ov + v8, 0, 0, 0);
     }
   };
-  if (nkb > 0) issue(0);
-  if (NS > 2 && nkb > 1) issue(1);
+#pragma unroll
+  for (int i = 0; i < NS - 1; ++i)
+    if (i < nkb) issue(i);
 
   u32x4 qf[MB][KC];
 #pragma unroll
@@ -304,7 +311,9 @@ __global__ __launch_bounds__(256, 2) void win_attn_kernel(WinParams p) {
   for (int i = 0; i < nkb; ++i) {
     const int st = i % NS, j = kbs.at(i);
     __builtin_amdgcn_sched_barrier(0);
-    if (NS == 3 && i + 1 < nkb)
+    if (NS == 4 && i + 2 < nkb)
+      __builtin_amdgcn_s_waitcnt(waitcnt_imm(2 * LPB, 0));
+    else if (NS >= 3 && i + 1 < nkb)
       __builtin_amdgcn_s_waitcnt(waitcnt_imm(LPB, 0));
     else
       __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 0));
@@ -469,15 +478,17 @@ __global__ __launch_bounds__(256, 2) void win_attn_kernel(WinParams p) {
     __builtin_amdgcn_s_setprio(1);
     sums(0);
     pv(0, h0, n0);
-    expo(1);
+    if constexpr (MB > 1) {
+      expo(1);
 #pragma unroll
-    for (int g = 0; g < 10; ++g) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x002, LSE ? 4 : 3, 0);
+      for (int g = 0; g < 10; ++g) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, LSE ? 4 : 3, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      sums(1);
+      pv(1, h0, n0);
     }
-    __builtin_amdgcn_sched_barrier(0);
-    sums(1);
-    pv(1, h0, n0);
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (HV > 1) {
       constexpr std::integral_constant<int, 1> h1{};
@@ -486,7 +497,7 @@ __global__ __launch_bounds__(256, 2) void win_attn_kernel(WinParams p) {
       __builtin_amdgcn_s_waitcnt(waitcnt_imm(63, 0));
       __builtin_amdgcn_sched_barrier(0);
       pv(0, h1, n1);
-      pv(1, h1, n1);
+      if constexpr (MB > 1) pv(1, h1, n1);
       __builtin_amdgcn_sched_barrier(0);
     }
     __builtin_amdgcn_s_setprio(0);
