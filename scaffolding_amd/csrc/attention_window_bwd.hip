@@ -21,10 +21,10 @@ static int64_t win_ranges(const WinShape& a) {
 static int64_t round256(int64_t n) { return cdiv64(n, 256) * 256; }
 static size_t part_floats(int64_t D) { return static_cast<size_t>(2 * 128) * win_width(D); }
 
-// delta, the ranges' starts, their sums.
+// The rows' statistics, the ranges' starts, their sums.
 int64_t win_back_work(const WinShape& a) {
   const int64_t n = win_ranges(a);
-  return round256(a.batch * a.heads * a.Sq * 4) + round256((n + 1) * static_cast<int64_t>(sizeof(WinStart))) +
+  return round256(2 * a.batch * a.heads * a.Sq * 4) + round256((n + 1) * static_cast<int64_t>(sizeof(WinStart))) +
          2 * n * static_cast<int64_t>(part_floats(a.D) * sizeof(float));
 }
 
@@ -50,8 +50,8 @@ int launch_window_back(const WinShape& a, const WinBack& g, sf_dtype dt, void* w
   p.scale = a.scale;
   p.KBS = (int)cdiv64(a.Sk, 128);
   p.ranges = (int)win_ranges(a);
-  p.delta = static_cast<float*>(work);
-  char* at = static_cast<char*>(work) + round256(a.batch * a.heads * a.Sq * 4);
+  p.stat = static_cast<float*>(work);
+  char* at = static_cast<char*>(work) + round256(2 * a.batch * a.heads * a.Sq * 4);
   p.start = reinterpret_cast<WinStart*>(at);
   p.ws = reinterpret_cast<float*>(at + round256((p.ranges + 1) * static_cast<int64_t>(sizeof(WinStart))));
   const bool h = dt == SF_F16;

@@ -52,7 +52,7 @@ struct WinBackParams {
   void *dQ, *dK, *dV;  // strides as Q's, K's and V's
   int64_t sG, hG, sDQ, hDQ, sDK, hDK, sDV, hDV;
   int ldg, lddq, lddk, lddv;
-  float* delta;     // [B, H, Sq]
+  float* stat;      // [2, B, H, Sq]: -lse / ln 2 (P's scale added), then -delta
   float* ws;        // two sums (WinDkvCfg::PART floats) a range: its first and its last key block's
   WinStart* start;  // where each range begins, and the end of the last
   int ranges;
@@ -266,9 +266,12 @@ __global__ __launch_bounds__(256, 2) void win_dq_kernel(WinBackParams bp) {
       }
     d += __shfl_xor(d, 16, 64);
     d += __shfl_xor(d, 32, 64);
-    dl[mb] = d;
+    dl[mb] = -d;
     nl[mb] = row < sq.rows ? S::log2 - p.lse[stat + row] * 1.4426950408889634f : 0.f;
-    if (row < sq.rows && lane < 16) bp.delta[stat + row] = d;
+    if (row < sq.rows && lane < 16) {
+      bp.stat[stat + row] = nl[mb];
+      bp.stat[(int64_t)p.B * p.H * p.Sq + stat + row] = -d;
+    }
   }
   f32x4 dq[MB][DB];
 #pragma unroll
@@ -310,7 +313,7 @@ __global__ __launch_bounds__(256, 2) void win_dq_kernel(WinBackParams bp) {
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb) {
-          dp[mb][N] = f32x4{0.f, 0.f, 0.f, 0.f};
+          dp[mb][N] = f32x4{dl[mb], dl[mb], dl[mb], dl[mb]};
 #pragma unroll
           for (int kc = 0; kc < KC; ++kc) dp[mb][N] = Mfma16<T>::run(vf[kc], gf[mb][kc], dp[mb][N]);
         }
@@ -332,7 +335,7 @@ __global__ __launch_bounds__(256, 2) void win_dq_kernel(WinBackParams bp) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mb][n][q], p.scale_log2e, nl[mb]));
-            v[q] = e * ((dp[mb][n][q] - dl[mb]) * S::down);
+            v[q] = e * (dp[mb][n][q] * S::down);
             if (edge && !win_sees(p, sq, pos, k0 + CH * 32 + n * 16 + 4 * (lane >> 4) + q)) v[q] = 0.f;
           }
           ds[mb][2 * n] = pack2<T>(v[0], v[1]);
@@ -395,7 +398,7 @@ __global__ __launch_bounds__(512, 2) void win_dkv_kernel(WinBackParams bp) {
       else win_load_tile<HV>(Gb + g * bp.hG, bp.ldg, row0, n, p.D, &sG[st][0], wave - 4, lane);
       if (wave < 2) {
         const int left = n - row0 < RB ? n - row0 : RB;
-        const float* src = (wave == 0 ? p.lse : bp.delta) + ((int64_t)b * p.H + hk * p.G + g) * p.Sq + row0;
+        const float* src = bp.stat + (((int64_t)wave * p.B + b) * p.H + hk * p.G + g) * p.Sq + row0;
         const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)src, (short)0, left * 4, 0x00020000);
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)&sL[st][wave][0], 4, (uint32_t)lane * 4u, 0, 0, 0);
       }
@@ -450,7 +453,7 @@ __global__ __launch_bounds__(512, 2) void win_dkv_kernel(WinBackParams bp) {
         static_for<DB>([&](auto d) { gt[decltype(d)::value] = win_frag_cols<CH, decltype(d)::value, HB>(ga, fr); });
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) s[i] = dp[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < 2; ++i) s[i] = f32x4{0.f, 0.f, 0.f, 0.f}, dp[i] = dl[CH][i];
 #pragma unroll
         for (int kc = 0; kc < KC; ++kc) {  // four sums side by side
 #pragma unroll
@@ -467,9 +470,8 @@ __global__ __launch_bounds__(512, 2) void win_dkv_kernel(WinBackParams bp) {
           float x[4], v[4];
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const float nl = __builtin_fmaf(ls[CH][i][q], -1.4426950408889634f, S::log2);
-            x[q] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][q], p.scale_log2e, nl));
-            v[q] = x[q] * ((dp[i][q] - dl[CH][i][q]) * S::down);
+            x[q] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][q], p.scale_log2e, ls[CH][i][q]));
+            v[q] = x[q] * (dp[i][q] * S::down);
           }
           if (edge) {
 #pragma unroll
