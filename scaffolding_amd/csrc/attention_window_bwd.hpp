@@ -13,10 +13,24 @@
 //
 //   win_dq_kernel   128 query rows a workgroup (32 a wave), Q and dO in
 //                   registers, blocks of 64 keys of K and V through LDS; it
-//                   forms delta first and leaves it for the other launch
-//   win_dkv_kernel  128 keys a workgroup (16 a wave), K and V in registers,
-//                   blocks of 64 rows of Q and dO of every query head of the
-//                   group through LDS: the sum over heads is part of it
+//                   forms delta first and leaves it, and lse as the exponents
+//                   want it, for the other launch
+//   win_dkv_kernel  128 keys a workgroup, 32 for two waves, their K and V in
+//                   registers, blocks of 64 rows of Q and dO of every query head
+//                   of the group through LDS: the sum over heads is part of it.
+//                   Of two waves each forms P and dS of half the rows, hands
+//                   them to the other through LDS and sums dK and dV of half the
+//                   columns: 320 KB of LDS a block where 16 keys a wave alone
+//                   read 512 (190 -> 179 us below)
+//
+// 2 x 4096 rows, 16 + 4 heads of 128, window 1024, 4 sinks, bf16: 132 us (90 GF,
+// 690 TF/s), 179 us (121 GF, 675 TF/s) and 17 for the cut blocks' sums, 130 MB
+// written and read.  Both products and LDS reading are busy about a third of the
+// time and hardly overlap: two waves a SIMD is what the sums' registers leave, and
+// the barriers keep them in step.  Forming the weights beside the products with V
+// gains 2 % of the second launch and nothing in the first.  A third stage of
+// tiles, or Q's rows asked for a tile ahead, takes more registers or LDS than
+// there are.
 //
 // Both take the forward kernel's operand layouts: scores come out with the
 // summed index (keys here, rows there) across a lane's registers, where the
@@ -362,22 +376,37 @@ struct WinDkvCfg {
   static constexpr int PART = 2 * 128 * DW;  // floats of the sums of a workgroup's 128 keys, dK and dV
 };
 
+// 16 bytes a lane to LDS, in the order of the ds_read16 around it.
+__device__ __forceinline__ void ds_write16(uint32_t addr, u32x4 v) {
+  asm volatile("ds_write_b128 %0, %1" ::"v"(addr), "v"(v) : "memory");
+}
+
 template <typename T, int DW>
 __global__ __launch_bounds__(512, 2) void win_dkv_kernel(WinBackParams bp) {
   using S = WinBackScale<T>;
-  constexpr int HV = WinCfg<DW>::HALVES, KC = DW / 32, DB = DW / 16, RB = 64, HB = RB * 128, NS = 2;
+  constexpr int HV = WinCfg<DW>::HALVES, KC = DW / 32, DB = DW / 16, DH = DB / 2, RB = 64, HB = RB * 128, NS = 2;
   const WinParams& p = bp.w;
   __shared__ __attribute__((aligned(1024))) uint8_t sQ[NS][HV * HB];
   __shared__ __attribute__((aligned(1024))) uint8_t sG[NS][HV * HB];
   __shared__ __attribute__((aligned(256))) float sL[NS][2][RB];
+  __shared__ __attribute__((aligned(1024))) u32x4 sX[8][4][64];  // a wave's P and dS
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int half = wave & 1;  // of a tile's rows, and of the columns of D
   // Each XCD takes a contiguous share of the ranges: neighbouring key blocks
   // read the same rows.
   const int w = xcd_remap((int)blockIdx.x, (int)gridDim.x);
   const WinStart from = bp.start[w], to = bp.start[w + 1];
   WinFrag fr;
   fr.set(lane);
+  uint32_t col[DH];  // transposed fragments of the wave's columns
+#pragma unroll
+  for (int x = 0; x < DH; ++x) {
+    const int db = half * DH + x;
+    col[x] = fr.trow + (uint32_t)(((2 * (db & 3) + fr.tch) ^ fr.tsw) << 4) + (uint32_t)((db >> 2) * HB);
+  }
+  const uint32_t xa = lds_addr(&sX[wave][0][0]) + (uint32_t)lane * 16u;
+  const uint32_t xb = lds_addr(&sX[wave ^ 1][0][0]) + (uint32_t)lane * 16u;
   for (int e = from.block; e < to.block || (e == to.block && to.at > 0); ++e) {
     const int kv = e / bp.KBS, kb = e % bp.KBS;
     const int b = kv / p.Hk, hk = kv % p.Hk;
@@ -386,7 +415,7 @@ __global__ __launch_bounds__(512, 2) void win_dkv_kernel(WinBackParams bp) {
     const WinKeyRows kr = win_key_rows(p, sq, kb);
     const int begin = e == from.block ? from.at : 0, end = e == to.block ? to.at : kr.products;
     const int t0 = begin, t1 = kr.n > 0 ? end : begin;  // past the sequence: nothing to add up
-    const int kw0 = kb * 128 + wave * 16, key = kw0 + (lane & 15);
+    const int kw0 = kb * 128 + (wave >> 1) * 32;
     const uint16_t* Kb = static_cast<const uint16_t*>(p.K) + b * p.sK + hk * p.hK;
     const uint16_t* Vb = static_cast<const uint16_t*>(p.V) + b * p.sV + hk * p.hV;
     const uint16_t* Qb = static_cast<const uint16_t*>(p.Q) + b * p.sQ + (int64_t)hk * p.G * p.hQ;
@@ -405,117 +434,192 @@ __global__ __launch_bounds__(512, 2) void win_dkv_kernel(WinBackParams bp) {
     };
     __syncthreads();  // every wave has read the last block's tiles
     if (t0 < t1) issue(t0);
-    u32x4 kf[KC], vf[KC];
-    f32x4 dk[DB], dv[DB];
-    win_load_rows<KC>(Kb, p.ldk, kw0, n, p.D, lane, kf);
-    win_load_rows<KC>(Vb, p.ldv, kw0, n, p.D, lane, vf);
+    u32x4 kf[2][KC], vf[2][KC];
+    f32x4 dk[2][DH], dv[2][DH];
 #pragma unroll
-    for (int db = 0; db < DB; ++db) dk[db] = dv[db] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < 2; ++j) {
+      win_load_rows<KC>(Kb, p.ldk, kw0 + 16 * j, n, p.D, lane, kf[j]);
+      win_load_rows<KC>(Vb, p.ldv, kw0 + 16 * j, n, p.D, lane, vf[j]);
+#pragma unroll
+      for (int x = 0; x < DH; ++x) dk[j][x] = dv[j][x] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
 
     for (int t = t0; t < t1; ++t) {
-      const int row0 = (kr.first + t % kr.n) * RB, row1 = row0 + RB - 1, st = (t - t0) % NS;
+      const int row0 = (kr.first + t % kr.n) * RB, st = (t - t0) % NS;
       __builtin_amdgcn_sched_barrier(0);
       __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 0));
       __builtin_amdgcn_s_barrier();
       __builtin_amdgcn_sched_barrier(0);
       if (t + 1 < t1) issue(t + 1);
       __builtin_amdgcn_sched_barrier(0);
-      if (row1 < kw0 || (kw0 + 15 <= row0 - p.window && kw0 >= p.sinks)) continue;
-      const bool edge = kw0 + 15 > row0 || row1 >= n || (kw0 <= row1 - p.window && kw0 + 15 >= p.sinks);
-      const uint32_t qa = lds_addr(&sQ[st][0]), ga = lds_addr(&sG[st][0]);
-      const uint32_t la = lds_addr(&sL[st][0][0]) + (uint32_t)(lane >> 4) * 16u;
-      // Rows 32 CH .. + 31 of the block are one chunk; the second's are read while
-      // the first is worked on, in the registers that it has left.
-      u32x4 qf[2][2][KC], gf[2][2][KC];
-      f32x4 ls[2][2], dl[2][2];
-      auto q_rows = [&](auto c) {
-        constexpr int CH = decltype(c)::value;
-        static_for<2>([&](auto i) { win_frag_rows<2 * CH + decltype(i)::value, KC, HB>(qa, fr, qf[CH][decltype(i)::value]); });
+      // whether rows c0 .. c0 + 31 see one of the wave's keys
+      auto meet = [&](int c0) {
+        return !(c0 + 31 < kw0 || (kw0 + 31 <= c0 - p.window && kw0 >= p.sinks) || c0 >= n);
       };
-      auto g_rows = [&](auto c) {
-        constexpr int CH = decltype(c)::value;
-        static_for<2>([&](auto i) {
-          constexpr int N = decltype(i)::value, NB = 2 * CH + N;
-          win_frag_rows<NB, KC, HB>(ga, fr, gf[CH][N]);
-          ls[CH][N] = __builtin_bit_cast(f32x4, ds_read16<NB * 64>(la));
-          dl[CH][N] = __builtin_bit_cast(f32x4, ds_read16<RB * 4 + NB * 64>(la));
+      const uint32_t qa = lds_addr(&sQ[st][0]), ga = lds_addr(&sG[st][0]);
+      // The gradients of the wave's columns from rows 32 c .. + 31: the reading,
+      // and the products.
+      auto columns = [&](uint32_t base, uint32_t c, u32x4 (&f)[DH]) {
+        static_for<DH>([&](auto x_c) {
+          constexpr int X = decltype(x_c)::value;
+          const uint32_t a = base + col[X] + c * 4096u;
+          const u32x2 lo = ds_read_tr16<0>(a), hi = ds_read_tr16<2048>(a);
+          f[X] = u32x4{lo.x, lo.y, hi.x, hi.y};
         });
       };
-      q_rows(std::integral_constant<int, 0>{});
-      g_rows(std::integral_constant<int, 0>{});
-      static_for<2>([&](auto c_c) {
-        constexpr int CH = decltype(c_c)::value;
-        u32x4 gt[DB], qt[DB], pf, ds;
-        f32x4 s[2], dp[2];
+      auto add = [&](const u32x4 (&f)[DH], const u32x4 (&pt)[2], f32x4 (&out)[2][DH]) {
+#pragma unroll
+        for (int x = 0; x < DH; ++x)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) out[j][x] = Mfma16<T>::run(f[x], pt[j], out[j][x]);
+      };
+      const int c0 = row0 + half * 32;
+      if (meet(c0)) {
+        const bool edge = kw0 + 31 > c0 || c0 + 31 >= n || (kw0 <= c0 + 31 - p.window && kw0 + 31 >= p.sinks);
+        const uint32_t la = lds_addr(&sL[st][0][0]) + (uint32_t)half * 128u + (uint32_t)(lane >> 4) * 16u;
+        const uint32_t q0 = qa + (uint32_t)half * 4096u, g0 = ga + (uint32_t)half * 4096u;
+        u32x4 qf[2][KC], gf[2][KC], ls[2], dl[2], pf[2], ds[2], gt[DH], qt[DH];
+        f32x4 s[2][2], dp[2][2];
+        static_for<2>([&](auto i) { win_frag_rows<decltype(i)::value, KC, HB>(q0, fr, qf[decltype(i)::value]); });
+        static_for<2>([&](auto i) {
+          constexpr int I = decltype(i)::value;
+          ls[I] = ds_read16<I * 64>(la);
+          dl[I] = ds_read16<RB * 4 + I * 64>(la);
+          win_frag_rows<I, KC, HB>(g0, fr, gf[I]);
+        });
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(waitcnt_imm(63, 2 * KC + 4));  // Q's rows
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) s[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kc = 0; kc < KC; ++kc)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) s[i][j] = Mfma16<T>::run(qf[i][kc], kf[j][kc], s[i][j]);
         __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_waitcnt(waitcnt_imm(63, 0));
         __builtin_amdgcn_sched_barrier(0);
-        static_for<DB>([&](auto d) { gt[decltype(d)::value] = win_frag_cols<CH, decltype(d)::value, HB>(ga, fr); });
+        columns(ga, (uint32_t)half, gt);
         __builtin_amdgcn_sched_barrier(0);
+        // the weights are formed while the products with V run
 #pragma unroll
-        for (int i = 0; i < 2; ++i) s[i] = f32x4{0.f, 0.f, 0.f, 0.f}, dp[i] = dl[CH][i];
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int kc = 0; kc < KC; ++kc) {  // four sums side by side
+          for (int j = 0; j < 2; ++j) {
+            const f32x4 nl = __builtin_bit_cast(f32x4, ls[i]);
+            dp[i][j] = __builtin_bit_cast(f32x4, dl[i]);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) s[i] = Mfma16<T>::run(qf[CH][i][kc], kf[kc], s[i]);
+            for (int q = 0; q < 4; ++q)
+              s[i][j][q] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][j][q], p.scale_log2e, nl[q]));
+          }
 #pragma unroll
-          for (int i = 0; i < 2; ++i) dp[i] = Mfma16<T>::run(gf[CH][i][kc], vf[kc], dp[i]);
+        for (int kc = 0; kc < KC; ++kc)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) dp[i][j] = Mfma16<T>::run(gf[i][kc], vf[j][kc], dp[i][j]);
+#pragma unroll
+        for (int g = 0; g < 4 * KC; ++g) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
-        static_for<DB>([&](auto d) { qt[decltype(d)::value] = win_frag_cols<CH, decltype(d)::value, HB>(qa, fr); });
+        columns(qa, (uint32_t)half, qt);
         __builtin_amdgcn_sched_barrier(0);
+        if (edge) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int row = row0 + (2 * CH + i) * 16 + 4 * (lane >> 4);
-          float x[4], v[4];
+          for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            x[q] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][q], p.scale_log2e, ls[CH][i][q]));
-            v[q] = x[q] * (dp[i][q] * S::down);
-          }
-          if (edge) {
+            for (int i = 0; i < 2; ++i) {
+              const int key = kw0 + 16 * j + (lane & 15), row = c0 + i * 16 + 4 * (lane >> 4);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const bool see = (row + q < n) & win_sees(p, sq, row + q, key);
-              x[q] = see ? x[q] : 0.f;
-              v[q] = see ? v[q] : 0.f;
+              for (int q = 0; q < 4; ++q) {
+                const bool see = (row + q < n) & win_sees(p, sq, row + q, key);
+                s[i][j][q] = see ? s[i][j][q] : 0.f;
+                dp[i][j][q] = see ? dp[i][j][q] : 0.f;
+              }
             }
-          }
-          pf[2 * i] = pack2<T>(x[0], x[1]);
-          pf[2 * i + 1] = pack2<T>(x[2], x[3]);
-          ds[2 * i] = pack2<T>(v[0], v[1]);
-          ds[2 * i + 1] = pack2<T>(v[2], v[3]);
         }
         __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_waitcnt(waitcnt_imm(63, 2 * DB < 16 ? 2 * DB : 15));  // dO columns
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            pf[j][2 * i] = pack2<T>(s[i][j][0], s[i][j][1]);
+            pf[j][2 * i + 1] = pack2<T>(s[i][j][2], s[i][j][3]);
+          }
+        __builtin_amdgcn_s_waitcnt(waitcnt_imm(63, 2 * DH));  // dO's columns
+        __builtin_amdgcn_sched_barrier(0);
+        add(gt, pf, dv);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float v[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] = s[i][j][q] * (dp[i][j][q] * S::down);
+            ds[j][2 * i] = pack2<T>(v[0], v[1]);
+            ds[j][2 * i + 1] = pack2<T>(v[2], v[3]);
+          }
+#pragma unroll
+        for (int g = 0; g < 2 * DH; ++g) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
+        }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int db = 0; db < DB; ++db) dv[db] = Mfma16<T>::run(gt[db], pf, dv[db]);
+        for (int j = 0; j < 2; ++j) {
+          ds_write16(xa + j * 1024, pf[j]);
+          ds_write16(xa + (2 + j) * 1024, ds[j]);
+        }
+        __builtin_amdgcn_s_waitcnt(waitcnt_imm(63, 4));  // Q's columns
         __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_waitcnt(waitcnt_imm(63, 0));  // Q columns
+        add(qt, ds, dk);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_waitcnt(waitcnt_imm(63, 0));
+      __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_sched_barrier(0);
+      if (meet(row0 + (half ^ 1) * 32)) {  // the neighbour's rows, for the wave's columns
+        u32x4 pf[2], ds[2], gt[DH], qt[DH];
+        pf[0] = ds_read16<0>(xb), pf[1] = ds_read16<1024>(xb);
+        columns(ga, (uint32_t)(half ^ 1), gt);
+        ds[0] = ds_read16<2048>(xb), ds[1] = ds_read16<3072>(xb);
+        columns(qa, (uint32_t)(half ^ 1), qt);
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (CH == 0) q_rows(std::integral_constant<int, 1>{});
+        __builtin_amdgcn_s_waitcnt(waitcnt_imm(63, 2 * DH + 2));
         __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int db = 0; db < DB; ++db) dk[db] = Mfma16<T>::run(qt[db], ds, dk[db]);
+        add(gt, pf, dv);
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (CH == 0) g_rows(std::integral_constant<int, 1>{});
+        __builtin_amdgcn_s_waitcnt(waitcnt_imm(63, 0));
         __builtin_amdgcn_sched_barrier(0);
-      });
+        add(qt, ds, dk);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
     if (begin == 0 && end == kr.products) {
-      win_store_16<T, DB>(static_cast<uint16_t*>(bp.dK) + b * bp.sDK + hk * bp.hDK, bp.lddk, key, n, p.Sk, p.D, bp.scale,
-                          lane, dk);
-      win_store_16<T, DB>(static_cast<uint16_t*>(bp.dV) + b * bp.sDV + hk * bp.hDV, bp.lddv, key, n, p.Sk, p.D, S::down,
-                          lane, dv);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int key = kw0 + 16 * j + (lane & 15), d0 = half * DH * 16;
+        win_store_16<T, DH>(static_cast<uint16_t*>(bp.dK) + b * bp.sDK + hk * bp.hDK + d0, bp.lddk, key, n, p.Sk,
+                            p.D - d0, bp.scale, lane, dk[j]);
+        win_store_16<T, DH>(static_cast<uint16_t*>(bp.dV) + b * bp.sDV + hk * bp.hDV + d0, bp.lddv, key, n, p.Sk,
+                            p.D - d0, S::down, lane, dv[j]);
+      }
     } else {
       f32x4* out = reinterpret_cast<f32x4*>(bp.ws + (int64_t)(2 * w + (begin == 0 ? 1 : 0)) * WinDkvCfg<DW>::PART) +
-                   (wave * DB) * 64 + lane;
+                   ((wave >> 1) * 2 * DB + half * DH) * 64 + lane;
 #pragma unroll
-      for (int db = 0; db < DB; ++db) {
-        out[db * 64] = dk[db];
-        out[(8 * DB + db) * 64] = dv[db];
-      }
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int x = 0; x < DH; ++x) {
+          out[(j * DB + x) * 64] = dk[j][x];
+          out[(8 * DB + j * DB + x) * 64] = dv[j][x];
+        }
     }
   }
 }
