@@ -69,20 +69,40 @@ static int gated_check(const char* name, int64_t M, int64_t F, int64_t K, sf_dty
   return SF_OK;
 }
 
-// Tiles of a gated product: lines of W a tile takes are half gate, half up.
+// Tiles of a gated product: lines of W a tile takes are half gate, half up.  The
+// times are fitted to a sweep of 20 to 4096 rows over layers of F 352 to 11008
+// and K 208 to 4096 (bf16): there the choice is within 6 % of the fastest.
 struct GatedTile {
   int cfg, bm, bn, occ;
-  float tau[4];  // us per 64 k when r workgroups share each CU
+  float tau[4];  // us per 64 k when r workgroups share each CU, in line between
 };
 static constexpr GatedTile kGatedDirect[] = {
-    {TILE_MID_128, 128, 128, 2, {0.72f, 1.15f}},
-    {TILE_MID_64, 64, 64, 3, {0.32f, 0.44f, 0.74f}},
-    {TILE_MID_32, 32, 64, 3, {0.22f, 0.30f, 0.48f}},
+    {TILE_MID_128, 128, 128, 2, {0.68f, 1.14f}},
+    {TILE_MID_64, 64, 64, 3, {0.29f, 0.44f, 0.60f}},
+    {TILE_MID_32, 32, 64, 3, {0.21f, 0.26f, 0.40f}},
 };
 static constexpr GatedTile kGatedStaged[] = {
     {TILE_RAG_128, 128, 128, 2, {0.90f, 1.50f}},
     {TILE_RAG_64, 64, 64, 4, {0.45f, 0.85f, 1.10f, 1.75f}},
 };
+
+static float gated_tiles_us(const GatedTile& c, int64_t tiles, int64_t K, int64_t cus) {
+  const int64_t slots = c.occ * cus, rem = tiles % slots;
+  float us = static_cast<float>(tiles / slots) * c.tau[c.occ - 1];
+  if (rem > 0) {
+    const int64_t r = rem / cus;
+    const float part = static_cast<float>(rem % cus) / static_cast<float>(cus);
+    us += r == 0 ? c.tau[0] : part == 0.0f ? c.tau[r - 1] : c.tau[r - 1] + part * (c.tau[r] - c.tau[r - 1]);
+  }
+  return us * static_cast<float>(cdiv(K, 64)) + 5.0f;  // launch, first loads, epilogue
+}
+
+// A round of 256 x 256 tiles; and one of `rem` of them, left whole or cut into
+// quarters for a second launch.
+static float gated_round_us(int64_t K) { return 12.4f + 0.0227f * static_cast<float>(K); }
+static bool gated_quarters(int64_t rem, int64_t K, int64_t cus) {
+  return rem > 0 && gated_tiles_us(kGatedDirect[0], 4 * rem, K, cus) < gated_round_us(K);
+}
 
 static int gated_tile(int64_t M, int64_t F, int64_t K, bool rows16, bool direct, int& bm, int& bn) {
   const int64_t cus = cu_count_current();
@@ -95,16 +115,15 @@ static int gated_tile(int64_t M, int64_t F, int64_t K, bool rows16, bool direct,
   int cfg = -1;
   if (direct && K % 128 == 0 && K >= 128 && F > 64) {
     const int64_t tiles = cdiv(M, 256) * cdiv(F, 128), rem = tiles % cus;
-    best = (static_cast<float>(tiles / cus) + (rem > 0 ? 1.0f : 0.0f)) * (12.4f + 0.0227f * static_cast<float>(K));
+    best = static_cast<float>(tiles / cus) * gated_round_us(K);
+    if (tiles > cus && gated_quarters(rem, K, cus)) best += gated_tiles_us(kGatedDirect[0], 4 * rem, K, cus);
+    else if (rem > 0) best += gated_round_us(K);
     cfg = TILE_NT_BIG;
     bm = bn = 256;
   }
   for (int i = 0; i < (direct ? 3 : 2); ++i) {
     const GatedTile& c = direct ? kGatedDirect[i] : kGatedStaged[i];
-    const int64_t tiles = cdiv(M, c.bm) * cdiv(2 * F, c.bn), slots = c.occ * cus, rem = tiles % slots;
-    float us = static_cast<float>(tiles / slots) * c.tau[c.occ - 1];
-    if (rem > 0) us += c.tau[cdiv(rem, cus) - 1];
-    us = us * static_cast<float>(cdiv(K, 64)) + 5.0f;  // launch, first loads, epilogue
+    const float us = gated_tiles_us(c, cdiv(M, c.bm) * cdiv(2 * F, c.bn), K, cus);
     if (us < best) {
       best = us;
       cfg = c.cfg;
@@ -142,11 +161,25 @@ static int gated16(const void* x, const void* W, const void* bias, void* y, void
   p.tiles_n = (int)cdiv(2 * F, bn);
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, cus = cu_count_current();
   if (tiles > (int64_t(1) << 22)) return fail(SF_ERR_UNSUPPORTED, "sf_gated_linear: more than 2^22 tiles");
-  // One workgroup a CU walks the tiles where the last round is at most half
-  // full, as sf_gemm's.
-  if (cfg == TILE_NT_BIG && tiles > cus && cus % kNumXcd == 0 && 2 * (tiles % cus) <= cus) p.persist = (int)cus;
-  const unsigned gx = p.persist > 0 ? (unsigned)p.persist : (unsigned)tiles;
-  return dtype == SF_BF16 ? launch_gated_bf16(cfg, p, gx, st) : launch_gated_f16(cfg, p, gx, st);
+  const auto launch = [&](int c, unsigned gx) {
+    return dtype == SF_BF16 ? launch_gated_bf16(c, p, gx, st) : launch_gated_f16(c, p, gx, st);
+  };
+  if (cfg != TILE_NT_BIG) return launch(cfg, (unsigned)tiles);
+  // A part round that its tiles' quarters fill better runs as those: 4096 rows, F
+  // 11008, K 4096 (5.4 rounds) 570 -> 552 us, F 2048 of 4352 rows (1.1) 172 -> 153;
+  // past about half a round the quarters take as long.
+  const int64_t rem = tiles % cus;
+  const bool quarters = tiles > cus && gated_quarters(rem, K, cus);
+  p.head = (int)(quarters ? tiles - rem : tiles);
+  // One workgroup a CU walks the tiles where the last round is full or at most
+  // half full, as sf_gemm's.
+  if (p.head > cus && cus % kNumXcd == 0 && 2 * (p.head % cus) <= cus) p.persist = (int)cus;
+  const int rc = launch(cfg, p.persist > 0 ? (unsigned)p.persist : (unsigned)p.head);
+  if (rc != SF_OK || !quarters) return rc;
+  p.persist = 0;
+  p.big_m = p.tiles_m;
+  p.big_n = p.tiles_n;
+  return launch(TILE_MID_128, (unsigned)(4 * rem));
 }
 
 // ---- windowed attention -------------------------------------------------------

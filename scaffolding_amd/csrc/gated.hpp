@@ -20,9 +20,14 @@
 namespace sf {
 
 // M, K, A, B, C (y, ldc = F), bias [2 F] and epi as GemmParams says; N = 2 F.
+//
+// A launch may leave the last, part round of 256 x 256 tiles to a second one:
+// the first runs tiles 0 .. head - 1, the second, of 128 x 128 tiles with big_n >
+// 0, the quarters of the tiles from `head` on of big_m x big_n.
 struct GatedParams : GemmParams {
   void* pre;
   int F;
+  int head, big_m, big_n;
 };
 
 // The product's columns (0: not a gated launch).

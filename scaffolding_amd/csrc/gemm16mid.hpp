@@ -131,6 +131,14 @@ __global__ __launch_bounds__(WVM* WVN * 64, OCC) void gemm16mid_kernel(Prm p) {
   } else {
     group_tile(tile, p.tiles_m, p.tiles_n, 8, tm, tn);
   }
+  if constexpr (GATED && BM == 128 && BN == 128) {
+    if (p.big_n > 0) {  // quarters of the tiles from p.head on
+      group_tile(p.head + (tile >> 2), p.big_m, p.big_n, 8, tm, tn);
+      tm = 2 * tm + ((tile >> 1) & 1);
+      tn = 2 * tn + (tile & 1);
+      if (tm * BM >= p.M || tn * (BN / 2) >= p.F) return;  // workgroup-uniform
+    }
+  }
   const int m0 = tm * BM, n0 = tn * (GATED ? BN / 2 : BN);  // GATED: the first column of the product
   if (ROWS && n0 >= N) return;  // a quarter past the last column
   const uint16_t* __restrict__ A = static_cast<const uint16_t*>(p.A) + (ROWS || SUMS ? row0 * p.lda : b * p.sA);

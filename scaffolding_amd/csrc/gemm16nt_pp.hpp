@@ -234,7 +234,8 @@ __global__ __launch_bounds__(512) void gemm16nt_pp_kernel(Prm p) {
     if constexpr (PERSIST) {
       const int G = (int)gridDim.x;
       const int slot = xcd * (G / kNumXcd) + xo;
-      const int whole = p.split > 0 ? p.full_tiles : n_tiles;
+      int whole = p.split > 0 ? p.full_tiles : n_tiles;
+      if constexpr (std::is_same<Prm, GatedParams>::value) whole = p.head;
       const int nr = (whole + G - 1) / G;
       if (k < nr) {
         const int pid = k * G + slot;

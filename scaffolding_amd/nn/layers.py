@@ -552,6 +552,8 @@ class WindowAttention(Module):
     def cache(self, batch: int, capacity: int) -> tuple[Tensor, Tensor]:
         """Zeroed caches of keys and values, (batch, capacity, kv_heads
         head_dim), on the weights' device in their type."""
+        if self.table is not None and capacity > self.table.shape[0]:
+            raise ValueError("WindowAttention: a cache of %d tokens, positions up to %d" % (capacity, self.table.shape[0]))
         w = self.qkv.weight
         shape = (batch, capacity, self.kv_heads * self.head_dim)
         return _zeros(*shape, dtype=w.dtype, device=w.device), _zeros(*shape, dtype=w.dtype, device=w.device)
@@ -563,6 +565,8 @@ class WindowAttention(Module):
         made = (self.norm_weight, self.norm_bias, self.norm, self.eps, None, self.interleaved)
         heads = (self.heads, self.kv_heads)
         if cache is None:
+            if self.table is not None and x.shape[-2] > self.table.shape[0]:
+                raise ValueError("WindowAttention: %d tokens, positions up to %d" % (x.shape[-2], self.table.shape[0]))
             qkv = F.qk_norm_rope(qkv, *heads, self.table, *made)
             y = F.window_attention(qkv, *heads, self.window, self.sinks, None, lengths)
         else:

@@ -611,3 +611,38 @@ def test_gated_fp32_of_few_rows(M, K, F, act, bias):
     y, p = cu().dev_gated_linear(up(x, "float32"), up(W, "float32"), up(b, "float32") if bias else None, act, True)
     check_bound(down(y), want, ty, "y")
     check_bound(down(p), pre, tp, "pre")
+
+
+def test_sequences_and_caches_past_the_table_are_refused():
+    import scaffolding_amd as sf
+    from scaffolding_amd import nn
+    att = nn.WindowAttention(64, 4, max_positions=6, dtype="float16")
+    with pytest.raises(ValueError):
+        att.cache(1, 7)
+    with pytest.raises(ValueError):
+        att(sf.Tensor(np.zeros((1, 7, 64), np.float32), dtype="float16", device="cuda"))
+    assert att(sf.Tensor(np.zeros((1, 6, 64), np.float32), dtype="float16", device="cuda")).shape == (1, 6, 64)
+    assert att.cache(1, 6)[0].shape == (1, 6, 64)
+
+
+@pytest.mark.parametrize("M,F,K", [(2 ** 20 + 300, 8, 1032), (2 ** 20 + 300, 8, 1027), (20, 2 ** 18 + 40, 2056),
+                                   (3, 2 ** 18 + 40, 2056), (3, 2 ** 18 + 40, 2051)])
+def test_gated_operands_past_2_gib(lib, M, F, K):
+    """The last rows of x, or of W's gate and up halves, lie past 2^31 bytes;
+    what is before them is 0."""
+    rng = np.random.default_rng(M)
+    tall = M > F
+    assert (M if tall else 2 * F) * K * 2 > 2 ** 31
+    m, f = (50, F) if tall else (M, 30)  # rows that are not 0, the last ones
+    x0, W0 = rnd(rng, (m, K), 1.0, "bfloat16"), rnd(rng, (2 * f, K), K ** -0.5, "bfloat16")
+    x, W = cu().zeros((M, K), cu().BFLOAT16), cu().zeros((2 * F, K), cu().BFLOAT16)
+    for dst, row, part in ((x, M - m, x0), (W, F - f, W0[:f]), (W, 2 * F - f, W0[f:])):
+        src = up(part, "bfloat16")
+        assert lib.sf_memcpy_d2d(P(dst.data_ptr + row * K * 2), P(src.data_ptr), ctypes.c_size_t(src.nbytes), None) == 0
+    y, pre = cu().dev_gated_linear(x, W, None, "silu", True)
+    want, wp, mag = ob.gated(x0, W0, None, "silu")
+    ty, tp = gated_bounds(wp, mag, K, "bfloat16", "silu")
+    y, pre = down(y), down(pre)
+    check_bound(y[M - m:, F - f:], want, ty, "y")
+    check_bound(np.concatenate([pre[M - m:, F - f:F], pre[M - m:, 2 * F - f:]], 1), wp, tp, "pre")
+    assert not y[:M - m].any() and not y[:, :F - f].any()
