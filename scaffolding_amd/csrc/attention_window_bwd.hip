@@ -8,13 +8,16 @@ static int64_t cdiv64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 static int win_width(int64_t D) { return D <= 64 ? 64 : (D <= 96 ? 96 : 128); }
 
 // Ranges of win_dkv_kernel's work: one a CU (its eight waves fill it), but at
-// least 8 products a range on average (each leaves at most 2 sums to be added).
+// least 4 products a range on average (each leaves at most 2 sums to be added).
+// All three launches, us, for at least 8 / 4 / 2: 2 x 20 rows of 3 + 1 heads
+// 27 / 23 / 20, 1024 of 8 + 8, window 256, 73 / 61 / 61, 512 of 16 + 4 60 / 62 /
+// 81.
 static int64_t win_ranges(const WinShape& a) {
   const int64_t blocks = cdiv64(a.Sk, 128), G = a.heads / a.kv_heads;
   const int64_t seen = a.window > 0 && a.window + 127 < a.Sq ? a.window + 127 : a.Sq;
   const int64_t products = a.batch * a.kv_heads * blocks * (cdiv64(seen, 64) + 1) * G;  // at most, but for the sinks'
   int64_t n = cu_count_current();
-  if (n > products / 8) n = products / 8;
+  if (n > products / 4) n = products / 4;
   return n < 1 ? 1 : n;
 }
 

@@ -588,7 +588,7 @@ __global__ __launch_bounds__(512, 2) void win_dkv_kernel(WinBackParams bp) {
         u32x4 pf[2], ds[2], gt[DH], qt[DH];
         pf[0] = ds_read16<0>(xb), pf[1] = ds_read16<1024>(xb);
         columns(ga, (uint32_t)(half ^ 1), gt);
-        ds[0] = ds_read16<2048>(xb), ds[1] = ds_read16<3072>(xb);
+        ds[0] = ds_read16<2048>(xb), ds[1] = ds_read16<3 * 1024>(xb);
         columns(qa, (uint32_t)(half ^ 1), qt);
         __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_waitcnt(waitcnt_imm(63, 2 * DH + 2));
