@@ -583,7 +583,7 @@ int sf_window_attention(const void* Q, int64_t ldq, int64_t strideQ, int64_t hea
  * sums fp32, in an order fixed by the sizes.  A NaN or infinity reaches the
  * gradients of the tokens around it.  The gradients may not overlap the
  * operands or each other.  `work`: sf_window_attention_backward_work bytes of
- * 256-byte aligned device memory, overwritten. */
+ * 16-byte aligned device memory of the call's device, overwritten. */
 int64_t sf_window_attention_backward_work(int64_t batch, int64_t heads, int64_t kv_heads, int64_t rows, int64_t D,
                                           int64_t window, int64_t sinks);
 int sf_window_attention_backward(const void* dO, int64_t lddo, int64_t strideDO, int64_t headDO, const void* Q,

@@ -373,6 +373,7 @@ int sf_window_attention_backward(const void* dO, int64_t lddo, int64_t strideDO,
   if (rc == SF_OK) rc = window_operand(name, "dV", dV, lddv, strideDV, headDV, D);
   if (rc != SF_OK) return rc;
   if (lse == nullptr || work == nullptr) return fail(SF_ERR_INVALID_ARG, "%s: null pointer (lse or work)", name);
+  if (!aligned16(work)) return fail(SF_ERR_INVALID_ARG, "%s: work must be 16-byte aligned", name);
   a.lse = const_cast<float*>(lse);
   a.lengths = lengths;
   WinBack g;
@@ -415,6 +416,7 @@ int sf_window_attention_cached(const void* Q, int64_t ldq, int64_t strideQ, int6
   if (rc != SF_OK) return rc;
   if (lengths == nullptr || (work == nullptr && win_cached_work(a) > 0))
     return fail(SF_ERR_INVALID_ARG, "%s: null pointer (lengths or work)", name);
+  if (!aligned16(work)) return fail(SF_ERR_INVALID_ARG, "%s: work must be 16-byte aligned", name);
   a.lengths = lengths;
   a.cached = 1;
   return launch_window(a, dtype, static_cast<float*>(work), static_cast<hipStream_t>(stream));

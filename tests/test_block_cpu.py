@@ -408,3 +408,9 @@ def test_rope_table_on_the_host():
     t = F.rope_table(300, 10, 500.0, device="cpu")
     assert t.shape == (300, 10)
     assert np.abs(t.numpy() - ox.rope_table(300, 10, 500.0)).max() <= 2.0 ** -24
+
+
+@pytest.mark.parametrize("entry", ["backward", "cached"])
+def test_window_refuses_misaligned_work(lib, entry):
+    assert dict(window_calls(lib, only=entry, work=P(4104))) == {entry: INVALID}
+    assert b"work" in lib.sf_last_error()
