@@ -407,11 +407,13 @@ __global__ __launch_bounds__(256) void qk_norm_rope_backward_kernel(NormRopePara
         for (int u = 0; u < PL; ++u)
 #pragma unroll
           for (int e = 0; e < V; ++e) q += xa[u][e] * xa[u][e] + xb[u][e] * xb[u][e];
-        const float r = 1.0f / sqrtf(sum_lanes(q, L) * inv_d + a.eps);
+        // Lanes past the last head add zeros to the sums, also where eps is 0 (their
+        // r would be infinite) or the angles are not finite.
+        const float r = live ? 1.0f / sqrtf(sum_lanes(q, L) * inv_d + a.eps) : 0.f;
         float m1 = 0.f, m2 = 0.f;
 #pragma unroll
         for (int u = 0; u < PL; ++u) {
-          if (ln.tix[u] >= 0) turn<V, NEXT>(da[u], db[u], c[u], s[u]);
+          if (live && ln.tix[u] >= 0) turn<V, NEXT>(da[u], db[u], c[u], s[u]);
 #pragma unroll
           for (int e = 0; e < V; ++e) {
             xa[u][e] *= r;  // hat

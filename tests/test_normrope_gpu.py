@@ -169,3 +169,27 @@ def test_empty():
     assert tuple(g.dev_qk_norm_rope(x, 2, 1).shape) == (2, 0, 256)
     dx, dw, db = g.dev_qk_norm_rope_backward(x, x, 2, 1, None, None, "layer")
     assert tuple(dx.shape) == (2, 0, 256) and (down(dw) == 0).all() and (down(db) == 0).all()
+
+
+@pytest.mark.parametrize("norm", ["rms", "layer"])
+@pytest.mark.parametrize("dtype,D,H,Hk", [
+    ("bfloat16", 64, 5, 1), ("float16", 64, 8, 3), ("bfloat16", 128, 30, 3), ("float32", 128, 4, 1),
+    ("float16", 256, 3, 1), ("float32", 37, 3, 2),
+])
+def test_backward_without_eps(dtype, D, H, Hk, norm):
+    """eps 0 with heads that leave lanes of a wave over: those lanes hold no head
+    and add nothing to the parameters' gradients."""
+    rng = np.random.default_rng(D + H)
+    B, N, R = 2, 9, D // 2 * 2
+    x, table, w, _ = make(rng, dtype, B, N, H, Hk, D, R, N)
+    g = rnd(rng, x.shape, 0.5, dtype)
+    pos = np.tile(np.arange(N), (B, 1))
+    dx, dw, db = cu().dev_qk_norm_rope_backward(up(g, dtype), up(x, dtype), H, Hk, f32(table), up(w, dtype), norm, 0.0)
+    (wx, ww, wb), (mx, mw, mb) = ob.qk_norm_rope_backward(g, x, H, Hk, table, pos, w, norm, 0.0)
+    hu = out_half_ulp_rel(dtype)
+    n = B * N * max(H, Hk)
+    check_bound(down(dx), wx, 3 * steps(D) * mx + hu * np.abs(wx) + 1e-7, "dx")
+    assert np.isfinite(down(dw)).all()
+    check_bound(down(dw), ww, (steps(D) + n * 2.0 ** -24) * mw + hu * np.abs(ww) + 1e-7, "dw")
+    if norm == "layer":
+        check_bound(down(db), wb, (n + 4) * 2.0 ** -24 * mb + hu * np.abs(wb) + 1e-7, "db")
