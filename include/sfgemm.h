@@ -535,6 +535,13 @@ int sf_qk_norm_rope(const void* x, int64_t ldx, void* q, int64_t ldq, int64_t st
                     const void* weight, const void* bias, sf_norm norm, float eps, int interleaved, int64_t batch,
                     int64_t rows, int64_t heads, int64_t kv_heads, int64_t D, sf_dtype dtype, void* stream);
 
+/* Diagnostic twin of sf_qk_norm_rope (backward 0; values: v is there) and
+ * sf_qk_norm_rope_backward (1), as sf_gemm_plan is sf_gemm's: writes what these
+ * sizes launch on the current device into buf[len] ("chunks of 8, 13332
+ * workgroups": columns that a lane loads at a time).  Host-only. */
+int sf_qk_norm_rope_plan(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads, int64_t D, int64_t rot,
+                         int values, int backward, char* buf, int len);
+
 /* Its gradients (without lengths: row i stands at i): grad, x and grad_x are
  * contiguous packed rows [batch * rows, (heads + 2 kv_heads) D]; grad is that
  * of the packed result, values included, whose gradient goes through.

@@ -278,6 +278,27 @@ int sf_qk_norm_rope(const void* x, int64_t ldx, void* q, int64_t ldq, int64_t st
   return launch_norm_rope(a, dtype, false, static_cast<hipStream_t>(stream));
 }
 
+int sf_qk_norm_rope_plan(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads, int64_t D, int64_t rot,
+                         int values, int backward, char* buf, int len) {
+  clear_error();
+  const char* name = "sf_qk_norm_rope_plan";
+  if (buf == nullptr || len <= 0) return fail(SF_ERR_INVALID_ARG, "%s: bad buffer", name);
+  buf[0] = 0;
+  const float none = 0.0f;  // stands for the table
+  const int rc = norm_rope_check(name, &none, 1, rot, SF_NORM_RMS, 0.0f, batch, rows, heads, kv_heads, D, SF_BF16);
+  if (rc != SF_OK) return rc;
+  if (batch == 0 || rows == 0) {
+    snprintf(buf, static_cast<size_t>(len), "noop");
+    return SF_OK;
+  }
+  NormRopeArgs a;
+  norm_rope_fill(a, nullptr, 0, nullptr, 0, rot, nullptr, nullptr, SF_NORM_RMS, 0.0f, 0, batch, rows, heads, kv_heads, D);
+  a.v = values != 0 || backward != 0 ? buf : nullptr;  // not followed
+  const NormRopePlan p = norm_rope_plan(a, backward != 0);
+  snprintf(buf, static_cast<size_t>(len), "chunks of %d, %u workgroups", p.chunk, p.blocks);
+  return SF_OK;
+}
+
 int64_t sf_qk_norm_rope_backward_work(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads, int64_t D,
                                       int64_t rot) {
   if (batch < 1 || rows < 1 || heads < 1 || kv_heads < 1 || D < 1 || D > 256 || rot < 0 || rot > D || (rot & 1) ||

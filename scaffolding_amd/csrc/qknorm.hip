@@ -534,6 +534,8 @@ static unsigned norm_rope_split(NormRopeParams& p, bool back) {
   int64_t groups = cdiv(tokens, 4);
   const int64_t most = back ? cdiv(4 * cus, slices) : 64 * cus;
   if (groups > most) groups = most;
+  const int64_t fit = ((int64_t(1) << 24) - 1) / slices;  // a launch holds fewer than 2^32 threads
+  if (groups > fit) groups = fit;
   if (groups < 1) groups = 1;
   p.stride = groups * 4;
   return (unsigned)(groups * slices);
@@ -544,6 +546,13 @@ int64_t norm_rope_work(int64_t batch, int64_t rows, int heads, int kv_heads, int
   p.a.batch = batch, p.a.rows = rows, p.a.heads = heads, p.a.kv_heads = kv_heads, p.a.D = D, p.a.rot = rot;
   p.a.v = &p;  // not followed
   return (int64_t)norm_rope_split(p, true) * 2 * D * 4;
+}
+
+NormRopePlan norm_rope_plan(const NormRopeArgs& a, bool back) {
+  NormRopeParams p{};
+  p.a = a;
+  const unsigned blocks = norm_rope_split(p, back);
+  return {chunk_of(a.D, a.rot, back), blocks};
 }
 
 template <typename T, int V, int PL>

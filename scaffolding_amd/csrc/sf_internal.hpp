@@ -251,6 +251,11 @@ struct NormRopeArgs {
 };
 int launch_norm_rope(const NormRopeArgs& a, sf_dtype dt, bool back, hipStream_t st);
 int64_t norm_rope_work(int64_t batch, int64_t rows, int heads, int kv_heads, int D, int rot);
+struct NormRopePlan {
+  int chunk;        // columns that a lane loads at a time
+  unsigned blocks;  // of 256 threads
+};
+NormRopePlan norm_rope_plan(const NormRopeArgs& a, bool back);
 
 // Gated feed-forward layers (gated.hpp, gated.hip).
 int launch_gated_bf16(int cfg, const GatedParams& p, unsigned gx, hipStream_t st);

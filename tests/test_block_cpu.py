@@ -414,3 +414,42 @@ def test_rope_table_on_the_host():
 def test_window_refuses_misaligned_work(lib, entry):
     assert dict(window_calls(lib, only=entry, work=P(4104))) == {entry: INVALID}
     assert b"work" in lib.sf_last_error()
+
+
+# ---- what the entries launch ------------------------------------------------------
+
+def plan_of(lib, name, *args):
+    buf = ctypes.create_string_buffer(128)
+    assert call(getattr(lib, name), *args, buf, c_int(128)) == 0, lib.sf_last_error()
+    return buf.value.decode()
+
+
+def norm_rope_plan(lib, *sizes, values=1, backward=0):
+    return plan_of(lib, "sf_qk_norm_rope_plan", *sizes, c_int(values), c_int(backward))
+
+
+def test_norm_rope_plans(lib):
+    sizes = 1, 17776, 30, 30, 64
+    assert norm_rope_plan(lib, *sizes, 64).startswith("chunks of 8,")
+    assert norm_rope_plan(lib, *sizes, 64, backward=1).startswith("chunks of 4,")
+    assert norm_rope_plan(lib, *sizes, 24).startswith("chunks of 4,")
+    assert norm_rope_plan(lib, *sizes, 20).startswith("chunks of 1,")
+    assert norm_rope_plan(lib, 0, 4, 2, 1, 16, 16) == norm_rope_plan(lib, 4, 0, 2, 1, 16, 16) == "noop"
+    buf = ctypes.create_string_buffer(8)
+    plan = lambda *a: call(lib.sf_qk_norm_rope_plan, *a)
+    assert plan(1, 4, 2, 1, 16, 16, c_int(1), c_int(0), None, c_int(8)) == INVALID
+    assert plan(1, 4, 2, 1, 16, 16, c_int(1), c_int(0), buf, c_int(0)) == INVALID
+    assert plan(1, 4, 0, 1, 16, 16, c_int(1), c_int(0), buf, c_int(8)) == INVALID
+    assert plan(1, 4, 4097, 1, 16, 16, c_int(1), c_int(0), buf, c_int(8)) == UNSUPPORTED
+    assert plan(1, 4, 2, 1, 257, 16, c_int(1), c_int(0), buf, c_int(8)) == UNSUPPORTED
+
+
+@pytest.mark.parametrize("D,rot", [(256, 256), (256, 8), (255, 254), (129, 0), (8, 2), (1, 0)])
+def test_norm_rope_of_every_size_fits_a_launch(lib, D, rot):
+    """Fewer than 2^32 threads: what a launch holds."""
+    for rows in (1, 1000, 2 ** 12 - 1, 2 ** 12, 2 ** 16, 2 ** 20 + 1, 2 ** 30):
+        for H, Hk in ((1, 1), (1366, 1366), (4096, 1), (4096, 4096)):
+            for values in (0, 1):
+                for backward in (0, 1):
+                    n = int(norm_rope_plan(lib, 1, rows, H, Hk, D, rot, values=values, backward=backward).split()[3])
+                    assert 0 < n * 256 < 2 ** 32, (rows, H, Hk, values, backward)
