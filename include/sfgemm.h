@@ -527,8 +527,9 @@ typedef enum sf_norm { SF_NORM_RMS = 0, SF_NORM_LAYER = 1 } sf_norm;
  * values, unchanged, to v + b strideV + p ldv where 0 <= p < capacity (other
  * rows are not written): a cache that holds lengths[b] rows takes the new ones
  * behind them.  v NULL: values are not read (x then needs no columns for
- * them).  q, k and v may be x's own columns (in place).  fp32 arithmetic, one
- * rounding.  D <= 256, heads and kv_heads <= 4096, batch * rows <= 2^30. */
+ * them).  q, k and v may be x's own columns (in place); with lengths, whose keys
+ * and values move to other rows, the ranges of k and v may not overlap that of
+ * x.  fp32 arithmetic, one rounding.  D <= 256, heads and kv_heads <= 4096, batch * rows <= 2^30. */
 int sf_qk_norm_rope(const void* x, int64_t ldx, void* q, int64_t ldq, int64_t strideQ, void* k, int64_t ldk,
                     int64_t strideK, void* v, int64_t ldv, int64_t strideV, const float* table, int64_t table_rows,
                     int64_t rot, const int32_t* positions, const int32_t* lengths, int64_t capacity,

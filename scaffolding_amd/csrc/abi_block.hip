@@ -56,6 +56,12 @@ static void norm_rope_fill(NormRopeArgs& a, const void* x, int64_t ldx, const fl
   a.pairs = interleaved != 0;
 }
 
+// Whether na elements from `a` on and nb from `b` on share memory.
+static bool ranges_meet(const void* a, __int128 na, const void* b, __int128 nb, int size) {
+  const __int128 a0 = reinterpret_cast<uintptr_t>(a), b0 = reinterpret_cast<uintptr_t>(b);
+  return a0 < b0 + nb * size && b0 < a0 + na * size;
+}
+
 // ---- gated feed-forward layers ----------------------------------------------
 
 static int gated_check(const char* name, int64_t M, int64_t F, int64_t K, sf_dtype dtype, sf_epilogue act) {
@@ -266,6 +272,16 @@ int sf_qk_norm_rope(const void* x, int64_t ldx, void* q, int64_t ldq, int64_t st
     return fail(SF_ERR_INVALID_ARG, "%s: a row is shorter than its heads", name);
   if (strideQ < 0 || strideK < 0 || strideV < 0) return fail(SF_ERR_INVALID_ARG, "%s: negative stride", name);
   if (capacity < 0 || capacity > kMostRows) return fail(SF_ERR_INVALID_ARG, "%s: capacity out of range", name);
+  if (lengths != nullptr && capacity > 0) {  // a row would be written while another wave has yet to read it
+    const int size = dtype == SF_F32 ? 4 : 2;
+    const __int128 nx = static_cast<__int128>(batch * rows - 1) * ldx + (heads + (v != nullptr ? 2 : 1) * kv_heads) * D;
+    const auto extent = [&](int64_t ld, int64_t stride) {
+      return static_cast<__int128>(batch - 1) * stride + static_cast<__int128>(capacity - 1) * ld + kv_heads * D;
+    };
+    if (ranges_meet(x, nx, k, extent(ldk, strideK), size) ||
+        (v != nullptr && ranges_meet(x, nx, v, extent(ldv, strideV), size)))
+      return fail(SF_ERR_INVALID_ARG, "%s: with lengths, k and v may not overlap x", name);
+  }
   NormRopeArgs a;
   norm_rope_fill(a, x, ldx, table, table_rows, rot, positions, weight, norm, eps, interleaved, batch, rows, heads,
                  kv_heads, D);

@@ -453,3 +453,22 @@ def test_norm_rope_of_every_size_fits_a_launch(lib, D, rot):
                 for backward in (0, 1):
                     n = int(norm_rope_plan(lib, 1, rows, H, Hk, D, rot, values=values, backward=backward).split()[3])
                     assert 0 < n * 256 < 2 ** 32, (rows, H, Hk, values, backward)
+
+
+def test_norm_rope_into_rows_of_its_own_input(lib):
+    """With lengths a row's key goes to another row: into x that would be written
+    ahead of another wave's reading, and is refused, down to one shared
+    element."""
+    def run(k, v, n=A, rows=4, capacity=4):
+        return call(lib.sf_qk_norm_rope, P(1 << 20), 64, P(1 << 22), 32, 128, P(k), 64, 256, P(v) if v else None, 64, 256, A,
+                    8, 16, None, n, capacity, None, None, c_int(0), F32(1e-6), c_int(0), 1, rows, 2, 1, 16, c_int(2), None)
+
+    x, far = 1 << 20, 1 << 24
+    size = (3 * 64 + 64) * 2  # of x
+    key = (3 * 64 + 16) * 2   # of a cache
+    for k, v in ((x + 64, far), (far, x + 96), (x, None), (x + size - 2, far), (x - key + 2, far), (far, x - key + 2)):
+        assert run(k, v) == INVALID
+        assert b"overlap" in lib.sf_last_error()
+    far_rows = call(lib.sf_qk_norm_rope, P(x), 64, P(1 << 22), 32, 128, P(x + size), 2 ** 62, 2 ** 62, P(far), 64, 256, A,
+                    8, 16, None, A, 2 ** 30, None, None, c_int(0), F32(1e-6), c_int(0), 2 ** 20, 4, 2, 1, 16, c_int(2), None)
+    assert far_rows == INVALID and b"overlap" in lib.sf_last_error()  # 2^22 rows of x reach k
