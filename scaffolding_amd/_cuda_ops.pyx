@@ -1615,10 +1615,10 @@ def dev_qk_norm_rope_cached(gt_x, int heads, int kv_heads, gt_table, gt_k, gt_v,
 
 
 def dev_qk_norm_rope_backward(gt_grad, gt_x, int heads, int kv_heads, gt_table=None, gt_weight=None, norm='rms',
-                              float eps=1e-6, gt_positions=None, bint interleaved=False):
+                              float eps=1e-6, gt_positions=None, bint interleaved=False, has_bias=None):
     """Gradients of dev_qk_norm_rope from grad, that of its result: (grad_x,
-    grad_weight (2, D), grad_bias (2, D)), the last for norm 'layer' only (else
-    None)."""
+    grad_weight (2, D), grad_bias (2, D) or None): the bias's with has_bias, or
+    where that is None for norm 'layer'."""
     name = 'dev_qk_norm_rope_backward'
     bnd = _packed_heads(name, gt_x, heads, kv_heads)
     _norm_rope_operands(name, gt_x, gt_table, gt_positions, gt_weight, None, norm, bnd)
@@ -1634,7 +1634,7 @@ def dev_qk_norm_rope_backward(gt_grad, gt_x, int heads, int kv_heads, gt_table=N
     cdef int dev = gt_x.device_id
     out = _alloc_like(tuple(gt_x.shape), gt_x.dtype, dev)
     dw = _alloc_like((2, int(D)), gt_x.dtype, dev)
-    db = _alloc_like((2, int(D)), gt_x.dtype, dev) if norm == 'layer' else None
+    db = _alloc_like((2, int(D)), gt_x.dtype, dev) if (norm == 'layer' if has_bias is None else has_bias) else None
     cdef int64_t need = sf_qk_norm_rope_backward_work(B, N, heads, kv_heads, D, rot)
     cdef CudaBuffer work = _make_buffer(need if need > 0 else 4, dev)
     cdef void* px = _ptr(gt_x)

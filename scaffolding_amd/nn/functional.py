@@ -290,13 +290,14 @@ def _written_on(op: str, dev: int, *written) -> None:
 
 def qk_norm_rope_backward(grad: Tensor, qkv: Tensor, heads: int, kv_heads: int, table: Tensor | None,
                           weight: Tensor | None = None, norm: str = "rms", eps: float = 1e-6,
-                          positions: Tensor | None = None, interleaved: bool = False
+                          positions: Tensor | None = None, interleaved: bool = False, has_bias: bool | None = None
                           ) -> tuple[Tensor, Tensor, Tensor | None]:
-    """(grad_qkv, grad_weight (2, D), grad_bias (2, D)) of qk_norm_rope, qkv
-    being its input; the bias's for norm 'layer' only (else None)."""
+    """(grad_qkv, grad_weight (2, D), grad_bias (2, D) or None) of qk_norm_rope,
+    qkv being its input; the bias's with has_bias, or where that is None for
+    norm 'layer'."""
     dev = _device_of("qk_norm_rope_backward", qkv, grad, table, weight, positions)
     out = _cuops.dev_qk_norm_rope_backward(_on(grad, dev), qkv._gpu, heads, kv_heads, _on(table, dev),
-                                           _on(weight, dev), norm, eps, _on(positions, dev), interleaved)
+                                           _on(weight, dev), norm, eps, _on(positions, dev), interleaved, has_bias)
     return tuple(None if t is None else Tensor._wrap_gpu(t, qkv._device) for t in out)
 
 

@@ -193,3 +193,33 @@ def test_backward_without_eps(dtype, D, H, Hk, norm):
     check_bound(down(dw), ww, (steps(D) + n * 2.0 ** -24) * mw + hu * np.abs(ww) + 1e-7, "dw")
     if norm == "layer":
         check_bound(down(db), wb, (n + 4) * 2.0 ** -24 * mb + hu * np.abs(wb) + 1e-7, "db")
+
+
+@pytest.mark.parametrize("norm,has_bias,given", [("rms", True, True), ("rms", None, False), ("rms", False, False),
+                                                 ("layer", True, True), ("layer", None, True), ("layer", False, False)])
+def test_gradient_of_a_bias(norm, has_bias, given):
+    """Either norm takes a bias and gives its gradient, by formula and by the
+    sums' differences: the loss is linear in it, so they are as exact as its own
+    fp64."""
+    from scaffolding_amd import Tensor
+    from scaffolding_amd.nn import functional as F
+    rng = np.random.default_rng(5)
+    dtype, B, N, H, Hk, D, R = "bfloat16", 2, 7, 3, 2, 64, 32
+    x, table, w, _ = make(rng, dtype, B, N, H, Hk, D, R, N)
+    g, bias = rnd(rng, x.shape, 0.5, dtype), rnd(rng, (2, D), 0.3, dtype)
+    pos = np.tile(np.arange(N), (B, 1))
+    t = lambda a, d=dtype: Tensor(a, dtype=d, device="cuda")
+    y = F.qk_norm_rope(t(x), H, Hk, t(table, "float32"), t(w), t(bias), norm)
+    want, mag = ob.qk_norm_rope(x, H, Hk, table, pos, w, bias, norm)
+    hu = out_half_ulp_rel(dtype)
+    check_bound(y.numpy(), want, steps(D) * mag + hu * np.abs(want) + 1e-7, "y")
+    dx, dw, db = F.qk_norm_rope_backward(t(g), t(x), H, Hk, t(table, "float32"), t(w), norm, has_bias=has_bias)
+    (wx, ww, wb), (mx, mw, mb) = ob.qk_norm_rope_backward(g, x, H, Hk, table, pos, w, norm)
+    n = B * N * H
+    check_bound(dx.numpy(), wx, 3 * steps(D) * mx + hu * np.abs(wx) + 1e-7, "dx")
+    check_bound(dw.numpy(), ww, (steps(D) + n * 2.0 ** -24) * mw + hu * np.abs(ww) + 1e-7, "dw")
+    assert (db is not None) == given
+    if given:
+        check_bound(db.numpy(), wb, (n + 4) * 2.0 ** -24 * mb + hu * np.abs(wb) + 1e-7, "db")
+        lo, hi = ((ob.qk_norm_rope(x, H, Hk, table, pos, w, bias + s, norm)[0] * g).sum() for s in (-0.5, 0.5))
+        assert abs(hi - lo - wb.sum()) < 1e-9 * np.abs(g).sum()
