@@ -17,7 +17,8 @@
 // Keys past the sequence's end are never read (the buffers end there), so what
 // a cache holds behind it does not matter.  A NaN or infinite V that a row does
 // not see meets its weight 0 in the products: rows that come out other than
-// finite are formed again over their own keys (win_exact_rows).
+// finite, or past the type's largest value, are formed again over their own keys
+// (win_exact_rows).
 //
 // The scale is applied to the fp32 scores (attn_wide_kernel's rounding of a
 // scaled Q would show in the rows' log-sums), and with the log-sums wanted a
@@ -138,11 +139,23 @@ __device__ __forceinline__ float win_dot(const uint16_t* a, const uint16_t* b, i
   return dot;
 }
 
+// The least size that rounds to infinity in T.  A row's weights are rounded for
+// their product with V and its sum is not (or held unnormalised, up to 2^8 times
+// the result), so a row of values next to T's largest one can come out past it,
+// which an average cannot.
+template <typename T>
+__device__ __forceinline__ float win_top() {
+  return std::is_same<T, F16>::value ? 65520.f : __builtin_bit_cast(float, 0x7f7f8000u);
+}
+
 // Output rows term by term over their own keys alone, scores and values from
 // global memory.  One wave; bit i of `rows` is the row at position pos0 + i,
 // whose query and output lie at Q + i ldq and O + i ldo.  Slow, for rows
-// beside values that are not finite.  Not inlined: it would cost the kernels
-// registers.  Columns d0 .. d1 - 1 are stored.
+// beside values that are not finite and rows that came out past T's largest
+// value: the weights are normalised ahead of their products and the terms added
+// 64 at a time, so that a sum over n keys is off by at most (n / 64 + 128) 2^-24 of
+// its terms' sizes (half a step of fp16 at n = 2^18).  Not inlined: it would cost
+// the kernels registers.  Columns d0 .. d1 - 1 are stored.
 template <typename T>
 __device__ __attribute__((noinline)) void win_exact_rows(const WinParams& p, const uint16_t* Q, int64_t ldq,
                                                          uint16_t* O, int64_t ldo, const uint16_t* K,
@@ -171,29 +184,34 @@ __device__ __attribute__((noinline)) void win_exact_rows(const WinParams& p, con
     }
     mx = wave_max(mx);
     bad = __builtin_amdgcn_ballot_w64(bad) != 0 || !(mx > -INFINITY) || mx == INFINITY;
-    float l = 0.f, a0 = 0.f, a1 = 0.f;
+    auto weight = [&](int t) {
+      return __builtin_amdgcn_exp2f(win_dot<T>(q, K + (int64_t)key(t) * p.ldk, p.D) * p.scale_log2e - mx);
+    };
+    float a0 = bad && n > 0 ? __builtin_nanf("") : 0.f, a1 = a0;
     if (!bad) {
+      float l = 0.f;
+#pragma nounroll
+      for (int t = lane; t < n; t += 64) l += weight(t);
+      const float inv = 1.0f / wave_sum(l);
 #pragma nounroll
       for (int t0 = 0; t0 < n; t0 += 64) {
         const int m = n - t0 < 64 ? n - t0 : 64;
-        const float pt = lane < m ? __builtin_amdgcn_exp2f(
-                                        win_dot<T>(q, K + (int64_t)key(t0 + lane) * p.ldk, p.D) * p.scale_log2e - mx)
-                                  : 0.f;
-        l += pt;
+        const float pt = lane < m ? weight(t0 + lane) * inv : 0.f;
+        float b0 = 0.f, b1 = 0.f;
 #pragma nounroll
         for (int u = 0; u < m; ++u) {
           const float pu = __shfl(pt, u, 64);
           const uint32_t w =
               *reinterpret_cast<const uint32_t*>(V + (int64_t)key(t0 + u) * p.ldv + (dok ? 2 * lane : 0));
-          a0 = __builtin_fmaf(pu, Elem<T>::to_f32((uint16_t)(w & 0xffffu)), a0);
-          a1 = __builtin_fmaf(pu, Elem<T>::to_f32((uint16_t)(w >> 16)), a1);
+          b0 = __builtin_fmaf(pu, Elem<T>::to_f32((uint16_t)(w & 0xffffu)), b0);
+          b1 = __builtin_fmaf(pu, Elem<T>::to_f32((uint16_t)(w >> 16)), b1);
         }
+        a0 += b0;
+        a1 += b1;
       }
-      l = wave_sum(l);
     }
-    const float inv = n > 0 ? 1.0f / l : 0.f;  // bad: 0 * inf = NaN
     if (dok && 2 * lane >= d0 && 2 * lane < d1)
-      *reinterpret_cast<uint32_t*>(O + (int64_t)i * ldo + 2 * lane) = pack2<T>(a0 * inv, a1 * inv);
+      *reinterpret_cast<uint32_t*>(O + (int64_t)i * ldo + 2 * lane) = pack2<T>(a0, a1);
   }
 }
 
@@ -517,16 +535,16 @@ __global__ __launch_bounds__(256, FEW && DW > 64 ? 1 : 2) void win_attn_kernel(W
     // cache's end and no sink is there
     const bool row = r < p.Sq, any = r < sq.rows && sq.keys > 0 && (sq.keys > pos - p.window + 1 || p.sinks > 0);
     const float inv = 1.0f / l;
-    float fin = 0.f;
+    float most = 0.f;
 #pragma unroll
     for (int db = 0; db < DB; ++db) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         o[mb][db][q] *= inv;
-        fin = __builtin_fmaf(o[mb][db][q], 0.f, fin);
+        most = __builtin_elementwise_maximum(most, __builtin_fabsf(o[mb][db][q]));
       }
     }
-    uint64_t bad = __builtin_amdgcn_ballot_w64(row && any && fin != 0.f);  // NaN
+    uint64_t bad = __builtin_amdgcn_ballot_w64(row && any && !(most < win_top<T>()));  // NaN too
     bad |= bad >> 32;
     bad = (bad | bad >> 16) & 0xffffull;
     odd |= bad << (16 * mb);
@@ -593,9 +611,9 @@ __device__ __forceinline__ WinRow win_row(const WinParams& p, int hk, int r) {
 }
 
 // Normalises and stores 16 rows' blocks of 16 columns db0, db0 + step, ... (NB
-// of them, those below DB); rows that are not finite are formed again (columns
-// d0 .. d1 - 1, all that the workgroup stores) by wave 0.  l: the sum of the
-// lane's row.
+// of them, those below DB); rows that are not below win_top are formed again
+// (columns d0 .. d1 - 1, all that the workgroup stores) by wave 0.  l: the sum of
+// the lane's row.
 template <typename T, int DB, int NB>
 __device__ __forceinline__ void win_finish_rows(const WinParams& p, const WinSeq& sq, int b, int hk, int rb, int wave,
                                                 int lane, int db0, int step, int d0, int d1, const f32x4 (&o)[NB],
@@ -605,7 +623,7 @@ __device__ __forceinline__ void win_finish_rows(const WinParams& p, const WinSeq
   const int pos = sq.off + w.token;
   const bool row = r < rows, any = sq.keys > 0 && (sq.keys > pos - p.window + 1 || p.sinks > 0);
   const float inv = 1.0f / l;
-  float fin = 0.f;
+  float most = 0.f;
   u32x2 v[NB];
 #pragma unroll
   for (int i = 0; i < NB; ++i) {
@@ -613,11 +631,11 @@ __device__ __forceinline__ void win_finish_rows(const WinParams& p, const WinSeq
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       x[q] = o[i][q] * inv;
-      if (db0 + step * i < DB) fin = __builtin_fmaf(x[q], 0.f, fin);
+      if (db0 + step * i < DB) most = __builtin_elementwise_maximum(most, __builtin_fabsf(x[q]));
     }
     v[i] = any ? u32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])} : u32x2{0u, 0u};
   }
-  uint64_t bad = __builtin_amdgcn_ballot_w64(row && any && fin != 0.f);  // NaN
+  uint64_t bad = __builtin_amdgcn_ballot_w64(row && any && !(most < win_top<T>()));  // NaN too
   bad |= bad >> 32;
   bad = (bad | bad >> 16) & 0xffffull;
   if (bad != 0 && lane == 0) __hip_atomic_fetch_or(flag, (uint32_t)bad, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);

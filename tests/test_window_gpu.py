@@ -314,3 +314,53 @@ def test_backward_against_differences():
         lo, hi = (ob.window_attention(x + s * way, H, Hk, window, sinks, D ** -0.5)[0] for s in (-h, h))
         num = ((hi - lo) * g).sum() / (2 * h)
         assert abs(num - (dx * way).sum()) < (tol * np.abs(way)).sum() + 1e-5
+
+
+# ---- values at the top of the type ---------------------------------------------------
+
+TOP = {"float16": 65504.0, "bfloat16": (2.0 - 2.0 ** -7) * 2.0 ** 127}
+
+
+def top_values(rng, v, dtype):
+    """v (..., D) with its last columns at the type's largest value, either sign."""
+    v[..., -8:] = TOP[dtype] * np.where(np.arange(8) % 2, 1.0, -1.0)
+    return v
+
+
+def check_top(y, H, D, dtype):
+    """An average of one number is that number (the bound of a sum over n keys, n
+    below 2^14: under a quarter of a step)."""
+    got = y.reshape(-1, H, D)[..., -8:]
+    assert np.isfinite(got).all()
+    assert (np.abs(got) >= TOP[dtype] * (1 - 2 * out_half_ulp_rel(dtype))).all()
+    assert (np.sign(got) == np.where(np.arange(8) % 2, 1.0, -1.0)).all()
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("N,H,D,window", [(333, 2, 64, None), (200, 3, 72, 50), (150, 2, 128, 90)])
+def test_values_at_the_top_of_the_type(dtype, N, H, D, window):
+    """The weights' rounding, or sums past the type's (or fp32's) largest value
+    ahead of the division, may not make an average infinite."""
+    rng = np.random.default_rng(N)
+    x = rnd(rng, (1, N, (H + 2) * D), 1.0, dtype)
+    x[..., :(H + 1) * D] *= 4.0
+    top_values(rng, x[..., (H + 1) * D:], dtype)
+    want, lse = ob.window_attention(x, H, 1, window, 2, 0.3)
+    for with_lse in (False, True):
+        y = cu().dev_window_attention(up(x, dtype), H, 1, window, 2, 0.3, None, with_lse)
+        y = down(y[0] if with_lse else y)
+        check_top(y, H, D, dtype)
+        tol, _ = forward_bound(x, H, 1, window, 2, 0.3, dtype)
+        check(y, want, tol, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("B,n,H,Hk,D,S", [(1, 1, 16, 2, 128, 5000), (2, 1, 8, 2, 72, 400), (3, 5, 4, 1, 64, 700), (1, 2, 4, 2, 96, 9000)])
+def test_cached_values_at_the_top_of_the_type(dtype, B, n, H, Hk, D, S):
+    rng = np.random.default_rng(S)
+    q = rnd(rng, (B, n, H * D), 4.0, dtype)
+    k, v = rnd(rng, (B, S, Hk * D), 1.0, dtype), rnd(rng, (B, S, Hk * D), 1.0, dtype)
+    top_values(rng, v.reshape(B, S, Hk, D), dtype)
+    y = down(cu().dev_window_attention_cached(up(q, dtype), up(k, dtype), up(v, dtype), ints([S - n] * B), H, Hk, None, 0,
+                                              0.2))
+    check_top(y, H, D, dtype)
