@@ -624,10 +624,21 @@ int sf_window_attention_cached(const void* Q, int64_t ldq, int64_t strideQ, int6
  *   y[m, f] = act(x[m] . W[f] + bias[f]) (x[m] . W[F + f] + bias[F + f])
  * x [M, K], y [M, F]; act SF_EPI_NONE, SF_EPI_SILU or SF_EPI_GELU_TANH; fp32
  * sums, one rounding.  pre [M, 2 F] (or NULL) takes the two projections,
- * rounded, for the backward pass; SF_F32 needs it (past 16 rows its products
- * and the gate are two launches).  M, K <= 2^30, F <= 2^29, at most 2^22 tiles. */
+ * rounded, for the backward pass; SF_F32 needs it.  One launch; 16-bit layers of
+ * many rows take a second one where a part round of tiles runs as quarters, and
+ * SF_F32 past 16 rows (or with rows that are not 16-byte aligned) its products
+ * and the gate.  M, K <= 2^30, F <= 2^29, at most 2^22 tiles. */
 int sf_gated_linear(const void* x, const void* W, const void* bias, void* y, void* pre, int64_t M, int64_t F, int64_t K,
                     sf_dtype dtype, sf_epilogue act, void* stream);
+/* Diagnostic twin of sf_gated_linear, as sf_gemm_plan is sf_gemm's: writes what
+ * these operands (of whose addresses only the alignment counts) launch on the
+ * current device into buf[len]: "gated 256x256 persistent, 48 quartered" (the
+ * tile, one workgroup a CU walking several, the tiles that a second launch takes
+ * as quarters), "gated 64x64 staged" (rows that are not 16-byte aligned), "gated
+ * 16x32" (up to 16 rows), "gated fp32 16 rows" or "gated fp32 product, then
+ * gate".  Host-only. */
+int sf_gated_linear_plan(const void* x, const void* W, int64_t M, int64_t F, int64_t K, sf_dtype dtype, char* buf,
+                         int len);
 /* The gradient of pre from that of y: grad_pre[m, f] = grad up act'(gate),
  * grad_pre[m, F + f] = grad act(gate), each rounded once; and with grad_bias
  * [2 F] (or NULL) its sums over the rows, fp32 in an order fixed by the sizes.

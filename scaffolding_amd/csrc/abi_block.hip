@@ -140,8 +140,40 @@ static int gated_tile(int64_t M, int64_t F, int64_t K, bool rows16, bool direct,
   return cfg;
 }
 
+// The launches of a 16-bit layer: `tiles` of kernel cfg, of which a second launch
+// takes those from `head` on as quarters.
+struct GatedPlan {
+  int cfg, bm, bn;
+  int64_t tiles, head;
+  bool persist;
+};
+
+static int gated_plan(const char* name, const void* x, const void* W, int64_t M, int64_t F, int64_t K, GatedPlan& g) {
+  const bool rows16 = K % 8 == 0 && aligned16(x) && aligned16(W);
+  // the direct loads' 32-bit offsets reach 2 GiB of either operand
+  const bool direct = rows16 && K > 0 && 2 * F * K < kMostRows && M * K < kMostRows;
+  g = GatedPlan{};
+  g.cfg = gated_tile(M, F, K, rows16, direct, g.bm, g.bn);
+  g.tiles = cdiv(M, g.bm) * cdiv(2 * F, g.bn);
+  g.head = g.tiles;
+  if (g.tiles > (int64_t(1) << 22)) return fail(SF_ERR_UNSUPPORTED, "%s: more than 2^22 tiles", name);
+  if (g.cfg != TILE_NT_BIG) return SF_OK;
+  // A part round that its tiles' quarters fill better runs as those: 4096 rows, F
+  // 11008, K 4096 (5.4 rounds) 570 -> 552 us, F 2048 of 4352 rows (1.1) 172 -> 153;
+  // past about half a round the quarters take as long.
+  const int64_t cus = cu_count_current(), rem = g.tiles % cus;
+  if (g.tiles > cus && gated_quarters(rem, K, cus)) g.head = g.tiles - rem;
+  // One workgroup a CU walks the tiles where the last round is full or at most
+  // half full, as sf_gemm's.
+  g.persist = g.head > cus && cus % kNumXcd == 0 && 2 * (g.head % cus) <= cus;
+  return SF_OK;
+}
+
 static int gated16(const void* x, const void* W, const void* bias, void* y, void* pre, int64_t M, int64_t F, int64_t K,
                    sf_dtype dtype, sf_epilogue act, hipStream_t st) {
+  GatedPlan g;
+  int rc = gated_plan("sf_gated_linear", x, W, M, F, K, g);
+  if (rc != SF_OK) return rc;
   GatedParams p{};
   p.A = x;
   p.B = W;
@@ -158,34 +190,26 @@ static int gated16(const void* x, const void* W, const void* bias, void* y, void
   p.epi = bias == nullptr ? act
           : act == SF_EPI_SILU ? SF_EPI_BIAS_SILU
           : act == SF_EPI_GELU_TANH ? SF_EPI_BIAS_GELU_TANH : SF_EPI_BIAS;
-  const bool rows16 = K % 8 == 0 && aligned16(x) && aligned16(W);
-  // the direct loads' 32-bit offsets reach 2 GiB of either operand
-  const bool direct = rows16 && K > 0 && 2 * F * K < kMostRows && M * K < kMostRows;
-  int bm = 0, bn = 0;
-  const int cfg = gated_tile(M, F, K, rows16, direct, bm, bn);
-  p.tiles_m = (int)cdiv(M, bm);
-  p.tiles_n = (int)cdiv(2 * F, bn);
-  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, cus = cu_count_current();
-  if (tiles > (int64_t(1) << 22)) return fail(SF_ERR_UNSUPPORTED, "sf_gated_linear: more than 2^22 tiles");
+  p.tiles_m = (int)cdiv(M, g.bm);
+  p.tiles_n = (int)cdiv(2 * F, g.bn);
+  p.head = (int)g.head;
+  p.persist = g.persist ? cu_count_current() : 0;
   const auto launch = [&](int c, unsigned gx) {
     return dtype == SF_BF16 ? launch_gated_bf16(c, p, gx, st) : launch_gated_f16(c, p, gx, st);
   };
-  if (cfg != TILE_NT_BIG) return launch(cfg, (unsigned)tiles);
-  // A part round that its tiles' quarters fill better runs as those: 4096 rows, F
-  // 11008, K 4096 (5.4 rounds) 570 -> 552 us, F 2048 of 4352 rows (1.1) 172 -> 153;
-  // past about half a round the quarters take as long.
-  const int64_t rem = tiles % cus;
-  const bool quarters = tiles > cus && gated_quarters(rem, K, cus);
-  p.head = (int)(quarters ? tiles - rem : tiles);
-  // One workgroup a CU walks the tiles where the last round is full or at most
-  // half full, as sf_gemm's.
-  if (p.head > cus && cus % kNumXcd == 0 && 2 * (p.head % cus) <= cus) p.persist = (int)cus;
-  const int rc = launch(cfg, p.persist > 0 ? (unsigned)p.persist : (unsigned)p.head);
-  if (rc != SF_OK || !quarters) return rc;
+  rc = launch(g.cfg, p.persist > 0 ? (unsigned)p.persist : (unsigned)g.head);
+  if (rc != SF_OK || g.head == g.tiles) return rc;
   p.persist = 0;
   p.big_m = p.tiles_m;
   p.big_n = p.tiles_n;
-  return launch(TILE_MID_128, (unsigned)(4 * rem));
+  return launch(TILE_MID_128, (unsigned)(4 * (g.tiles - g.head)));
+}
+
+// fp32 layers of few rows, in one launch, bound by the weight's reading (F 5312, K
+// 2416: 25 us for one row and 36 for 16, the product and the gate 86; F 11008, K
+// 4096: 81 and 122, 145).
+static bool gated_few32(const void* x, const void* W, int64_t M, int64_t F, int64_t K) {
+  return M <= 16 && K > 0 && K % 4 == 0 && aligned16(x) && aligned16(W) && F < (int64_t(1) << 26);
 }
 
 // ---- windowed attention -------------------------------------------------------
@@ -469,15 +493,36 @@ int sf_gated_linear(const void* x, const void* W, const void* bias, void* y, voi
     return fail(SF_ERR_INVALID_ARG, "%s: null pointer", name);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype != SF_F32) return gated16(x, W, bias, y, pre, M, F, K, dtype, act, st);
-  // few rows: in one launch, bound by the weight's reading (F 5312, K 2416: 25 us
-  // for one row and 36 for 16, the product and the gate 86; F 11008, K 4096: 81
-  // and 122, 145)
-  if (M <= 16 && K > 0 && K % 4 == 0 && aligned16(x) && aligned16(W) && F < (int64_t(1) << 26))
-    return launch_gated_skinny32(x, W, bias, y, pre, M, F, K, epi_act(act), st);
+  if (gated_few32(x, W, M, F, K)) return launch_gated_skinny32(x, W, bias, y, pre, M, F, K, epi_act(act), st);
   rc = sf_gemm(0, 1, M, 2 * F, K, 1, x, K > 0 ? K : 1, 0, W, K > 0 ? K : 1, 0, pre, 2 * F, 0, SF_F32, SF_F32, 1.0f,
                bias, bias != nullptr ? SF_EPI_BIAS : SF_EPI_NONE, stream);
   if (rc != SF_OK) return rc;
   return launch_gate(epi_act(act), false, nullptr, pre, y, M, F, dtype, st);
+}
+
+int sf_gated_linear_plan(const void* x, const void* W, int64_t M, int64_t F, int64_t K, sf_dtype dtype, char* buf,
+                         int len) {
+  clear_error();
+  const char* name = "sf_gated_linear_plan";
+  if (buf == nullptr || len <= 0) return fail(SF_ERR_INVALID_ARG, "%s: bad buffer", name);
+  buf[0] = 0;
+  int rc = gated_check(name, M, F, K, dtype, SF_EPI_NONE);
+  if (rc != SF_OK) return rc;
+  const size_t n = static_cast<size_t>(len);
+  if (M == 0 || F == 0) {
+    snprintf(buf, n, "noop");
+  } else if (dtype == SF_F32) {
+    snprintf(buf, n, "gated fp32 %s", gated_few32(x, W, M, F, K) ? "16 rows" : "product, then gate");
+  } else {
+    GatedPlan g;
+    rc = gated_plan(name, x, W, M, F, K, g);
+    if (rc != SF_OK) return rc;
+    const bool staged = g.cfg == TILE_RAG_128 || g.cfg == TILE_RAG_64;
+    char quarters[32] = "";
+    if (g.head < g.tiles) snprintf(quarters, sizeof(quarters), ", %lld quartered", (long long)(g.tiles - g.head));
+    snprintf(buf, n, "gated %dx%d%s%s%s", g.bm, g.bn, staged ? " staged" : "", g.persist ? " persistent" : "", quarters);
+  }
+  return SF_OK;
 }
 
 int64_t sf_gated_backward_work(int64_t M, int64_t F) {

@@ -472,3 +472,23 @@ def test_norm_rope_into_rows_of_its_own_input(lib):
     far_rows = call(lib.sf_qk_norm_rope, P(x), 64, P(1 << 22), 32, 128, P(x + size), 2 ** 62, 2 ** 62, P(far), 64, 256, A,
                     8, 16, None, A, 2 ** 30, None, None, c_int(0), F32(1e-6), c_int(0), 2 ** 20, 4, 2, 1, 16, c_int(2), None)
     assert far_rows == INVALID and b"overlap" in lib.sf_last_error()  # 2^22 rows of x reach k
+
+
+def test_gated_plans(lib):
+    """Every kernel of the table has a size in the GPU's tests that chooses it."""
+    import gated_cases as gc
+    import test_gated_gpu as small
+    for dtype, M, K, F, want in gc.LARGE:
+        assert gc.plan(dtype, M, K, F) == want, (M, K, F)
+    assert [gc.plan(*c) for c in small.CASES] == gc.SMALL
+    assert gc.plan("bfloat16", 300, 64, 64, x=4098) == "gated 64x64 staged"
+    assert gc.plan("float32", 3, 64, 64, W=4100) == "gated fp32 product, then gate"
+    assert gc.plan("float16", 0, 64, 64) == gc.plan("float32", 3, 64, 0) == "noop"
+    buf = ctypes.create_string_buffer(8)
+    f = lib.sf_gated_linear_plan
+    assert call(f, A, A, 4, 16, 16, c_int(2), None, c_int(8)) == INVALID
+    assert call(f, A, A, 4, 16, 16, c_int(2), buf, c_int(0)) == INVALID
+    assert call(f, A, A, 4, 16, 16, c_int(3), buf, c_int(8)) == INVALID
+    assert call(f, A, A, -4, 16, 16, c_int(2), buf, c_int(8)) == INVALID
+    assert call(f, A, A, 2 ** 20, 2 ** 24, 64, c_int(2), buf, c_int(8)) == UNSUPPORTED
+    assert call(f, A, A, 4, 16, 16, c_int(2), buf, c_int(8)) == 0 and buf.value == b"gated 1"  # cut to the buffer
