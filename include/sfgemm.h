@@ -619,6 +619,14 @@ int sf_window_attention_cached(const void* Q, int64_t ldq, int64_t strideQ, int6
                                int64_t capacity, int64_t D, int64_t window, int64_t sinks, float scale, sf_dtype dtype,
                                void* work, void* stream);
 
+/* Diagnostic twin of sf_window_attention (capacity 0) and of
+ * sf_window_attention_cached, as sf_gemm_plan is sf_gemm's: writes what these
+ * sizes launch on the current device into buf[len]: "window 128 rows, heads up to
+ * 96" (query rows of a workgroup) or "window split 4, heads up to 128" (ranges of
+ * the keys; past 1 a second launch merges them).  Host-only. */
+int sf_window_attention_plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_t rows, int64_t capacity, int64_t D,
+                             int64_t window, int64_t sinks, char* buf, int len);
+
 /* The up side of a gated feed-forward layer: with W [2 F, K] holding the
  * gate's rows, then the up-projection's (bias [2 F] likewise, or NULL),
  *   y[m, f] = act(x[m] . W[f] + bias[f]) (x[m] . W[F + f] + bias[F + f])

@@ -483,6 +483,29 @@ int sf_window_attention_cached(const void* Q, int64_t ldq, int64_t strideQ, int6
   return launch_window(a, dtype, static_cast<float*>(work), static_cast<hipStream_t>(stream));
 }
 
+int sf_window_attention_plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_t rows, int64_t capacity, int64_t D,
+                             int64_t window, int64_t sinks, char* buf, int len) {
+  clear_error();
+  const char* name = "sf_window_attention_plan";
+  if (buf == nullptr || len <= 0) return fail(SF_ERR_INVALID_ARG, "%s: bad buffer", name);
+  buf[0] = 0;
+  bool noop;
+  const int rc = window_sizes(name, batch, heads, kv_heads, rows, capacity, D, window, sinks, &noop);
+  if (rc != SF_OK) return rc;
+  const size_t n = static_cast<size_t>(len);
+  if (noop) {
+    snprintf(buf, n, "noop");
+    return SF_OK;
+  }
+  WinShape a;
+  window_shape(a, batch, heads, kv_heads, rows, capacity > 0 ? capacity : rows, D, window, sinks);
+  a.cached = capacity > 0;
+  const WinPlan p = win_plan(a);
+  if (p.parts > 0) snprintf(buf, n, "window split %d, heads up to %d", p.parts, p.width);
+  else snprintf(buf, n, "window %d rows, heads up to %d", p.few ? 64 : 128, p.width);
+  return SF_OK;
+}
+
 int sf_gated_linear(const void* x, const void* W, const void* bias, void* y, void* pre, int64_t M, int64_t F, int64_t K,
                     sf_dtype dtype, sf_epilogue act, void* stream) {
   clear_error();

@@ -88,21 +88,26 @@ static int launch_win(const WinParams& p, int parts, bool few, hipStream_t st) {
   return few ? launch_win_rows<T, DW, true>(p, st) : launch_win_rows<T, DW, false>(p, st);
 }
 
+WinPlan win_plan(const WinShape& a) {
+  const int cus = cu_count_current();
+  const int64_t halves = a.batch * a.heads * cdiv64(a.Sq, WinCfg<64, true>::ROWS);
+  return {win_width(a.D), a.cached ? win_split_parts(a, cus) : 0, halves <= (a.D > 64 ? 1 : 2) * cus};
+}
+
 int launch_window(const WinShape& a, sf_dtype dt, float* ws, hipStream_t st) {
   WinParams p;
   win_fill_params(a, p);
-  int parts = 0;
+  const WinPlan plan = win_plan(a);
+  const int parts = plan.parts;
+  const bool few = plan.few;
   if (a.cached) {
-    parts = win_split_parts(a, cu_count_current());
     p.parts = parts;
     p.RB = (int)cdiv64(a.Sq * p.G, 16);
     p.ws = ws;
   }
-  const int64_t halves = a.batch * a.heads * cdiv64(a.Sq, WinCfg<64, true>::ROWS);
-  const bool few = halves <= (a.D > 64 ? 1 : 2) * cu_count_current();
   if (few) p.QB = (int)cdiv64(a.Sq, WinCfg<64, true>::ROWS);
   const bool h = dt == SF_F16;
-  switch (win_width(a.D)) {
+  switch (plan.width) {
     case 64: return h ? launch_win<F16, 64>(p, parts, few, st) : launch_win<BF16, 64>(p, parts, few, st);
     case 96: return h ? launch_win<F16, 96>(p, parts, few, st) : launch_win<BF16, 96>(p, parts, few, st);
   }

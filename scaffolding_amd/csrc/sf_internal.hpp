@@ -283,6 +283,13 @@ struct WinShape {
 };
 int launch_window(const WinShape& a, sf_dtype dt, float* ws, hipStream_t st);
 int64_t win_cached_work(const WinShape& a);
+// The kernels of a call: head sizes up to `width`; parts of the split kernel (0:
+// not split), else workgroups of 64 (few) or 128 rows.
+struct WinPlan {
+  int width, parts;
+  bool few;
+};
+WinPlan win_plan(const WinShape& a);
 
 struct WinParams;
 void win_fill_params(const WinShape& a, WinParams& p);

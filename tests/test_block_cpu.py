@@ -492,3 +492,39 @@ def test_gated_plans(lib):
     assert call(f, A, A, -4, 16, 16, c_int(2), buf, c_int(8)) == INVALID
     assert call(f, A, A, 2 ** 20, 2 ** 24, 64, c_int(2), buf, c_int(8)) == UNSUPPORTED
     assert call(f, A, A, 4, 16, 16, c_int(2), buf, c_int(8)) == 0 and buf.value == b"gated 1"  # cut to the buffer
+
+
+def test_window_plans(lib):
+    """The sizes of the GPU's tests choose the kernels that they are there for:
+    each width with 128 rows a workgroup, split and merged."""
+    import window_cases as wc
+    for _, B, N, H, Hk, D, window, sinks, _l, want in wc.LARGE:
+        assert wc.plan(B, H, Hk, N, 0, D, window, sinks) == want
+    for _, B, n, H, Hk, D, S, window, sinks, want in wc.CACHED:
+        assert wc.plan(B, H, Hk, n, S, D, window, sinks) == want
+    for cases, kinds in ((wc.LARGE, ["window 128 rows"]), (wc.CACHED, ["window 128 rows", "window split 1"])):
+        for kind in kinds:
+            assert {c[-1] for c in cases if c[-1].startswith(kind + ",")} == {
+                "%s, heads up to %d" % (kind, w) for w in (64, 96, 128)}
+    assert {c[-1].split()[-1] for c in wc.CACHED if "split" in c[-1] and "split 1," not in c[-1]} == {"64", "96", "128"}
+    assert wc.plan(3, 6, 2, 777, 0, 72, 100, 3) == "window 64 rows, heads up to 96"
+    assert wc.plan(0, 6, 2, 777, 0, 72, 100, 3) == wc.plan(3, 6, 2, 0, 9, 72, 100, 3) == "noop"
+    buf, f = ctypes.create_string_buffer(8), lib.sf_window_attention_plan
+    assert call(f, 1, 4, 2, 4, 8, 16, 2, 1, None, c_int(8)) == INVALID
+    assert call(f, 1, 4, 2, 4, 8, 16, 2, 1, buf, c_int(0)) == INVALID
+    assert call(f, 1, 3, 2, 4, 8, 16, 2, 1, buf, c_int(8)) == INVALID
+    assert call(f, 1, 4, 2, 4, 8, 12, 2, 1, buf, c_int(8)) == UNSUPPORTED
+    assert call(f, 1, 4, 2, 4, -1, 16, 2, 1, buf, c_int(8)) == INVALID
+
+
+@pytest.mark.parametrize("first,window,sinks", [(0, None, 0), (5, 3, 2), (20, 2, 0), (0, 1, 4)])
+def test_rows_in_64_bits_are_the_oracle_s(first, window, sinks):
+    import window_cases as wc
+    rng = np.random.default_rng(first)
+    q, k, v = rng.standard_normal((6, 4)), rng.standard_normal((11, 4)), rng.standard_normal((11, 4))
+    out, lse, p = ox.window_rows(q, k, v, first, window, sinks, 0.7)
+    o, s, w, avg, size = wc.rows64(q, k, v, first, window, sinks, 0.7)
+    assert np.abs(o - out).max() < 1e-13 and np.abs(w - p).max() < 1e-14 and (np.isinf(s) == np.isinf(lse)).all()
+    there = np.isfinite(lse)
+    assert np.abs(s[there] - lse[there]).max(initial=0) < 1e-13
+    assert np.abs(avg - p @ np.abs(v)).max() < 1e-13
