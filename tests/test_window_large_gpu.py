@@ -198,3 +198,58 @@ def test_caches_at_the_top_of_the_type(dtype, B, n, H, Hk, D, S, window, sinks, 
     y = down(cu().dev_window_attention_cached(up(q, dtype), up(k, dtype), up(v, dtype), ints([S - n] * B), H, Hk, window,
                                               sinks, 0.2))
     check_top(y, H, D, dtype)
+
+
+# ---- gradients of many key blocks ----------------------------------------------------
+
+def gradients(g, x, H, Hk, D, window, sinks, scale, dtype, lengths=None):
+    """(dx, bound), the bound as test_window_gpu's: P and dS rounded once for their
+    products, delta and the log-sums within another half step of the magnitudes,
+    the scores' D fp32 roundings, sums of up to N rows of every head 2^-23 a term,
+    the result's rounding; fp16's smallest steps of dS (2^-24)."""
+    B, N, _ = x.shape
+    h, gh = x.astype(np.float64).reshape(B, N, H + 2 * Hk, D), g.astype(np.float64).reshape(B, N, H, D)
+    out, mag = np.zeros(h.shape), np.zeros(h.shape)
+    for b in range(B):
+        n = N if lengths is None else lengths[b]
+        for a in range(H):
+            u, v = H + a // (H // Hk), H + Hk + a // (H // Hk)
+            qh, kh, vh, go = h[b, :n, a], h[b, :n, u], h[b, :n, v], gh[b, :n, a]
+            o, _, p, avg, _ = rows64(qh, kh, vh, 0, window, sinks, scale)
+            ds = p * (go @ vh.T - (go * o).sum(1, keepdims=True)) * scale
+            size = p * (np.abs(go) @ np.abs(vh).T + (np.abs(go) * avg).sum(1, keepdims=True)) * abs(scale)
+            for t, e, f in ((out, ds, lambda z: z), (mag, size, np.abs)):
+                t[b, :n, a] = e @ f(kh)
+                t[b, :n, u] += e.T @ f(qh)
+                t[b, :n, v] += p.T @ f(go)
+    hu = out_half_ulp_rel(dtype)
+    most = np.abs(h[:, :, :H]).sum(-1).max() * np.abs(h[:, :, H:H + Hk]).max()
+    rel = 3 * hu + 4 * D * 2.0 ** -23 * abs(scale) * most + (N * H // Hk + D) * 2.0 ** -23 + 2.0 ** -16
+    tiny = 2.0 ** -24 * N * (H // Hk) * np.abs(x).max() * max(abs(scale), 1.0) if dtype == "float16" else 0.0
+    tol = rel * mag + tiny
+    return out.reshape(x.shape), (tol + hu * (np.abs(out) + tol) + 2.0 ** -24).reshape(x.shape)
+
+
+@pytest.mark.parametrize("dtype,B,N,H,Hk,D,window,sinks,ragged", [
+    ("bfloat16", 40, 300, 4, 4, 64, 100, 3, True), ("float16", 70, 130, 4, 2, 72, None, 0, True),
+    ("bfloat16", 2, 1100, 16, 4, 128, 300, 70, False), ("float16", 3, 700, 12, 3, 96, 2, 640, False),
+])
+def test_gradients_of_many_key_blocks(dtype, B, N, H, Hk, D, window, sinks, ragged):
+    """More key blocks than the plan's workgroup has threads, as many ranges as
+    CUs, key blocks cut into many ranges."""
+    rng = np.random.default_rng(N)
+    x, g = rnd(rng, (B, N, (H + 2 * Hk) * D), 1.0, dtype), rnd(rng, (B, N, H * D), 0.5, dtype)
+    lengths = None
+    if ragged:
+        lengths = rng.integers(0, N + 1, B)
+        lengths[:3] = 0, N, 1
+    want, tol = gradients(g, x, H, Hk, D, window, sinks, D ** -0.5, dtype, lengths)
+    if ragged:
+        for b, n in enumerate(lengths):
+            x[b, n:], g[b, n:] = np.nan, np.nan
+    gx, gg, gn = up(x, dtype), up(g, dtype), None if lengths is None else ints(lengths)
+    out, lse = cu().dev_window_attention(gx, H, Hk, window, sinks, None, gn, True)
+    args = gg, gx, out, lse, H, Hk, window, sinks, None, gn
+    dx = down(cu().dev_window_attention_backward(*args))
+    check_bound(dx, want, tol)
+    assert (down(cu().dev_window_attention_backward(*args)) == dx).all()
