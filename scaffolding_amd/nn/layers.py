@@ -525,7 +525,7 @@ class WindowAttention(Module):
             raise ValueError("WindowAttention: rotary must be an even number up to %d, got %d" % (head_dim, rotary))
         if norm not in ("rms", "layer"):
             raise ValueError("WindowAttention: unknown norm %r" % (norm,))
-        self._check_dtype(dtype)
+        self._check_dtype("float32" if dtype is None else dtype)  # what a layer without a type gets
         from .functional import rope_table
         self.heads, self.kv_heads, self.head_dim = heads, kv_heads, head_dim
         self.window, self.sinks = window, sinks
