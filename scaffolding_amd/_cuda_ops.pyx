@@ -1506,11 +1506,11 @@ _ACT_EPI = (SF_EPI_NONE, SF_EPI_SILU, SF_EPI_GELU_TANH)
 cdef tuple _packed_heads(str name, gt, int heads, int kv_heads):
     """(B, N, D) of a packed projection (..., N, (heads + 2 kv_heads) D)."""
     shape = tuple(gt.shape)
-    if heads < 1 or kv_heads < 1 or len(shape) not in (2, 3) or shape[-1] % (heads + 2 * kv_heads) != 0 \
-            or shape[-1] == 0:
+    cdef int64_t per = heads + 2 * <int64_t>kv_heads
+    if heads < 1 or kv_heads < 1 or len(shape) not in (2, 3) or shape[-1] % per != 0 or shape[-1] == 0:
         raise ValueError("%s: the projection must be (B, N, (%d + 2 * %d) * D), got %s"
                          % (name, heads, kv_heads, shape))
-    return (shape[0] if len(shape) == 3 else 1), shape[-2], shape[-1] // (heads + 2 * kv_heads)
+    return (shape[0] if len(shape) == 3 else 1), shape[-2], shape[-1] // per
 
 
 cdef object _norm_rope_operands(str name, x, table, positions, weight, bias, norm, tuple bnd):

@@ -536,3 +536,11 @@ def test_attention_modules_refuse_fp32_where_they_are_made(dtype):
     raises(TypeError, nn.WindowAttention, 64, 4, device="cpu", dtype=dtype)
     raises(TypeError, nn.DecoderBlock, 64, 96, 4, device="cpu", dtype=dtype)
     assert nn.WindowAttention(64, 4, device="cpu", dtype="float16").qkv.weight.dtype.value == "float16"
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(2, 2 ** 31 - 1), (3, 2 ** 31 - 1), (2 ** 31 - 1, 2 ** 30), (2 ** 30, 2 ** 30)])
+def test_heads_whose_sum_passes_32_bits(heads, kv_heads):
+    from scaffolding_amd import _cuda_ops as g
+    for f in (g.dev_qk_norm_rope, g.dev_window_attention):
+        with pytest.raises(ValueError, match="projection must be"):
+            f(fake((2, 3, 64)), heads, kv_heads)
