@@ -587,8 +587,9 @@ int sf_window_attention(const void* Q, int64_t ldq, int64_t strideQ, int64_t hea
  * and scale; O and lse as it wrote them) from dO, that of O: dQ laid out with
  * strides of its own, dK and dV with kv_heads heads, summed over the query
  * heads that share them; 0 for rows behind lengths.  P and dS are rounded to
- * dtype for their products (dS unscaled: fp16 gradients past 65504 overflow);
- * sums fp32, in an order fixed by the sizes.  A NaN or infinity reaches the
+ * dtype for their products (dS unscaled: in fp16 terms past 65504 overflow, those
+ * below 2^-14 keep fewer digits and those below 2^-25 are lost; P is held times
+ * 2^8); sums fp32, in an order fixed by the sizes.  A NaN or infinity reaches the
  * gradients of the tokens around it.  The gradients may not overlap the
  * operands or each other.  `work`: sf_window_attention_backward_work bytes of
  * 16-byte aligned device memory of the call's device, overwritten. */
@@ -606,7 +607,8 @@ int sf_window_attention_backward(const void* dO, int64_t lddo, int64_t strideDO,
 
 /* Over a cache of `capacity` rows: query i of sequence b stands at lengths[b]
  * + i and sees keys up to its own, which are there already (sf_qk_norm_rope
- * writes them).  lengths int32 [batch], cut to [0, capacity].  Few rows over
+ * writes them): every token keeps a row of its own, and a window bounds what is
+ * read of the cache, not its memory.  lengths int32 [batch], cut to [0, capacity].  Few rows over
  * many keys are split over ranges of the keys: `work` is
  * sf_window_attention_cached_work bytes of 16-byte aligned device memory of
  * the call's device (may be NULL where that is 0), overwritten. */

@@ -1793,8 +1793,10 @@ def dev_window_attention_cached(gt_q, gt_k, gt_v, gt_lengths, int heads, int kv_
 
 def dev_gated_linear(gt_x, gt_weight, gt_bias=None, activation='silu', bint with_pre=False):
     """y = act(x @ Wg^T + bg) * (x @ Wu^T + bu), W (2 F, K) holding Wg's rows,
-    then Wu's, b (2 F,) likewise: x (..., K) -> y (..., F), one launch (two in
-    fp32).  with_pre: (y, pre), pre (..., 2 F) the two projections."""
+    then Wu's, b (2 F,) likewise: x (..., K) -> y (..., F).  One launch, two where
+    a part round of tiles runs as quarters (16-bit, many rows) and in fp32 past 16
+    rows (or with rows that are not 16-byte aligned).  with_pre: (y, pre), pre
+    (..., 2 F) the two projections."""
     name = 'dev_gated_linear'
     _same_dtype(gt_x, gt_weight, name)
     if len(gt_x.shape) < 1 or len(gt_weight.shape) != 2 or gt_weight.shape[0] % 2 \

@@ -77,7 +77,8 @@ static int gated_check(const char* name, int64_t M, int64_t F, int64_t K, sf_dty
 
 // Tiles of a gated product: lines of W a tile takes are half gate, half up.  The
 // times are fitted to a sweep of 20 to 4096 rows over layers of F 352 to 11008
-// and K 208 to 4096 (bf16): there the choice is within 6 % of the fastest.
+// and K 208 to 4096 (bf16): there the choice is within 1 % of the fastest in 82 of
+// 88 sizes and within 7 % in all.
 struct GatedTile {
   int cfg, bm, bn, occ;
   float tau[4];  // us per 64 k when r workgroups share each CU, in line between

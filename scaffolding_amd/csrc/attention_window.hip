@@ -29,7 +29,14 @@ void win_fill_params(const WinShape& a, WinParams& p) {
 // the better choice.  Estimated us: a workgroup of the split kernel (one a CU
 // at head sizes past 64, else two) takes 3 and 2.6 per four blocks of 32 keys
 // (its share of the memory's rate), the merge 3; one of win_attn_kernel (two a
-// CU) 5 and 1 per block of 64 keys.
+// CU, 128 rows) 5 and 1 per block of 64 keys.  Both sides measured over 216 caches
+// (1, 8, 32 sequences of 256 to 4096 tokens, 1 to 64 new ones, 8 or 32 heads of 64
+// and 128 on 1 to 8 key heads): the choice is within 6 % of the better one in 153
+// and within 30 % in 207.  It misses where several row blocks share a key head,
+// whose keys the second one finds in L2 while the estimate counts them again: 16
+// tokens over 32 x 4096, 32 heads of 64 on one, take 167 us in whole rows and 54
+// split.  The other way by at most 29 %: 16 tokens over 8 x 1024, 32 heads of 64 on
+// 8, 18.8 us in two ranges, 14.5 in workgroups of 64 rows.
 static int win_split_parts(const WinShape& a, int cus) {
   const int64_t G = a.heads / a.kv_heads, RB = cdiv64(a.Sq * G, 16), items = a.batch * a.kv_heads * RB;
   const int64_t W = a.window > 0 ? a.window : a.Sk;

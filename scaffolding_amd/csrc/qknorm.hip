@@ -502,9 +502,11 @@ __global__ __launch_bounds__(1024) void qk_norm_sums_kernel(NormRopeParams p, un
 }
 
 // The widest chunk that the sizes take: chunks divide the head and, in twos,
-// what is rotated of it.  Backward at most 4 columns: with 8, the sums and
-// operands take 230 registers, and half as many waves are there to hide the
-// memory's latency.
+// what is rotated of it.  Backward at most 4 columns (124 registers, four waves a
+// SIMD): with 8, the sums of both parameters and the operands take 231, and half
+// as many waves are there to hide the memory's latency.  (The kernel takes either
+// norm at run time and sums both parameters; one for the rms norm without its
+// bias would take 94, and 150 with 8 columns.  None is built.)
 static int chunk_of(int D, int rot, bool back) {
   if (!back && D % 8 == 0 && rot % 16 == 0) return 8;
   if (D % 4 == 0 && rot % 8 == 0) return 4;

@@ -343,10 +343,11 @@ def window_attention_cached(q: Tensor, k_cache: Tensor, v_cache: Tensor, lengths
 
 def gated_linear(input: Tensor, weight: Tensor, bias: Tensor | None = None, activation: str | None = "silu",
                  return_pre: bool = False):
-    """The up side of a gated feed-forward layer, one launch: act(input Wg^T +
-    bg) * (input Wu^T + bu), weight (2 F, K) holding Wg's rows, then Wu's, bias
-    (2 F,) likewise; (..., K) -> (..., F).  return_pre: (output, pre), pre
-    (..., 2 F) the two projections, for gated_linear_backward."""
+    """The up side of a gated feed-forward layer: act(input Wg^T + bg) * (input
+    Wu^T + bu), weight (2 F, K) holding Wg's rows, then Wu's, bias (2 F,)
+    likewise; (..., K) -> (..., F).  One launch; two for some 16-bit layers of
+    many rows and for fp32 past 16 rows.  return_pre: (output, pre), pre (..., 2
+    F) the two projections, for gated_linear_backward."""
     dev = _device_of("gated_linear", input, weight, bias)
     out = _cuops.dev_gated_linear(input._gpu, _on(weight, dev), _on(bias, dev), activation, return_pre)
     if return_pre:

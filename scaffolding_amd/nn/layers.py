@@ -471,7 +471,7 @@ class _ExpertLinear(Module):
 
 class GatedMLP(Module):
     """A gated feed-forward layer: down(act(x Wg^T + bg) * (x Wu^T + bu)), the
-    part in brackets in one launch (F.gated_linear).  up.weight (2 hidden, dim)
+    part in brackets fused (F.gated_linear).  up.weight (2 hidden, dim)
     holds Wg's rows, then Wu's, up.bias (2 hidden,) likewise; down.weight (dim,
     hidden).  Inference, as Linear (F.gated_linear_backward gives the
     gradients)."""
@@ -551,7 +551,8 @@ class WindowAttention(Module):
 
     def cache(self, batch: int, capacity: int) -> tuple[Tensor, Tensor]:
         """Zeroed caches of keys and values, (batch, capacity, kv_heads
-        head_dim), on the weights' device in their type."""
+        head_dim), on the weights' device in their type: every token has a row of
+        its own, whatever the window."""
         if self.table is not None and capacity > self.table.shape[0]:
             raise ValueError("WindowAttention: a cache of %d tokens, positions up to %d" % (capacity, self.table.shape[0]))
         w = self.qkv.weight
